@@ -365,6 +365,82 @@ int lq_q8_decode_append_attn_noalloc(const uint16_t* q, const uint16_t* k_new,
                                      int64_t n, const int32_t* lens_host, float scale,
                                      uint16_t* out, void* stream);
 
+/*
+ * A paged 8-bit cache (no counterpart in the reference, whose caches hold one sequence each in one
+ * buffer): the K/V of one layer for several sequences, in pages of 64 positions,
+ *   codes uint8 [pages, Hkv, 64, 128], scales and biases bf16 [pages, Hkv, 64, 2]  (K and V each)
+ * -- every page the cache layout above with cap = 64. Row b of `table` (int32, device, rows
+ * table_stride entries apart, table_width entries) lists the pages of sequence b in order: position p
+ * lies in slot p % 64 of page table[b][p / 64]. Pool buffers 16-byte aligned; ids outside
+ * [0, pages) are never followed.
+ *
+ * lq_paged_append: rows of up to LQ_MAX_SEQS sequences, packed one sequence behind the other
+ * (sequence b has counts_host[b] rows), quantized as lq_quantize_append_kv into positions starts[b],
+ * starts[b] + 1, .. of sequence b. k and v bf16, row t of head h at k + t k_tok + h k_head (elements;
+ * strides multiples of 8, rows 16-byte aligned). Rows whose position or page does not exist are not
+ * stored. No two rows of a call may go to one slot (a page that two sequences share is copied
+ * first): what such a slot holds afterwards is undefined.
+ */
+int lq_paged_append(const uint16_t* k, const uint16_t* v, int64_t k_tok, int64_t k_head,
+                    int64_t v_tok, int64_t v_head, uint8_t* kc, uint16_t* ks, uint16_t* kb,
+                    uint8_t* vc, uint16_t* vs, uint16_t* vb, int64_t pages, int64_t Hkv, int64_t D,
+                    const int32_t* table, int64_t table_stride, int64_t table_width,
+                    const int32_t* starts, const int32_t* counts_host, int64_t nseq, void* stream);
+
+/*
+ * Positions starts[b] .. starts[b] + counts_host[b] - 1 of each sequence as bf16 rows, dequantized
+ * as lq_dequantize, packed one sequence behind the other: k_out, v_out bf16 [rows, Hkv, 128].
+ * Positions whose page does not exist read as NaN.
+ */
+int lq_paged_gather(const uint8_t* kc, const uint16_t* ks, const uint16_t* kb, const uint8_t* vc,
+                    const uint16_t* vs, const uint16_t* vb, int64_t pages, int64_t Hkv, int64_t D,
+                    const int32_t* table, int64_t table_stride, int64_t table_width,
+                    const int32_t* starts, const int32_t* counts_host, int64_t nseq,
+                    uint16_t* k_out, uint16_t* v_out, void* stream);
+
+/*
+ * Copies n pages of the pool, all heads of K and V: page src_host[i] to page dst_host[i] (host
+ * arrays). A page may be copied to several; no page may be written twice, or both read and written
+ * (LQ_EINVAL).
+ */
+int lq_copy_pages(uint8_t* kc, uint16_t* ks, uint16_t* kb, uint8_t* vc, uint16_t* vs, uint16_t* vb,
+                  int64_t pages, int64_t Hkv, int64_t D, const int32_t* src_host,
+                  const int32_t* dst_host, int64_t n, void* stream);
+
+/*
+ * Attention of one new token per sequence over a paged cache: q, out bf16 [B, Hq, 1, 128], sequence b
+ * attends to its first lens[b] positions (int32, device; read by the kernel, so a captured call
+ * follows them), values as lq_paged_gather reads them. The first shared_pages pages are promised to be
+ * the same in the table rows of all sequences that are at least that long, and are read once for them;
+ * shorter sequences are attended on their own. lens[b] == 0: the sequence's rows are 0; a length
+ * outside [0, 64 table_width] or a page outside the pool: NaN. Hq / Hkv <= 16, B <= 4096. Workspace:
+ * lq_paged_decode_workspace_bytes, any contents; calls that may overlap need their own.
+ */
+int64_t lq_paged_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t shared_pages);
+int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const uint16_t* ks,
+                         const uint16_t* kb, const uint8_t* vc, const uint16_t* vs,
+                         const uint16_t* vb, int64_t pages, int64_t B, int64_t Hq, int64_t Hkv,
+                         int64_t D, const int32_t* table, int64_t table_stride, int64_t table_width,
+                         const int32_t* lens, int64_t shared_pages, float scale, uint16_t* out,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Causal attention of packed prompts (bf16), without padding or a score matrix: sequence s has
+ * q_lens_host[s] query rows and k_lens_host[s] keys (host arrays, up to LQ_MAX_SEQS), each packed one
+ * sequence behind the other; its row i sees keys 0 .. k_lens - q_lens + i (a prompt has as many of
+ * both, a later chunk more keys). Rows that see no key are 0.
+ *   q bf16: row t of head h at q + t q_tok + h q_head; k, v alike (elements; strides multiples of 8,
+ *   rows 16-byte aligned); out bf16 [rows, Hq, 128] contiguous. Hq / Hkv <= 64.
+ * Workspace: lq_prompt_workspace_bytes (0 for many calls), any contents.
+ */
+int64_t lq_prompt_workspace_bytes(const int32_t* q_lens_host, const int32_t* k_lens_host,
+                                  int64_t nseq, int64_t Hq, int64_t Hkv);
+int lq_prompt_attn(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t q_tok,
+                   int64_t q_head, int64_t k_tok, int64_t k_head, int64_t v_tok, int64_t v_head,
+                   const int32_t* q_lens_host, const int32_t* k_lens_host, int64_t nseq, int64_t Hq,
+                   int64_t Hkv, int64_t D, float scale, uint16_t* out, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

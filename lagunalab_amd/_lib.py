@@ -67,6 +67,17 @@ SIGNATURES = {
                                 i64, vp, vp, vp]),
     "lq_q8_decode_append_attn_pos": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64,
                                            i64, i64, vp, f32, vp, vp, i64, vp]),
+    "lq_paged_append": (i32, [vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp,
+                              i64, i64, vp, vp, i64, vp]),
+    "lq_paged_gather": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, i64, i64, vp, vp, i64, vp, vp,
+                              vp]),
+    "lq_copy_pages": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, vp, i64, vp]),
+    "lq_paged_decode_workspace_bytes": (i64, [i64, i64, i64, i64]),
+    "lq_paged_decode_attn": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, i64, i64, vp,
+                                   i64, f32, vp, vp, i64, vp]),
+    "lq_prompt_workspace_bytes": (i64, [vp, vp, i64, i64, i64]),
+    "lq_prompt_attn": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i64, vp, vp, i64, i64, i64, i64, f32,
+                             vp, vp, i64, vp]),
     "lq_q8_decode_append_attn_noalloc": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64,
                                                i64, i64, i64, vp, f32, vp, vp]),
 }

@@ -1,0 +1,219 @@
+// Attention of 16 NT query rows per wave over one 64-key tile of bf16 K and V in LDS, on the matrix
+// cores: the inner step of the paged prefix and the packed prompt kernels.
+//
+// S = K Q^T as v_mfma_f32_16x16x32_bf16 (M = 16 keys, N = 16 rows, K = 32 dims): lane (lc = lane % 16,
+// lq4 = lane / 16) ends with the scores of keys 16 mt + 4 lq4 + r of row lc. P of key tiles 2 e and
+// 2 e + 1 is then, as it lies in the lane's registers, the B operand of k-step e of O^T = V^T P^T: slot
+// 4 h + r of lane group lq4 is key 32 e + 16 h + 4 lq4 + r. V^T's A operand takes the keys in that order
+// with two transposed LDS reads (ds_read_b64_tr_b16: of 4 keys x 16 dims per 16 lanes, lane i gets dim
+// i of the four keys), so neither P nor V is moved between lanes.
+//
+// Softmax in fp32 with a running maximum that moves only when a tile's exceeds it by 2^8; P rounded to
+// bf16 for its product (2^-8 relative at most per key, of either sign, against an output of the same
+// type; bf16 keeps the range of V). The row sums are those of the rounded P, one more product with ones.
+#pragma once
+
+#include "attn_dev.h"
+
+namespace lq {
+namespace attn {
+
+constexpr int TKEYS = 64;  // keys of a tile, positions of a page
+
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4_t lds_s4_t;
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+// A tile in LDS. K: 16-byte chunk j of key r at chunk j ^ (r & 15); V: 32-byte window w of key r at
+// window w ^ (r & 7): operand reads touch every bank equally.
+struct alignas(256) KvTile {
+  uint16_t k[TKEYS * D];
+  uint16_t v[TKEYS * D];
+};
+__device__ __forceinline__ uint4* k_chunk(KvTile& t, int key, int chunk) {
+  return reinterpret_cast<uint4*>(t.k) + 16 * key + (chunk ^ (key & 15));
+}
+__device__ __forceinline__ uint4* v_chunk(KvTile& t, int key, int chunk) {
+  return reinterpret_cast<uint4*>(t.v) + 16 * key + (chunk ^ (2 * (key & 7)));
+}
+
+// Two floats as one dword of bf16, round to nearest even, x in the low half (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ uint32_t pack_bf2(float x, float y) {
+  typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+  const bf2_t p = {(__bf16)x, (__bf16)y};
+  return __builtin_bit_cast(uint32_t, p);
+}
+__device__ __forceinline__ bf16x8_t words_as_bf8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const u4_t u = {a, b, c, d};
+  return __builtin_bit_cast(bf16x8_t, u);
+}
+__device__ __forceinline__ bf16x8_t u4_as_bf8(uint4 u) { return words_as_bf8(u.x, u.y, u.z, u.w); }
+
+// Codes 0..3 of a word as scale * code + bias in bf16: the product is exact in fp32, so the fused
+// multiply-add rounds as the two operations of the dequantizer do.
+__device__ __forceinline__ uint2 dequant4(uint32_t w, float s, float b) {
+  return make_uint2(pack_bf2(fmaf(s, (float)(w & 0xffu), b), fmaf(s, (float)((w >> 8) & 0xffu), b)),
+                    pack_bf2(fmaf(s, (float)((w >> 16) & 0xffu), b), fmaf(s, (float)(w >> 24), b)));
+}
+
+__device__ __forceinline__ bf16x8_t bf16_ones() {
+  return words_as_bf8(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+}
+
+// The softmax scale in log2 units, as its magnitude (the sign goes into q): never 0, so that a masked
+// score of -infinity stays one.
+__device__ __forceinline__ float abs_scale(float sl2) { return fmaxf(fabsf(sl2), 1e-37f); }
+// A q row's 16 bytes with the scale's sign.
+__device__ __forceinline__ uint4 signed_q(uint4 u, float sl2) {
+  const uint32_t x = sl2 < 0.0f ? 0x80008000u : 0u;
+  return make_uint4(u.x ^ x, u.y ^ x, u.z ^ x, u.w ^ x);
+}
+
+// State of a wave's rows: row 16 nt + lc in column lc of N tile nt.
+template <int NT>
+struct TileRows {
+  bf16x8_t q[NT][4];  // B operands: dims 32 kk + 8 lq4 .. + 7
+  f4_t o[NT][8];      // O^T: dims 16 w + 4 lq4 + r
+  f4_t l[NT];         // row sums of P, the same in all four
+  float m[NT];        // running maximum, log2 units
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int w = 0; w < 8; ++w) o[nt][w] = f4_t{0.f, 0.f, 0.f, 0.f};
+      l[nt] = f4_t{0.f, 0.f, 0.f, 0.f};
+      m[nt] = -INFINITY;
+    }
+  }
+};
+
+// Raw scores of the tile's keys.
+template <int NT>
+__device__ __forceinline__ void tile_scores(const KvTile& t, const TileRows<NT>& st, int lane,
+                                            f4_t (&c)[NT][4]) {
+  const int lc = lane & 15, lq4 = lane >> 4;
+  const bf16x8_t* k = reinterpret_cast<const bf16x8_t*>(t.k) + 16 * lc;
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const bf16x8_t a = k[256 * mt + ((4 * kk + lq4) ^ lc)];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        c[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            a, st.q[nt][kk], kk == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : c[nt][mt], 0, 0, 0);
+    }
+}
+
+// Scores to weights: raises the running maximum where needed (and rescales the row), P in bf16 as the
+// B operands of the two k-steps.
+template <int NT>
+__device__ __forceinline__ void tile_softmax(f4_t (&c)[NT][4], TileRows<NT>& st, float scale,
+                                             bf16x8_t (&p)[NT][2]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float t = -INFINITY;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t = max_ieee(t, c[nt][mt][r]);
+    t = max_xor32(max_xor16(t)) * scale;
+    const bool bump = t > (st.m[nt] == -INFINITY ? -INFINITY : st.m[nt] + RESCALE_LOG2);
+    if (__builtin_amdgcn_ballot_w64(bump)) {
+      const float mn = bump ? t : st.m[nt];
+      const float alpha = st.m[nt] == -INFINITY ? 0.0f : exp2_nonpos(st.m[nt] - mn);
+      st.m[nt] = mn;
+      st.l[nt] *= alpha;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) st.o[nt][w] *= alpha;
+    }
+    const float off = st.m[nt] == -INFINITY ? 0.0f : -st.m[nt];
+    uint32_t w[8];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[2 * mt + h] = pack_bf2(__builtin_amdgcn_exp2f(fmaf(c[nt][mt][2 * h], scale, off)),
+                                 __builtin_amdgcn_exp2f(fmaf(c[nt][mt][2 * h + 1], scale, off)));
+    p[nt][0] = words_as_bf8(w[0], w[1], w[2], w[3]);
+    p[nt][1] = words_as_bf8(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// A operand of dims 16 w .. 16 w + 15 and k-step e of a tile's V^T.
+__device__ __forceinline__ uint32_t v_lane(const KvTile& t, int lane) {
+  const int rk = 4 * (lane >> 4) + ((lane >> 2) & 3);  // key of this lane's source within 16
+  return lds_addr(t.v) + (uint32_t)(256 * rk + 8 * (lane & 3) + 32 * (rk & 7));
+}
+__device__ __forceinline__ bf16x8_t v_operand(uint32_t vl, int w, int e) {
+  const uint32_t a = (vl ^ (uint32_t)(32 * w)) + 8192u * e;
+  const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(uintptr_t)a);
+  const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(uintptr_t)(a + 4096u));
+  typedef short s8_t __attribute__((ext_vector_type(8)));
+  const s8_t u = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(bf16x8_t, u);
+}
+
+// The bf16 pairs of an operand with infinities and NaN as 0.
+__device__ __forceinline__ bf16x8_t finite_only(bf16x8_t x) {
+  u4_t u = __builtin_bit_cast(u4_t, x);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if ((u[j] & 0x7f80u) == 0x7f80u) u[j] &= 0xffff0000u;
+    if ((u[j] & 0x7f800000u) == 0x7f800000u) u[j] &= 0xffffu;
+  }
+  return __builtin_bit_cast(bf16x8_t, u);
+}
+
+// FINITE: infinities and NaN of V are left out (0 times one of them is no 0).
+template <int NT, bool FINITE = false>
+__device__ __forceinline__ void tile_values(const KvTile& t, TileRows<NT>& st, int lane,
+                                            const bf16x8_t (&p)[NT][2]) {
+  const uint32_t vl = v_lane(t, lane);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      st.l[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_ones(), p[nt][e], st.l[nt], 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      bf16x8_t a = v_operand(vl, w, e);
+      if constexpr (FINITE) a = finite_only(a);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        st.o[nt][w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p[nt][e], st.o[nt][w], 0, 0, 0);
+    }
+  }
+}
+
+// What tile_values<NT, true> left out, for the rows that see the key (lim: last key of each row, counted
+// from the tile): keys' infinities and NaN, one key of `mask` at a time. Rare.
+template <int NT>
+__device__ __forceinline__ void tile_nonfinite(const KvTile& t, TileRows<NT>& st, int lane,
+                                               const bf16x8_t (&p)[NT][2], const int (&lim)[NT],
+                                               uint64_t mask) {
+  const int lc = lane & 15, lq4 = lane >> 4;
+  for (; mask; mask &= mask - 1) {
+    const int key = __builtin_ctzll(mask);
+    const int word = 2 * ((key >> 4) & 1) + ((key >> 1) & 1);
+    const uint16_t* vrow = t.v + key * D + 4 * lq4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const u4_t pe = __builtin_bit_cast(u4_t, key < 32 ? p[nt][0] : p[nt][1]);
+      const uint32_t mine = word < 2 ? (word == 0 ? pe[0] : pe[1]) : (word == 2 ? pe[2] : pe[3]);
+      const uint32_t pw = __shfl(mine, 16 * ((key >> 2) & 3) + lc, 64);
+      const float pk = key & 1 ? bf16_hi(pw) : bf16_lo(pw);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const uint2 v2 = *reinterpret_cast<const uint2*>(vrow + 16 * (w ^ (key & 7)));
+        const float v[4] = {bf16_lo(v2.x), bf16_hi(v2.x), bf16_lo(v2.y), bf16_hi(v2.y)};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (key <= lim[nt] && !(fabsf(v[r]) < INFINITY)) st.o[nt][w][r] = fmaf(pk, v[r], st.o[nt][w][r]);
+      }
+    }
+  }
+}
+
+}  // namespace attn
+}  // namespace lq

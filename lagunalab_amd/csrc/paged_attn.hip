@@ -1,0 +1,581 @@
+// Attention of one new token per sequence over a paged 8-bit cache, the pages that all sequences share
+// read once for the batch (a prompt and the answers sampled from it, a long system prompt).
+//
+// Work. A KV head's shared pages are cut into np parts; a workgroup takes one part for a block of 64 or
+// 128 query rows (the G rows of each sequence, one sequence behind the other), dequantizes each page
+// once into LDS and runs the matrix-core tile of attn_tile.h on it. A sequence's own pages are cut into
+// chunks; a workgroup takes one chunk for the sequence's G <= 16 rows, one page per wave at a time, K
+// straight from memory into MFMA operands, V transposed through the wave's own LDS. Both kinds write
+// partial rows (max, sum, weighted values), which a second launch merges.
+//
+// Lengths are read on the device, so one recorded launch serves every step of a growing batch: every
+// workgroup adds up the sequences' own pages, takes the chunk size that splits them over the workgroups
+// that fill the GPU, and finds its own chunk. Workgroups without one leave at once.
+//
+// Values: an attended K or V is bf16(scale * code + bias), what dequantizing the page gives; products on
+// bf16 operands with fp32 sums, P rounded to bf16. Positions past a length are not attended whatever
+// their slots hold: their scores are -infinity and their V terms 0. A length outside [0, 64 width] or a
+// page outside the pool makes the sequence's rows NaN; length 0 makes them 0. A sequence shorter than the
+// shared part takes no part in it: its own chunks cover it whole.
+#include "attn_tile.h"
+#include "paged.h"
+
+namespace lq {
+namespace {
+
+using namespace attn;
+
+constexpr int DW = 4;         // waves per workgroup
+constexpr int CHUNK_MIN = 4;  // pages of a sequence's chunk: one per wave
+constexpr int WAVE_V = PAGE * D;
+
+struct PagedArgs {
+  const uint16_t* q;
+  PagedBufs buf;
+  PageTable tab;
+  const int32_t* lens;
+  float* part_acc;    // [Hkv][slots][128], slots: own chunks x G, then np x rows of all sequences
+  float2* part_ml;
+  uint16_t* out;
+  int B, Hkv, G;
+  int shared;         // pages that all sequences share
+  int np, rb;         // their parts, blocks of query rows
+  int target;         // own chunks of a KV head that fill the GPU
+  float sl2;          // softmax scale, log2 units
+};
+
+__device__ __forceinline__ bool len_ok(const PagedArgs& a, int len) {
+  return len >= 0 && len <= (int64_t)a.tab.width * PAGE;
+}
+// First own page of a sequence, and how many.
+__device__ __forceinline__ int own_first(const PagedArgs& a, int len) {
+  return len >= a.shared * PAGE ? a.shared : 0;
+}
+__device__ __forceinline__ int own_pages(const PagedArgs& a, int len) {
+  return len_ok(a, len) ? (len + PAGE - 1) / PAGE - own_first(a, len) : 0;
+}
+
+__device__ __forceinline__ int wave_sum_i(int x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+__device__ __forceinline__ int wave_scan_i(int x, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    x += lane >= o ? y : 0;
+  }
+  return x;
+}
+
+// Pages per own chunk: the same in every workgroup of a call.
+__device__ __forceinline__ int chunk_pages(const PagedArgs& a, int lane) {
+  int total = 0;
+  for (int i = lane; i < a.B; i += 64) total += own_pages(a, a.lens[i]);
+  total = wave_sum_i(total);
+  return max(CHUNK_MIN, (total + a.target - 1) / a.target);
+}
+
+struct OwnSmem {
+  alignas(16) uint8_t v[DW][WAVE_V];  // a page's V codes, 16-byte chunk c of row r at c ^ vswz(r)
+  uint32_t w[DW][2][PAGE];            // its scale and bias words
+  float2 ml[DW][16];
+};
+// A page's operands on their way: K of keys 16 mt + lc (16 codes at dims 16 lq4 and 64 + 16 lq4), its
+// words, V rows 8 i + lane / 8, the words of V row `lane`.
+struct PageRegs {
+  uint4 k[4][2], v[8];
+  uint32_t ks[4], kb[4], vs, vb;
+};
+
+__device__ __forceinline__ void load_page(const PagedArgs& a, int64_t row, int lane, PageRegs& p) {
+  const int lc = lane & 15, lq4 = lane >> 4;
+  const uint8_t* kc = a.buf.kc + row * D;
+  const uint8_t* vc = a.buf.vc + row * D;
+  const uint32_t* ks = reinterpret_cast<const uint32_t*>(a.buf.ks) + row;
+  const uint32_t* kb = reinterpret_cast<const uint32_t*>(a.buf.kb) + row;
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      p.k[mt][h] = *reinterpret_cast<const uint4*>(kc + (16 * mt + lc) * D + 64 * h + 16 * lq4);
+    p.ks[mt] = ks[16 * mt + lc];
+    p.kb[mt] = kb[16 * mt + lc];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p.v[i] = *reinterpret_cast<const uint4*>(vc + 1024 * i + 16 * lane);
+  p.vs = reinterpret_cast<const uint32_t*>(a.buf.vs)[row + lane];
+  p.vb = reinterpret_cast<const uint32_t*>(a.buf.vb)[row + lane];
+}
+
+__device__ __forceinline__ int vswz(int r) { return (r & 3) | ((r >> 2) & 4); }
+
+__device__ __forceinline__ void wave_fence() {  // LDS of the wave's own: order across its lanes
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A sequence's chunk [p0, p1) of pages for its G rows.
+__device__ __forceinline__ void own_chunk(const PagedArgs& a, OwnSmem& sm, int b, int hk, int p0, int p1,
+                                          int len, int64_t slot) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lc = lane & 15, lq4 = lane >> 4;
+  const int32_t* ids = a.tab.ids + b * a.tab.stride;
+  const float scale = abs_scale(a.sl2);
+  const int64_t qrow = ((int64_t)b * a.Hkv + hk) * a.G;
+  // q as B operands in K's order of dims: k-step 2 h + j holds dims 64 h + 16 lq4 + 8 j .. + 7
+  bf16x8_t qf[4];
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (lc < a.G)
+      u = *reinterpret_cast<const uint4*>(a.q + (qrow + lc) * D + 64 * (kk >> 1) + 16 * lq4 + 8 * (kk & 1));
+    qf[kk] = u4_as_bf8(signed_q(u, a.sl2));
+  }
+  f4_t o[8];
+#pragma unroll
+  for (int w = 0; w < 8; ++w) o[w] = f4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.0f;
+  bool bad = false;
+
+  auto page_row = [&](int p) {
+    const int id = __builtin_amdgcn_readfirstlane(ids[p]);
+    const bool ok = id >= 0 && id < a.tab.pages;
+    bad |= !ok;
+    return ((int64_t)(ok ? id : 0) * a.Hkv + hk) * PAGE;
+  };
+
+  PageRegs cur;
+  int p = p0 + wv;
+  if (p < p1) load_page(a, page_row(p), lane, cur);
+  for (; p < p1; p += DW) {
+    const int limit = min(PAGE, len - p * PAGE);  // keys of the page that are the sequence's
+    // V to LDS; words of keys past the length 0, so that their slots' contents reach nothing
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 8 * i + (lane >> 3);
+      reinterpret_cast<uint4*>(sm.v[wv])[8 * r + ((lane & 7) ^ vswz(r))] = cur.v[i];
+    }
+    sm.w[wv][0][lane] = lane < limit ? cur.vs : 0u;
+    sm.w[wv][1][lane] = lane < limit ? cur.vb : 0u;
+    // scores
+    f4_t c[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      c[mt] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float s = h ? bf16_hi(cur.ks[mt]) : bf16_lo(cur.ks[mt]);
+        const float z = h ? bf16_hi(cur.kb[mt]) : bf16_lo(cur.kb[mt]);
+        const uint4 w = cur.k[mt][h];
+        const uint2 d0 = dequant4(w.x, s, z), d1 = dequant4(w.y, s, z);
+        const uint2 d2 = dequant4(w.z, s, z), d3 = dequant4(w.w, s, z);
+        c[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words_as_bf8(d0.x, d0.y, d1.x, d1.y), qf[2 * h],
+                                                        c[mt], 0, 0, 0);
+        c[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words_as_bf8(d2.x, d2.y, d3.x, d3.y),
+                                                        qf[2 * h + 1], c[mt], 0, 0, 0);
+      }
+    }
+    const int pn = p + DW;
+    if (pn < p1) load_page(a, page_row(pn), lane, cur);
+    if (limit < PAGE) {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          c[mt][r] = 16 * mt + 4 * lq4 + r < limit ? c[mt][r] : -INFINITY;
+    }
+    float t = -INFINITY;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t = max_ieee(t, c[mt][r]);
+    t = max_xor32(max_xor16(t)) * scale;
+    const bool bump = t > (m == -INFINITY ? -INFINITY : m + RESCALE_LOG2);
+    if (__builtin_amdgcn_ballot_w64(bump)) {
+      const float mn = bump ? t : m;
+      const float alpha = m == -INFINITY ? 0.0f : exp2_nonpos(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) o[w] *= alpha;
+    }
+    const float off = m == -INFINITY ? 0.0f : -m;
+    uint32_t pw[8];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      float e[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        e[r] = __builtin_amdgcn_exp2f(fmaf(c[mt][r], scale, off));
+        l += e[r];
+      }
+      pw[2 * mt] = pack_bf2(e[0], e[1]);
+      pw[2 * mt + 1] = pack_bf2(e[2], e[3]);
+    }
+    wave_fence();
+    // values: lane (lq4, lc) gets the codes of keys 32 e + 16 h + 4 lq4 + r at dim 16 w + lc
+    const int skey = 4 * lq4 + 16 * (lc >> 3) + ((lc >> 1) & 3);  // this lane's source key
+    const uint8_t* src = sm.v[wv] + skey * D + 8 * (lc & 1);
+    const int ssw = vswz(skey);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bf16x8_t pe = words_as_bf8(pw[4 * e], pw[4 * e + 1], pw[4 * e + 2], pw[4 * e + 3]);
+      const uint4 s0 = *reinterpret_cast<const uint4*>(&sm.w[wv][0][32 * e + 4 * lq4]);
+      const uint4 s1 = *reinterpret_cast<const uint4*>(&sm.w[wv][0][32 * e + 4 * lq4 + 16]);
+      const uint4 z0 = *reinterpret_cast<const uint4*>(&sm.w[wv][1][32 * e + 4 * lq4]);
+      const uint4 z1 = *reinterpret_cast<const uint4*>(&sm.w[wv][1][32 * e + 4 * lq4 + 16]);
+      const uint32_t sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+      const uint32_t zw[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const v2i_t raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_v2i_t*)(src + 32 * e * D + 16 * (w ^ ssw)));
+        const uint32_t r0 = (uint32_t)raw.x, r1 = (uint32_t)raw.y;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float s = w < 4 ? bf16_lo(sw[j]) : bf16_hi(sw[j]);
+          const float z = w < 4 ? bf16_lo(zw[j]) : bf16_hi(zw[j]);
+          v[j] = fmaf(s, (float)(((j < 4 ? r0 : r1) >> (8 * (j & 3))) & 0xffu), z);
+        }
+        o[w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            words_as_bf8(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]),
+                         pack_bf2(v[6], v[7])),
+            pe, o[w], 0, 0, 0);
+      }
+    }
+  }
+
+  // ---- the waves' rows meet in LDS (wave wv's in its own V area: 16 rows of 128 floats)
+  l = sum_xor32(sum_xor16(l));
+  wave_fence();
+  float* acc = reinterpret_cast<float*>(sm.v[wv]);
+  if (lc < a.G) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+      *reinterpret_cast<float4*>(acc + lc * D + 16 * w + 4 * lq4) =
+          make_float4(o[w][0], o[w][1], o[w][2], o[w][3]);
+    if (lq4 == 0) sm.ml[wv][lc] = make_float2(m, bad ? NAN : l);
+  }
+  __syncthreads();
+  for (int i = tid; i < a.G * (D / 4); i += 64 * DW) {
+    const int row = i >> 5, d = 4 * (i & 31);
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < DW; ++w) M = max_ieee(M, sm.ml[w][row].x);
+    const float Mr = M == -INFINITY ? 0.0f : M;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < DW; ++w) {
+      const float2 ml = sm.ml[w][row];
+      const float e = ml.x == -INFINITY ? 0.0f : exp2_nonpos(ml.x - Mr);
+      const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.v[w]) + row * D + d);
+      s.x = fmaf(e, x.x, s.x);
+      s.y = fmaf(e, x.y, s.y);
+      s.z = fmaf(e, x.z, s.z);
+      s.w = fmaf(e, x.w, s.w);
+      L = fmaf(ml.x == -INFINITY ? 1.0f : e, ml.y, L);
+    }
+    *reinterpret_cast<float4*>(a.part_acc + (slot + row) * D + d) = s;
+    if (d == 0) a.part_ml[slot + row] = make_float2(M, L);
+  }
+}
+
+// A part [p0, p1) of the shared pages (listed in the table at ids) for query rows f0 .. f0 + 64 NT - 1 of
+// a KV head.
+struct RawPage {  // keys tid / 8 and tid / 8 + 32, codes 16 (tid % 8) ..
+  uint4 k[2], v[2];
+  uint32_t ks[2], kb[2], vs[2], vb[2];
+};
+
+template <int NT>
+__device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2], const int32_t* ids, int hk,
+                                            int p0, int p1, int f0, int64_t slot) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lc = lane & 15, lq4 = lane >> 4;
+  const int rows = a.B * a.G;
+  const float scale = abs_scale(a.sl2);
+  const int key0 = tid >> 3, chunk = tid & 7;
+  bool bad = false;
+  RawPage raw;
+  auto load = [&](int p) {
+    const int id = __builtin_amdgcn_readfirstlane(ids[p]);
+    const bool ok = id >= 0 && id < a.tab.pages;
+    bad |= !ok;
+    const int64_t row = ((int64_t)(ok ? id : 0) * a.Hkv + hk) * PAGE;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      raw.k[i] = *reinterpret_cast<const uint4*>(a.buf.kc + row * D + 4096 * i + 16 * tid);
+      raw.v[i] = *reinterpret_cast<const uint4*>(a.buf.vc + row * D + 4096 * i + 16 * tid);
+      const int64_t r = row + key0 + 32 * i;
+      raw.ks[i] = reinterpret_cast<const uint32_t*>(a.buf.ks)[r];
+      raw.kb[i] = reinterpret_cast<const uint32_t*>(a.buf.kb)[r];
+      raw.vs[i] = reinterpret_cast<const uint32_t*>(a.buf.vs)[r];
+      raw.vb[i] = reinterpret_cast<const uint32_t*>(a.buf.vb)[r];
+    }
+  };
+  auto pick = [&](uint32_t w) { return chunk < 4 ? bf16_lo(w) : bf16_hi(w); };
+  auto stage = [&](KvTile& t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = key0 + 32 * i;
+      const float s = pick(raw.ks[i]), z = pick(raw.kb[i]);
+      const uint2 k0 = dequant4(raw.k[i].x, s, z), k1 = dequant4(raw.k[i].y, s, z);
+      const uint2 k2 = dequant4(raw.k[i].z, s, z), k3 = dequant4(raw.k[i].w, s, z);
+      *k_chunk(t, key, 2 * chunk) = make_uint4(k0.x, k0.y, k1.x, k1.y);
+      *k_chunk(t, key, 2 * chunk + 1) = make_uint4(k2.x, k2.y, k3.x, k3.y);
+      const float vs = pick(raw.vs[i]), vz = pick(raw.vb[i]);
+      const uint2 v0 = dequant4(raw.v[i].x, vs, vz), v1 = dequant4(raw.v[i].y, vs, vz);
+      const uint2 v2 = dequant4(raw.v[i].z, vs, vz), v3 = dequant4(raw.v[i].w, vs, vz);
+      *v_chunk(t, key, 2 * chunk) = make_uint4(v0.x, v0.y, v1.x, v1.y);
+      *v_chunk(t, key, 2 * chunk + 1) = make_uint4(v2.x, v2.y, v3.x, v3.y);
+    }
+  };
+  load(p0);
+  TileRows<NT> st;
+  st.clear();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int f = f0 + 16 * (NT * wv + nt) + lc;
+    const int b = f / a.G;
+    const int64_t row = ((int64_t)b * a.Hkv + hk) * a.G + (f - b * a.G);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (f < rows) u = *reinterpret_cast<const uint4*>(a.q + row * D + 32 * kk + 8 * lq4);
+      st.q[nt][kk] = u4_as_bf8(signed_q(u, a.sl2));
+    }
+  }
+  stage(sm[0]);
+  if (p0 + 1 < p1) load(p0 + 1);
+  __syncthreads();
+  for (int p = p0; p < p1; ++p) {
+    const int s = (p - p0) & 1;
+    f4_t c[NT][4];
+    bf16x8_t pr[NT][2];
+    tile_scores<NT>(sm[s], st, lane, c);
+    tile_softmax<NT>(c, st, scale, pr);
+    tile_values<NT>(sm[s], st, lane, pr);
+    if (p + 1 < p1) {
+      stage(sm[s ^ 1]);
+      if (p + 2 < p1) load(p + 2);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int f = f0 + 16 * (NT * wv + nt) + lc;
+    if (f >= rows) continue;
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+      *reinterpret_cast<float4*>(a.part_acc + (slot + f) * D + 16 * w + 4 * lq4) =
+          make_float4(st.o[nt][w][0], st.o[nt][w][1], st.o[nt][w][2], st.o[nt][w][3]);
+    if (lq4 == 0) a.part_ml[slot + f] = make_float2(st.m[nt], bad ? NAN : st.l[nt][0]);
+  }
+}
+
+// Partial rows of one KV head: own chunks first.
+__device__ __forceinline__ int64_t head_slots(const PagedArgs& a) {
+  return (int64_t)(a.target + a.B) * a.G + (int64_t)a.np * a.B * a.G;
+}
+
+template <int NT>  // 16-row tiles of a wave in the shared part; 0: nothing is shared
+__global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
+  __shared__ union Smem {
+    OwnSmem own;
+    KvTile tile[NT ? 2 : 1];
+    __device__ Smem() {}
+  } sm;
+  const int lane = threadIdx.x & 63;
+  const int hk = blockIdx.x % a.Hkv;
+  int x = blockIdx.x / a.Hkv;
+  const int64_t slot0 = hk * head_slots(a);
+  if constexpr (NT > 0) {
+    if (x < a.np * a.rb) {  // the shared parts first: they take longest
+      const int part = x / a.rb, block = x - part * a.rb;
+      const int p0 = (int)((int64_t)a.shared * part / a.np);
+      const int p1 = (int)((int64_t)a.shared * (part + 1) / a.np);
+      // listed by the first sequence that is long enough; a shorter one's row may end before them
+      for (int i = 0; i < a.B; i += 64) {
+        const int len = i + lane < a.B ? a.lens[i + lane] : -1;
+        const uint64_t joins = __builtin_amdgcn_ballot_w64(len_ok(a, len) && len >= a.shared * PAGE);
+        if (joins) {
+          shared_part<NT>(a, sm.tile, a.tab.ids + (i + __builtin_ctzll(joins)) * a.tab.stride, hk, p0, p1,
+                          block * 64 * NT,
+                          slot0 + (int64_t)(a.target + a.B) * a.G + (int64_t)part * a.B * a.G);
+          return;
+        }
+      }
+      return;
+    }
+    x -= a.np * a.rb;
+  }
+  // own chunk x of this KV head
+  const int C = chunk_pages(a, lane);
+  int before = 0;
+  for (int i = 0; i < a.B; i += 64) {
+    const int len = i + lane < a.B ? a.lens[i + lane] : 0;
+    const int n = (own_pages(a, len) + C - 1) / C;
+    const int upto = before + wave_scan_i(n, lane);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > x);
+    if (past) {
+      const int src = __builtin_ctzll(past);
+      const int blen = __builtin_amdgcn_readlane(len, src);
+      const int first = __builtin_amdgcn_readlane(upto - n, src);
+      const int p0 = own_first(a, blen) + (x - first) * C;
+      const int p1 = min(p0 + C, (blen + PAGE - 1) / PAGE);
+      own_chunk(a, sm.own, i + src, hk, p0, p1, blen, slot0 + (int64_t)x * a.G);
+      return;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+
+// One wave per output row: lane (half, 4 dims) takes every other partial, the halves meet by a swap.
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  if (row >= a.B * a.Hkv * a.G) return;
+  const int b = row / (a.Hkv * a.G), h = row - b * a.Hkv * a.G, hk = h / a.G, g = h - hk * a.G;
+  const int C = chunk_pages(a, lane);
+  int first = 0;
+  for (int i = lane; i < b; i += 64) first += (own_pages(a, a.lens[i]) + C - 1) / C;
+  first = wave_sum_i(first);
+  const int len = a.lens[b];
+  const int n = (own_pages(a, len) + C - 1) / C;
+  const bool joins = len_ok(a, len) && a.shared > 0 && len >= a.shared * PAGE;
+  const int64_t slot0 = hk * head_slots(a);
+  const int64_t own0 = slot0 + (int64_t)first * a.G + g;
+  const int64_t sh0 = slot0 + (int64_t)(a.target + a.B) * a.G + (int64_t)b * a.G + g;
+  const int parts = n + (joins ? a.np : 0);
+  const int d = 4 * (lane & 31);
+  float M = -INFINITY, den = 0.0f;
+  f4_t acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i = lane >> 5; i < parts; i += 2) {
+    const int64_t s = i < n ? own0 + (int64_t)i * a.G : sh0 + (int64_t)(i - n) * a.B * a.G;
+    const float2 ml = a.part_ml[s];
+    const f4_t x = *reinterpret_cast<const f4_t*>(a.part_acc + s * D + d);
+    const float mn = max_ieee(M, ml.x);
+    const float mr = mn == -INFINITY ? 0.0f : mn;
+    const float e0 = M == -INFINITY ? 0.0f : exp2_nonpos(M - mr);
+    const float e1 = ml.x == -INFINITY ? 0.0f : exp2_nonpos(ml.x - mr);
+    acc = acc * e0 + x * e1;
+    den = den * e0 + ml.y * (ml.x == -INFINITY ? 1.0f : e1);
+    M = mn;
+  }
+  // the two halves
+  const float Mo = __shfl_xor(M, 32, 64), deno = __shfl_xor(den, 32, 64);
+  f4_t acco;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acco[r] = __shfl_xor(acc[r], 32, 64);
+  const float mx = max_ieee(M, Mo);
+  const float mr = mx == -INFINITY ? 0.0f : mx;
+  const float e0 = M == -INFINITY ? 0.0f : exp2_nonpos(M - mr);
+  const float e1 = Mo == -INFINITY ? 0.0f : exp2_nonpos(Mo - mr);
+  acc = acc * e0 + acco * e1;
+  den = (M == -INFINITY ? den : den * e0) + (Mo == -INFINITY ? deno : deno * e1);
+  float inv = den == 0.0f ? 0.0f : 1.0f / den;  // no keys: 0; a sum that is NaN stays
+  if (!len_ok(a, len)) inv = NAN;
+  const f4_t o = acc * inv;
+  if (lane < 32)
+    *reinterpret_cast<uint2*>(a.out + (int64_t)row * D + d) =
+        make_uint2((uint32_t)f32_to_bf16(o[0]) | ((uint32_t)f32_to_bf16(o[1]) << 16),
+                   (uint32_t)f32_to_bf16(o[2]) | ((uint32_t)f32_to_bf16(o[3]) << 16));
+}
+
+struct DecodeShape {
+  int np, rb, target, nt;
+  int64_t slots;  // partial rows, all heads
+};
+
+DecodeShape decode_shape(int64_t B, int64_t Hkv, int64_t G, int64_t shared, int cus) {
+  DecodeShape s{0, 0, 1, 0, 0};
+  const int64_t fill = 2 * cus;  // workgroups that the GPU holds at once
+  if (shared > 0) {
+    s.nt = B * G > 64 ? 2 : 1;
+    s.rb = (int)((B * G + 64 * s.nt - 1) / (64 * s.nt));
+    s.np = (int)std::min<int64_t>((shared + 3) / 4, std::max<int64_t>(1, fill / (Hkv * s.rb)));
+  }
+  s.target = (int)std::max<int64_t>(1, fill / Hkv);
+  s.slots = Hkv * G * (s.target + B + s.np * B);
+  return s;
+}
+
+int64_t decode_bytes(const DecodeShape& s) { return s.slots * (int64_t)(D * sizeof(float) + sizeof(float2)); }
+
+int check_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t shared_pages) {
+  LQ_CHECK_ARG(Hkv >= 1 && Hkv <= 1024 && Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= 16,
+               "Hq=%lld must be 1 to 16 times Hkv=%lld", (long long)Hq, (long long)Hkv);
+  LQ_CHECK_ARG(B >= 1 && B <= 4096, "a batch of %lld is not in [1, 4096]", (long long)B);
+  LQ_CHECK_ARG(shared_pages >= 0, "%lld shared pages", (long long)shared_pages);
+  return LQ_OK;
+}
+
+}  // namespace
+}  // namespace lq
+
+extern "C" int64_t lq_paged_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv,
+                                                   int64_t shared_pages) {
+  using namespace lq;
+  clear_error();
+  if (check_decode(B, Hq, Hkv, shared_pages)) return -1;
+  return decode_bytes(decode_shape(B, Hkv, Hq / Hkv, shared_pages, device_cu_count()));
+}
+
+extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const uint16_t* ks,
+                                    const uint16_t* kb, const uint8_t* vc, const uint16_t* vs,
+                                    const uint16_t* vb, int64_t pages, int64_t B, int64_t Hq,
+                                    int64_t Hkv, int64_t D, const int32_t* table, int64_t table_stride,
+                                    int64_t table_width, const int32_t* lens, int64_t shared_pages,
+                                    float scale, uint16_t* out, void* workspace, int64_t workspace_bytes,
+                                    void* stream) {
+  using namespace lq;
+  clear_error();
+  PagedArgs a{};
+  a.q = q;
+  a.buf = {const_cast<uint8_t*>(kc),  const_cast<uint16_t*>(ks), const_cast<uint16_t*>(kb),
+           const_cast<uint8_t*>(vc),  const_cast<uint16_t*>(vs), const_cast<uint16_t*>(vb)};
+  a.tab = {table, table_stride, (int)table_width, (int)pages};
+  if (const int st = check_pool(a.buf, a.tab, table_stride, table_width, pages, Hkv, D)) return st;
+  if (const int st = check_decode(B, Hq, Hkv, shared_pages)) return st;
+  LQ_CHECK_ARG(shared_pages <= table_width, "%lld shared pages of table rows of %lld",
+               (long long)shared_pages, (long long)table_width);
+  LQ_CHECK_ARG(q && lens && out, "null pointer");
+  LQ_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "q and out must be 16-byte aligned");
+  LQ_CHECK_ARG(std::isfinite(scale), "the softmax scale is not finite");
+  const int64_t G = Hq / Hkv;
+  const DecodeShape s = decode_shape(B, Hkv, G, shared_pages, device_cu_count());
+  if (!workspace || workspace_bytes < decode_bytes(s)) {
+    set_error("workspace of %lld bytes is smaller than the %lld needed", (long long)workspace_bytes,
+              (long long)decode_bytes(s));
+    return LQ_EWORKSPACE;
+  }
+  LQ_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
+  const int64_t wgs = Hkv * ((int64_t)s.np * s.rb + s.target + B);
+  LQ_CHECK_ARG(wgs <= INT32_MAX, "too many workgroups");
+  a.lens = lens;
+  a.part_acc = (float*)workspace;
+  a.part_ml = (float2*)(a.part_acc + s.slots * 128);
+  a.out = out;
+  a.B = (int)B;
+  a.Hkv = (int)Hkv;
+  a.G = (int)G;
+  a.shared = (int)shared_pages;
+  a.np = s.np;
+  a.rb = s.rb;
+  a.target = s.target;
+  a.sl2 = scale * 1.4426950408889634f;
+  auto* kern = s.nt == 2 ? paged_decode_kernel<2> : s.nt == 1 ? paged_decode_kernel<1> : paged_decode_kernel<0>;
+  kern<<<dim3((unsigned)wgs), dim3(64 * DW), 0, (hipStream_t)stream>>>(a);
+  LQ_CHECK_LAUNCH("paged_decode_kernel");
+  paged_merge_kernel<<<dim3((unsigned)((B * Hq + 3) / 4)), dim3(256), 0, (hipStream_t)stream>>>(a);
+  LQ_CHECK_LAUNCH("paged_merge_kernel");
+  return LQ_OK;
+}

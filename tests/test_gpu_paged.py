@@ -1,0 +1,475 @@
+"""The paged 8-bit cache and packed-prompt attention against plain computations in 64 bits."""
+import pytest
+import torch
+
+from lagunalab_amd.paged import (copy_pages, page_pool, paged_append, paged_decode_attention,
+                                 paged_gather)
+from lagunalab_amd.prompt_attn import prompt_attention
+from paged_util import (D, PAGE, assert_within, exact_attention, fill_pool, make_table, randn,
+                        read_rows, write_rows)
+
+pytestmark = pytest.mark.gpu
+SCALE = D ** -0.5
+
+
+def gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def bits(t):
+    return t.view(torch.int16) if t.dtype == torch.bfloat16 else t
+
+
+# ------------------------------------------------------------------------------- rows in and out
+
+@pytest.mark.parametrize("kv,starts,counts", [
+    (1, [0], [1]),
+    (8, [5, 0, 63, 64, 130], [1, 1, 1, 1, 1]),
+    (2, [0, 7, 64, 200, 3], [64, 130, 0, 1, 61]),
+    (3, [1] * 70, [2] * 70),  # more sequences than one launch takes
+])
+def test_append_is_the_quantizer_at_the_tables_slots(dev, kv, starts, counts):
+    from lagunalab_amd.quant import quantize
+    g = gen(1)
+    ends = [s + c for s, c in zip(starts, counts)]
+    table, pages = make_table(g, ends, 0)
+    pool = fill_pool(g, pages, kv, dev)
+    before = [tuple(t.clone() for t in buf) for buf in pool]
+    T = sum(counts)
+    k, v = randn(g, T, kv, D).to(dev), randn(g, T, kv, D, std=3.0).to(dev)
+    paged_append(k, v, *pool, table.to(dev), torch.tensor(starts, dtype=torch.int32, device=dev), counts)
+    b = torch.cat([torch.full((c,), i) for i, c in enumerate(counts)])
+    at = torch.cat([torch.arange(s, s + c) for s, c in zip(starts, counts)])
+    where = table[b, at // PAGE].long().to(dev), (at % PAGE).to(dev)
+    for rows, buf, old in zip((k, v), pool, before):
+        for t, x, o in zip(buf, quantize(rows), old):
+            assert torch.equal(bits(t[where[0], :, where[1]]), bits(x))
+            o[where[0], :, where[1]] = x
+            assert torch.equal(bits(t), bits(o)), "a slot that no row goes to changed"
+
+
+def test_append_special_rows_and_strides(dev):
+    from lagunalab_amd.quant import quantize
+    from gpu_util import special_rows
+    rows = torch.from_numpy(special_rows()).to(torch.bfloat16)  # [n, 128]
+    n = rows.shape[0]
+    wide = torch.zeros((n, 5, 2, D + 8), dtype=torch.bfloat16)  # heads and rows apart
+    wide[:, 1, :, :D] = rows[:, None]
+    wide[:, 3, :, :D] = rows.flip(0)[:, None]
+    wide = wide.to(dev)
+    k, v = wide[:, 1, :, :D], wide[:, 3, :, :D]
+    pool = page_pool(2, 2, dev)
+    table = torch.tensor([[1, 0]], dtype=torch.int32, device=dev)
+    paged_append(k, v, *pool, table, torch.tensor([60], dtype=torch.int32, device=dev))
+    at = torch.arange(60, 60 + n)
+    where = table[0].cpu()[at // PAGE].long().to(dev), (at % PAGE).to(dev)
+    for x, buf in ((k, pool[0]), (v, pool[1])):
+        for t, y in zip(buf, quantize(x.contiguous())):
+            assert torch.equal(bits(t[where[0], :, where[1]]), bits(y))
+
+
+def test_append_skips_positions_and_pages_that_do_not_exist(dev):
+    g = gen(2)
+    pool = fill_pool(g, 3, 2, dev)
+    before = [tuple(t.clone() for t in buf) for buf in pool]
+    k = randn(g, 12, 2, D).to(dev)
+    # pages -1 and 3 do not exist, position 128 is beyond the row, negative positions are before it
+    table = torch.tensor([[-1, 3], [3, 2], [0, -7]], dtype=torch.int32, device=dev)
+    starts = torch.tensor([62, 126, -3], dtype=torch.int32, device=dev)
+    paged_append(k, k, *pool, table, starts, [4, 4, 4])
+    for buf, old in zip(pool, before):
+        for t, o in zip(buf, old):
+            changed = torch.zeros(t.shape[:3], dtype=torch.bool)
+            changed[2, :, 62:64] = True  # rows 126, 127 of sequence 1
+            changed[0, :, 0:1] = True    # row 0 of sequence 2
+            same = (bits(t) == bits(o)).all(-1).cpu()
+            assert same[~changed].all()
+            assert not same[changed].any()
+
+
+@pytest.mark.parametrize("kv,starts,counts", [
+    (8, [0], [1]), (2, [0, 63, 64, 1], [64, 2, 65, 200]), (1, [100, 5, 0], [0, 59, 128]),
+    (4, list(range(67)), [3] * 67),
+])
+def test_gather_is_the_dequantizer(dev, kv, starts, counts):
+    g = gen(3)
+    ends = [s + c for s, c in zip(starts, counts)]
+    table, pages = make_table(g, ends, 0)
+    pool = fill_pool(g, pages, kv, dev)
+    rows = [(randn(g, n, kv, D), randn(g, n, kv, D)) for n in ends]
+    for b, (k, v) in enumerate(rows):
+        if ends[b]:
+            write_rows(pool, table[b], k, v)
+    got = paged_gather(*pool, table.to(dev), torch.tensor(starts, dtype=torch.int32, device=dev), counts)
+    for x, buf in zip(got, pool):
+        want = torch.cat([read_rows(buf, table[b], ends[b])[starts[b]:] for b in range(len(ends))])
+        assert x.shape == want.shape and torch.equal(x.cpu().double(), want)
+
+
+def test_gather_of_positions_that_do_not_exist_is_nan(dev):
+    g = gen(4)
+    pool = fill_pool(g, 2, 1, dev, poison=False)
+    table = torch.tensor([[1, 5]], dtype=torch.int32, device=dev)
+    k, v = paged_gather(*pool, table, torch.tensor([-2], dtype=torch.int32, device=dev), [140])
+    for x in (k, v):
+        lost = torch.isnan(x).all(-1).all(-1).cpu()
+        assert lost.tolist() == [True] * 2 + [False] * 64 + [True] * 74
+
+
+@pytest.mark.parametrize("kv,pages,n", [(8, 10, 1), (1, 2500, 1000), (3, 40, 17)])
+def test_copy_pages(dev, kv, pages, n):
+    g = gen(5)
+    pool = fill_pool(g, pages, kv, dev, poison=False)
+    for buf in pool:
+        buf[1].copy_(torch.randn(buf[1].shape, generator=g))
+        buf[2].copy_(torch.randn(buf[1].shape, generator=g))
+    order = torch.randperm(pages, generator=g)
+    src, dst = order[:n], order[n:2 * n]
+    want = [[t.clone() for t in buf] for buf in pool]
+    for buf in want:
+        for t in buf:
+            t[dst.to(dev)] = t[src.to(dev)]
+    copy_pages(*pool, src, dst.tolist())
+    copy_pages(*pool, [], [])
+    for buf, w in zip(pool, want):
+        for t, x in zip(buf, w):
+            assert torch.equal(bits(t), bits(x))
+
+
+def test_one_page_copied_to_several(dev):
+    g = gen(6)
+    pool = fill_pool(g, 6, 2, dev, poison=False)
+    want = [[t.clone() for t in buf] for buf in pool]
+    for buf in want:
+        for t in buf:
+            t[[0, 1, 5]] = t[3].clone()
+    copy_pages(*pool, [3, 3, 3], [0, 5, 1])
+    for buf, w in zip(pool, want):
+        for t, x in zip(buf, w):
+            assert torch.equal(bits(t), bits(x))
+
+
+# ------------------------------------------------------------------------------------- decoding
+
+def decode_case(seed, hq, kv, lens, shared, dev, std=1.0, width_spare=0):
+    g = gen(seed)
+    table, pages = make_table(g, lens, shared, width_spare=width_spare)
+    pool = fill_pool(g, pages, kv, dev)
+    common = shared // PAGE * PAGE
+    if common:
+        row = max(range(len(lens)), key=lambda b: lens[b])
+        n = min(common, lens[row])
+        write_rows(pool, table[row], randn(g, n, kv, D), randn(g, n, kv, D))
+    for b, n in enumerate(lens):
+        if n > common:
+            write_rows(pool, table[b], randn(g, n - common, kv, D), randn(g, n - common, kv, D), common)
+    q = randn(g, len(lens), hq, 1, D, std=std)
+    return q, pool, table
+
+
+def check_decode(out, q, pool, table, lens, scale=SCALE, rows=None):
+    hq, kv = q.shape[1], pool[0][0].shape[1]
+    G = hq // kv
+    for b in rows if rows is not None else range(len(lens)):
+        k, v = (read_rows(buf, table[b], lens[b]) for buf in pool)
+        for h in range(kv):
+            want, bound = exact_attention(q[b, h * G:(h + 1) * G, 0].double(), k[:, h], v[:, h],
+                                          [lens[b] - 1] * G, scale)
+            assert_within(out[b, h * G:(h + 1) * G, 0], want, bound, f"sequence {b} head {h}")
+
+
+@pytest.mark.parametrize("hq,kv,lens", [
+    (4, 1, [1]), (8, 8, [64]), (32, 8, [1037]), (6, 1, [63, 64, 65, 0, 1]), (16, 1, [300, 5]),
+    (10, 2, [129, 1000, 2]), (48, 8, [4099]), (2, 2, [17] * 70), (3, 1, [20011, 1]),
+])
+def test_decode_without_a_shared_prefix(dev, hq, kv, lens):
+    q, pool, table = decode_case(7, hq, kv, lens, 0, dev, width_spare=2)
+    out = paged_decode_attention(q.to(dev), *pool, table.to(dev),
+                                 torch.tensor(lens, dtype=torch.int32, device=dev), SCALE)
+    assert out.shape == q.shape and out.dtype == torch.bfloat16
+    check_decode(out, q, pool, table, lens)
+
+
+@pytest.mark.parametrize("hq,kv,shared,own", [
+    (4, 1, 64, [1]), (8, 2, 64, [0, 1, 64, 65]), (32, 8, 640, [3] * 16), (16, 1, 192, [5, 0, 70, 1000, 9]),
+    (12, 2, 2048, list(range(1, 34))), (6, 6, 130, [62, 63, 64, 300]), (3, 1, 4096, [11] * 70),
+])
+def test_decode_with_a_shared_prefix(dev, hq, kv, shared, own):
+    lens = [shared + n for n in own]
+    q, pool, table = decode_case(8, hq, kv, lens, shared, dev)
+    args = (q.to(dev), *pool, table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), SCALE)
+    out = paged_decode_attention(*args, shared=shared)
+    rows = sorted({0, 1, len(lens) // 2, len(lens) - 1} & set(range(len(lens))))
+    check_decode(out, q, pool, table, lens, rows=rows)
+    # the same numbers whether the batch is told of the shared pages or not, to the roundings of both
+    plain = paged_decode_attention(*args)
+    assert (out.float() - plain.float()).abs().max() < 2 ** -5
+
+
+def test_decode_of_sequences_shorter_than_the_shared_part(dev):
+    """The longest is not the first; one ends inside the shared part, one is empty, one ends with it."""
+    lens = [70, 0, 200, 128, 129, 1]
+    q, pool, table = decode_case(9, 8, 2, lens, 128, dev)
+    out = paged_decode_attention(q.to(dev), *pool, table.to(dev),
+                                 torch.tensor(lens, dtype=torch.int32, device=dev), SCALE, shared=128)
+    check_decode(out, q, pool, table, lens)
+    assert (out[1] == 0).all()
+    # no sequence as long as the shared part
+    short = [70, 0, 100, 127, 64, 1]
+    out = paged_decode_attention(q.to(dev), *pool, table.to(dev),
+                                 torch.tensor(short, dtype=torch.int32, device=dev), SCALE, shared=128)
+    check_decode(out, q, pool, table, short)
+
+
+@pytest.mark.parametrize("shared", [0, 128])
+@pytest.mark.parametrize("scale,std", [(-SCALE, 1.0), (0.0, 1.0), (1.0, 1.0), (SCALE, 30.0), (SCALE, 1e-6)])
+def test_decode_scales(dev, scale, std, shared):
+    lens = [200, 131]
+    q, pool, table = decode_case(10, 8, 2, lens, shared, dev, std=std)
+    out = paged_decode_attention(q.to(dev), *pool, table.to(dev),
+                                 torch.tensor(lens, dtype=torch.int32, device=dev), scale, shared=shared)
+    check_decode(out, q, pool, table, lens, scale=scale)
+
+
+def test_decode_of_large_and_tiny_values(dev):
+    """K and V far outside the fp16 range, as bf16 rows may be."""
+    g = gen(11)
+    lens = [150, 200]
+    for vstd in (1e20, 1e-20):
+        table, pages = make_table(g, lens, 128)
+        pool = fill_pool(g, pages, 2, dev)
+        write_rows(pool, table[0], randn(g, 128, 2, D), randn(g, 128, 2, D, std=vstd))
+        for b, n in enumerate(lens):
+            write_rows(pool, table[b], randn(g, n - 128, 2, D), randn(g, n - 128, 2, D, std=vstd), 128)
+        q = randn(g, 2, 4, 1, D)
+        args = (q.to(dev), *pool, table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), SCALE)
+        for shared in (0, 128):
+            check_decode(paged_decode_attention(*args, shared=shared), q, pool, table, lens)
+
+
+@pytest.mark.parametrize("shared", [0, 64])
+def test_decode_of_bad_lengths_and_pages_is_nan_for_their_sequence_alone(dev, shared):
+    lens = [100, 300, 150, 90, 128]
+    q, pool, table = decode_case(12, 4, 2, lens, shared, dev)
+    told = list(lens)
+    told[0] = -1
+    told[1] = 64 * table.shape[1] + 1
+    bad = table.clone()
+    bad[2, 2] = pool[0][0].shape[0]
+    bad[3, 1] = -5
+    out = paged_decode_attention(q.to(dev), *pool, bad.to(dev),
+                                 torch.tensor(told, dtype=torch.int32, device=dev), SCALE, shared=shared)
+    assert torch.isnan(out[:4]).all()
+    check_decode(out, q, pool, table, lens, rows=[4])
+    if shared:  # a bad page in the shared part: NaN for all that attend to it
+        bad = table.clone()
+        bad[:, 0] = 1 << 30
+        out = paged_decode_attention(q.to(dev), *pool, bad.to(dev),
+                                     torch.tensor(lens, dtype=torch.int32, device=dev), SCALE, shared=shared)
+        assert torch.isnan(out).all()
+
+
+def test_decode_reads_table_rows_of_any_stride_and_no_row_behind_the_batch(dev):
+    lens = [100, 200, 70]
+    q, pool, table = decode_case(13, 8, 2, lens, 0, dev)
+    wide = torch.full((5, table.shape[1] + 9), -1, dtype=torch.int32)
+    wide[:3, :table.shape[1]] = table
+    view = wide.to(dev)[:3, :table.shape[1]]
+    out = paged_decode_attention(q.to(dev), *pool, view,
+                                 torch.tensor(lens, dtype=torch.int32, device=dev), SCALE)
+    check_decode(out, q, pool, table, lens)
+
+
+def test_decode_captured_follows_lengths_and_tables(dev):
+    lens = [190, 130]
+    q, pool, table = decode_case(14, 8, 2, [256, 256], 128, dev)
+    q_d, t_d = q.to(dev), table.to(dev)
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    stream = torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):
+        paged_decode_attention(q_d, *pool, t_d, n_d, SCALE, shared=128)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = paged_decode_attention(q_d, *pool, t_d, n_d, SCALE, shared=128)
+    torch.cuda.current_stream(dev).wait_stream(stream)
+    for step in ([190, 130], [191, 131], [256, 1], [0, 129], [192, 256]):
+        n_d.copy_(torch.tensor(step, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        eager = paged_decode_attention(q_d, *pool, t_d, n_d, SCALE, shared=128)
+        assert torch.equal(bits(out), bits(eager))
+        check_decode(out, q, pool, table, step)
+
+
+def test_decode_on_two_streams_at_once(dev):
+    cases = [decode_case(s, 8, 2, [1500, 700], 512, dev) for s in (15, 16)]
+    lens = torch.tensor([1500, 700], dtype=torch.int32, device=dev)
+    args = [(q.to(dev), *pool, table.to(dev), lens, SCALE) for q, pool, table in cases]
+    want = [paged_decode_attention(*a, shared=512) for a in args]
+    torch.cuda.synchronize(dev)
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    for _ in range(10):
+        got = []
+        for st, a in zip(streams, args):
+            with torch.cuda.stream(st):
+                got.append(paged_decode_attention(*a, shared=512))
+        torch.cuda.synchronize(dev)
+        for x, y in zip(got, want):
+            assert torch.equal(bits(x), bits(y))
+
+
+def test_pool_beyond_32_bit_offsets(dev):
+    """Pages whose codes lie more than 4 GB into the pool: appended, attended, copied and read back."""
+    pages, kv = 67000, 8
+    pool = [(torch.empty((pages, kv, PAGE, D), dtype=torch.uint8, device=dev),
+             torch.empty((pages, kv, PAGE, 2), dtype=torch.bfloat16, device=dev),
+             torch.empty((pages, kv, PAGE, 2), dtype=torch.bfloat16, device=dev)) for _ in range(2)]
+    g = gen(17)
+    table = torch.tensor([[66999, 66001, 3]], dtype=torch.int32)
+    k, v = randn(g, 150, kv, D), randn(g, 150, kv, D)
+    zero = torch.zeros(1, dtype=torch.int32, device=dev)
+    paged_append(k.to(dev), v.to(dev), *pool, table.to(dev), zero)
+    copy_pages(*pool, [66999, 3], [65999, 66500])
+    moved = torch.tensor([[65999, 66001, 66500]], dtype=torch.int32)
+    q = randn(g, 1, 16, 1, D)
+    n = torch.tensor([150], dtype=torch.int32, device=dev)
+    small = [tuple(t[[66999, 66001, 3]].cpu() for t in buf) for buf in pool]
+    straight = torch.arange(3, dtype=torch.int32)[None]
+    for t in (table, moved):
+        out = paged_decode_attention(q.to(dev), *pool, t.to(dev), n, SCALE)
+        check_decode(out, q, small, straight, [150])
+        out = paged_decode_attention(q.to(dev), *pool, t.to(dev), n, SCALE, shared=128)
+        check_decode(out, q, small, straight, [150])
+        for x, buf in zip(paged_gather(*pool, t.to(dev), zero, [150]), small):
+            assert torch.equal(x.cpu().double(), read_rows(buf, straight[0], 150))
+
+
+# -------------------------------------------------------------------------------- packed prompts
+
+def check_prompt(out, q, k, v, q_lens, k_lens, scale=SCALE, some=None):
+    hq, kv = q.shape[1], k.shape[1]
+    G = hq // kv
+    a = c = 0
+    q, k, v = (x.cpu().double() for x in (q, k, v))
+    for s, (lq, lk) in enumerate(zip(q_lens, k_lens)):
+        rows = range(lq) if some is None or lq <= some else sorted(
+            {0, 1, lq - 1, lq // 2} | {int(i) for i in torch.linspace(0, lq - 1, some)})
+        for h in range(hq):
+            if lk == 0:
+                assert (out[a:a + lq, h] == 0).all()
+                continue
+            rows = list(rows)
+            want, bound = exact_attention(q[a:a + lq, h][rows], k[c:c + lk, h // G], v[c:c + lk, h // G],
+                                          [lk - lq + i for i in rows], scale)
+            assert_within(out[a:a + lq, h][rows], want, bound, f"sequence {s} head {h}")
+        a, c = a + lq, c + lk
+
+
+@pytest.mark.parametrize("hq,kv,q_lens,k_lens", [
+    (1, 1, [1], None), (4, 1, [64], None), (8, 2, [65, 1, 63, 128, 200], None), (6, 1, [43, 0, 86], None),
+    (3, 3, [300], None), (16, 1, [33], None), (64, 1, [9, 5], None), (5, 1, [103], None),
+    (8, 2, [1, 1, 1], [1, 64, 65]), (4, 2, [70, 5], [200, 5]), (48, 8, [17], [900]),
+    (4, 1, [10, 7, 3], [4, 0, 3]), (2, 1, [700], [1500]), (32, 8, [12] * 66, None),
+])
+def test_prompts(dev, hq, kv, q_lens, k_lens):
+    g = gen(20)
+    k_lens = q_lens if k_lens is None else k_lens
+    q = randn(g, sum(q_lens), hq, D)
+    k, v = randn(g, sum(k_lens), kv, D), randn(g, sum(k_lens), kv, D)
+    out = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens)
+    assert out.shape == q.shape and out.dtype == torch.bfloat16
+    check_prompt(out, q, k, v, q_lens, k_lens, some=24)
+
+
+@pytest.mark.parametrize("hq,kv,q_lens,k_lens", [
+    (32, 8, [2048], [2048]), (6, 1, [3001, 900], [3001, 2500]), (8, 1, [20], [40000]), (12, 2, [512], [8193]),
+])
+def test_long_prompts(dev, hq, kv, q_lens, k_lens):
+    g = gen(21)
+    q = randn(g, sum(q_lens), hq, D)
+    k, v = randn(g, sum(k_lens), kv, D), randn(g, sum(k_lens), kv, D)
+    out = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens)
+    check_prompt(out, q, k, v, q_lens, k_lens, some=10)
+
+
+@pytest.mark.parametrize("scale,std", [(-SCALE, 1.0), (0.0, 1.0), (1.0, 1.0), (SCALE, 30.0)])
+def test_prompt_scales(dev, scale, std):
+    g = gen(22)
+    q, k, v = randn(g, 150, 4, D, std=std), randn(g, 150, 2, D), randn(g, 150, 2, D)
+    out = prompt_attention(q.to(dev), k.to(dev), v.to(dev), [150], scale)
+    check_prompt(out, q, k, v, [150], [150], scale=scale)
+
+
+def test_prompt_rows_of_a_fused_projection(dev):
+    """q, k and v as views of one projection, and of rows that are not 16-byte aligned."""
+    g = gen(23)
+    T, hq, kv = 130, 8, 2
+    for pad in (0, 1):
+        proj = randn(g, T, (hq + 2 * kv) * D + 24 + pad)
+        d = proj.to(dev)
+        q, k, v = (d[:, a * D + pad:b * D + pad].unflatten(1, (b - a, D))
+                   for a, b in ((0, hq), (hq, hq + kv), (hq + kv, hq + 2 * kv)))
+        out = prompt_attention(q, k, v, [100, 30], SCALE)
+        check_prompt(out, q, k, v, [100, 30], [100, 30], some=20)
+
+
+def test_prompt_heads_first_layout(dev):
+    g = gen(24)
+    q, k, v = (randn(g, h, 90, D).to(dev).transpose(0, 1) for h in (6, 2, 2))
+    check_prompt(prompt_attention(q, k, v, [90], SCALE), q, k, v, [90], [90])
+
+
+@pytest.mark.parametrize("what", ["k nan", "k inf", "v nan", "v inf"])
+@pytest.mark.parametrize("q_lens,k_lens,at", [([200], [200], 130), ([100], [164], 150), ([3, 60], [3, 60], 40)])
+def test_prompt_keys_that_a_row_does_not_see_do_not_reach_it(dev, what, q_lens, k_lens, at):
+    g = gen(25)
+    q, k, v = randn(g, sum(q_lens), 8, D), randn(g, sum(k_lens), 2, D), randn(g, sum(k_lens), 2, D)
+    seq = len(k_lens) - 1
+    row = sum(k_lens[:seq]) + at
+    clean = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens)
+    x = (k if what[0] == "k" else v)
+    bad = x.clone()
+    bad[row, 1, 7 if what[0] == "v" else slice(None)] = float(what[2:])
+    args = (bad, v) if what[0] == "k" else (k, bad)
+    out = prompt_attention(q.to(dev), *(t.to(dev) for t in args), q_lens, SCALE, k_lens=k_lens)
+    first = sum(q_lens[:seq]) + max(0, at - (k_lens[seq] - q_lens[seq]))  # first row that sees it
+    assert torch.equal(bits(out[:first]), bits(clean[:first]))
+    assert torch.equal(bits(out[:, :4]), bits(clean[:, :4])), "heads of another KV head"
+    if what[0] == "v":  # the rows that do see it: that dim alone
+        dim = out[first:, 4:, 7].float()
+        assert torch.isnan(dim).all() if "nan" in what else not torch.isfinite(dim).any()
+        rest = [d for d in range(D) if d != 7]
+        assert torch.equal(bits(out[first:, :, rest]), bits(clean[first:, :, rest]))
+    elif "nan" in what:
+        assert torch.isnan(out[first:, 4:]).all()
+
+
+def test_prompt_captured(dev):
+    g = gen(26)
+    q_lens, k_lens = [65, 300], [65, 700]
+    q, k, v = (randn(g, n, h, D).to(dev) for n, h in ((365, 8), (765, 2), (765, 2)))
+    stream = torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):
+        prompt_attention(q, k, v, q_lens, SCALE, k_lens=k_lens)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = prompt_attention(q, k, v, q_lens, SCALE, k_lens=k_lens)
+    torch.cuda.current_stream(dev).wait_stream(stream)
+    for i in range(3):
+        q.copy_(randn(g, 365, 8, D))
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        eager = prompt_attention(q, k, v, q_lens, SCALE, k_lens=k_lens)
+        assert torch.equal(bits(out), bits(eager))
+        check_prompt(out, q, k, v, q_lens, k_lens, some=12)
+
+
+def test_prompt_of_no_rows(dev):
+    e = torch.empty((0, 8, D), dtype=torch.bfloat16, device=dev)
+    kv = torch.empty((0, 2, D), dtype=torch.bfloat16, device=dev)
+    assert prompt_attention(e, kv, kv, [], SCALE).shape == (0, 8, D)
+    assert prompt_attention(e, kv, kv, [0, 0], SCALE).shape == (0, 8, D)
+    q = torch.ones((5, 8, D), dtype=torch.bfloat16, device=dev)
+    assert (prompt_attention(q, kv, kv, [2, 3], SCALE, k_lens=[0, 0]) == 0).all()
