@@ -87,22 +87,31 @@ struct TileRows {
   }
 };
 
-// Raw scores of the tile's keys.
+// Raw scores of the tile's keys. K fragments are read one key tile ahead of the MFMAs that use them (the
+// scheduling barriers keep it so).
 template <int NT>
-__device__ __forceinline__ void tile_scores(const KvTile& t, const TileRows<NT>& st, int lane,
+__device__ __forceinline__ void tile_scores(const uint16_t* kt, const TileRows<NT>& st, int lane,
                                             f4_t (&c)[NT][4]) {
   const int lc = lane & 15, lq4 = lane >> 4;
-  const bf16x8_t* k = reinterpret_cast<const bf16x8_t*>(t.k) + 16 * lc;
+  const bf16x8_t* k = reinterpret_cast<const bf16x8_t*>(kt) + 16 * lc;
+  bf16x8_t f[2][4];
 #pragma unroll
-  for (int mt = 0; mt < 4; ++mt)
+  for (int kk = 0; kk < 4; ++kk) f[0][kk] = k[(4 * kk + lq4) ^ lc];
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const bf16x8_t a = k[256 * mt + ((4 * kk + lq4) ^ lc)];
+  for (int mt = 0; mt < 4; ++mt) {
+    if (mt + 1 < 4) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) f[(mt + 1) & 1][kk] = k[256 * (mt + 1) + ((4 * kk + lq4) ^ lc)];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
         c[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            a, st.q[nt][kk], kk == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : c[nt][mt], 0, 0, 0);
-    }
+            f[mt & 1][kk], st.q[nt][kk], kk == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : c[nt][mt], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // Scores to weights: raises the running maximum where needed (and rescales the row), P in bf16 as the
@@ -140,10 +149,10 @@ __device__ __forceinline__ void tile_softmax(f4_t (&c)[NT][4], TileRows<NT>& st,
   }
 }
 
-// A operand of dims 16 w .. 16 w + 15 and k-step e of a tile's V^T.
-__device__ __forceinline__ uint32_t v_lane(const KvTile& t, int lane) {
+// A operand of dims 16 w .. 16 w + 15 and k-step e of a tile's V^T (v 256-byte aligned).
+__device__ __forceinline__ uint32_t v_lane(const uint16_t* v, int lane) {
   const int rk = 4 * (lane >> 4) + ((lane >> 2) & 3);  // key of this lane's source within 16
-  return lds_addr(t.v) + (uint32_t)(256 * rk + 8 * (lane & 3) + 32 * (rk & 7));
+  return lds_addr(v) + (uint32_t)(256 * rk + 8 * (lane & 3) + 32 * (rk & 7));
 }
 __device__ __forceinline__ bf16x8_t v_operand(uint32_t vl, int w, int e) {
   const uint32_t a = (vl ^ (uint32_t)(32 * w)) + 8192u * e;
@@ -154,64 +163,72 @@ __device__ __forceinline__ bf16x8_t v_operand(uint32_t vl, int w, int e) {
   return __builtin_bit_cast(bf16x8_t, u);
 }
 
-// The bf16 pairs of an operand with infinities and NaN as 0.
-__device__ __forceinline__ bf16x8_t finite_only(bf16x8_t x) {
-  u4_t u = __builtin_bit_cast(u4_t, x);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if ((u[j] & 0x7f80u) == 0x7f80u) u[j] &= 0xffff0000u;
-    if ((u[j] & 0x7f800000u) == 0x7f800000u) u[j] &= 0xffffu;
-  }
-  return __builtin_bit_cast(bf16x8_t, u);
+// A bf16 pair with infinities and NaN as 0.
+__device__ __forceinline__ uint32_t finite_bf2(uint32_t u) {
+  if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
+  if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
+  return u;
 }
 
-// FINITE: infinities and NaN of V are left out (0 times one of them is no 0).
-template <int NT, bool FINITE = false>
-__device__ __forceinline__ void tile_values(const KvTile& t, TileRows<NT>& st, int lane,
+// O^T += V^T P^T. Fragments of half a k-step (four windows of 16 dims) are read ahead of the MFMAs, as in
+// tile_scores.
+template <int NT>
+__device__ __forceinline__ void tile_values(const uint16_t* v, TileRows<NT>& st, int lane,
                                             const bf16x8_t (&p)[NT][2]) {
-  const uint32_t vl = v_lane(t, lane);
+  const uint32_t vl = v_lane(v, lane);
+  bf16x8_t f[2][4];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
+  for (int j = 0; j < 4; ++j) f[0][j] = v_operand(vl, j, 0);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      st.l[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_ones(), p[nt][e], st.l[nt], 0, 0, 0);
+  for (int u = 0; u < 4; ++u) {  // k-step u / 2, windows 4 (u % 2) ..
+    if (u + 1 < 4) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      bf16x8_t a = v_operand(vl, w, e);
-      if constexpr (FINITE) a = finite_only(a);
+      for (int j = 0; j < 4; ++j) f[(u + 1) & 1][j] = v_operand(vl, 4 * ((u + 1) & 1) + j, (u + 1) >> 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const int e = u >> 1, w0 = 4 * (u & 1);
+    if (u & 1) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        st.o[nt][w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p[nt][e], st.o[nt][w], 0, 0, 0);
+        st.l[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_ones(), p[nt][e], st.l[nt], 0, 0, 0);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        st.o[nt][w0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[u & 1][j], p[nt][e],
+                                                                 st.o[nt][w0 + j], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// What tile_values<NT, true> left out, for the rows that see the key (lim: last key of each row, counted
-// from the tile): keys' infinities and NaN, one key of `mask` at a time. Rare.
+// The infinities and NaN of one V row (key `key` of a tile whose P is p, position `at`), for the rows that see
+// it: O^T took 0 in their place, since 0 times one of them is no 0.
 template <int NT>
-__device__ __forceinline__ void tile_nonfinite(const KvTile& t, TileRows<NT>& st, int lane,
-                                               const bf16x8_t (&p)[NT][2], const int (&lim)[NT],
-                                               uint64_t mask) {
+__device__ __forceinline__ void tile_nonfinite(const uint8_t* vrow, int key, int at, TileRows<NT>& st, int lane,
+                                               const bf16x8_t (&p)[NT][2], const int (&lim)[NT]) {
   const int lc = lane & 15, lq4 = lane >> 4;
-  for (; mask; mask &= mask - 1) {
-    const int key = __builtin_ctzll(mask);
-    const int word = 2 * ((key >> 4) & 1) + ((key >> 1) & 1);
-    const uint16_t* vrow = t.v + key * D + 4 * lq4;
+  const int word = 2 * ((key >> 4) & 1) + ((key >> 1) & 1);
+  float pk[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const u4_t pe = __builtin_bit_cast(u4_t, key < 32 ? p[nt][0] : p[nt][1]);
-      const uint32_t mine = word < 2 ? (word == 0 ? pe[0] : pe[1]) : (word == 2 ? pe[2] : pe[3]);
-      const uint32_t pw = __shfl(mine, 16 * ((key >> 2) & 3) + lc, 64);
-      const float pk = key & 1 ? bf16_hi(pw) : bf16_lo(pw);
+  for (int nt = 0; nt < NT; ++nt) {
+    const u4_t p0 = __builtin_bit_cast(u4_t, p[nt][0]), p1 = __builtin_bit_cast(u4_t, p[nt][1]);
+    uint32_t mine = 0;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const uint2 v2 = *reinterpret_cast<const uint2*>(vrow + 16 * (w ^ (key & 7)));
-        const float v[4] = {bf16_lo(v2.x), bf16_hi(v2.x), bf16_lo(v2.y), bf16_hi(v2.y)};
+    for (int j = 0; j < 4; ++j) mine = j == word ? (key < 32 ? p0[j] : p1[j]) : mine;
+    const uint32_t w = __shfl(mine, 16 * ((key >> 2) & 3) + lc, 64);
+    pk[nt] = key & 1 ? bf16_hi(w) : bf16_lo(w);
+  }
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (key <= lim[nt] && !(fabsf(v[r]) < INFINITY)) st.o[nt][w][r] = fmaf(pk, v[r], st.o[nt][w][r]);
-      }
-    }
+  for (int w = 0; w < 8; ++w) {
+    const uint2 v2 = *reinterpret_cast<const uint2*>(vrow + 2 * (16 * w + 4 * lq4));
+    const float v[4] = {bf16_lo(v2.x), bf16_hi(v2.x), bf16_lo(v2.y), bf16_hi(v2.y)};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (at <= lim[nt] && !(fabsf(v[r]) < INFINITY)) st.o[nt][w][r] = fmaf(pk[nt], v[r], st.o[nt][w][r]);
   }
 }
 

@@ -360,9 +360,9 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
     const int s = (p - p0) & 1;
     f4_t c[NT][4];
     bf16x8_t pr[NT][2];
-    tile_scores<NT>(sm[s], st, lane, c);
+    tile_scores<NT>(sm[s].k, st, lane, c);
     tile_softmax<NT>(c, st, scale, pr);
-    tile_values<NT>(sm[s], st, lane, pr);
+    tile_values<NT>(sm[s].v, st, lane, pr);
     if (p + 1 < p1) {
       stage(sm[s ^ 1]);
       if (p + 2 < p1) load(p + 2);

@@ -7,8 +7,16 @@
 // Work: a workgroup of 8 waves takes 256 query rows of a KV head, numbered position-major (row f is
 // position f / G of query head f % G), so that any grouping fills the matrix cores and a block's rows see
 // nearly the same keys; a wave has 32 of them. It walks the 64-key tiles up to its last row's bound, each
-// staged in LDS once for all waves (two buffers; the next tile's global loads are in flight while one
-// is computed, one barrier per tile) and run through attn_tile.h. Where whole blocks would leave CUs idle
+// copied into LDS once for all waves (three buffers of K and of V, copies two tiles ahead) and run through
+// attn_tile.h. A SIMD holds one wave of each half of the workgroup, and the halves run one phase apart, so
+// that one's matrix phase (P.V of a tile, Q.K^T of the next) lies beside the other's vector phase (softmax,
+// copies), with a barrier after each:
+//
+//   slot    group A                   group B
+//   2t      P.V(t-1), Q.K^T(t)        softmax(t-1), copies K(t+2) V(t+1)
+//   2t+1    softmax(t), copies        P.V(t-1), Q.K^T(t)
+//
+// Where whole blocks would leave CUs idle
 // (short or few prompts behind long pasts) a block's tiles are cut into parts whose partial rows a second
 // launch merges.
 //
@@ -65,15 +73,18 @@ __host__ __device__ __forceinline__ int block_tiles(int blk, int R, FastDiv g, i
   return last < 0 ? 0 : last / TKEYS + 1;
 }
 
+constexpr int STAGES = 3;  // tiles of K and of V in LDS
 struct PromptSmem {
-  KvTile t[2];
-  uint32_t nonfinite[3][2];  // keys of a masked tile whose V holds an infinity or NaN
+  alignas(256) uint16_t k[STAGES][TKEYS * D];
+  alignas(256) uint16_t v[STAGES][TKEYS * D];
+  uint32_t nonfinite[STAGES][2];  // keys of a masked tile whose V holds an infinity or NaN
 };
 
 __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArgs a, int first) {
   __shared__ PromptSmem sm;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool grp_a = wv < PW / 2;
   const int lc = lane & 15, lq4 = lane >> 4;
   const int x = blockIdx.x / a.Hkv, hk = blockIdx.x - x * a.Hkv;
   const Entry en = a.list[x];
@@ -90,32 +101,45 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   const int low = base + (int)fdiv_u((uint32_t)(blk * PROWS), a.g);
   const int t_masked = low < 0 ? 0 : (low + 1) / TKEYS;
 
-  // ---- staging: 16-byte chunk tid % 16 of keys tid / 16 and tid / 16 + 32
-  const int key0 = tid >> 4, chunk = tid & 15;
-  const uint16_t* kp = a.k + (int64_t)k0 * a.k_tok + hk * a.k_head + 8 * chunk;
-  const uint16_t* vp = a.v + (int64_t)k0 * a.v_tok + hk * a.v_head + 8 * chunk;
-  uint4 rk[2], rv[2];
-  auto load = [&](int t) {
+  // ---- copies: wave wv brings keys 8 wv .. 8 wv + 7 of every tile, K and V 1 KB (4 keys) at a time; a
+  // lane's 16 bytes land at lane x 16, so the swizzle is in the chunk it reads. Keys past the last one
+  // read it again.
+  const int krow = 8 * wv + (lane >> 4);  // and + 4
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + (int64_t)k0 * a.k_tok + hk * a.k_head);
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + (int64_t)k0 * a.v_tok + hk * a.v_head);
+  const uint32_t k_at = lds_u32(sm.k) + 2048u * wv, v_at = lds_u32(sm.v) + 2048u * wv;
+  auto copy_k = [&](int t) {
+    const int r = TKEYS * min(t, t1 - 1) + krow;
+    const uint32_t m = __builtin_amdgcn_readfirstlane(k_at + (uint32_t)(t % STAGES) * (TKEYS * D * 2));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int key = TKEYS * t + key0 + 32 * i;
-      const int64_t r = min(key, lk - 1);
-      rk[i] = *reinterpret_cast<const uint4*>(kp + r * a.k_tok);
-      rv[i] = *reinterpret_cast<const uint4*>(vp + r * a.v_tok);
-      if (key >= lk) rv[i] = make_uint4(0, 0, 0, 0);
+      const uint8_t* p = kbase + 2 * a.k_tok * min(r + 4 * i, lk - 1) + 16 * (lc ^ ((krow + 4 * i) & 15));
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                   :: "v"(p), "s"(m + 1024u * i) : "memory");
     }
   };
-  auto stage = [&](int t) {
-    KvTile& d = sm.t[t & 1];
+  auto copy_v = [&](int t) {
+    const int r = TKEYS * min(t, t1 - 1) + krow;
+    const uint32_t m = __builtin_amdgcn_readfirstlane(v_at + (uint32_t)(t % STAGES) * (TKEYS * D * 2));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      *k_chunk(d, key0 + 32 * i, chunk) = rk[i];
-      *v_chunk(d, key0 + 32 * i, chunk) = rv[i];
-      if (t >= t_masked) {  // workgroup-uniform
-        uint32_t m = bf16x2_absmax_bits(bf16x2_absmax_bits(0, rv[i].x), rv[i].y);
-        m = bf16x2_absmax_bits(bf16x2_absmax_bits(m, rv[i].z), rv[i].w);
-        if ((m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u)
-          atomicOr(&sm.nonfinite[t % 3][i], 1u << key0);
+      const uint8_t* p = vbase + 2 * a.v_tok * min(r + 4 * i, lk - 1) + 16 * (lc ^ (2 * ((krow + 4 * i) & 7)));
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                   :: "v"(p), "s"(m + 1024u * i) : "memory");
+    }
+  };
+  // The wave's own V rows of tile t, in LDS: infinities and NaN become 0 and their keys are noted.
+  auto scan_v = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint4* at = reinterpret_cast<uint4*>(&sm.v[t % STAGES][(8 * wv + 4 * i) * D + 8 * lane]);
+      const uint4 u = *at;
+      uint32_t m = bf16x2_absmax_bits(bf16x2_absmax_bits(0, u.x), u.y);
+      m = bf16x2_absmax_bits(bf16x2_absmax_bits(m, u.z), u.w);
+      const int key = krow + 4 * i;
+      if ((m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u) {
+        *at = make_uint4(finite_bf2(u.x), finite_bf2(u.y), finite_bf2(u.z), finite_bf2(u.w));
+        atomicOr(&sm.nonfinite[t % STAGES][key >> 5], 1u << (key & 31));
       }
     }
   };
@@ -123,7 +147,6 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   // ---- the wave's rows
   const int f0 = blk * PROWS + 16 * NT * wv;
   TileRows<NT> st;
-  st.clear();
   int lim[NT];  // last key of the lane's row, -1: none
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -136,25 +159,37 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
     for (int kk = 0; kk < 4; ++kk)
       st.q[nt][kk] = u4_as_bf8(signed_q(*reinterpret_cast<const uint4*>(qr + 32 * kk), a.sl2));
   }
+  st.clear();
   const int lim_lo = f0 < R ? base + (int)fdiv_u((uint32_t)f0, a.g) : -1;
-  const int lim_hi = f0 < R ? base + (int)fdiv_u((uint32_t)min(f0 + 16 * NT - 1, R - 1), a.g) : -1;
 
+  f4_t c[NT][4];
+  bf16x8_t p[NT][2];
+  // end of a tile's two slots: the wave's copies of K(t + 1) and V(t) have landed (4 newer ones are out)
+  auto landed = [&](int t) {
+    asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    if (t >= t_masked) scan_v(t);  // workgroup-uniform
+  };
   if (t0 < t1) {
-    if (tid < 6) sm.nonfinite[tid >> 1][tid & 1] = 0;
-    load(t0);
-    __syncthreads();
-    stage(t0);
-    if (t0 + 1 < t1) load(t0 + 1);
-    __syncthreads();
-  }
-  for (int t = t0; t < t1; ++t) {
-    const KvTile& tile = sm.t[t & 1];
-    if (TKEYS * t <= lim_hi) {  // wave-uniform: some row sees the tile
-      f4_t c[NT][4];
-      bf16x8_t p[NT][2];
-      tile_scores<NT>(tile, st, lane, c);
-      const bool masked = TKEYS * t + TKEYS - 1 > lim_lo;
-      if (masked) {
+    if (tid < 2 * STAGES) sm.nonfinite[tid >> 1][tid & 1] = 0;
+    copy_k(t0);
+    copy_k(t0 + 1);
+    copy_v(t0);
+    asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    lds_barrier();
+    if (!grp_a) {  // half a tile behind
+      copy_k(t0 + 2);
+      copy_v(t0 + 1);
+      lds_barrier();
+    }
+    tile_scores<NT>(sm.k[t0 % STAGES], st, lane, c);
+    for (int t = t0; t < t1; ++t) {
+      if (!grp_a) landed(t);
+      lds_barrier();
+      // vector phase
+      __builtin_amdgcn_s_setprio(2);
+      copy_k(t + (grp_a ? 2 : 3));
+      copy_v(t + (grp_a ? 1 : 2));
+      if (TKEYS * t + TKEYS - 1 > lim_lo) {  // wave-uniform: masked for some row
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -164,26 +199,25 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
               c[nt][mt][r] = TKEYS * t + 16 * mt + 4 * lq4 + r <= lim[nt] ? c[nt][mt][r] : -INFINITY;
       }
       tile_softmax<NT>(c, st, scale, p);
-      const uint64_t nf = masked ? (uint64_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % 3][0]) |
-                                       (uint64_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % 3][1]) << 32
-                                 : 0;
-      if (nf) {
-        int rel[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) rel[nt] = lim[nt] - TKEYS * t;
-        tile_values<NT, true>(tile, st, lane, p);
-        tile_nonfinite<NT>(tile, st, lane, p, rel, nf);
-      } else {
-        tile_values<NT>(tile, st, lane, p);
+      if (grp_a) landed(t);
+      lds_barrier();
+      // matrix phase: P.V of tile t, Q.K^T of tile t + 1 (behind the last one, of a copy nobody reads)
+      __builtin_amdgcn_s_setprio(0);
+      tile_values<NT>(sm.v[t % STAGES], st, lane, p);
+      if (t >= t_masked) {
+        uint64_t nf = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % STAGES][0]) |
+                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % STAGES][1]) << 32;
+        for (; nf; nf &= nf - 1) {  // rare
+          const int key = __builtin_ctzll(nf), at = TKEYS * t + key;
+          if (at < lk) tile_nonfinite<NT>(vbase + 2 * a.v_tok * at, key, at, st, lane, p, lim);
+        }
       }
+      tile_scores<NT>(sm.k[(t + 1) % STAGES], st, lane, c);
+      // read by the other half for the last time a slot ago: group A clears what tile t + 2 will note
+      if (tid < 2) sm.nonfinite[(t + 2) % STAGES][tid] = 0;
     }
-    if (t + 1 < t1) {
-      stage(t + 1);
-      if (t + 2 < t1) load(t + 2);
-    }
-    // tile t + 2's flags, last read for tile t - 1
-    if (tid < 2) sm.nonfinite[(t + 2) % 3][tid] = 0;
-    __syncthreads();
+    if (grp_a) lds_barrier();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies past the last tile
   }
 
   // ---- rows out: dims 16 w + 4 lq4 + r
