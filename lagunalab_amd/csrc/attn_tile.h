@@ -144,6 +144,8 @@ __device__ __forceinline__ void tile_softmax(f4_t (&c)[NT][4], TileRows<NT>& st,
       for (int h = 0; h < 2; ++h)
         w[2 * mt + h] = pack_bf2(__builtin_amdgcn_exp2f(fmaf(c[nt][mt][2 * h], scale, off)),
                                  __builtin_amdgcn_exp2f(fmaf(c[nt][mt][2 * h + 1], scale, off)));
+    // made here, not sunk into the product's phase
+    asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]), "+v"(w[4]), "+v"(w[5]), "+v"(w[6]), "+v"(w[7]));
     p[nt][0] = words_as_bf8(w[0], w[1], w[2], w[3]);
     p[nt][1] = words_as_bf8(w[4], w[5], w[6], w[7]);
   }
