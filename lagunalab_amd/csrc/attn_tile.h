@@ -119,35 +119,54 @@ __device__ __forceinline__ void tile_scores(const uint16_t* kt, const TileRows<N
 template <int NT>
 __device__ __forceinline__ void tile_softmax(f4_t (&c)[NT][4], TileRows<NT>& st, float scale,
                                              bf16x8_t (&p)[NT][2]) {
+  float t[NT];
+  bool bump[NT], any = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    float t = -INFINITY;
+    // four chains
+    float x[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
+      x[mt] = max_ieee(max_ieee(max_ieee(c[nt][mt][0], c[nt][mt][1]), c[nt][mt][2]), c[nt][mt][3]);
+    t[nt] = max_ieee(max_ieee(x[0], x[1]), max_ieee(x[2], x[3]));
+  }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t = max_ieee(t, c[nt][mt][r]);
-    t = max_xor32(max_xor16(t)) * scale;
-    const bool bump = t > (st.m[nt] == -INFINITY ? -INFINITY : st.m[nt] + RESCALE_LOG2);
-    if (__builtin_amdgcn_ballot_w64(bump)) {
-      const float mn = bump ? t : st.m[nt];
+  for (int nt = 0; nt < NT; ++nt) t[nt] = max_xor16(t[nt]);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    t[nt] = max_xor32(t[nt]) * scale;
+    bump[nt] = t[nt] > (st.m[nt] == -INFINITY ? -INFINITY : st.m[nt] + RESCALE_LOG2);
+    any |= bump[nt];
+  }
+  if (__builtin_amdgcn_ballot_w64(any)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float mn = bump[nt] ? t[nt] : st.m[nt];
       const float alpha = st.m[nt] == -INFINITY ? 0.0f : exp2_nonpos(st.m[nt] - mn);
       st.m[nt] = mn;
       st.l[nt] *= alpha;
 #pragma unroll
       for (int w = 0; w < 8; ++w) st.o[nt][w] *= alpha;
     }
-    const float off = st.m[nt] == -INFINITY ? 0.0f : -st.m[nt];
-    uint32_t w[8];
+  }
+  uint32_t w[NT][8];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+  for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float off = st.m[nt] == -INFINITY ? 0.0f : -st.m[nt];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        w[2 * mt + h] = pack_bf2(__builtin_amdgcn_exp2f(fmaf(c[nt][mt][2 * h], scale, off)),
-                                 __builtin_amdgcn_exp2f(fmaf(c[nt][mt][2 * h + 1], scale, off)));
+        w[nt][2 * mt + h] = pack_bf2(__builtin_amdgcn_exp2f(fmaf(c[nt][mt][2 * h], scale, off)),
+                                     __builtin_amdgcn_exp2f(fmaf(c[nt][mt][2 * h + 1], scale, off)));
+    }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
     // made here, not sunk into the product's phase
-    asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]), "+v"(w[4]), "+v"(w[5]), "+v"(w[6]), "+v"(w[7]));
-    p[nt][0] = words_as_bf8(w[0], w[1], w[2], w[3]);
-    p[nt][1] = words_as_bf8(w[4], w[5], w[6], w[7]);
+    asm volatile("" : "+v"(w[nt][0]), "+v"(w[nt][1]), "+v"(w[nt][2]), "+v"(w[nt][3]), "+v"(w[nt][4]),
+                      "+v"(w[nt][5]), "+v"(w[nt][6]), "+v"(w[nt][7]));
+    p[nt][0] = words_as_bf8(w[nt][0], w[nt][1], w[nt][2], w[nt][3]);
+    p[nt][1] = words_as_bf8(w[nt][4], w[nt][5], w[nt][6], w[nt][7]);
   }
 }
 

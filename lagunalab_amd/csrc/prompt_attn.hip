@@ -108,26 +108,33 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + (int64_t)k0 * a.k_tok + hk * a.k_head);
   const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + (int64_t)k0 * a.v_tok + hk * a.v_head);
   const uint32_t k_at = lds_u32(sm.k) + 2048u * wv, v_at = lds_u32(sm.v) + 2048u * wv;
-  auto copy_k = [&](int t) {
-    const int r = TKEYS * min(t, t1 - 1) + krow;
-    const uint32_t m = __builtin_amdgcn_readfirstlane(k_at + (uint32_t)(t % STAGES) * (TKEYS * D * 2));
+  // A tile's base is scalar, a lane's offset in it fixed but in the tile that ends behind the last key.
+  auto copy = [&](const uint8_t* from, int64_t tok, int t, uint32_t to, const uint32_t (&at)[2], bool is_v) {
+    const int tt = min(t, t1 - 1);
+    const uint8_t* sb = from + 2 * TKEYS * tok * tt;
+    const uint32_t m = __builtin_amdgcn_readfirstlane(to + (uint32_t)(t % STAGES) * (TKEYS * D * 2));
+    uint32_t o[2] = {at[0], at[1]};
+    if (TKEYS * tt + TKEYS > lk) {  // uniform
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint8_t* p = kbase + 2 * a.k_tok * min(r + 4 * i, lk - 1) + 16 * (lc ^ ((krow + 4 * i) & 15));
-      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                   :: "v"(p), "s"(m + 1024u * i) : "memory");
+      for (int i = 0; i < 2; ++i) {
+        const int r = krow + 4 * i;
+        o[i] = 2 * (uint32_t)tok * (uint32_t)min(r, lk - 1 - TKEYS * tt) + 16 * (lc ^ (is_v ? 2 * (r & 7) : r & 15));
+      }
     }
-  };
-  auto copy_v = [&](int t) {
-    const int r = TKEYS * min(t, t1 - 1) + krow;
-    const uint32_t m = __builtin_amdgcn_readfirstlane(v_at + (uint32_t)(t % STAGES) * (TKEYS * D * 2));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint8_t* p = vbase + 2 * a.v_tok * min(r + 4 * i, lk - 1) + 16 * (lc ^ (2 * ((krow + 4 * i) & 7)));
-      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                   :: "v"(p), "s"(m + 1024u * i) : "memory");
-    }
+    for (int i = 0; i < 2; ++i)
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                   :: "v"(o[i]), "s"(sb), "s"(m + 1024u * i) : "memory");
   };
+  uint32_t ko[2], vo[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = krow + 4 * i;
+    ko[i] = 2 * (uint32_t)a.k_tok * r + 16 * (lc ^ (r & 15));
+    vo[i] = 2 * (uint32_t)a.v_tok * r + 16 * (lc ^ (2 * (r & 7)));
+  }
+  auto copy_k = [&](int t) { copy(kbase, a.k_tok, t, k_at, ko, false); };
+  auto copy_v = [&](int t) { copy(vbase, a.v_tok, t, v_at, vo, true); };
   // The wave's own V rows of tile t, in LDS: infinities and NaN become 0 and their keys are noted.
   auto scan_v = [&](int t) {
 #pragma unroll
@@ -383,6 +390,8 @@ extern "C" int lq_prompt_attn(const uint16_t* q, const uint16_t* k, const uint16
   LQ_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0 &&
                    ((q_tok | q_head | k_tok | k_head | v_tok | v_head) & 7) == 0,
                "rows must be 16-byte aligned (strides a multiple of 8)");
+  LQ_CHECK_ARG(k_tok >= 0 && v_tok >= 0 && k_tok < (1 << 24) && v_tok < (1 << 24),
+               "rows of k or v 2^24 values apart or more");
   LQ_CHECK_ARG(std::isfinite(scale), "the softmax scale is not finite");
   PromptArgs a;
   std::vector<Entry> list;
