@@ -224,6 +224,58 @@ __device__ __forceinline__ void tile_values(const uint16_t* v, TileRows<NT>& st,
   }
 }
 
+// Q.K^T of one tile, then P.V of another, in eight steps of 4 NT MFMAs: key tile u of K, then half a
+// k-step of V. A step's four fragments are read two steps ahead (tile_ahead: the first two, which may
+// lie in the phase before), so that no MFMA waits for LDS.
+struct Ahead {
+  bf16x8_t f[3][4];
+};
+__device__ __forceinline__ void tile_fetch(const bf16x8_t* k, uint32_t vl, int lane, int step, bf16x8_t (&f)[4]) {
+  const int lc = lane & 15, lq4 = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    f[j] = step < 4 ? k[256 * step + ((4 * j + lq4) ^ lc)]
+                    : v_operand(vl, 4 * (step & 1) + j, (step - 4) >> 1);
+}
+__device__ __forceinline__ void tile_ahead(const uint16_t* kt, int lane, Ahead& a) {
+  const bf16x8_t* k = reinterpret_cast<const bf16x8_t*>(kt) + 16 * (lane & 15);
+  tile_fetch(k, 0, lane, 0, a.f[0]);
+  tile_fetch(k, 0, lane, 1, a.f[1]);
+}
+template <int NT>
+__device__ __forceinline__ void tile_matrix(const uint16_t* kt, const uint16_t* vt, TileRows<NT>& st, int lane,
+                                            f4_t (&c)[NT][4], const bf16x8_t (&p)[NT][2], Ahead& a) {
+  const bf16x8_t* k = reinterpret_cast<const bf16x8_t*>(kt) + 16 * (lane & 15);
+  const uint32_t vl = v_lane(vt, lane);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    if (u + 2 < 8) tile_fetch(k, vl, lane, u + 2, a.f[(u + 2) % 3]);
+    __builtin_amdgcn_sched_barrier(0);
+    if (u < 4) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          c[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              a.f[u % 3][kk], st.q[nt][kk], kk == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : c[nt][u], 0, 0, 0);
+    } else {
+      const int e = (u - 4) >> 1, w0 = 4 * (u & 1);
+      if (u & 1) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          st.l[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_ones(), p[nt][e], st.l[nt], 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          st.o[nt][w0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.f[u % 3][j], p[nt][e],
+                                                                     st.o[nt][w0 + j], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // The infinities and NaN of one V row (key `key` of a tile whose P is p, position `at`), for the rows that see
 // it: O^T took 0 in their place, since 0 times one of them is no 0.
 template <int NT>

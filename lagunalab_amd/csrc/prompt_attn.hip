@@ -13,8 +13,8 @@
 // copies), with a barrier after each:
 //
 //   slot    group A                   group B
-//   2t      P.V(t-1), Q.K^T(t)        softmax(t-1), copies K(t+2) V(t+1)
-//   2t+1    softmax(t), copies        P.V(t-1), Q.K^T(t)
+//   2t      Q.K^T(t), P.V(t-1)        softmax(t-1), copies K(t+2) V(t+1)
+//   2t+1    softmax(t), copies        Q.K^T(t), P.V(t-1)
 //
 // Where whole blocks would leave CUs idle
 // (short or few prompts behind long pasts) a block's tiles are cut into parts whose partial rows a second
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
 
   f4_t c[NT][4];
   bf16x8_t p[NT][2];
-  // end of a tile's two slots: the wave's copies of K(t + 1) and V(t) have landed (4 newer ones are out)
+  // V(t) of the wave's copies has landed (4 newer ones are out)
   auto landed = [&](int t) {
     asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     if (t >= t_masked) scan_v(t);  // workgroup-uniform
@@ -186,14 +186,18 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
     if (!grp_a) {  // half a tile behind
       copy_k(t0 + 2);
       copy_v(t0 + 1);
+      asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t0 + 1)
       lds_barrier();
     }
     tile_scores<NT>(sm.k[t0 % STAGES], st, lane, c);
     for (int t = t0; t < t1; ++t) {
-      if (!grp_a) landed(t);
+      if (grp_a)
+        asm volatile("s_waitcnt vmcnt(2)" ::: "memory");  // K(t + 1)
+      else
+        landed(t);
       lds_barrier();
       // vector phase
-      __builtin_amdgcn_s_setprio(2);
+      __builtin_amdgcn_s_setprio(1);
       copy_k(t + (grp_a ? 2 : 3));
       copy_v(t + (grp_a ? 1 : 2));
       if (TKEYS * t + TKEYS - 1 > lim_lo) {  // wave-uniform: masked for some row
@@ -206,11 +210,16 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
               c[nt][mt][r] = TKEYS * t + 16 * mt + 4 * lq4 + r <= lim[nt] ? c[nt][mt][r] : -INFINITY;
       }
       tile_softmax<NT>(c, st, scale, p);
-      if (grp_a) landed(t);
+      Ahead ahead;
+      tile_ahead(sm.k[(t + 1) % STAGES], lane, ahead);
+      if (grp_a)
+        landed(t);
+      else
+        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t + 2)
       lds_barrier();
-      // matrix phase: P.V of tile t, Q.K^T of tile t + 1 (behind the last one, of a copy nobody reads)
+      // matrix phase: Q.K^T of tile t + 1 (behind the last one, of a copy nobody reads), P.V of tile t
       __builtin_amdgcn_s_setprio(0);
-      tile_values<NT>(sm.v[t % STAGES], st, lane, p);
+      tile_matrix<NT>(sm.k[(t + 1) % STAGES], sm.v[t % STAGES], st, lane, c, p, ahead);
       if (t >= t_masked) {
         uint64_t nf = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % STAGES][0]) |
                       (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % STAGES][1]) << 32;
@@ -219,7 +228,6 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
           if (at < lk) tile_nonfinite<NT>(vbase + 2 * a.v_tok * at, key, at, st, lane, p, lim);
         }
       }
-      tile_scores<NT>(sm.k[(t + 1) % STAGES], st, lane, c);
       // read by the other half for the last time a slot ago: group A clears what tile t + 2 will note
       if (tid < 2) sm.nonfinite[(t + 2) % STAGES][tid] = 0;
     }
