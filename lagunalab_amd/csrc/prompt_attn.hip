@@ -16,19 +16,19 @@
 //   2t      Q.K^T(t), P.V(t-1)        softmax(t-1), copies K(t+2) V(t+1)
 //   2t+1    softmax(t), copies        Q.K^T(t), P.V(t-1)
 //
-// Where whole blocks would leave CUs idle
-// (short or few prompts behind long pasts) a block's tiles are cut into parts whose partial rows a second
-// launch merges.
-//
-// The blocks of a launch come as a list in the kernel's arguments, made on the host from the lengths,
-// longest first; the KV head is the fastest index, so that neighbouring workgroups (XCDs) hold different
-// heads and each XCD's L2 the K and V of few.
+// The work is dealt out in equal shares of tiles: the blocks of all sequences stand one behind the other, a
+// block costing its tiles and BLOCK_COST for its start and end, and a workgroup takes one share, which may
+// begin and end inside blocks. Parts of blocks go to the workspace and a second launch merges them. One
+// share per CU (several where they are long), so that every CU ends at the same time whatever the lengths
+// are: 2,048 rows, 32/8 heads, in whole blocks would be 32 tiles for the last workgroup and 1 for the
+// first. A workgroup finds its share by scanning the blocks of a sequence, a lane each; nothing of the
+// plan but the sequences' costs comes from the host. The KV head is the fastest index, so that neighbouring
+// workgroups (XCDs) hold different heads and each XCD's L2 the K and V of few.
 //
 // Keys that a row does not see reach it in no way: masked scores are -infinity, and an infinity or NaN in
 // V of a tile that is masked for some row of the block goes only to the rows that see its key (0 times it
 // would be NaN): such tiles are rare and take the two-pass form.
 #include <algorithm>
-#include <vector>
 
 #include "attn_tile.h"
 
@@ -40,17 +40,8 @@ using namespace attn;
 constexpr int PW = 8;          // waves per workgroup
 constexpr int NT = 2;          // 16-row tiles per wave
 constexpr int PROWS = 16 * NT * PW;
-constexpr int LIST = 768;      // blocks of one launch: kernel arguments are limited to 4 KB
-constexpr int MAX_PARTS = 63;
-
-// A block of a sequence (or part j of n of its tiles): seq | block << 6 | j << 20 | n << 26.
-struct Entry {
-  uint32_t x;
-  __host__ __device__ int seq() const { return x & 63; }
-  __host__ __device__ int block() const { return (x >> 6) & 16383; }
-  __host__ __device__ int part() const { return (x >> 20) & 63; }
-  __host__ __device__ int parts() const { return x >> 26; }
-};
+constexpr int BLOCK_COST = 4;  // of a block's start and end, in tiles
+constexpr int MIN_PART = 2;    // tiles of a block's part: nearer cuts move to the block's end
 
 struct PromptArgs {
   const uint16_t* q;
@@ -58,19 +49,97 @@ struct PromptArgs {
   const uint16_t* v;
   uint16_t* out;           // [rows, Hq, 128]
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
-  float* part_acc;         // [entries of the call x Hkv][256][128], of entries that are parts
-  float2* part_ml;
-  int Hkv, G;
+  float* part_acc;         // [2 x shares x Hkv][256][128] rows of parts: slot 0 of a share those of the block
+  float2* part_ml;         // that began in an earlier one, slot 1 of the block that goes on in a later one
+  int Hkv, G, nseq;
   FastDiv g;
   float sl2;
+  int64_t share;           // cost of a share; 0: a workgroup takes one whole block
+  int longest;             // tiles of the longest block
   int q_begin[LQ_MAX_SEQS + 1], k_begin[LQ_MAX_SEQS + 1];
-  Entry list[LIST];
+  int64_t cost[LQ_MAX_SEQS + 1];  // of the blocks before each sequence
 };
 
 // 64-key tiles that block blk of a sequence of R rows needs; base: row i sees keys <= base + i.
 __host__ __device__ __forceinline__ int block_tiles(int blk, int R, FastDiv g, int base) {
   const int last = base + (int)fdiv_u((uint32_t)min(blk * PROWS + PROWS - 1, R - 1), g);
   return last < 0 ? 0 : last / TKEYS + 1;
+}
+
+// A block and where its cost begins.
+struct Block {
+  int seq, blk, tiles;
+  int64_t begin;
+};
+__device__ __forceinline__ int seq_rows(const PromptArgs& a, int s) {
+  return (a.q_begin[s + 1] - a.q_begin[s]) * a.G;
+}
+__device__ __forceinline__ int seq_base(const PromptArgs& a, int s) {
+  return a.k_begin[s + 1] - a.k_begin[s] - (a.q_begin[s + 1] - a.q_begin[s]);
+}
+// The block that holds cost u (below the total): the sequence by a lane each, then its blocks 64 at a time.
+__device__ __forceinline__ Block find_block(const PromptArgs& a, int64_t u, int lane) {
+  const int64_t end = lane < a.nseq ? a.cost[lane + 1] : INT64_MAX;
+  const int s = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= u));
+  const int R = seq_rows(a, s), base = seq_base(a, s), nb = (R + PROWS - 1) / PROWS;
+  int64_t before = a.cost[s];
+  for (int i = 0;; i += 64) {
+    const int tiles = i + lane < nb ? block_tiles(i + lane, R, a.g, base) : 0;
+    const int c = i + lane < nb ? tiles + BLOCK_COST : 0;
+    int upto = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o, 64);
+      upto += lane >= o ? y : 0;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > u);
+    if (past || i + 64 >= nb) {
+      const int l = past ? __builtin_ctzll(past) : 0;
+      return {s, i + l, __builtin_amdgcn_readlane(tiles, l), before + __builtin_amdgcn_readlane(upto - c, l)};
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+// The block of rank x when all are in order of their tiles, most first: how many have at least n tiles is a
+// sum over the sequences, a lane each, and the largest n that more than x have is found by halving. Its cost
+// is counted from its own begin.
+__device__ __forceinline__ Block ranked_block(const PromptArgs& a, int x, int lane) {
+  const int sl = min(lane, a.nseq - 1);
+  const int R = lane < a.nseq ? seq_rows(a, sl) : 0, base = seq_base(a, sl), nb = (R + PROWS - 1) / PROWS;
+  auto from = [&](int n) {  // first block of the lane's sequence with at least n tiles (of nb: none)
+    const int64_t y = a.G * ((int64_t)TKEYS * (n - 1) - base);  // the row that has to be reached
+    return n <= 0 || y <= 0 ? 0 : y > R - 1 ? nb : (int)(y / PROWS);
+  };
+  auto wave_sum_i = [&](int v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+    return __builtin_amdgcn_readfirstlane(v);
+  };
+  int lo = 0, hi = a.longest + 1;  // all have lo, none has hi
+  int above = 0;                   // blocks with at least hi tiles
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, n = wave_sum_i(nb - from(mid));
+    if (n > x) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = n;
+    }
+  }
+  const int n = from(lo + 1) - from(lo);
+  int upto = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(upto, o, 64);
+    upto += lane >= o ? y : 0;
+  }
+  const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > x - above));
+  return {l, __builtin_amdgcn_readlane(from(lo), l) + x - above - __builtin_amdgcn_readlane(upto - n, l), lo, 0};
+}
+// The tile of a block at which a cut at cost u (anywhere) lies: not within MIN_PART of its ends.
+__device__ __forceinline__ int cut_tile(const Block& b, int64_t u) {
+  const int64_t t = u - b.begin - BLOCK_COST;
+  return t >= b.tiles ? b.tiles : t < MIN_PART ? 0 : t > b.tiles - MIN_PART ? b.tiles : (int)t;
 }
 
 constexpr int STAGES = 3;  // tiles of K and of V in LDS
@@ -80,22 +149,30 @@ struct PromptSmem {
   uint32_t nonfinite[STAGES][2];  // keys of a masked tile whose V holds an infinity or NaN
 };
 
-__global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArgs a, int first) {
+__global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArgs a) {
   __shared__ PromptSmem sm;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int share = blockIdx.x / a.Hkv, hk = blockIdx.x - share * a.Hkv;
+  Block b = a.share ? find_block(a, a.share * share, threadIdx.x & 63)
+                    : ranked_block(a, share, threadIdx.x & 63);
+  const int64_t u0 = a.share * share;  // 0 for a whole block
+  const int64_t u1 = a.share ? min(u0 + a.share, a.cost[a.nseq]) : b.tiles + BLOCK_COST;
+  for (bool more = true; more;) {
+  // re-read per block, so that no lane value made of it is kept across blocks
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool grp_a = wv < PW / 2;
   const int lc = lane & 15, lq4 = lane >> 4;
-  const int x = blockIdx.x / a.Hkv, hk = blockIdx.x - x * a.Hkv;
-  const Entry en = a.list[x];
-  if (en.parts() == 0) return;  // fills up a launch
-  const int s = en.seq(), blk = en.block();
+  const int s = b.seq, blk = b.blk;
   const int q0 = a.q_begin[s], lq = a.q_begin[s + 1] - q0;
   const int k0 = a.k_begin[s], lk = a.k_begin[s + 1] - k0;
   const int R = lq * a.G, base = lk - lq;
-  const int tiles = block_tiles(blk, R, a.g, base);
-  const int t0 = (int)((int64_t)tiles * en.part() / en.parts());
-  const int t1 = (int)((int64_t)tiles * (en.part() + 1) / en.parts());
+  const int tiles = b.tiles;
+  const int t0 = cut_tile(b, u0), t1 = cut_tile(b, u1);
+  // a block without a tile (rows without keys) belongs to the share that its begin lies in
+  const bool mine = t0 < t1 || (tiles == 0 && b.begin >= u0 && b.begin < u1);
+  if (mine) {
   const float scale = abs_scale(a.sl2);
   // tiles from here on are masked for some row of the block (or end behind the last key)
   const int low = base + (int)fdiv_u((uint32_t)(blk * PROWS), a.g);
@@ -151,6 +228,13 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
     }
   };
 
+  lds_barrier();  // the other half is done with the block before
+  if (t0 < t1) {  // out before the rows of q are asked for
+    copy_k(t0);
+    copy_k(t0 + 1);
+    copy_v(t0);
+  }
+
   // ---- the wave's rows
   const int f0 = blk * PROWS + 16 * NT * wv;
   TileRows<NT> st;
@@ -178,9 +262,6 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   };
   if (t0 < t1) {
     if (tid < 2 * STAGES) sm.nonfinite[tid >> 1][tid & 1] = 0;
-    copy_k(t0);
-    copy_k(t0 + 1);
-    copy_v(t0);
     asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     lds_barrier();
     if (!grp_a) {  // half a tile behind
@@ -236,12 +317,13 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   }
 
   // ---- rows out: dims 16 w + 4 lq4 + r
-  const int64_t prow = ((int64_t)(first + x) * a.Hkv + hk) * PROWS;
+  const bool part = t1 - t0 < tiles;
+  const int64_t prow = ((int64_t)(2 * share + (t0 == 0)) * a.Hkv + hk) * PROWS;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int f = f0 + 16 * nt + lc;
     if (f >= R) continue;
-    if (en.parts() > 1) {
+    if (part) {
       const int64_t pr = prow + 16 * (NT * wv + nt) + lc;
 #pragma unroll
       for (int w = 0; w < 8; ++w)
@@ -258,89 +340,100 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
           make_uint2(pack_bf2(st.o[nt][w][0] * inv, st.o[nt][w][1] * inv),
                      pack_bf2(st.o[nt][w][2] * inv, st.o[nt][w][3] * inv));
   }
-}
-
-// The parts of a block (consecutive entries) into output rows: 32 lanes x 4 dims per row, 8 rows per
-// workgroup.
-__global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptArgs a, int first) {
-  const int x = blockIdx.x / a.Hkv, hk = blockIdx.x - x * a.Hkv;
-  const Entry en = a.list[x];
-  if (en.parts() < 2 || en.part() != 0) return;
-  const int s = en.seq();
-  const int q0 = a.q_begin[s], R = (a.q_begin[s + 1] - q0) * a.G;
-  const int wrow = 8 * blockIdx.y + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
-  const int f = en.block() * PROWS + wrow;
-  if (f >= R) return;
-  float M = -INFINITY, den = 0.0f;
-  f4_t acc = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < en.parts(); ++j) {
-    const int64_t pr = ((int64_t)(first + x + j) * a.Hkv + hk) * PROWS + wrow;
-    const float2 ml = a.part_ml[pr];
-    const f4_t o = *reinterpret_cast<const f4_t*>(a.part_acc + pr * D + d);
-    const float mn = max_ieee(M, ml.x);
-    const float mr = mn == -INFINITY ? 0.0f : mn;
-    const float e0 = M == -INFINITY ? 0.0f : exp2_nonpos(M - mr);
-    const float e1 = ml.x == -INFINITY ? 0.0f : exp2_nonpos(ml.x - mr);
-    acc = acc * e0 + o * e1;
-    den = den * e0 + ml.y * e1;
-    M = mn;
   }
-  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-  const int i = (int)fdiv_u((uint32_t)f, a.g), head = f - i * a.G;
-  *reinterpret_cast<uint2*>(a.out + ((int64_t)(q0 + i) * a.Hkv * a.G + hk * a.G + head) * D + d) =
-      make_uint2(pack_bf2(acc[0] * inv, acc[1] * inv), pack_bf2(acc[2] * inv, acc[3] * inv));
-}
-
-struct PromptPlan {
-  std::vector<Entry> list;
-  bool split = false;
-};
-
-// The blocks of the call, longest first, cut into parts where whole blocks would not fill the CUs.
-// Returns an LQ_ status.
-int prompt_plan(const int32_t* q_lens, const int32_t* k_lens, int64_t nseq, int64_t Hkv, int64_t G,
-                int cus, PromptPlan* plan) {
-  struct Block {
-    int tiles, seq, blk;
-  };
-  const FastDiv g = make_fastdiv((uint32_t)G);
-  std::vector<Block> blocks;
-  int64_t total = 0;
-  int longest = 0;
-  for (int s = 0; s < nseq; ++s) {
-    const int64_t R = (int64_t)q_lens[s] * G;
-    LQ_CHECK_ARG((R + PROWS - 1) / PROWS <= 16384, "%d query rows of one sequence are too many",
-                 (int)q_lens[s]);
-    for (int b = 0; b * PROWS < R; ++b) {
-      const int t = block_tiles(b, (int)R, g, k_lens[s] - q_lens[s]);
-      blocks.push_back({t, s, b});
-      total += t;
-      longest = std::max(longest, t);
+  // the next block
+  const int64_t next = b.begin + b.tiles + BLOCK_COST;
+  more = next < u1;
+  if (more) {
+    int ns = b.seq, nblk = b.blk + 1;
+    if (nblk * PROWS >= R) {
+      nblk = 0;
+      do ++ns;
+      while (a.cost[ns + 1] == a.cost[ns]);  // sequences without rows cost nothing
     }
+    b = Block{ns, nblk, block_tiles(nblk, seq_rows(a, ns), a.g, seq_base(a, ns)), next};
   }
-  // a CU's equal share of the tiles, as the size of a part
-  const int64_t share = std::max<int64_t>(4, (total * Hkv + cus - 1) / cus);
-  plan->split = longest > share + share / 4;
-  auto parts = [&](int t) {
-    return plan->split ? (int)std::min<int64_t>(MAX_PARTS, std::max<int64_t>(1, (t + share - 1) / share))
-                       : 1;
-  };
-  std::stable_sort(blocks.begin(), blocks.end(), [&](const Block& x, const Block& y) {
-    return x.tiles * parts(y.tiles) > y.tiles * parts(x.tiles);
-  });
-  for (const Block& b : blocks) {
-    const int n = parts(b.tiles);
-    // a block's parts stay in one launch
-    if ((int)(plan->list.size() % LIST) + n > LIST)
-      while (plan->list.size() % LIST) plan->list.push_back({0u});
-    for (int j = 0; j < n; ++j)
-      plan->list.push_back({(uint32_t)b.seq | (uint32_t)b.blk << 6 | (uint32_t)j << 20 | (uint32_t)n << 26});
   }
-  return LQ_OK;
+}
+
+constexpr int MERGE_ROWS = 32;  // of a workgroup
+// The parts of a block into output rows, by the workgroups of its first cut: share j's end. 32 lanes x 4
+// dims per row, 8 rows at a time.
+__global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptArgs a) {
+  const int j = blockIdx.x / a.Hkv, hk = blockIdx.x - j * a.Hkv;
+  const int64_t u = a.share * (j + 1);
+  const Block b = find_block(a, u, threadIdx.x & 63);
+  const int t = cut_tile(b, u);
+  if (t == 0 || t == b.tiles || cut_tile(b, u - a.share) != 0) return;  // no cut, or not its first
+  const int R = seq_rows(a, b.seq);
+  const int d = 4 * (threadIdx.x & 31);
+  int n = 1;  // parts
+  while (cut_tile(b, u + n * a.share - a.share) < b.tiles) ++n;
+#pragma unroll 1
+  for (int i = 0; i < MERGE_ROWS / 8; ++i) {
+    const int wrow = MERGE_ROWS * blockIdx.y + 8 * i + (threadIdx.x >> 5);
+    const int f = b.blk * PROWS + wrow;
+    if (f >= R) return;
+    float M = -INFINITY, den = 0.0f;
+    f4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k = 0; k < n; ++k) {
+      const int64_t pr = ((int64_t)(2 * (j + k) + (k == 0)) * a.Hkv + hk) * PROWS + wrow;
+      const float2 ml = a.part_ml[pr];
+      const f4_t o = *reinterpret_cast<const f4_t*>(a.part_acc + pr * D + d);
+      const float mn = max_ieee(M, ml.x);
+      const float mr = mn == -INFINITY ? 0.0f : mn;
+      const float e0 = M == -INFINITY ? 0.0f : exp2_nonpos(M - mr);
+      const float e1 = ml.x == -INFINITY ? 0.0f : exp2_nonpos(ml.x - mr);
+      acc = acc * e0 + o * e1;
+      den = den * e0 + ml.y * e1;
+      M = mn;
+    }
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    const int p = (int)fdiv_u((uint32_t)f, a.g), head = f - p * a.G;
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)(a.q_begin[b.seq] + p) * a.Hkv * a.G + hk * a.G + head) * D + d) =
+        make_uint2(pack_bf2(acc[0] * inv, acc[1] * inv), pack_bf2(acc[2] * inv, acc[3] * inv));
+  }
+}
+
+// Cost of the blocks of every sequence, and the share of a workgroup: one per CU. Where there are
+// WHOLE_ROUNDS blocks and more for each CU they are taken whole instead, longest first: then the last
+// round evens itself out, nothing is merged, and the workgroups of a head walk its keys together, which the
+// L2 likes (16,384 rows, 32/8 heads, 8 blocks per CU: 1,825 us whole, 2,040 in shares; 2,048 rows, one
+// block per CU: see above).
+constexpr int64_t WHOLE_ROUNDS = 6;
+struct PromptPlan {
+  int64_t cost[LQ_MAX_SEQS + 1], share, shares;  // share 0: whole blocks, `shares` of them
+  int longest;
+};
+PromptPlan prompt_plan(const int32_t* q_lens, const int32_t* k_lens, int64_t nseq, int64_t Hkv, int64_t G,
+                       int cus) {
+  PromptPlan p{};
+  const FastDiv g = make_fastdiv((uint32_t)G);
+  int64_t blocks = 0;
+  for (int s = 0; s < LQ_MAX_SEQS; ++s) {
+    int64_t c = 0;
+    const int R = s < nseq ? (int)(q_lens[s] * G) : 0;
+    for (int b = 0; (int64_t)b * PROWS < R; ++b) {
+      const int t = block_tiles(b, R, g, k_lens[s] - q_lens[s]);
+      p.longest = std::max(p.longest, t);
+      c += t + BLOCK_COST;
+      ++blocks;
+    }
+    p.cost[s + 1] = p.cost[s] + c;
+  }
+  if (blocks * Hkv >= WHOLE_ROUNDS * cus) {
+    p.shares = blocks;
+    return p;
+  }
+  const int64_t total = p.cost[nseq], per_head = std::max<int64_t>(1, cus / Hkv);
+  p.share = std::max<int64_t>(BLOCK_COST + MIN_PART, (total + per_head - 1) / per_head);
+  p.shares = (total + p.share - 1) / p.share;
+  return p;
 }
 
 int64_t prompt_bytes(const PromptPlan& p, int64_t Hkv) {
-  return p.split ? (int64_t)p.list.size() * Hkv * PROWS * (int64_t)(D * sizeof(float) + sizeof(float2)) : 0;
+  return p.share && p.shares > 1 ? 2 * p.shares * Hkv * PROWS * (int64_t)(D * sizeof(float) + sizeof(float2)) : 0;
 }
 
 int check_prompt(int64_t Hq, int64_t Hkv, int64_t D, const int32_t* q_lens, const int32_t* k_lens,
@@ -355,6 +448,8 @@ int check_prompt(int64_t Hq, int64_t Hkv, int64_t D, const int32_t* q_lens, cons
   for (int s = 0; s < nseq; ++s) {
     LQ_CHECK_ARG(q_lens[s] >= 0 && k_lens[s] >= 0 && q_lens[s] <= (1 << 24) && k_lens[s] <= (1 << 24),
                  "sequence %d has %d rows and %d keys (at most 2^24)", s, (int)q_lens[s], (int)k_lens[s]);
+    LQ_CHECK_ARG((int64_t)q_lens[s] * (Hq / Hkv) < (1 << 30), "%d rows of one sequence are too many",
+                 (int)q_lens[s]);
     tq += q_lens[s];
     tk += k_lens[s];
   }
@@ -370,14 +465,7 @@ extern "C" int64_t lq_prompt_workspace_bytes(const int32_t* q_lens_host, const i
   using namespace lq;
   clear_error();
   if (check_prompt(Hq, Hkv, 128, q_lens_host, k_lens_host, nseq)) return -1;
-  try {
-    PromptPlan plan;
-    if (prompt_plan(q_lens_host, k_lens_host, nseq, Hkv, Hq / Hkv, device_cu_count(), &plan)) return -1;
-    return prompt_bytes(plan, Hkv);
-  } catch (...) {
-    set_error("no host memory for the plan");
-    return -1;
-  }
+  return prompt_bytes(prompt_plan(q_lens_host, k_lens_host, nseq, Hkv, Hq / Hkv, device_cu_count()), Hkv);
 }
 
 extern "C" int lq_prompt_attn(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t q_tok,
@@ -401,56 +489,48 @@ extern "C" int lq_prompt_attn(const uint16_t* q, const uint16_t* k, const uint16
   LQ_CHECK_ARG(k_tok >= 0 && v_tok >= 0 && k_tok < (1 << 24) && v_tok < (1 << 24),
                "rows of k or v 2^24 values apart or more");
   LQ_CHECK_ARG(std::isfinite(scale), "the softmax scale is not finite");
+  const PromptPlan plan = prompt_plan(q_lens_host, k_lens_host, nseq, Hkv, Hq / Hkv, device_cu_count());
+  const int64_t need = prompt_bytes(plan, Hkv);
+  if (need > 0 && (!workspace || workspace_bytes < need)) {
+    set_error("workspace of %lld bytes is smaller than the %lld needed", (long long)workspace_bytes,
+              (long long)need);
+    return LQ_EWORKSPACE;
+  }
+  LQ_CHECK_ARG(plan.shares * Hkv <= INT32_MAX, "too many workgroups");
+  LQ_CHECK_ARG(need == 0 || ((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
   PromptArgs a;
-  std::vector<Entry> list;
-  try {
-    PromptPlan plan;
-    if (const int st = prompt_plan(q_lens_host, k_lens_host, nseq, Hkv, Hq / Hkv, device_cu_count(), &plan))
-      return st;
-    const int64_t need = prompt_bytes(plan, Hkv);
-    if (need > 0 && (!workspace || workspace_bytes < need)) {
-      set_error("workspace of %lld bytes is smaller than the %lld needed", (long long)workspace_bytes,
-                (long long)need);
-      return LQ_EWORKSPACE;
-    }
-    LQ_CHECK_ARG(need == 0 || ((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
-    a.part_acc = (float*)workspace;
-    a.part_ml = need ? (float2*)(a.part_acc + (int64_t)plan.list.size() * Hkv * PROWS * 128) : nullptr;
-    list.swap(plan.list);
-    a.q = q;
-    a.k = k;
-    a.v = v;
-    a.out = out;
-    a.q_tok = q_tok;
-    a.q_head = q_head;
-    a.k_tok = k_tok;
-    a.k_head = k_head;
-    a.v_tok = v_tok;
-    a.v_head = v_head;
-    a.Hkv = (int)Hkv;
-    a.G = (int)(Hq / Hkv);
-    a.g = make_fastdiv((uint32_t)a.G);
-    a.sl2 = scale * 1.4426950408889634f;
-    a.q_begin[0] = a.k_begin[0] = 0;
-    for (int s = 0; s < LQ_MAX_SEQS; ++s) {
-      a.q_begin[s + 1] = a.q_begin[s] + (s < nseq ? q_lens_host[s] : 0);
-      a.k_begin[s + 1] = a.k_begin[s] + (s < nseq ? k_lens_host[s] : 0);
-    }
-    const bool split = plan.split;
-    for (size_t at = 0; at < list.size(); at += LIST) {
-      const int n = (int)std::min<size_t>(LIST, list.size() - at);
-      for (int i = 0; i < LIST; ++i) a.list[i] = i < n ? list[at + i] : Entry{0u};
-      prompt_attn_kernel<<<dim3((unsigned)(n * Hkv)), dim3(64 * PW), 0, (hipStream_t)stream>>>(a, (int)at);
-      LQ_CHECK_LAUNCH("prompt_attn_kernel");
-      if (split) {
-        prompt_merge_kernel<<<dim3((unsigned)(n * Hkv), PROWS / 8), dim3(256), 0, (hipStream_t)stream>>>(
-            a, (int)at);
-        LQ_CHECK_LAUNCH("prompt_merge_kernel");
-      }
-    }
-  } catch (...) {
-    set_error("no host memory for the plan");
-    return LQ_EHIP;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.q_tok = q_tok;
+  a.q_head = q_head;
+  a.k_tok = k_tok;
+  a.k_head = k_head;
+  a.v_tok = v_tok;
+  a.v_head = v_head;
+  a.part_acc = (float*)workspace;
+  a.part_ml = need ? (float2*)(a.part_acc + 2 * plan.shares * Hkv * PROWS * lq::D) : nullptr;
+  a.Hkv = (int)Hkv;
+  a.G = (int)(Hq / Hkv);
+  a.nseq = (int)nseq;
+  a.g = make_fastdiv((uint32_t)a.G);
+  a.sl2 = scale * 1.4426950408889634f;
+  a.share = plan.share;
+  a.longest = plan.longest;
+  a.q_begin[0] = a.k_begin[0] = 0;
+  for (int s = 0; s < LQ_MAX_SEQS; ++s) {
+    a.q_begin[s + 1] = a.q_begin[s] + (s < nseq ? q_lens_host[s] : 0);
+    a.k_begin[s + 1] = a.k_begin[s] + (s < nseq ? k_lens_host[s] : 0);
+    a.cost[s] = plan.cost[s];
+  }
+  a.cost[LQ_MAX_SEQS] = plan.cost[LQ_MAX_SEQS];
+  prompt_attn_kernel<<<dim3((unsigned)(plan.shares * Hkv)), dim3(64 * PW), 0, (hipStream_t)stream>>>(a);
+  LQ_CHECK_LAUNCH("prompt_attn_kernel");
+  if (need > 0) {
+    prompt_merge_kernel<<<dim3((unsigned)((plan.shares - 1) * Hkv), PROWS / MERGE_ROWS), dim3(256), 0,
+                          (hipStream_t)stream>>>(a);
+    LQ_CHECK_LAUNCH("prompt_merge_kernel");
   }
   return LQ_OK;
 }
