@@ -3,20 +3,21 @@
 //
 // Work. A KV head's shared pages are cut into np parts; a workgroup takes one part for a block of 64 or
 // 128 query rows (the G rows of each sequence, one sequence behind the other), dequantizes each page
-// once into LDS and runs the matrix-core tile of attn_tile.h on it. A sequence's own pages are cut into
-// chunks; a workgroup takes one chunk for the sequence's G <= 16 rows, one page per wave at a time, K
-// straight from memory into MFMA operands, V transposed through the wave's own LDS. Both kinds write
+// once into LDS and runs the matrix-core tile of attn_tile.h on it. The sequences' own pages, one sequence
+// behind the other, are dealt out to the workgroups in equal shares; a workgroup runs its pages of a sequence
+// for the G <= 16 rows, one page per wave at a time, through the wave's own LDS (no barriers), the next
+// page's loads out while it computes. Both kinds write
 // partial rows (max, sum, weighted values), which a second launch merges.
 //
 // Lengths are read on the device, so one recorded launch serves every step of a growing batch: every
-// workgroup adds up the sequences' own pages, takes the chunk size that splits them over the workgroups
-// that fill the GPU, and finds its own chunk. Workgroups without one leave at once.
+// workgroup adds up the sequences' own pages and finds its share of them. Workgroups without one leave at
+// once.
 //
 // Values: an attended K or V is bf16(scale * code + bias), what dequantizing the page gives; products on
 // bf16 operands with fp32 sums, P rounded to bf16. Positions past a length are not attended whatever
 // their slots hold: their scores are -infinity and their V terms 0. A length outside [0, 64 width] or a
 // page outside the pool makes the sequence's rows NaN; length 0 makes them 0. A sequence shorter than the
-// shared part takes no part in it: its own chunks cover it whole.
+// shared part takes no part in it: its own parts cover it whole.
 #include "attn_tile.h"
 #include "paged.h"
 
@@ -26,21 +27,20 @@ namespace {
 using namespace attn;
 
 constexpr int DW = 4;         // waves per workgroup
-constexpr int CHUNK_MIN = 4;  // pages of a sequence's chunk: one per wave
-constexpr int WAVE_V = PAGE * D;
+constexpr int SHARE_MIN = 4;  // pages of a share: one per wave
 
 struct PagedArgs {
   const uint16_t* q;
   PagedBufs buf;
   PageTable tab;
   const int32_t* lens;
-  float* part_acc;    // [Hkv][slots][128], slots: own chunks x G, then np x rows of all sequences
+  float* part_acc;    // [Hkv][slots][128], slots: (share + sequence) x G, then np x rows of all
   float2* part_ml;
   uint16_t* out;
   int B, Hkv, G;
   int shared;         // pages that all sequences share
   int np, rb;         // their parts, blocks of query rows
-  int target;         // own chunks of a KV head that fill the GPU
+  int shares;         // workgroups for the own pages of a KV head
   float sl2;          // softmax scale, log2 units
 };
 
@@ -69,46 +69,39 @@ __device__ __forceinline__ int wave_scan_i(int x, int lane) {  // inclusive
   return x;
 }
 
-// Pages per own chunk: the same in every workgroup of a call.
-__device__ __forceinline__ int chunk_pages(const PagedArgs& a, int lane) {
-  int total = 0;
-  for (int i = lane; i < a.B; i += 64) total += own_pages(a, a.lens[i]);
-  total = wave_sum_i(total);
-  return max(CHUNK_MIN, (total + a.target - 1) / a.target);
+// Pages of a share: the same in every workgroup of a call.
+__device__ __forceinline__ int share_pages(const PagedArgs& a, int total) {
+  return max(SHARE_MIN, (total + a.shares - 1) / a.shares);
 }
 
 struct OwnSmem {
-  alignas(16) uint8_t v[DW][WAVE_V];  // a page's V codes, 16-byte chunk c of row r at c ^ vswz(r)
-  uint32_t w[DW][2][PAGE];            // its scale and bias words
+  // a page's codes, per wave: 16-byte chunk c of row r of K at c ^ kswz(r), of V at c ^ vswz(r)
+  alignas(16) uint8_t k[DW][PAGE * D], v[DW][PAGE * D];
+  uint32_t w[DW][4][PAGE];  // its K scale, K bias, V scale, V bias words
   float2 ml[DW][16];
 };
-// A page's operands on their way: K of keys 16 mt + lc (16 codes at dims 16 lq4 and 64 + 16 lq4), its
-// words, V rows 8 i + lane / 8, the words of V row `lane`.
+// A page on its way: rows 8 i + lane / 8 of K and V, the words of row `lane`. Read once: non-temporal (8
+// sessions of 42,771 to 82,671 rows 244 -> 229 us), in whole lines (K as MFMA operands straight from memory
+// takes half lines: 220 -> 238).
 struct PageRegs {
-  uint4 k[4][2], v[8];
-  uint32_t ks[4], kb[4], vs, vb;
+  u4_t k[8], v[8];
+  uint32_t w[4];
 };
 
 __device__ __forceinline__ void load_page(const PagedArgs& a, int64_t row, int lane, PageRegs& p) {
-  const int lc = lane & 15, lq4 = lane >> 4;
-  const uint8_t* kc = a.buf.kc + row * D;
-  const uint8_t* vc = a.buf.vc + row * D;
-  const uint32_t* ks = reinterpret_cast<const uint32_t*>(a.buf.ks) + row;
-  const uint32_t* kb = reinterpret_cast<const uint32_t*>(a.buf.kb) + row;
+  const u4_t* k = reinterpret_cast<const u4_t*>(a.buf.kc + row * D) + lane;
+  const u4_t* v = reinterpret_cast<const u4_t*>(a.buf.vc + row * D) + lane;
 #pragma unroll
-  for (int mt = 0; mt < 4; ++mt) {
+  for (int i = 0; i < 8; ++i) p.k[i] = __builtin_nontemporal_load(k + 64 * i);
+  p.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(a.buf.ks) + row + lane);
+  p.w[1] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(a.buf.kb) + row + lane);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      p.k[mt][h] = *reinterpret_cast<const uint4*>(kc + (16 * mt + lc) * D + 64 * h + 16 * lq4);
-    p.ks[mt] = ks[16 * mt + lc];
-    p.kb[mt] = kb[16 * mt + lc];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) p.v[i] = *reinterpret_cast<const uint4*>(vc + 1024 * i + 16 * lane);
-  p.vs = reinterpret_cast<const uint32_t*>(a.buf.vs)[row + lane];
-  p.vb = reinterpret_cast<const uint32_t*>(a.buf.vb)[row + lane];
+  for (int i = 0; i < 8; ++i) p.v[i] = __builtin_nontemporal_load(v + 64 * i);
+  p.w[2] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(a.buf.vs) + row + lane);
+  p.w[3] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(a.buf.vb) + row + lane);
 }
 
+__device__ __forceinline__ int kswz(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int vswz(int r) { return (r & 3) | ((r >> 2) & 4); }
 
 __device__ __forceinline__ void wave_fence() {  // LDS of the wave's own: order across its lanes
@@ -117,12 +110,13 @@ __device__ __forceinline__ void wave_fence() {  // LDS of the wave's own: order 
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A sequence's chunk [p0, p1) of pages for its G rows.
-__device__ __forceinline__ void own_chunk(const PagedArgs& a, OwnSmem& sm, int b, int hk, int p0, int p1,
+// Pages [p0, p1) of a sequence for its G rows.
+__device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, int b, int hk, int p0, int p1,
                                           int len, int64_t slot) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 15, lq4 = lane >> 4;
+  __syncthreads();  // the sequence before is written
   const int32_t* ids = a.tab.ids + b * a.tab.stride;
   const float scale = abs_scale(a.sl2);
   const int64_t qrow = ((int64_t)b * a.Hkv + hk) * a.G;
@@ -153,35 +147,39 @@ __device__ __forceinline__ void own_chunk(const PagedArgs& a, OwnSmem& sm, int b
   if (p < p1) load_page(a, page_row(p), lane, cur);
   for (; p < p1; p += DW) {
     const int limit = min(PAGE, len - p * PAGE);  // keys of the page that are the sequence's
-    // V to LDS; words of keys past the length 0, so that their slots' contents reach nothing
+    // to LDS, and the next page's loads out at once; V words of keys past the length 0, so that their
+    // slots' contents reach nothing
     wave_fence();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int r = 8 * i + (lane >> 3);
-      reinterpret_cast<uint4*>(sm.v[wv])[8 * r + ((lane & 7) ^ vswz(r))] = cur.v[i];
+      const int r = 8 * i + (lane >> 3), c = lane & 7;
+      reinterpret_cast<u4_t*>(sm.k[wv])[8 * r + (c ^ kswz(r))] = cur.k[i];
+      reinterpret_cast<u4_t*>(sm.v[wv])[8 * r + (c ^ vswz(r))] = cur.v[i];
     }
-    sm.w[wv][0][lane] = lane < limit ? cur.vs : 0u;
-    sm.w[wv][1][lane] = lane < limit ? cur.vb : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sm.w[wv][i][lane] = i < 2 || lane < limit ? cur.w[i] : 0u;
+    if (p + DW < p1) load_page(a, page_row(p + DW), lane, cur);
+    wave_fence();
     // scores
     f4_t c[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       c[mt] = f4_t{0.f, 0.f, 0.f, 0.f};
+      const int key = 16 * mt + lc;
+      const uint32_t sw = sm.w[wv][0][key], zw = sm.w[wv][1][key];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float s = h ? bf16_hi(cur.ks[mt]) : bf16_lo(cur.ks[mt]);
-        const float z = h ? bf16_hi(cur.kb[mt]) : bf16_lo(cur.kb[mt]);
-        const uint4 w = cur.k[mt][h];
-        const uint2 d0 = dequant4(w.x, s, z), d1 = dequant4(w.y, s, z);
-        const uint2 d2 = dequant4(w.z, s, z), d3 = dequant4(w.w, s, z);
+        const float s = h ? bf16_hi(sw) : bf16_lo(sw), z = h ? bf16_hi(zw) : bf16_lo(zw);
+        const u4_t w = reinterpret_cast<const u4_t*>(sm.k[wv])[8 * key + ((lq4 + 4 * h) ^ kswz(lc))];
+        const uint2 d0 = dequant4(w[0], s, z), d1 = dequant4(w[1], s, z);
+        const uint2 d2 = dequant4(w[2], s, z), d3 = dequant4(w[3], s, z);
         c[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words_as_bf8(d0.x, d0.y, d1.x, d1.y), qf[2 * h],
                                                         c[mt], 0, 0, 0);
         c[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words_as_bf8(d2.x, d2.y, d3.x, d3.y),
                                                         qf[2 * h + 1], c[mt], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const int pn = p + DW;
-    if (pn < p1) load_page(a, page_row(pn), lane, cur);
     if (limit < PAGE) {
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
@@ -217,7 +215,6 @@ __device__ __forceinline__ void own_chunk(const PagedArgs& a, OwnSmem& sm, int b
       pw[2 * mt] = pack_bf2(e[0], e[1]);
       pw[2 * mt + 1] = pack_bf2(e[2], e[3]);
     }
-    wave_fence();
     // values: lane (lq4, lc) gets the codes of keys 32 e + 16 h + 4 lq4 + r at dim 16 w + lc
     const int skey = 4 * lq4 + 16 * (lc >> 3) + ((lc >> 1) & 3);  // this lane's source key
     const uint8_t* src = sm.v[wv] + skey * D + 8 * (lc & 1);
@@ -225,10 +222,10 @@ __device__ __forceinline__ void own_chunk(const PagedArgs& a, OwnSmem& sm, int b
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const bf16x8_t pe = words_as_bf8(pw[4 * e], pw[4 * e + 1], pw[4 * e + 2], pw[4 * e + 3]);
-      const uint4 s0 = *reinterpret_cast<const uint4*>(&sm.w[wv][0][32 * e + 4 * lq4]);
-      const uint4 s1 = *reinterpret_cast<const uint4*>(&sm.w[wv][0][32 * e + 4 * lq4 + 16]);
-      const uint4 z0 = *reinterpret_cast<const uint4*>(&sm.w[wv][1][32 * e + 4 * lq4]);
-      const uint4 z1 = *reinterpret_cast<const uint4*>(&sm.w[wv][1][32 * e + 4 * lq4 + 16]);
+      const uint4 s0 = *reinterpret_cast<const uint4*>(&sm.w[wv][2][32 * e + 4 * lq4]);
+      const uint4 s1 = *reinterpret_cast<const uint4*>(&sm.w[wv][2][32 * e + 4 * lq4 + 16]);
+      const uint4 z0 = *reinterpret_cast<const uint4*>(&sm.w[wv][3][32 * e + 4 * lq4]);
+      const uint4 z1 = *reinterpret_cast<const uint4*>(&sm.w[wv][3][32 * e + 4 * lq4 + 16]);
       const uint32_t sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
       const uint32_t zw[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
 #pragma unroll
@@ -247,6 +244,7 @@ __device__ __forceinline__ void own_chunk(const PagedArgs& a, OwnSmem& sm, int b
             words_as_bf8(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]),
                          pack_bf2(v[6], v[7])),
             pe, o[w], 0, 0, 0);
+        if (w & 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -381,9 +379,9 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
   }
 }
 
-// Partial rows of one KV head: own chunks first.
+// Partial rows of one KV head: own parts first. Along the shares and sequences each part adds one to their sum.
 __device__ __forceinline__ int64_t head_slots(const PagedArgs& a) {
-  return (int64_t)(a.target + a.B) * a.G + (int64_t)a.np * a.B * a.G;
+  return (int64_t)(a.shares + a.B) * a.G + (int64_t)a.np * a.B * a.G;
 }
 
 template <int NT>  // 16-row tiles of a wave in the shared part; 0: nothing is shared
@@ -409,7 +407,7 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
         if (joins) {
           shared_part<NT>(a, sm.tile, a.tab.ids + (i + __builtin_ctzll(joins)) * a.tab.stride, hk, p0, p1,
                           block * 64 * NT,
-                          slot0 + (int64_t)(a.target + a.B) * a.G + (int64_t)part * a.B * a.G);
+                          slot0 + (int64_t)(a.shares + a.B) * a.G + (int64_t)part * a.B * a.G);
           return;
         }
       }
@@ -417,24 +415,32 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
     }
     x -= a.np * a.rb;
   }
-  // own chunk x of this KV head
-  const int C = chunk_pages(a, lane);
-  int before = 0;
-  for (int i = 0; i < a.B; i += 64) {
-    const int len = i + lane < a.B ? a.lens[i + lane] : 0;
-    const int n = (own_pages(a, len) + C - 1) / C;
-    const int upto = before + wave_scan_i(n, lane);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > x);
-    if (past) {
-      const int src = __builtin_ctzll(past);
-      const int blen = __builtin_amdgcn_readlane(len, src);
-      const int first = __builtin_amdgcn_readlane(upto - n, src);
-      const int p0 = own_first(a, blen) + (x - first) * C;
-      const int p1 = min(p0 + C, (blen + PAGE - 1) / PAGE);
-      own_chunk(a, sm.own, i + src, hk, p0, p1, blen, slot0 + (int64_t)x * a.G);
-      return;
+  // share x of the own pages of this KV head
+  int total = 0;
+  for (int i = lane; i < a.B; i += 64) total += own_pages(a, a.lens[i]);
+  total = wave_sum_i(total);
+  const int S = share_pages(a, total), u0 = x * S, u1 = min(u0 + S, total);
+  if (u0 >= u1) return;
+  int b = 0, begin = 0;  // the sequence that holds page u0, and the pages before it
+  for (int i = 0;; i += 64) {
+    const int n = i + lane < a.B ? own_pages(a, a.lens[i + lane]) : 0;
+    const int upto = begin + wave_scan_i(n, lane);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > u0);
+    if (past || i + 64 >= a.B) {
+      const int src = past ? __builtin_ctzll(past) : 0;
+      b = i + src;
+      begin = __builtin_amdgcn_readlane(upto - n, src);
+      break;
     }
-    before = __builtin_amdgcn_readlane(upto, 63);
+    begin = __builtin_amdgcn_readlane(upto, 63);
+  }
+  for (int u = u0; u < u1; ++b) {
+    const int len = a.lens[b], n = own_pages(a, len);
+    if (n == 0) continue;
+    const int e = min(u1, begin + n), first = own_first(a, len) - begin;
+    own_part(a, sm.own, b, hk, first + u, first + e, len, slot0 + (int64_t)(x + b) * a.G);
+    begin += n;
+    u = e;
   }
 }
 
@@ -444,16 +450,23 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (row >= a.B * a.Hkv * a.G) return;
   const int b = row / (a.Hkv * a.G), h = row - b * a.Hkv * a.G, hk = h / a.G, g = h - hk * a.G;
-  const int C = chunk_pages(a, lane);
-  int first = 0;
-  for (int i = lane; i < b; i += 64) first += (own_pages(a, a.lens[i]) + C - 1) / C;
-  first = wave_sum_i(first);
+  int before = 0, total = 0;
+  for (int i = lane; i < a.B; i += 64) {
+    const int n = own_pages(a, a.lens[i]);
+    before += i < b ? n : 0;
+    total += n;
+  }
+  before = wave_sum_i(before);
+  total = wave_sum_i(total);
+  const int S = share_pages(a, total);
   const int len = a.lens[b];
-  const int n = (own_pages(a, len) + C - 1) / C;
+  const int pages = own_pages(a, len);
+  const int first = before / S;
+  const int n = pages ? (before + pages - 1) / S - first + 1 : 0;  // shares that hold own pages
   const bool joins = len_ok(a, len) && a.shared > 0 && len >= a.shared * PAGE;
   const int64_t slot0 = hk * head_slots(a);
-  const int64_t own0 = slot0 + (int64_t)first * a.G + g;
-  const int64_t sh0 = slot0 + (int64_t)(a.target + a.B) * a.G + (int64_t)b * a.G + g;
+  const int64_t own0 = slot0 + (int64_t)(first + b) * a.G + g;
+  const int64_t sh0 = slot0 + (int64_t)(a.shares + a.B) * a.G + (int64_t)b * a.G + g;
   const int parts = n + (joins ? a.np : 0);
   const int d = 4 * (lane & 31);
   float M = -INFINITY, den = 0.0f;
@@ -491,7 +504,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 }
 
 struct DecodeShape {
-  int np, rb, target, nt;
+  int np, rb, shares, nt;
   int64_t slots;  // partial rows, all heads
 };
 
@@ -503,8 +516,8 @@ DecodeShape decode_shape(int64_t B, int64_t Hkv, int64_t G, int64_t shared, int 
     s.rb = (int)((B * G + 64 * s.nt - 1) / (64 * s.nt));
     s.np = (int)std::min<int64_t>((shared + 3) / 4, std::max<int64_t>(1, fill / (Hkv * s.rb)));
   }
-  s.target = (int)std::max<int64_t>(1, fill / Hkv);
-  s.slots = Hkv * G * (s.target + B + s.np * B);
+  s.shares = (int)std::max<int64_t>(1, fill / Hkv);
+  s.slots = Hkv * G * (s.shares + B + s.np * B);
   return s;
 }
 
@@ -558,7 +571,7 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
     return LQ_EWORKSPACE;
   }
   LQ_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
-  const int64_t wgs = Hkv * ((int64_t)s.np * s.rb + s.target + B);
+  const int64_t wgs = Hkv * ((int64_t)s.np * s.rb + s.shares + B);
   LQ_CHECK_ARG(wgs <= INT32_MAX, "too many workgroups");
   a.lens = lens;
   a.part_acc = (float*)workspace;
@@ -570,7 +583,7 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
   a.shared = (int)shared_pages;
   a.np = s.np;
   a.rb = s.rb;
-  a.target = s.target;
+  a.shares = s.shares;
   a.sl2 = scale * 1.4426950408889634f;
   auto* kern = s.nt == 2 ? paged_decode_kernel<2> : s.nt == 1 ? paged_decode_kernel<1> : paged_decode_kernel<0>;
   kern<<<dim3((unsigned)wgs), dim3(64 * DW), 0, (hipStream_t)stream>>>(a);
