@@ -302,8 +302,8 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
   const float scale = abs_scale(a.sl2);
   const int key0 = tid >> 3, chunk = tid & 7;
   bool bad = false;
-  RawPage raw;
-  auto load = [&](int p) {
+  RawPage pre[2];  // pages p + 1 and p + 2
+  auto load = [&](int p, RawPage& raw) {
     const int id = __builtin_amdgcn_readfirstlane(ids[p]);
     const bool ok = id >= 0 && id < a.tab.pages;
     bad |= !ok;
@@ -320,7 +320,7 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
     }
   };
   auto pick = [&](uint32_t w) { return chunk < 4 ? bf16_lo(w) : bf16_hi(w); };
-  auto stage = [&](KvTile& t) {
+  auto stage = [&](KvTile& t, const RawPage& raw) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int key = key0 + 32 * i;
@@ -336,7 +336,8 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
       *v_chunk(t, key, 2 * chunk + 1) = make_uint4(v2.x, v2.y, v3.x, v3.y);
     }
   };
-  load(p0);
+  load(p0, pre[0]);
+  load(min(p0 + 1, p1 - 1), pre[1]);
   TileRows<NT> st;
   st.clear();
 #pragma unroll
@@ -351,21 +352,24 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
       st.q[nt][kk] = u4_as_bf8(signed_q(u, a.sl2));
     }
   }
-  stage(sm[0]);
-  if (p0 + 1 < p1) load(p0 + 1);
+  stage(sm[0], pre[0]);
+  load(min(p0 + 2, p1 - 1), pre[0]);
   __syncthreads();
-  for (int p = p0; p < p1; ++p) {
-    const int s = (p - p0) & 1;
-    f4_t c[NT][4];
-    bf16x8_t pr[NT][2];
-    tile_scores<NT>(sm[s].k, st, lane, c);
-    tile_softmax<NT>(c, st, scale, pr);
-    tile_values<NT>(sm[s].v, st, lane, pr);
-    if (p + 1 < p1) {
-      stage(sm[s ^ 1]);
-      if (p + 2 < p1) load(p + 2);
+  for (int p = p0; p < p1; p += 2) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {  // page p + s in tile s
+      if (p + s >= p1) break;
+      f4_t c[NT][4];
+      bf16x8_t pr[NT][2];
+      tile_scores<NT>(sm[s].k, st, lane, c);
+      tile_softmax<NT>(c, st, scale, pr);
+      tile_values<NT>(sm[s].v, st, lane, pr);
+      if (p + s + 1 < p1) {
+        stage(sm[s ^ 1], pre[s ^ 1]);
+        load(min(p + s + 3, p1 - 1), pre[s ^ 1]);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -444,11 +448,23 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
   }
 }
 
-// One wave per output row: lane (half, 4 dims) takes every other partial, the halves meet by a swap.
+// Adds a partial (maximum m, sum l, values x) to another; one without keys (m = -infinity) has x = 0.
+__device__ __forceinline__ void merge_into(float& M, float& den, f4_t& acc, float m, float l, f4_t x) {
+  const float mn = max_ieee(M, m);
+  const float mr = mn == -INFINITY ? 0.0f : mn;
+  const float e0 = exp2_nonpos(M - mr), e1 = exp2_nonpos(m - mr);
+  acc = acc * e0 + x * e1;
+  den = den * e0 + l * e1;
+  M = mn;
+}
+
+// One workgroup per output row: group g of 32 lanes (4 dims each) takes every eighth partial, four at a
+// time, and the groups meet in LDS.
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
+  __shared__ float2 sh_ml[8];
+  __shared__ f4_t sh_acc[8][32];
   const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  if (row >= a.B * a.Hkv * a.G) return;
+  const int row = blockIdx.x;
   const int b = row / (a.Hkv * a.G), h = row - b * a.Hkv * a.G, hk = h / a.G, g = h - hk * a.G;
   int before = 0, total = 0;
   for (int i = lane; i < a.B; i += 64) {
@@ -468,39 +484,34 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   const int64_t own0 = slot0 + (int64_t)(first + b) * a.G + g;
   const int64_t sh0 = slot0 + (int64_t)(a.shares + a.B) * a.G + (int64_t)b * a.G + g;
   const int parts = n + (joins ? a.np : 0);
-  const int d = 4 * (lane & 31);
+  const int grp = threadIdx.x >> 5, ln = threadIdx.x & 31;
   float M = -INFINITY, den = 0.0f;
   f4_t acc = {0.f, 0.f, 0.f, 0.f};
-  for (int i = lane >> 5; i < parts; i += 2) {
-    const int64_t s = i < n ? own0 + (int64_t)i * a.G : sh0 + (int64_t)(i - n) * a.B * a.G;
-    const float2 ml = a.part_ml[s];
-    const f4_t x = *reinterpret_cast<const f4_t*>(a.part_acc + s * D + d);
-    const float mn = max_ieee(M, ml.x);
-    const float mr = mn == -INFINITY ? 0.0f : mn;
-    const float e0 = M == -INFINITY ? 0.0f : exp2_nonpos(M - mr);
-    const float e1 = ml.x == -INFINITY ? 0.0f : exp2_nonpos(ml.x - mr);
-    acc = acc * e0 + x * e1;
-    den = den * e0 + ml.y * (ml.x == -INFINITY ? 1.0f : e1);
-    M = mn;
-  }
-  // the two halves
-  const float Mo = __shfl_xor(M, 32, 64), deno = __shfl_xor(den, 32, 64);
-  f4_t acco;
+  for (int i0 = grp; i0 < parts; i0 += 32) {
+    float2 ml[4];
+    f4_t x[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) acco[r] = __shfl_xor(acc[r], 32, 64);
-  const float mx = max_ieee(M, Mo);
-  const float mr = mx == -INFINITY ? 0.0f : mx;
-  const float e0 = M == -INFINITY ? 0.0f : exp2_nonpos(M - mr);
-  const float e1 = Mo == -INFINITY ? 0.0f : exp2_nonpos(Mo - mr);
-  acc = acc * e0 + acco * e1;
-  den = (M == -INFINITY ? den : den * e0) + (Mo == -INFINITY ? deno : deno * e1);
+    for (int j = 0; j < 4; ++j) {
+      const int i = min(i0 + 8 * j, parts - 1);
+      const int64_t s = i < n ? own0 + (int64_t)i * a.G : sh0 + (int64_t)(i - n) * a.B * a.G;
+      ml[j] = a.part_ml[s];
+      x[j] = *reinterpret_cast<const f4_t*>(a.part_acc + s * D + 4 * ln);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + 8 * j < parts) merge_into(M, den, acc, ml[j].x, ml[j].y, x[j]);
+  }
+  sh_acc[grp][ln] = acc;
+  if (ln == 0) sh_ml[grp] = make_float2(M, den);
+  __syncthreads();
+  if (grp != 0) return;
+#pragma unroll
+  for (int j = 1; j < 8; ++j) merge_into(M, den, acc, sh_ml[j].x, sh_ml[j].y, sh_acc[j][ln]);
   float inv = den == 0.0f ? 0.0f : 1.0f / den;  // no keys: 0; a sum that is NaN stays
   if (!len_ok(a, len)) inv = NAN;
   const f4_t o = acc * inv;
-  if (lane < 32)
-    *reinterpret_cast<uint2*>(a.out + (int64_t)row * D + d) =
-        make_uint2((uint32_t)f32_to_bf16(o[0]) | ((uint32_t)f32_to_bf16(o[1]) << 16),
-                   (uint32_t)f32_to_bf16(o[2]) | ((uint32_t)f32_to_bf16(o[3]) << 16));
+  *reinterpret_cast<uint2*>(a.out + (int64_t)row * D + 4 * ln) =
+      make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
 }
 
 struct DecodeShape {
@@ -514,7 +525,7 @@ DecodeShape decode_shape(int64_t B, int64_t Hkv, int64_t G, int64_t shared, int 
   if (shared > 0) {
     s.nt = B * G > 64 ? 2 : 1;
     s.rb = (int)((B * G + 64 * s.nt - 1) / (64 * s.nt));
-    s.np = (int)std::min<int64_t>((shared + 3) / 4, std::max<int64_t>(1, fill / (Hkv * s.rb)));
+    s.np = (int)std::min<int64_t>((shared + 3) / 4, std::max<int64_t>(1, fill / 2 / (Hkv * s.rb)));
   }
   s.shares = (int)std::max<int64_t>(1, fill / Hkv);
   s.slots = Hkv * G * (s.shares + B + s.np * B);
@@ -588,7 +599,7 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
   auto* kern = s.nt == 2 ? paged_decode_kernel<2> : s.nt == 1 ? paged_decode_kernel<1> : paged_decode_kernel<0>;
   kern<<<dim3((unsigned)wgs), dim3(64 * DW), 0, (hipStream_t)stream>>>(a);
   LQ_CHECK_LAUNCH("paged_decode_kernel");
-  paged_merge_kernel<<<dim3((unsigned)((B * Hq + 3) / 4)), dim3(256), 0, (hipStream_t)stream>>>(a);
+  paged_merge_kernel<<<dim3((unsigned)(B * Hq)), dim3(256), 0, (hipStream_t)stream>>>(a);
   LQ_CHECK_LAUNCH("paged_merge_kernel");
   return LQ_OK;
 }
