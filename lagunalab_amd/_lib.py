@@ -125,6 +125,28 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, for launches on tensors of another device than the current one; nothing
+    (2 us less) where it is the current one."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def raw_stream(device: torch.device) -> int:
+    """:func:`stream_ptr` of a tensor's device, without the stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def require_device(*tensors: torch.Tensor):
     """All tensors on one ROCm device; returns it."""
     dev = None

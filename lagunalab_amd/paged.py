@@ -15,7 +15,7 @@ sequence ``b`` in order; position ``p`` is slot ``p % 64`` of page ``table[b, p 
 """
 from __future__ import annotations
 
-import ctypes as C
+import functools
 from array import array
 import heapq
 
@@ -41,16 +41,17 @@ def page_pool(pages: int, n_kv_heads: int, device="cuda"):
 
 def _pool(keys, values):
     """(pages, Hkv, device, the six buffers' pointers) of a checked pool."""
-    bufs = (*keys, *values)
     if len(keys) != 3 or len(values) != 3:
         raise ValueError("a pool's keys and values are (codes, scales, biases)")
-    P, H = keys[0].shape[0], keys[0].shape[1] if keys[0].dim() == 4 else 0
+    bufs = (*keys, *values)
+    lead = keys[0].shape[:2]
+    wide, narrow = (*lead, PAGE, HEAD_DIM), (*lead, PAGE, HEAD_DIM // 64)
     for i, t in enumerate(bufs):
-        want = (P, H, PAGE, HEAD_DIM if i % 3 == 0 else HEAD_DIM // 64)
-        dtype = torch.uint8 if i % 3 == 0 else torch.bfloat16
-        if tuple(t.shape) != want or t.dtype != dtype or not t.is_contiguous():
+        want, dtype = (narrow, torch.bfloat16) if i % 3 else (wide, torch.uint8)
+        if t.shape != want or t.dtype != dtype or not t.is_contiguous():
             raise ValueError(f"pool buffer {tuple(t.shape)} {t.dtype} is not contiguous {want} {dtype}")
-    return P, H, _lib.require_device(*bufs), [t.data_ptr() for t in bufs]
+    dev = _lib.require_device(*bufs)
+    return lead[0], lead[1], dev, [t.data_ptr() for t in bufs]
 
 
 def _ints(x, n, what, dev, dims=1):
@@ -60,45 +61,47 @@ def _ints(x, n, what, dev, dims=1):
                          f"{(tuple(x.shape), x.dtype) if torch.is_tensor(x) else type(x)}")
     if x.device != dev:
         raise ValueError(f"{what} is on {x.device}, the pool on {dev}")
-    return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
+    return x if x.is_contiguous() or x.stride(-1) == 1 else x.contiguous()
 
 
 def _table(table, n, dev):
+    """(table, entries from one row to the next, entries of a row)."""
     table = _ints(table, n, "table", dev, 2)
-    if table.shape[1] < 1:
+    width = table.shape[1]
+    if width < 1:
         raise ValueError("table rows of no pages")
-    return table, table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    return table, table.stride(0) if n > 1 else width, width
 
 
 def _counts(counts, B):
-    counts = [int(c) for c in (counts.tolist() if torch.is_tensor(counts) else counts)]
+    """Host row counts as the C arrays take them."""
+    counts = array("i", counts.tolist() if torch.is_tensor(counts) else counts)
     if len(counts) != B:
         raise ValueError(f"{len(counts)} counts for {B} sequences")
-    if min(counts, default=0) < 0:
-        raise ValueError(f"negative count in {counts}")
+    if B and min(counts) < 0:
+        raise ValueError(f"negative count in {counts.tolist()}")
     return counts
 
 
 def _rows(x, T, H, what):
     """Rows [T, H, 128] as the kernels read them: bf16, any token and head strides of 16-byte steps."""
-    if x.dtype != torch.bfloat16 or tuple(x.shape) != (T, H, HEAD_DIM):
+    if x.dtype != torch.bfloat16 or x.shape != (T, H, HEAD_DIM):
         raise ValueError(f"{what} must be bfloat16 {(T, H, HEAD_DIM)}, got {tuple(x.shape)} {x.dtype}")
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+    st = x.stride()
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
+        st = x.stride()
+    return x, st[0], st[1]
 
 
-def _slices(counts):
-    """The sequences of a call in launches of at most LQ_MAX_SEQS: (first, last + 1, rows before)."""
-    at = 0
+def _launches(counts):
+    """The sequences of a call in launches of at most LQ_MAX_SEQS: (first, how many, rows before, its
+    counts' address)."""
+    at, ptr = 0, counts.buffer_info()[0]
     for a in range(0, len(counts), _lib.LQ_MAX_SEQS):
-        e = min(len(counts), a + _lib.LQ_MAX_SEQS)
-        yield a, e, at
-        at += sum(counts[a:e])
-
-
-def _c_ints(xs):
-    return (C.c_int32 * len(xs))(*xs)
+        n = min(len(counts) - a, _lib.LQ_MAX_SEQS)
+        yield a, n, at, ptr + 4 * a
+        at += sum(counts[a:a + n])
 
 
 def paged_append(k, v, keys, values, table, starts, counts=None):
@@ -108,8 +111,7 @@ def paged_append(k, v, keys, values, table, starts, counts=None):
     and biases are those of :func:`lagunalab_amd.quant.quantize`. Rows whose position or page does not
     exist are not stored; no two rows may go to one slot."""
     P, H, dev, ptrs = _pool(keys, values)
-    B = table.shape[0]
-    T = k.shape[0]
+    B, T = table.shape[0], k.shape[0]
     if counts is None:
         if B == 0 or T % B:
             raise ValueError(f"{T} rows are not the same number for each of {B} sequences")
@@ -118,17 +120,17 @@ def paged_append(k, v, keys, values, table, starts, counts=None):
     if sum(counts) != T:
         raise ValueError(f"counts add up to {sum(counts)}, not to the {T} rows")
     _lib.require_device(k, v, keys[0])
-    k, v = _rows(k, T, H, "k"), _rows(v, T, H, "v")
-    table, ts = _table(table, B, dev)
+    k, kt, kh = _rows(k, T, H, "k")
+    v, vt, vh = _rows(v, T, H, "v")
+    table, ts, width = _table(table, B, dev)
     starts = _ints(starts, B, "starts", dev)
+    kp, vp, tp, sp = k.data_ptr(), v.data_ptr(), table.data_ptr(), starts.data_ptr()
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        for a, e, at in _slices(counts):
-            kk, vv = k[at:], v[at:]
-            _lib.check(lib.lq_paged_append(
-                kk.data_ptr(), vv.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), *ptrs,
-                P, H, HEAD_DIM, table[a:].data_ptr(), ts, table.shape[1], starts[a:].data_ptr(),
-                _c_ints(counts[a:e]), e - a, _lib.stream_ptr(dev)), "lq_paged_append")
+    with _lib.on_device(dev):
+        for a, n, at, cp in _launches(counts):
+            _lib.check(lib.lq_paged_append(kp + 2 * at * kt, vp + 2 * at * vt, kt, kh, vt, vh, *ptrs, P, H,
+                                           HEAD_DIM, tp + 4 * a * ts, ts, width, sp + 4 * a, cp, n,
+                                           _lib.raw_stream(dev)), "lq_paged_append")
 
 
 def paged_gather(keys, values, table, starts, counts):
@@ -138,20 +140,27 @@ def paged_gather(keys, values, table, starts, counts):
     P, H, dev, ptrs = _pool(keys, values)
     B = table.shape[0]
     counts = _counts(counts, B)
-    table, ts = _table(table, B, dev)
+    table, ts, width = _table(table, B, dev)
     starts = _ints(starts, B, "starts", dev)
-    k = torch.empty((sum(counts), H, HEAD_DIM), dtype=torch.bfloat16, device=dev)
-    v = torch.empty_like(k)
+    out = torch.empty((2, sum(counts), H, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    k, v = out.unbind()
+    kp, vp, tp, sp = k.data_ptr(), v.data_ptr(), table.data_ptr(), starts.data_ptr()
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        for a, e, at in _slices(counts):
-            if not sum(counts[a:e]):
-                continue
-            _lib.check(lib.lq_paged_gather(
-                *ptrs, P, H, HEAD_DIM, table[a:].data_ptr(), ts, table.shape[1], starts[a:].data_ptr(),
-                _c_ints(counts[a:e]), e - a, k[at:].data_ptr(), v[at:].data_ptr(), _lib.stream_ptr(dev)),
-                "lq_paged_gather")
+    with _lib.on_device(dev):
+        for a, n, at, cp in _launches(counts) if len(k) else ():
+            o = 2 * at * H * HEAD_DIM
+            _lib.check(lib.lq_paged_gather(*ptrs, P, H, HEAD_DIM, tp + 4 * a * ts, ts, width, sp + 4 * a, cp,
+                                           n, kp + o, vp + o, _lib.raw_stream(dev)), "lq_paged_gather")
     return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode_workspace(device, B, Hq, Hkv, pages):
+    """Bytes of workspace of a decode call (of its shape alone)."""
+    need = _lib.load().lq_paged_decode_workspace_bytes(B, Hq, Hkv, pages)
+    if need < 0:
+        _lib.check(_lib.LQ_EINVAL, "lq_paged_decode_workspace_bytes")
+    return need
 
 
 def paged_decode_attention(q, keys, values, table, lens, scale, shared: int = 0):
@@ -162,34 +171,31 @@ def paged_decode_attention(q, keys, values, table, lens, scale, shared: int = 0)
     outside the pool gives NaN. The table and the lengths are read by the kernel: a captured call
     follows them."""
     P, H, dev, ptrs = _pool(keys, values)
-    if q.dim() != 4 or q.shape[2] != 1 or q.shape[3] != HEAD_DIM or q.dtype != torch.bfloat16:
+    if q.dim() != 4 or q.shape[2:] != (1, HEAD_DIM) or q.dtype != torch.bfloat16:
         raise ValueError(f"q must be bfloat16 [B, Hq, 1, {HEAD_DIM}], got {tuple(q.shape)} {q.dtype}")
     _lib.require_device(q, keys[0])
     _refuse_grad(q)
     B, Hq = q.shape[:2]
     if B == 0:
         return torch.empty_like(q)
-    if Hq % H or not 1 <= Hq // H <= 16:
+    if H < 1 or Hq % H or not 1 <= Hq // H <= 16:
         raise ValueError(f"{Hq} query heads are not 1 to 16 per KV head ({H})")
-    table, ts = _table(table, B, dev)
+    table, ts, width = _table(table, B, dev)
     lens = _ints(lens, B, "lens", dev)
     pages = int(shared) // PAGE
-    if shared < 0 or pages > table.shape[1]:
-        raise ValueError(f"{shared} shared positions of table rows of {table.shape[1]} pages")
-    q = q.contiguous()
-    if q.data_ptr() % 16:
-        q = q.clone()
+    if shared < 0 or pages > width:
+        raise ValueError(f"{shared} shared positions of table rows of {width} pages")
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        need = lib.lq_paged_decode_workspace_bytes(B, Hq, H, pages)
-        if need < 0:
-            _lib.check(_lib.LQ_EINVAL, "lq_paged_decode_workspace_bytes")
+    with _lib.on_device(dev):
+        need = _decode_workspace(dev.index, B, Hq, H, pages)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        out = torch.empty((B, Hq, 1, HEAD_DIM), dtype=torch.bfloat16, device=dev)
-        _lib.check(lib.lq_paged_decode_attn(
-            q.data_ptr(), *ptrs, P, B, Hq, H, HEAD_DIM, table.data_ptr(), ts, table.shape[1],
-            lens.data_ptr(), pages, float(scale), out.data_ptr(), ws.data_ptr(), need,
-            _lib.stream_ptr(dev)), "lq_paged_decode_attn")
+        out = torch.empty_like(q)
+        _lib.check(lib.lq_paged_decode_attn(q.data_ptr(), *ptrs, P, B, Hq, H, HEAD_DIM, table.data_ptr(), ts,
+                                            width, lens.data_ptr(), pages, scale, out.data_ptr(),
+                                            ws.data_ptr(), need, _lib.raw_stream(dev)),
+                   "lq_paged_decode_attn")
     return out
 
 
@@ -201,6 +207,6 @@ def copy_pages(keys, values, src, dst):
     if len(src) != len(dst):
         raise ValueError(f"{len(src)} pages to copy to {len(dst)}")
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.check(lib.lq_copy_pages(*ptrs, P, H, HEAD_DIM, src.buffer_info()[0], dst.buffer_info()[0],
-                                     len(src), _lib.stream_ptr(dev)), "lq_copy_pages")
+                                     len(src), _lib.raw_stream(dev)), "lq_copy_pages")

@@ -4,7 +4,7 @@ that are not in a cache yet or were read back from one, of the SDPA that ``lagun
 runs with the causal mask."""
 from __future__ import annotations
 
-import ctypes as C
+from array import array
 
 import torch
 
@@ -19,8 +19,8 @@ def _refuse_grad(*tensors):
 
 
 def _lens(lens, what):
-    lens = [int(n) for n in (lens.tolist() if torch.is_tensor(lens) else lens)]
-    if min(lens, default=0) < 0:
+    lens = array("i", lens.tolist() if torch.is_tensor(lens) else lens)
+    if lens and min(lens) < 0:
         raise ValueError(f"negative length in {what}")
     return lens
 
@@ -31,9 +31,11 @@ def _rows(x, heads, total, what):
     if x.shape[0] != total or (heads and x.shape[1] != heads):
         raise ValueError(f"{what} {tuple(x.shape)} does not have {total} rows"
                          + (f" of {heads} heads" if heads else ""))
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+    st = x.stride()
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
+        st = x.stride()
+    return x, st[0], st[1]
 
 
 def prompt_attention(q, k, v, q_lens, scale, k_lens=None):
@@ -47,27 +49,27 @@ def prompt_attention(q, k, v, q_lens, scale, k_lens=None):
         raise ValueError(f"{len(q_lens)} q_lens and {len(k_lens)} k_lens")
     dev = _lib.require_device(q, k, v)
     _refuse_grad(q, k, v)
-    q = _rows(q, 0, sum(q_lens), "q")
-    k = _rows(k, 0, sum(k_lens), "k")
+    q, qt, qh = _rows(q, 0, sum(q_lens), "q")
+    k, kt, kh = _rows(k, 0, sum(k_lens), "k")
     Hq, Hkv = q.shape[1], k.shape[1]
-    v = _rows(v, Hkv, sum(k_lens), "v")
+    v, vt, vh = _rows(v, Hkv, sum(k_lens), "v")
     if Hkv < 1 or Hq % Hkv or not 1 <= Hq // Hkv <= 64:
         raise ValueError(f"{Hq} query heads are not 1 to 64 per KV head ({Hkv})")
     lib = _lib.load()
-    out = torch.empty((q.shape[0], Hq, HEAD_DIM), dtype=torch.bfloat16, device=dev)
-    with torch.cuda.device(dev):
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    lq, lk = q_lens.buffer_info()[0], k_lens.buffer_info()[0]
+    with _lib.on_device(dev):
         qa = ka = 0
         for a in range(0, len(q_lens), _lib.LQ_MAX_SEQS):  # sequences per launch
-            ql, kl = q_lens[a:a + _lib.LQ_MAX_SEQS], k_lens[a:a + _lib.LQ_MAX_SEQS]
-            cq, ck = (C.c_int32 * len(ql))(*ql), (C.c_int32 * len(kl))(*kl)
-            need = lib.lq_prompt_workspace_bytes(cq, ck, len(ql), Hq, Hkv)
+            n = min(len(q_lens) - a, _lib.LQ_MAX_SEQS)
+            need = lib.lq_prompt_workspace_bytes(lq + 4 * a, lk + 4 * a, n, Hq, Hkv)
             if need < 0:
                 _lib.check(_lib.LQ_EINVAL, "lq_prompt_workspace_bytes")
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _lib.check(lib.lq_prompt_attn(
-                q[qa:].data_ptr(), k[ka:].data_ptr(), v[ka:].data_ptr(), q.stride(0), q.stride(1),
-                k.stride(0), k.stride(1), v.stride(0), v.stride(1), cq, ck, len(ql), Hq, Hkv, HEAD_DIM,
-                float(scale), out[qa:].data_ptr(), _lib.ptr(ws), need, _lib.stream_ptr(dev)),
-                "lq_prompt_attn")
-            qa, ka = qa + sum(ql), ka + sum(kl)
+            _lib.check(lib.lq_prompt_attn(qp + 2 * qa * qt, kp + 2 * ka * kt, vp + 2 * ka * vt, qt, qh, kt, kh,
+                                          vt, vh, lq + 4 * a, lk + 4 * a, n, Hq, Hkv, HEAD_DIM, scale,
+                                          op + 2 * qa * Hq * HEAD_DIM, _lib.ptr(ws), need,
+                                          _lib.raw_stream(dev)), "lq_prompt_attn")
+            qa, ka = qa + sum(q_lens[a:a + n]), ka + sum(k_lens[a:a + n])
     return out
