@@ -17,22 +17,6 @@
 namespace lq {
 namespace {
 
-// Code of one value: round-half-away(fl(fl(x - bias) / scale)) clamped to 2^BITS - 1, as
-// affine_code. Fast path: u = (x - bias) * (1 / scale) + 0.5 (v_rcp_f32, 1 ulp) is within
-// 6.1e-5 of fl(fl(x - bias) / scale) + 0.5 for quotients below 512 (ours stay below 257), so
-// floor(u) is the code unless u lies within 2e-4 of an integer; those lanes (and NaN/inf) take the
-// correctly rounded division instead. u >= 0 up to rounding (the bias is the group's edge on the
-// side the scale's sign points away from), so truncation is the floor and a slightly negative u
-// converts to 0, as its floor clamps there. Returns the code; sets `slow` for the lanes that need
-// the division.
-template <int BITS>
-__device__ __forceinline__ uint32_t fast_code(float x, const AffineParams& p, float rs, bool& slow) {
-  const float u = fmaf(x - p.bias, rs, 0.5f);
-  const float f = __builtin_amdgcn_fractf(u);
-  slow = !(fabsf(f - 0.5f) < 0.4998f);
-  return min((uint32_t)u, (uint32_t)((1 << BITS) - 1));
-}
-
 // One lane per group of GS values (CH = GS / 8 chunks of 16 bytes); a wave takes 64 consecutive
 // groups (every group of the update lies in one row: GS divides the head dim). Groups [0, groups_a)
 // belong to target a, [groups_a, groups) to target b (K and V of one update in one launch). Group
