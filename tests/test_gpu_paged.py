@@ -473,3 +473,173 @@ def test_prompt_of_no_rows(dev):
     assert prompt_attention(e, kv, kv, [0, 0], SCALE).shape == (0, 8, D)
     q = torch.ones((5, 8, D), dtype=torch.bfloat16, device=dev)
     assert (prompt_attention(q, kv, kv, [2, 3], SCALE, k_lens=[0, 0]) == 0).all()
+
+
+# ------------------------------------------------------------------- a server's use of them together
+
+def test_sessions_prompted_forked_decoded_and_compacted(dev):
+    """Prompts attended packed and appended, one forked, tokens appended to all and attended, sessions closed
+    and the pool compacted: every step against the contiguous cache of each session."""
+    from lagunalab_amd.cache import DequantKVCache
+    from lagunalab_amd.paged import PagedKVCache
+    g = gen(30)
+    hq, kv = 12, 2
+    cache = PagedKVCache(60, kv, dev)
+    prompts = [300, 64, 1, 130]
+    k, v = randn(g, sum(prompts), kv, D).to(dev), randn(g, sum(prompts), kv, D).to(dev)
+    q = randn(g, sum(prompts), hq, D).to(dev)
+    check_prompt(prompt_attention(q, k, v, prompts, SCALE), q, k, v, prompts, prompts, some=8)
+    ids = [cache.open() for _ in prompts]
+    cache.append(ids, k, v, prompts)
+    plain = {}
+    for s, kk, vv in zip(ids, k.split(prompts), v.split(prompts)):
+        plain[s] = DequantKVCache(fused_decode=True)
+        plain[s].update_and_fetch(kk.transpose(0, 1)[None], vv.transpose(0, 1)[None])
+        plain[s].state  # a short prompt's rows are pending until they are asked for
+    forks = [cache.fork(ids[0]) for _ in range(5)]
+    for s in forks:
+        plain[s] = DequantKVCache(fused_decode=True)
+        plain[s].update_and_fetch(k[:300].transpose(0, 1)[None], v[:300].transpose(0, 1)[None])
+
+    def step(sessions, n=1):
+        T = n * len(sessions)
+        kk, vv = randn(g, T, kv, D).to(dev), randn(g, T, kv, D).to(dev)
+        qq = randn(g, len(sessions), hq, 1, D).to(dev)
+        cache.append(sessions, kk, vv)
+        out = cache.attention(sessions, qq, SCALE)
+        rows = cache.rows(sessions)[0].split([cache.length(s) for s in sessions])
+        for i, s in enumerate(sessions):
+            part = slice(i * n, (i + 1) * n)
+            qk, qv = plain[s].q.update_and_fetch(kk[part].transpose(0, 1)[None], vv[part].transpose(0, 1)[None])
+            assert plain[s].offset == cache.length(s)
+            held = [tuple(t[0].cpu() for t in x) for x in (qk, qv)]  # [kv, rows, .]
+            n_rows = plain[s].offset
+            c, sc, bi = (t.double() for t in held[0])
+            val = [(x[0].double() * x[1].double().repeat_interleave(64, -1)
+                    + x[2].double().repeat_interleave(64, -1)).to(torch.bfloat16).double() for x in held]
+            assert (rows[i].cpu().double() == val[0].transpose(0, 1)).all().item()
+            for h in range(kv):
+                G = hq // kv
+                want, bound = exact_attention(qq[i, h * G:(h + 1) * G, 0].cpu().double(), val[0][h], val[1][h],
+                                              [n_rows - 1] * G, SCALE)
+                assert_within(out[i, h * G:(h + 1) * G, 0], want, bound, f"session {s} head {h}")
+            # the contiguous cache's fused kernel, to both kernels' roundings
+            fused = plain[s].attend(qq[i:i + 1], SCALE)
+            assert (out[i].float() - fused[0].float()).abs().max() < 2e-2
+
+    step(ids + forks)
+    step([ids[0], *forks])
+    step(forks, 40)
+    for s in (ids[0], ids[2], forks[1]):
+        cache.close(s)
+        del plain[s]
+    assert cache.trim(forks[0], 30) == 30
+    plain[forks[0]].trim(30)
+    used = cache.compact()
+    assert used == 60 - cache.free_pages and max(max(cache.pages(s)) for s in plain) < used
+    step(sorted(plain))
+    cache.resize(used + 8)
+    step(sorted(plain))
+    step([forks[2], ids[3]], 3)
+
+
+def test_adopted_session(dev):
+    from lagunalab_amd.cache import DequantKVCache, QuantizedKVCache
+    from lagunalab_amd.paged import PagedKVCache
+    g = gen(31)
+    for cls, n in ((DequantKVCache, 200), (QuantizedKVCache, 128), (DequantKVCache, 5), (DequantKVCache, 0)):
+        src = cls()
+        cache = PagedKVCache(6, 2, dev)
+        cache.open()
+        if n:
+            src.update_and_fetch(randn(g, 1, 2, n, D).to(dev), randn(g, 1, 2, n, D).to(dev))
+        s = cache.adopt(src)
+        assert cache.length(s) == n
+        if n:
+            from lagunalab_amd.quant import dequantize
+            for x, buf in zip(cache.rows([s]), src.state):
+                assert torch.equal(bits(x), bits(dequantize(*buf)[0].transpose(0, 1)))
+    four = DequantKVCache(bits=4)
+    four.update_and_fetch(randn(g, 1, 2, 3, D).to(dev), randn(g, 1, 2, 3, D).to(dev))
+    with pytest.raises(ValueError, match="8 bits"):
+        cache.adopt(four)
+    two = DequantKVCache()
+    two.update_and_fetch(randn(g, 2, 2, 3, D).to(dev), randn(g, 2, 2, 3, D).to(dev))
+    with pytest.raises(ValueError, match="one sequence"):
+        cache.adopt(two)
+
+
+@torch.no_grad()
+def test_model_over_paged_batches(dev):
+    """The tiny model's forward pass on PagedBatch caches: a prompt, forked into a batch, decoded; logits as
+    over the dequantizing cache of the same rows."""
+    from lagunalab_amd.cache import DequantKVCache
+    from lagunalab_amd.paged import PagedKVCache
+    from tiny_model import TinyArgs, TinyLM
+    model = TinyLM(TinyArgs(layer_types=["full_attention"] * 2), device="cuda", seed=2)
+    pools = [PagedKVCache(40, 2, dev) for _ in range(2)]
+    first = [p.open() for p in pools]
+    ids = torch.tensor([[5, 9, 2, 7, 1, 3, 8, 4] * 25], device="cuda")
+    plain = [DequantKVCache() for _ in range(2)]
+    one = [p.batch([s]) for p, s in zip(pools, first)]
+    for part in ids.split(120, dim=1):  # two chunks
+        got, want = model(part, cache=one), model(part, cache=plain)
+        assert (got - want).abs().max() < 5e-2 * want.abs().max()
+    forks = [[s] + [p.fork(s) for _ in range(2)] for p, s in zip(pools, first)]
+    batch = [p.batch(f) for p, f in zip(pools, forks)]
+    wide = []
+    for c in plain:
+        w = DequantKVCache()
+        w.state = tuple(tuple(t.expand(3, -1, -1, -1).contiguous() for t in x) for x in c.state)
+        wide.append(w)
+    for i in range(3):
+        tok = torch.tensor([[i + 1], [i + 70], [i + 300]], device="cuda")
+        got, want = model(tok, cache=batch), model(tok, cache=wide)
+        assert (got - want).abs().max() < 5e-2 * want.abs().max()
+        assert batch[0].offset == 201 + i
+    assert pools[0].free_pages == 40 - 3 - 3  # 3 shared whole pages, the fourth one for each
+    for b in batch:
+        assert b.trim(2) == 2
+
+
+@torch.no_grad()
+def test_lookup_generation_over_paged_caches(dev):
+    from lagunalab_amd.generate import generate_greedy, generate_lookup
+    from lagunalab_amd.paged import PagedKVCache
+    from tiny_model import TinyArgs, TinyLM
+    model = TinyLM(TinyArgs(layer_types=["full_attention"] * 2), device="cuda", seed=2)
+
+    def make():
+        pools = [PagedKVCache(8, 2, dev) for _ in range(2)]
+        return [p.batch([p.open()]) for p in pools]
+    prompt = [3, 1, 4, 1, 5, 9, 2, 6, 3, 1, 4, 1]
+    want = generate_greedy(model, prompt, 24, cache=make())
+    got, stats = generate_lookup(model, prompt, 24, g=2, n_draft=5, make_cache=make)
+    assert got == want
+
+
+def test_attention_block_over_a_paged_batch(dev):
+    """The attention block of a layer on sessions of one prompt, beside the same block on the dequantizing
+    cache."""
+    from lagunalab_amd.attention import Attention
+    from lagunalab_amd.cache import DequantKVCache
+    from lagunalab_amd.paged import PagedKVCache
+    g = gen(32)
+    C, hq, kv = 256, 8, 2
+    w = lambda *s: randn(g, *s, std=0.06).to(dev)  # noqa: E731
+    block = Attention(w(hq * D, C), w(kv * D, C), w(kv * D, C), w(C, hq * D), w(hq, C), w(D) + 1, w(D) + 1, hq, kv,
+                      {"rope_theta": 5e5, "partial_rotary_factor": 0.5})
+    pool = PagedKVCache(20, kv, dev)
+    s = pool.open()
+    x = randn(g, 1, 150, C).to(dev)
+    plain = DequantKVCache()
+    got, want = block(x, "causal", pool.batch([s])), block(x, "causal", plain)
+    assert (got.float() - want.float()).abs().max() < 3e-2 * want.float().abs().max()
+    wide = DequantKVCache()
+    wide.state = tuple(tuple(t.expand(4, -1, -1, -1).contiguous() for t in y) for y in plain.state)
+    batch = pool.batch([s] + [pool.fork(s) for _ in range(3)])
+    for L in (1, 3, 1):
+        x = randn(g, 4, L, C).to(dev)
+        mask = None if L == 1 else "causal"
+        got, want = block(x, mask, batch), block(x, mask, wide)
+        assert (got.float() - want.float()).abs().max() < 3e-2 * want.float().abs().max()
