@@ -233,6 +233,32 @@ __device__ __forceinline__ float wave_sum(float x) {
   return sum_xor32(sum_xor16(x));
 }
 
+// Whole numbers: sum over the wave in every lane (DPP steps within rows of 16, then the row and half swaps).
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int x) {
+  return __builtin_amdgcn_mov_dpp(x, CTRL, 0xF, 0xF, true);
+}
+__device__ __forceinline__ int wave_sum_i(int x) {
+  x += dpp_i<DPP_QUAD_XOR1>(x);
+  x += dpp_i<DPP_QUAD_XOR2>(x);
+  x += dpp_i<DPP_ROW_ROR4>(x);
+  x += dpp_i<DPP_ROW_ROR8>(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = (int)r[0] + (int)r[1];
+  const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return (int)h[0] + (int)h[1];
+}
+// Inclusive sum over the lanes: within rows of 16 by shifts, then the rows' last values broadcast on.
+__device__ __forceinline__ int wave_scan_i(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 // RMSNorm (times w, rounded to bf16) and RoPE at position `pos` of one 128-dim head row held by
 // one wave (the reference's q_norm / k_norm, then rope, laguna_mlx/laguna.py:97-101): lane l
 // holds dims 2l and 2l + 1 as the bf16 pair x2 (norm weights w2); returns the lane's output pair.

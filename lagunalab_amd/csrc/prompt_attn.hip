@@ -16,9 +16,10 @@
 //   2t      Q.K^T(t), P.V(t-1)        softmax(t-1), copies K(t+2) V(t+1)
 //   2t+1    softmax(t), copies        Q.K^T(t), P.V(t-1)
 //
-// The work is dealt out in equal shares of tiles: the blocks of all sequences stand one behind the other, a
-// block costing its tiles and BLOCK_COST for its start and end, and a workgroup takes one share, which may
-// begin and end inside blocks. Parts of blocks go to the workspace and a second launch merges them. One
+// The work is dealt out in equal shares of tiles: the blocks of all sequences stand one behind the other (of
+// a sequence the last, the first, the last but one, .., so that two neighbours cost about the same
+// everywhere and cuts are few), a block costing its tiles and BLOCK_COST for its start and end, and a
+// workgroup takes one share, which may begin and end inside blocks. Parts of blocks go to the workspace and a second launch merges them. One
 // share per CU (several where they are long), so that every CU ends at the same time whatever the lengths
 // are: 2,048 rows, 32/8 heads, in whole blocks would be 32 tiles for the last workgroup and 1 for the
 // first. A workgroup finds its share by scanning the blocks of a sequence, a lane each; nothing of the
@@ -66,11 +67,16 @@ __host__ __device__ __forceinline__ int block_tiles(int blk, int R, FastDiv g, i
   return last < 0 ? 0 : last / TKEYS + 1;
 }
 
-// A block and where its cost begins.
+// A block, its place among its sequence's blocks and where its cost begins.
 struct Block {
   int seq, blk, tiles;
   int64_t begin;
+  int place;
 };
+// The block at a place among nb: the last, the first, the last but one, ..
+__device__ __forceinline__ int block_at(int place, int nb) {
+  return place & 1 ? place >> 1 : nb - 1 - (place >> 1);
+}
 __device__ __forceinline__ int seq_rows(const PromptArgs& a, int s) {
   return (a.q_begin[s + 1] - a.q_begin[s]) * a.G;
 }
@@ -84,18 +90,14 @@ __device__ __forceinline__ Block find_block(const PromptArgs& a, int64_t u, int 
   const int R = seq_rows(a, s), base = seq_base(a, s), nb = (R + PROWS - 1) / PROWS;
   int64_t before = a.cost[s];
   for (int i = 0;; i += 64) {
-    const int tiles = i + lane < nb ? block_tiles(i + lane, R, a.g, base) : 0;
+    const int tiles = i + lane < nb ? block_tiles(block_at(i + lane, nb), R, a.g, base) : 0;
     const int c = i + lane < nb ? tiles + BLOCK_COST : 0;
-    int upto = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(upto, o, 64);
-      upto += lane >= o ? y : 0;
-    }
+    const int upto = wave_scan_i(c);
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > u);
     if (past || i + 64 >= nb) {
       const int l = past ? __builtin_ctzll(past) : 0;
-      return {s, i + l, __builtin_amdgcn_readlane(tiles, l), before + __builtin_amdgcn_readlane(upto - c, l)};
+      return {s, block_at(i + l, nb), __builtin_amdgcn_readlane(tiles, l),
+              before + __builtin_amdgcn_readlane(upto - c, l), i + l};
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
@@ -110,15 +112,10 @@ __device__ __forceinline__ Block ranked_block(const PromptArgs& a, int x, int la
     const int64_t y = a.G * ((int64_t)TKEYS * (n - 1) - base);  // the row that has to be reached
     return n <= 0 || y <= 0 ? 0 : y > R - 1 ? nb : (int)(y / PROWS);
   };
-  auto wave_sum_i = [&](int v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-    return __builtin_amdgcn_readfirstlane(v);
-  };
   int lo = 0, hi = a.longest + 1;  // all have lo, none has hi
   int above = 0;                   // blocks with at least hi tiles
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1, n = wave_sum_i(nb - from(mid));
+    const int mid = (lo + hi) >> 1, n = __builtin_amdgcn_readfirstlane(wave_sum_i(nb - from(mid)));
     if (n > x) {
       lo = mid;
     } else {
@@ -127,14 +124,9 @@ __device__ __forceinline__ Block ranked_block(const PromptArgs& a, int x, int la
     }
   }
   const int n = from(lo + 1) - from(lo);
-  int upto = n;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(upto, o, 64);
-    upto += lane >= o ? y : 0;
-  }
+  const int upto = wave_scan_i(n);
   const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > x - above));
-  return {l, __builtin_amdgcn_readlane(from(lo), l) + x - above - __builtin_amdgcn_readlane(upto - n, l), lo, 0};
+  return {l, __builtin_amdgcn_readlane(from(lo), l) + x - above - __builtin_amdgcn_readlane(upto - n, l), lo, 0, 0};
 }
 // The tile of a block at which a cut at cost u (anywhere) lies: not within MIN_PART of its ends.
 __device__ __forceinline__ int cut_tile(const Block& b, int64_t u) {
@@ -345,20 +337,21 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   const int64_t next = b.begin + b.tiles + BLOCK_COST;
   more = next < u1;
   if (more) {
-    int ns = b.seq, nblk = b.blk + 1;
-    if (nblk * PROWS >= R) {
-      nblk = 0;
+    int ns = b.seq, place = b.place + 1;
+    if (place * PROWS >= R) {
+      place = 0;
       do ++ns;
       while (a.cost[ns + 1] == a.cost[ns]);  // sequences without rows cost nothing
     }
-    b = Block{ns, nblk, block_tiles(nblk, seq_rows(a, ns), a.g, seq_base(a, ns)), next};
+    const int nr = seq_rows(a, ns), nblk = block_at(place, (nr + PROWS - 1) / PROWS);
+    b = Block{ns, nblk, block_tiles(nblk, nr, a.g, seq_base(a, ns)), next, place};
   }
   }
 }
 
 constexpr int MERGE_ROWS = 32;  // of a workgroup
 // The parts of a block into output rows, by the workgroups of its first cut: share j's end. 32 lanes x 4
-// dims per row, 8 rows at a time.
+// dims per row.
 __global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptArgs a) {
   const int j = blockIdx.x / a.Hkv, hk = blockIdx.x - j * a.Hkv;
   const int64_t u = a.share * (j + 1);
@@ -369,30 +362,45 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptArgs a) {
   const int d = 4 * (threadIdx.x & 31);
   int n = 1;  // parts
   while (cut_tile(b, u + n * a.share - a.share) < b.tiles) ++n;
-#pragma unroll 1
-  for (int i = 0; i < MERGE_ROWS / 8; ++i) {
-    const int wrow = MERGE_ROWS * blockIdx.y + 8 * i + (threadIdx.x >> 5);
-    const int f = b.blk * PROWS + wrow;
-    if (f >= R) return;
-    float M = -INFINITY, den = 0.0f;
-    f4_t acc = {0.f, 0.f, 0.f, 0.f};
+  constexpr int RT = MERGE_ROWS / 8;  // rows per thread: all their loads of a part together
+  const int row0 = MERGE_ROWS * blockIdx.y + (threadIdx.x >> 5);
+  if (b.blk * PROWS + MERGE_ROWS * (int)blockIdx.y >= R) return;
+  float M[RT], den[RT];
+  f4_t acc[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    M[i] = -INFINITY;
+    den[i] = 0.0f;
+    acc[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
 #pragma unroll 2
-    for (int k = 0; k < n; ++k) {
-      const int64_t pr = ((int64_t)(2 * (j + k) + (k == 0)) * a.Hkv + hk) * PROWS + wrow;
-      const float2 ml = a.part_ml[pr];
-      const f4_t o = *reinterpret_cast<const f4_t*>(a.part_acc + pr * D + d);
-      const float mn = max_ieee(M, ml.x);
-      const float mr = mn == -INFINITY ? 0.0f : mn;
-      const float e0 = M == -INFINITY ? 0.0f : exp2_nonpos(M - mr);
-      const float e1 = ml.x == -INFINITY ? 0.0f : exp2_nonpos(ml.x - mr);
-      acc = acc * e0 + o * e1;
-      den = den * e0 + ml.y * e1;
-      M = mn;
+  for (int k = 0; k < n; ++k) {
+    const int64_t part = ((int64_t)(2 * (j + k) + (k == 0)) * a.Hkv + hk) * PROWS;
+    float2 ml[RT];
+    f4_t o[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {  // rows past the sequence's are read, of the workspace, and not used
+      ml[i] = a.part_ml[part + row0 + 8 * i];
+      o[i] = *reinterpret_cast<const f4_t*>(a.part_acc + (part + row0 + 8 * i) * D + d);
     }
-    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const float mn = max_ieee(M[i], ml[i].x);
+      const float mr = mn == -INFINITY ? 0.0f : mn;
+      const float e0 = exp2_nonpos(M[i] - mr), e1 = exp2_nonpos(ml[i].x - mr);
+      acc[i] = acc[i] * e0 + o[i] * e1;
+      den[i] = den[i] * e0 + ml[i].y * e1;
+      M[i] = mn;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int f = b.blk * PROWS + row0 + 8 * i;
+    if (f >= R) return;
+    const float inv = den[i] == 0.0f ? 0.0f : 1.0f / den[i];
     const int p = (int)fdiv_u((uint32_t)f, a.g), head = f - p * a.G;
     *reinterpret_cast<uint2*>(a.out + ((int64_t)(a.q_begin[b.seq] + p) * a.Hkv * a.G + hk * a.G + head) * D + d) =
-        make_uint2(pack_bf2(acc[0] * inv, acc[1] * inv), pack_bf2(acc[2] * inv, acc[3] * inv));
+        make_uint2(pack_bf2(acc[i][0] * inv, acc[i][1] * inv), pack_bf2(acc[i][2] * inv, acc[i][3] * inv));
   }
 }
 
