@@ -224,8 +224,8 @@ __device__ __forceinline__ void tile_values(const uint16_t* v, TileRows<NT>& st,
   }
 }
 
-// Q.K^T of one tile, then P.V of another, in eight steps of 4 NT MFMAs: key tile u of K, then half a
-// k-step of V. A step's four fragments are read two steps ahead (tile_ahead: the first two, which may
+// Q.K^T of one tile, then P.V of another, in eight steps of 4 NT MFMAs: two key tiles of K by half the
+// dims (so that an MFMA's accumulator was last written 2 NT MFMAs before), then half a k-step of V. A step's four fragments are read two steps ahead (tile_ahead: the first two, which may
 // lie in the phase before), so that no MFMA waits for LDS.
 struct Ahead {
   bf16x8_t f[3][4];
@@ -234,7 +234,7 @@ __device__ __forceinline__ void tile_fetch(const bf16x8_t* k, uint32_t vl, int l
   const int lc = lane & 15, lq4 = lane >> 4;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    f[j] = step < 4 ? k[256 * step + ((4 * j + lq4) ^ lc)]
+    f[j] = step < 4 ? k[256 * (2 * (step >> 1) + (j >> 1)) + ((4 * (2 * (step & 1) + (j & 1)) + lq4) ^ lc)]
                     : v_operand(vl, 4 * (step & 1) + j, (step - 4) >> 1);
 }
 __device__ __forceinline__ void tile_ahead(const uint16_t* kt, int lane, Ahead& a) {
@@ -253,11 +253,14 @@ __device__ __forceinline__ void tile_matrix(const uint16_t* kt, const uint16_t* 
     __builtin_amdgcn_sched_barrier(0);
     if (u < 4) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
+      for (int i = 0; i < 4; ++i) {
+        const int mt = 2 * (u >> 1) + (i & 1), kk = 2 * (u & 1) + (i >> 1);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-          c[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              a.f[u % 3][kk], st.q[nt][kk], kk == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : c[nt][u], 0, 0, 0);
+          c[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              a.f[u % 3][2 * (i & 1) + (i >> 1)], st.q[nt][kk],
+              kk == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : c[nt][mt], 0, 0, 0);
+      }
     } else {
       const int e = (u - 4) >> 1, w0 = 4 * (u & 1);
       if (u & 1) {
