@@ -6,7 +6,8 @@
 // once into LDS and runs the matrix-core tile of attn_tile.h on it. The sequences' own pages, one sequence
 // behind the other, are dealt out to the workgroups in equal shares; a workgroup runs its pages of a sequence
 // for the G <= 16 rows, one page per wave at a time, through the wave's own LDS (no barriers), the next
-// page's loads out while it computes. Both kinds write
+// page's loads out while it computes. With up to 16 query rows in the batch the shared pages are dealt out
+// with the own ones, in front of them, as those of one sequence with all the rows. Both kinds write
 // partial rows (max, sum, weighted values), which a second launch merges.
 //
 // Lengths are read on the device, so one recorded launch serves every step of a growing batch: every
@@ -28,6 +29,10 @@ using namespace attn;
 
 constexpr int DW = 4;         // waves per workgroup
 constexpr int SHARE_MIN = 4;  // pages of a share: one per wave
+// Cost of starting on a sequence, in pages: shares of many short ones would end last. us at 0 / 2 / 4 / 8: 64
+// sessions of 10 to 500 positions, 32/8 heads 26.9 / 21.7 / 20.8 / 20.8, 8 of 100 to 4,000 21.8 / 19.2 / 17.8 /
+// 19.6, 4 of 100 to 300 behind 65,536 50.2 / 42.0 / 40.2 / 39.8.
+constexpr int SEQ_COST = 4;
 
 struct PagedArgs {
   const uint16_t* q;
@@ -39,7 +44,7 @@ struct PagedArgs {
   uint16_t* out;
   int B, Hkv, G;
   int shared;         // pages that all sequences share
-  int np, rb;         // their parts, blocks of query rows
+  int np, rb;         // their parts, blocks of query rows; 0: dealt out with the own pages
   int shares;         // workgroups for the own pages of a KV head
   float sl2;          // softmax scale, log2 units
 };
@@ -55,9 +60,38 @@ __device__ __forceinline__ int own_pages(const PagedArgs& a, int len) {
   return len_ok(a, len) ? (len + PAGE - 1) / PAGE - own_first(a, len) : 0;
 }
 
-// Pages of a share: the same in every workgroup of a call.
-__device__ __forceinline__ int share_pages(const PagedArgs& a, int total) {
-  return max(SHARE_MIN, (total + a.shares - 1) / a.shares);
+// What a sequence's own pages cost: one each, and a constant in front.
+__device__ __forceinline__ int own_cost(const PagedArgs& a, int len) {
+  const int n = own_pages(a, len);
+  return n ? n + SEQ_COST : 0;
+}
+
+// What the call deals out, in pages, the shared ones in front (0: no sequence is long enough, or the shared
+// part is not dealt out), and a share. The same in every workgroup of a call.
+struct Deal {
+  int lead, total, share;
+};
+__device__ __forceinline__ Deal deal_out(const PagedArgs& a, int lane) {
+  int total = 0;
+  bool joins = false;
+  for (int i = lane; i < a.B; i += 64) {
+    const int len = a.lens[i];
+    total += own_cost(a, len);
+    joins |= len_ok(a, len) && len >= a.shared * PAGE;
+  }
+  const int lead = a.np == 0 && __builtin_amdgcn_ballot_w64(joins) ? a.shared : 0;
+  total = wave_sum_i(total) + lead;
+  return {lead, total, max(SHARE_MIN, (total + a.shares - 1) / a.shares)};
+}
+// The table row that lists the shared pages: of the first sequence that is long enough (a shorter one's may
+// end before them); null: there is none.
+__device__ __forceinline__ const int32_t* shared_ids(const PagedArgs& a, int lane) {
+  for (int i = 0; i < a.B; i += 64) {
+    const int len = i + lane < a.B ? a.lens[i + lane] : -1;
+    const uint64_t joins = __builtin_amdgcn_ballot_w64(len_ok(a, len) && len >= a.shared * PAGE);
+    if (joins) return a.tab.ids + (i + __builtin_ctzll(joins)) * a.tab.stride;
+  }
+  return nullptr;
 }
 
 struct OwnSmem {
@@ -96,23 +130,22 @@ __device__ __forceinline__ void wave_fence() {  // LDS of the wave's own: order 
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Pages [p0, p1) of a sequence for its G rows.
-__device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, int b, int hk, int p0, int p1,
-                                          int len, int64_t slot) {
+// Pages [p0, p1) listed at ids, of a sequence of len positions, for R <= 16 query rows (row lane % 16 of them
+// at qrow).
+__device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, const int32_t* ids, int R,
+                                         int64_t qrow, int hk, int p0, int p1, int len, int64_t slot) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 15, lq4 = lane >> 4;
   __syncthreads();  // the sequence before is written
-  const int32_t* ids = a.tab.ids + b * a.tab.stride;
   const float scale = abs_scale(a.sl2);
-  const int64_t qrow = ((int64_t)b * a.Hkv + hk) * a.G;
   // q as B operands in K's order of dims: k-step 2 h + j holds dims 64 h + 16 lq4 + 8 j .. + 7
   bf16x8_t qf[4];
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (lc < a.G)
-      u = *reinterpret_cast<const uint4*>(a.q + (qrow + lc) * D + 64 * (kk >> 1) + 16 * lq4 + 8 * (kk & 1));
+    if (lc < R)
+      u = *reinterpret_cast<const uint4*>(a.q + qrow * D + 64 * (kk >> 1) + 16 * lq4 + 8 * (kk & 1));
     qf[kk] = u4_as_bf8(signed_q(u, a.sl2));
   }
   f4_t o[8];
@@ -239,7 +272,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, int b,
   l = sum_xor32(sum_xor16(l));
   wave_fence();
   float* acc = reinterpret_cast<float*>(sm.v[wv]);
-  if (lc < a.G) {
+  if (lc < R) {
 #pragma unroll
     for (int w = 0; w < 8; ++w)
       *reinterpret_cast<float4*>(acc + lc * D + 16 * w + 4 * lq4) =
@@ -247,7 +280,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, int b,
     if (lq4 == 0) sm.ml[wv][lc] = make_float2(m, bad ? NAN : l);
   }
   __syncthreads();
-  for (int i = tid; i < a.G * (D / 4); i += 64 * DW) {
+  for (int i = tid; i < R * (D / 4); i += 64 * DW) {
     const int row = i >> 5, d = 4 * (i & 31);
     float M = -INFINITY;
 #pragma unroll
@@ -369,9 +402,11 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
   }
 }
 
-// Partial rows of one KV head: own parts first. Along the shares and sequences each part adds one to their sum.
+// Partial rows of one KV head: own parts first (along the shares and sequences each part adds one to their
+// sum), then those of the shared pages, by part or by share.
+__device__ __forceinline__ int64_t shared_slots(const PagedArgs& a) { return (int64_t)(a.shares + a.B) * a.G; }
 __device__ __forceinline__ int64_t head_slots(const PagedArgs& a) {
-  return (int64_t)(a.shares + a.B) * a.G + (int64_t)a.np * a.B * a.G;
+  return shared_slots(a) + (int64_t)(a.np ? a.np : a.shared ? a.shares : 0) * a.B * a.G;
 }
 
 template <int NT>  // 16-row tiles of a wave in the shared part; 0: nothing is shared
@@ -390,32 +425,31 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
       const int part = x / a.rb, block = x - part * a.rb;
       const int p0 = (int)((int64_t)a.shared * part / a.np);
       const int p1 = (int)((int64_t)a.shared * (part + 1) / a.np);
-      // listed by the first sequence that is long enough; a shorter one's row may end before them
-      for (int i = 0; i < a.B; i += 64) {
-        const int len = i + lane < a.B ? a.lens[i + lane] : -1;
-        const uint64_t joins = __builtin_amdgcn_ballot_w64(len_ok(a, len) && len >= a.shared * PAGE);
-        if (joins) {
-          shared_part<NT>(a, sm.tile, a.tab.ids + (i + __builtin_ctzll(joins)) * a.tab.stride, hk, p0, p1,
-                          block * 64 * NT,
-                          slot0 + (int64_t)(a.shares + a.B) * a.G + (int64_t)part * a.B * a.G);
-          return;
-        }
-      }
+      if (const int32_t* ids = shared_ids(a, lane))
+        shared_part<NT>(a, sm.tile, ids, hk, p0, p1, block * 64 * NT,
+                        slot0 + shared_slots(a) + (int64_t)part * a.B * a.G);
       return;
     }
     x -= a.np * a.rb;
   }
-  // share x of the own pages of this KV head
-  int total = 0;
-  for (int i = lane; i < a.B; i += 64) total += own_pages(a, a.lens[i]);
-  total = wave_sum_i(total);
-  const int S = share_pages(a, total), u0 = x * S, u1 = min(u0 + S, total);
+  // share x of the pages of this KV head
+  const Deal deal = deal_out(a, lane);
+  const int u0 = x * deal.share, u1 = min(u0 + deal.share, deal.total);
   if (u0 >= u1) return;
-  int b = 0, begin = 0;  // the sequence that holds page u0, and the pages before it
+  const int lc = lane & 15;
+  int u = u0;
+  if (u < deal.lead) {  // shared pages, for all rows of the batch
+    const int e = min(u1, deal.lead), b = lc / a.G;
+    own_part(a, sm.own, shared_ids(a, lane), a.B * a.G, ((int64_t)b * a.Hkv + hk) * a.G + (lc - b * a.G), hk, u, e,
+             a.shared * PAGE, slot0 + shared_slots(a) + (int64_t)x * a.B * a.G);
+    u = e;
+  }
+  if (u == u1) return;
+  int b = 0, begin = deal.lead;  // the sequence that holds u, and the cost before it
   for (int i = 0;; i += 64) {
-    const int n = i + lane < a.B ? own_pages(a, a.lens[i + lane]) : 0;
+    const int n = i + lane < a.B ? own_cost(a, a.lens[i + lane]) : 0;
     const int upto = begin + wave_scan_i(n);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > u0);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > u);
     if (past || i + 64 >= a.B) {
       const int src = past ? __builtin_ctzll(past) : 0;
       b = i + src;
@@ -424,13 +458,16 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
     }
     begin = __builtin_amdgcn_readlane(upto, 63);
   }
-  for (int u = u0; u < u1; ++b) {
+  for (; u < u1; ++b) {
     const int len = a.lens[b], n = own_pages(a, len);
     if (n == 0) continue;
-    const int e = min(u1, begin + n), first = own_first(a, len) - begin;
-    own_part(a, sm.own, b, hk, first + u, first + e, len, slot0 + (int64_t)(x + b) * a.G);
+    begin += SEQ_COST;
+    const int p0 = max(u - begin, 0), p1 = min(u1 - begin, n), first = own_first(a, len);
+    if (p0 < p1)
+      own_part(a, sm.own, a.tab.ids + b * a.tab.stride, a.G, ((int64_t)b * a.Hkv + hk) * a.G + lc, hk, first + p0,
+               first + p1, len, slot0 + (int64_t)(x + b) * a.G);
     begin += n;
-    u = e;
+    u = begin;
   }
 }
 
@@ -455,15 +492,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   const int r = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / (32 * GR)));
   const int row = min((int)(blockIdx.x * (8 / GR)) + r, a.B * a.Hkv * a.G - 1);  // past the last: that again
   const int b = row / (a.Hkv * a.G), h = row - b * a.Hkv * a.G, hk = h / a.G, g = h - hk * a.G;
-  int before = 0, total = 0;
-  for (int i = lane; i < a.B; i += 64) {
-    const int n = own_pages(a, a.lens[i]);
-    before += i < b ? n : 0;
-    total += n;
-  }
-  before = wave_sum_i(before);
-  total = wave_sum_i(total);
-  const int S = share_pages(a, total);
+  const Deal deal = deal_out(a, lane);
+  int before = 0;
+  for (int i = lane; i < b; i += 64) before += own_cost(a, a.lens[i]);
+  before = wave_sum_i(before) + deal.lead + SEQ_COST;
+  const int S = deal.share;
   const int len = a.lens[b];
   const int pages = own_pages(a, len);
   const int first = before / S;
@@ -471,8 +504,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   const bool joins = len_ok(a, len) && a.shared > 0 && len >= a.shared * PAGE;
   const int64_t slot0 = hk * head_slots(a);
   const int64_t own0 = slot0 + (int64_t)(first + b) * a.G + g;
-  const int64_t sh0 = slot0 + (int64_t)(a.shares + a.B) * a.G + (int64_t)b * a.G + g;
-  const int parts = n + (joins ? a.np : 0);
+  const int64_t sh0 = slot0 + shared_slots(a) + (int64_t)b * a.G + g;
+  const int parts = n + (!joins ? 0 : a.np ? a.np : (deal.lead - 1) / S + 1);
   const int grp = (threadIdx.x >> 5) % GR, ln = threadIdx.x & 31;
   float M = -INFINITY, den = 0.0f;
   f4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -506,22 +539,28 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 }
 
 struct DecodeShape {
-  int np, rb, shares, nt;
+  int np, rb, shares, nt, shared;
   int64_t slots;  // partial rows, all heads
 };
 
+// Reading the shared pages once saves B - 1 readings of them; where these are fewer than SHARED_MIN pages of
+// a head, the sequences are attended on their own. (us, shared / each on its own, 8 KV heads: 512 positions
+// of 16 sequences 20.6 / 17.2, 4,096 of 3 18.7 / 17.3, of 6 17.6 / 21.9, 16,384 of 2 22.0 / 23.3.)
+constexpr int64_t SHARED_MIN = 1024;
 DecodeShape decode_shape(int64_t B, int64_t Hkv, int64_t G, int64_t shared, int cus) {
-  DecodeShape s{0, 0, 1, 0, 0};
+  DecodeShape s{0, 0, 1, 0, 0, 0};
+  if ((B - 1) * shared * Hkv >= SHARED_MIN) s.shared = (int)shared;
   const int64_t fill = 2 * cus;  // workgroups that the GPU holds at once
-  if (shared > 0) {
+  const bool blocks = s.shared > 0 && B * G > 16;
+  if (blocks) {
     s.nt = B * G > 64 ? 2 : 1;
     s.rb = (int)((B * G + 64 * s.nt - 1) / (64 * s.nt));
     s.np = (int)std::min<int64_t>((shared + 3) / 4, std::max<int64_t>(1, fill / 2 / (Hkv * s.rb)));
   }
   // beside a shared part's workgroup a CU holds one of the own pages': all run at once (48 sessions behind
   // 16,384 rows 70 -> 65 us, against twice as many in two rounds)
-  s.shares = (int)std::max<int64_t>(1, (shared > 0 ? fill / 2 : fill) / Hkv);
-  s.slots = Hkv * G * (s.shares + B + s.np * B);
+  s.shares = (int)std::max<int64_t>(1, (blocks ? fill / 2 : fill) / Hkv);
+  s.slots = Hkv * G * (s.shares + B + (s.np ? s.np : s.shared ? s.shares : 0) * B);
   return s;
 }
 
@@ -584,7 +623,7 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
   a.B = (int)B;
   a.Hkv = (int)Hkv;
   a.G = (int)G;
-  a.shared = (int)shared_pages;
+  a.shared = s.shared;
   a.np = s.np;
   a.rb = s.rb;
   a.shares = s.shares;
@@ -593,7 +632,7 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
   kern<<<dim3((unsigned)wgs), dim3(64 * DW), 0, (hipStream_t)stream>>>(a);
   LQ_CHECK_LAUNCH("paged_decode_kernel");
   // a row's partials: the shared parts and its share of the own ones
-  if (s.np + s.shares / B > 16)
+  if (s.np + s.shares / std::min<int64_t>(B, 4) > 16)
     paged_merge_kernel<8><<<dim3((unsigned)(B * Hq)), dim3(256), 0, (hipStream_t)stream>>>(a);
   else
     paged_merge_kernel<2><<<dim3((unsigned)((B * Hq + 3) / 4)), dim3(256), 0, (hipStream_t)stream>>>(a);

@@ -280,6 +280,88 @@ def test_decode_reads_table_rows_of_any_stride_and_no_row_behind_the_batch(dev):
     check_decode(out, q, pool, table, lens)
 
 
+# Head layouts, batches and shared positions whose shared pages are read once: dealt out with the own ones (up
+# to 16 query rows), and in blocks of 64 and 128 rows.
+SHARED = [(16, 16, 9, 512), (32, 16, 9, 512), (64, 8, 9, 1024), (6, 1, 23, 4096), (10, 2, 3, 16400)]
+
+
+@pytest.mark.parametrize("hq,kv,B,shared", SHARED)
+def test_shared_pages_read_once(dev, hq, kv, B, shared):
+    """Own lengths from none to several pages; some sequences end before the shared part does or with it,
+    one is empty, the first of all is short."""
+    g = gen(33)
+    lens = [shared + int(n) for n in torch.randint(0, 300, (B,), generator=g)]
+    lens[0] = shared // PAGE * PAGE - 1
+    lens[1] = shared // PAGE * PAGE
+    if B > 3:
+        lens[2], lens[3], lens[B - 1] = 0, 1, shared + 700
+    q, pool, table = decode_case(33, hq, kv, lens, shared, dev)
+    args = (q.to(dev), *pool, table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev))
+    out = paged_decode_attention(*args, SCALE, shared=shared)
+    check_decode(out, q, pool, table, lens)
+    assert (out.float() - paged_decode_attention(*args, SCALE).float()).abs().max() < 2 ** -5
+    check_decode(paged_decode_attention(*args, -0.3, shared=shared), q, pool, table, lens, scale=-0.3,
+                 rows=[0, 1, B - 1])
+    # none as long as the shared part
+    short = [min(n, shared // PAGE * PAGE - 1) for n in lens]
+    args = (*args[:-1], torch.tensor(short, dtype=torch.int32, device=dev))
+    check_decode(paged_decode_attention(*args, SCALE, shared=shared), q, pool, table, short)
+
+
+@pytest.mark.parametrize("hq,kv,B,shared", SHARED[:4])
+def test_shared_pages_that_are_bad(dev, hq, kv, B, shared):
+    lens = [shared + 30 * b for b in range(B)]
+    q, pool, table = decode_case(34, hq, kv, lens, shared, dev)
+    args = (q.to(dev), *pool)
+    n_d = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    told = list(lens)
+    told[0], told[B - 1] = -5, 64 * table.shape[1] + 1
+    own = table.clone()
+    own[2, shared // PAGE] = -1  # sequence 2's first own page
+    out = paged_decode_attention(*args, own.to(dev), n_d(told), SCALE, shared=shared)
+    assert torch.isnan(out[[0, 2, B - 1]]).all()
+    check_decode(out, q, pool, table, lens, rows=[1, 3])
+    bad = table.clone()
+    bad[:, 3] = pool[0][0].shape[0]
+    told = list(lens)
+    told[1] = 150  # ends before the bad page
+    out = paged_decode_attention(*args, bad.to(dev), n_d(told), SCALE, shared=shared)
+    assert torch.isnan(out[[b for b in range(B) if b != 1]]).all()
+    check_decode(out, q, pool, table, told, rows=[1])
+
+
+@pytest.mark.parametrize("hq,kv,B,shared", SHARED[:3])
+def test_shared_pages_captured_and_on_two_streams(dev, hq, kv, B, shared):
+    most = [shared + 200] * B
+    q, pool, table = decode_case(35, hq, kv, most, shared, dev)
+    q_d, t_d = q.to(dev), table.to(dev)
+    n_d = torch.tensor(most, dtype=torch.int32, device=dev)
+    call = lambda: paged_decode_attention(q_d, *pool, t_d, n_d, SCALE, shared=shared)  # noqa: E731
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    graphs, outs = [], []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(st):
+            call()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=st):
+                outs.append(call())
+    torch.cuda.synchronize(dev)
+    for i in range(4):
+        lens = [shared + (37 * b + 50 * i) % 201 for b in range(B)]
+        lens[i] = 40 * i
+        n_d.copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize(dev)
+        for st, graph in zip(streams, graphs):  # both at once
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize(dev)
+        eager = call()
+        for out in outs:
+            assert torch.equal(bits(out), bits(eager))
+        check_decode(eager, q, pool, table, lens, rows=[0, i, B - 1])
+
+
 def test_decode_captured_follows_lengths_and_tables(dev):
     lens = [190, 130]
     q, pool, table = decode_case(14, 8, 2, [256, 256], 128, dev)
