@@ -225,14 +225,14 @@ extern "C" int lq_paged_append(const uint16_t* k, const uint16_t* v, int64_t k_t
   PackedRows rows;
   const int64_t T = pack_rows(counts_host, nseq, &rows);
   if (T < 0) return LQ_EINVAL;
+  if (T == 0) return LQ_OK;
   LQ_CHECK_ARG(k && v && starts, "null pointer");
   LQ_CHECK_ARG((((uintptr_t)k | (uintptr_t)v) & 15) == 0 &&
                    ((k_tok | k_head | v_tok | v_head) & 7) == 0,
                "rows must be 16-byte aligned (strides a multiple of 8)");
   const int64_t units = T * Hkv;
-  LQ_CHECK_ARG(units < (int64_t)1 << 31, "an append of %lld rows is too large for one call",
+  LQ_CHECK_ARG(units < (int64_t)1 << 28, "an append of %lld rows is too large for one call",
                (long long)T);
-  if (T == 0) return LQ_OK;
   paged_append_kernel<<<dim3((unsigned)((units + 15) / 16), 2), dim3(256), 0, (hipStream_t)stream>>>(
       k, v, k_tok, k_head, v_tok, v_head, buf, tab, starts, rows, (uint32_t)units,
       make_fastdiv((uint32_t)Hkv), (int)Hkv);
@@ -254,15 +254,15 @@ extern "C" int lq_paged_gather(const uint8_t* kc, const uint16_t* ks, const uint
   PackedRows rows;
   const int64_t T = pack_rows(counts_host, nseq, &rows);
   if (T < 0) return LQ_EINVAL;
+  if (T == 0) return LQ_OK;
   LQ_CHECK_ARG(k_out && v_out && starts, "null pointer");
   LQ_CHECK_ARG((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "outputs must be 16-byte aligned");
-  if (T == 0) return LQ_OK;
   GatherUnits units;
   units.begin[0] = 0;
   for (int i = 0; i < nseq; ++i)
     units.begin[i + 1] = units.begin[i] + (counts_host[i] ? (counts_host[i] + 62) / PAGE + 1 : 0);
   const int64_t wgs = (int64_t)units.begin[nseq] * Hkv;
-  LQ_CHECK_ARG(wgs < (int64_t)1 << 31, "a gather of %lld rows is too large for one call", (long long)T);
+  LQ_CHECK_ARG(wgs < (int64_t)1 << 24, "a gather of %lld rows is too large for one call", (long long)T);
   paged_gather_kernel<<<dim3((unsigned)wgs, 2), dim3(256), 0, (hipStream_t)stream>>>(
       buf, tab, starts, rows, units, (int)Hkv, k_out, v_out);
   LQ_CHECK_LAUNCH("paged_gather_kernel");

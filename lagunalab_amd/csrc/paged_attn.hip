@@ -570,6 +570,7 @@ int check_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t shared_pages) {
   LQ_CHECK_ARG(Hkv >= 1 && Hkv <= 1024 && Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= 16,
                "Hq=%lld must be 1 to 16 times Hkv=%lld", (long long)Hq, (long long)Hkv);
   LQ_CHECK_ARG(B >= 1 && B <= 4096, "a batch of %lld is not in [1, 4096]", (long long)B);
+  LQ_CHECK_ARG(B * Hq < (1 << 23), "%lld query rows are too many", (long long)(B * Hq));
   LQ_CHECK_ARG(shared_pages >= 0, "%lld shared pages", (long long)shared_pages);
   return LQ_OK;
 }
@@ -615,7 +616,7 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
   }
   LQ_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
   const int64_t wgs = Hkv * ((int64_t)s.np * s.rb + s.shares);
-  LQ_CHECK_ARG(wgs <= INT32_MAX, "too many workgroups");
+  LQ_CHECK_ARG(wgs < (1 << 23), "too many workgroups");
   a.lens = lens;
   a.part_acc = (float*)workspace;
   a.part_ml = (float2*)(a.part_acc + s.slots * 128);

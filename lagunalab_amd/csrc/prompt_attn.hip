@@ -504,7 +504,7 @@ extern "C" int lq_prompt_attn(const uint16_t* q, const uint16_t* k, const uint16
               (long long)need);
     return LQ_EWORKSPACE;
   }
-  LQ_CHECK_ARG(plan.shares * Hkv <= INT32_MAX, "too many workgroups");
+  LQ_CHECK_ARG(plan.shares * Hkv < (1 << 23), "too many workgroups");
   LQ_CHECK_ARG(need == 0 || ((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
   PromptArgs a;
   a.q = q;

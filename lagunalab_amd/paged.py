@@ -55,6 +55,13 @@ def _pool(keys, values):
     return lead[0], lead[1], dev, [t.data_ptr() for t in bufs]
 
 
+def _length(table):
+    """Sequences of a table."""
+    if not torch.is_tensor(table) or table.dim() != 2:
+        raise ValueError("table must be an int32 tensor [sequences, pages]")
+    return table.shape[0]
+
+
 def _ints(x, n, what, dev, dims=1):
     """An int32 tensor on the pool's device, as the kernels read it (``n``: its first dimension)."""
     if not torch.is_tensor(x) or x.dtype != torch.int32 or x.dim() != dims or x.shape[0] != n:
@@ -112,7 +119,7 @@ def paged_append(k, v, keys, values, table, starts, counts=None):
     and biases are those of :func:`lagunalab_amd.quant.quantize`. Rows whose position or page does not
     exist are not stored; no two rows may go to one slot."""
     P, H, dev, ptrs = _pool(keys, values)
-    B, T = table.shape[0], k.shape[0]
+    B, T = _length(table), k.shape[0]
     if counts is None:
         if B == 0 or T % B:
             raise ValueError(f"{T} rows are not the same number for each of {B} sequences")
@@ -139,7 +146,7 @@ def paged_gather(keys, values, table, starts, counts):
     sequence behind the other: ``(k, v)``, each ``[sum(counts), Hkv, 128]``, as
     :func:`lagunalab_amd.quant.dequantize` gives them. Positions whose page does not exist read as NaN."""
     P, H, dev, ptrs = _pool(keys, values)
-    B = table.shape[0]
+    B = _length(table)
     counts = _counts(counts, B)
     table, ts, width = _table(table, B, dev)
     starts = _ints(starts, B, "starts", dev)

@@ -437,7 +437,7 @@ def check_prompt(out, q, k, v, q_lens, k_lens, scale=SCALE, some=None):
     for s, (lq, lk) in enumerate(zip(q_lens, k_lens)):
         rows = range(lq) if some is None or lq <= some else sorted(
             {0, 1, lq - 1, lq // 2} | {int(i) for i in torch.linspace(0, lq - 1, some)})
-        for h in range(hq):
+        for h in range(hq if lq else 0):
             if lk == 0:
                 assert (out[a:a + lq, h] == 0).all()
                 continue
@@ -473,6 +473,24 @@ def test_long_prompts(dev, hq, kv, q_lens, k_lens):
     k, v = randn(g, sum(k_lens), kv, D), randn(g, sum(k_lens), kv, D)
     out = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens)
     check_prompt(out, q, k, v, q_lens, k_lens, some=10)
+
+
+def test_prompts_of_many_blocks(dev):
+    """Enough blocks for every CU to take several whole ones, longest first: chunks, an empty sequence, rows
+    without keys, a V row with an infinity."""
+    g = gen(27)
+    q_lens, k_lens = [3000, 0, 300, 1, 3107], [3000, 50, 100, 1, 3500]
+    q = randn(g, sum(q_lens), 64, D)
+    k, v = randn(g, sum(k_lens), 32, D), randn(g, sum(k_lens), 32, D)
+    out = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens)
+    assert (out[3000:3200] == 0).all()  # of the sequence with more rows than keys
+    check_prompt(out, q, k, v, q_lens, k_lens, some=4)
+    v[1234, 5, 7] = float("inf")
+    hit = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens)
+    same = torch.ones(hit.shape, dtype=torch.bool)
+    same[1234:3000, 10:12, 7] = False
+    assert (bits(hit) == bits(out)).cpu()[same].all()
+    assert torch.isinf(hit[1234:3000, 10:12, 7]).all()
 
 
 @pytest.mark.parametrize("scale,std", [(-SCALE, 1.0), (0.0, 1.0), (1.0, 1.0), (SCALE, 30.0)])
@@ -546,6 +564,66 @@ def test_prompt_captured(dev):
         eager = prompt_attention(q, k, v, q_lens, SCALE, k_lens=k_lens)
         assert torch.equal(bits(out), bits(eager))
         check_prompt(out, q, k, v, q_lens, k_lens, some=12)
+
+
+def test_a_step_captured(dev):
+    """Rows appended, pages copied, rows read back and attended, all in one graph, replayed on new contents."""
+    g = gen(28)
+    lens = [100, 63]
+    q, pool, table = decode_case(28, 8, 2, [n + 1 for n in lens], 0, dev)
+    q_d, t_d = q.to(dev), table.to(dev)
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    k, v = randn(g, 2, 2, D).to(dev), randn(g, 2, 2, D).to(dev)
+    zero = torch.zeros_like(n_d)
+    spare = [p for p in range(pool[0][0].shape[0]) if p not in table.flatten().tolist() + [0]][0]
+
+    def step():
+        paged_append(k, v, *pool, t_d, n_d)
+        copy_pages(*pool, [int(table[0, 0])], [spare])
+        rows = paged_gather(*pool, t_d, zero, [n + 1 for n in lens])
+        out = paged_decode_attention(q_d, *pool, t_d, n_d + 1, SCALE)
+        wide = prompt_attention(q_d.transpose(1, 2).reshape(2, 8, D), *rows, [1, 1], SCALE,
+                                k_lens=[n + 1 for n in lens])
+        return (*rows, out, wide)
+
+    stream = torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = step()
+    torch.cuda.current_stream(dev).wait_stream(stream)
+    for i in range(4):
+        k.copy_(randn(g, 2, 2, D))
+        v.copy_(randn(g, 2, 2, D))
+        q_d.copy_(randn(g, 2, 8, 1, D))
+        torch.cuda.synchronize(dev)
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        held = [x.clone() for x in got]
+        for x, y in zip(held, step()):
+            assert torch.equal(bits(x), bits(y))
+        check_decode(held[2], q_d.cpu(), pool, table, [n + 1 for n in lens])
+        assert (held[2].float().flatten() - held[3].float().flatten()).abs().max() < 2 ** -5
+        for buf in pool:
+            for t in buf:
+                assert torch.equal(bits(t[spare]), bits(t[int(table[0, 0])]))
+
+
+def test_nothing_to_do(dev):
+    pool = page_pool(2, 2, dev)
+    e = torch.empty((0, 2, D), dtype=torch.bfloat16, device=dev)
+    one = torch.zeros((1, 1), dtype=torch.int32, device=dev)
+    n = torch.zeros(1, dtype=torch.int32, device=dev)
+    paged_append(e, e, *pool, one, n, [0])
+    paged_append(e, e, *pool, one[:0], n[:0], [])
+    assert paged_gather(*pool, one, n, [0])[0].shape == (0, 2, D)
+    assert paged_gather(*pool, one[:0], n[:0], [])[1].shape == (0, 2, D)
+    q = torch.ones((0, 4, 1, D), dtype=torch.bfloat16, device=dev)
+    assert paged_decode_attention(q, *pool, one[:0], n[:0], SCALE).shape == (0, 4, 1, D)
+    q = torch.ones((1, 4, 1, D), dtype=torch.bfloat16, device=dev)
+    assert (paged_decode_attention(q, *pool, one, n, SCALE) == 0).all()
 
 
 def test_prompt_of_no_rows(dev):

@@ -40,15 +40,18 @@ def append(lib, **kw):
     (dict(k=260), b"aligned"), (dict(k_tok=130), b"aligned"), (dict(v_head=4), b"aligned"),
     (dict(counts=ints(1, -2)), b"count"), (dict(counts=None), b"counts"), (dict(n=0), b"sequences"),
     (dict(n=65, counts=ints(*[1] * 65)), b"sequences"), (dict(counts=ints(1 << 29, 1 << 29)), b"count"),
-    (dict(kv=8, counts=ints(1 << 28, 1)), b"too large"),
+    (dict(kv=8, counts=ints(1 << 25, 1)), b"too large"),
 ])
 def test_append_refusals(lib, bad, word):
     assert append(lib, **bad) == _lib.LQ_EINVAL
     assert word in lib.lq_last_error()
 
 
-def test_append_of_no_rows_is_no_launch(lib):
-    assert append(lib, counts=ints(0, 0)) == _lib.LQ_OK
+def test_no_rows_are_no_launch(lib):
+    assert append(lib, counts=ints(0, 0), k=None, v=None) == _lib.LQ_OK
+    assert lib.lq_paged_gather(*POOL, 4, 2, 128, 256, 4, 4, 256, ints(0, 0), 2, None, None, None) == _lib.LQ_OK
+    assert lib.lq_prompt_attn(None, None, None, 128, 128, 128, 128, 128, 128, ints(0), ints(5), 1, 4, 2, 128, 0.1,
+                              None, None, 0, None) == _lib.LQ_OK
 
 
 def test_gather_refusals(lib):
@@ -78,7 +81,7 @@ def test_copy_of_no_pages_is_no_launch(lib):
 
 @pytest.mark.parametrize("bad,word", [
     (dict(q=None), b"null"), (dict(q=264), b"aligned"), (dict(lens=None), b"null"), (dict(D=96), b"head_dim"),
-    (dict(hq=9), b"Hq"), (dict(hq=34), b"Hq"), (dict(B=0), b"batch"), (dict(B=4097), b"batch"),
+    (dict(hq=9), b"Hq"), (dict(hq=34), b"Hq"), (dict(kv=1024, hq=16384, B=512), b"too many"), (dict(B=0), b"batch"), (dict(B=4097), b"batch"),
     (dict(shared=5), b"shared"), (dict(shared=-1), b"shared"), (dict(scale=float("nan")), b"scale"),
     (dict(scale=float("inf")), b"scale"), (dict(wsb=1000), b"workspace"), (dict(ws=None), b"workspace"),
 ])
@@ -146,6 +149,8 @@ def test_arguments_that_do_not_fit():
     with pytest.raises(ValueError):
         paged.page_pool(0, 2, device="cpu")
     keys, values = paged.page_pool(4, 2, device="cpu")
+    with pytest.raises(ValueError, match="values are"):
+        paged.paged_gather(keys[:2], values, torch.zeros(1, 1), None, [1])
     with pytest.raises(ValueError, match="contiguous"):
         paged.paged_gather((keys[0].transpose(0, 1), *keys[1:]), values, torch.zeros(1, 1), None, [1])
     with pytest.raises(ValueError, match="contiguous"):
