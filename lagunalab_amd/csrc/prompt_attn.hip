@@ -4,9 +4,9 @@
 // keys 0 .. k_lens[s] - q_lens[s] + i, so a prompt has as many of both and a chunk of one more keys. Rows
 // without a key are 0.
 //
-// Work: a workgroup of 8 waves takes 256 query rows of a KV head, numbered position-major (row f is
-// position f / G of query head f % G), so that any grouping fills the matrix cores and a block's rows see
-// nearly the same keys; a wave has 32 of them. It walks the 64-key tiles up to its last row's bound, each
+// Work: a workgroup of 8 waves (or 4, see below) takes 256 query rows (128) of a KV head, numbered
+// position-major (row f is position f / G of query head f % G), so that any grouping fills the matrix cores
+// and a block's rows see nearly the same keys; a wave has 32 of them. It walks the 64-key tiles up to its last row's bound, each
 // copied into LDS once for all waves (three buffers of K and of V, copies two tiles ahead) and run through
 // attn_tile.h. A SIMD holds one wave of each half of the workgroup, and the halves run one phase apart, so
 // that one's matrix phase (P.V of a tile, Q.K^T of the next) lies beside the other's vector phase (softmax,
@@ -16,15 +16,19 @@
 //   2t      Q.K^T(t), P.V(t-1)        softmax(t-1), copies K(t+2) V(t+1)
 //   2t+1    softmax(t), copies        Q.K^T(t), P.V(t-1)
 //
-// The work is dealt out in equal shares of tiles: the blocks of all sequences stand one behind the other (of
-// a sequence the last, the first, the last but one, .., so that two neighbours cost about the same
-// everywhere and cuts are few), a block costing its tiles and BLOCK_COST for its start and end, and a
-// workgroup takes one share, which may begin and end inside blocks. Parts of blocks go to the workspace and a second launch merges them. One
-// share per CU (several where they are long), so that every CU ends at the same time whatever the lengths
-// are: 2,048 rows, 32/8 heads, in whole blocks would be 32 tiles for the last workgroup and 1 for the
-// first. A workgroup finds its share by scanning the blocks of a sequence, a lane each; nothing of the
-// plan but the sequences' costs comes from the host. The KV head is the fastest index, so that neighbouring
-// workgroups (XCDs) hold different heads and each XCD's L2 the K and V of few.
+// The small workgroups have 4 waves, 128 rows and two buffers each, a barrier per tile, and share a CU in
+// twos: what the halves above do for each other, the two do by chance. Slower by 3% where blocks are long,
+// faster where they are short (prompt_plan has the rule and what it measured).
+//
+// The work is dealt out in whole blocks, longest first, or in equal shares of tiles. For these the blocks of
+// all sequences stand one behind the other (of a sequence the last, the first, the last but one, .., so that
+// two neighbours cost about the same everywhere and cuts are few), a block costing its tiles and BLOCK_COST
+// for its start and end, and a workgroup takes one share, which may begin and end inside blocks. Parts of
+// blocks go to the workspace and a second launch merges them. A workgroup finds its block or share by scanning
+// the blocks, a lane each; nothing of the plan but the sequences' costs comes from the host. Where all small
+// workgroups are resident at once, those beyond one per CU stand in ascending order, so that a CU holds a
+// long and a short one (2,048 rows, 32/8 heads: 53.3 -> 51.4 us). The KV head is the fastest index, so that
+// neighbouring workgroups (XCDs) hold different heads and each XCD's L2 the K and V of few.
 //
 // Keys that a row does not see reach it in no way: masked scores are -infinity, and an infinity or NaN in
 // V of a tile that is masked for some row of the block goes only to the rows that see its key (0 times it
@@ -38,9 +42,9 @@ namespace {
 
 using namespace attn;
 
-constexpr int PW = 8;          // waves per workgroup
 constexpr int NT = 2;          // 16-row tiles per wave
-constexpr int PROWS = 16 * NT * PW;
+constexpr int PROWS = 256;     // rows of a block; SROWS where the workgroups are small
+constexpr int SROWS = 128;
 constexpr int BLOCK_COST = 4;  // of a block's start and end, in tiles
 constexpr int MIN_PART = 2;    // tiles of a block's part: nearer cuts move to the block's end
 
@@ -57,13 +61,15 @@ struct PromptArgs {
   float sl2;
   int64_t share;           // cost of a share; 0: a workgroup takes one whole block
   int longest;             // tiles of the longest block
+  int paired;              // whole blocks from this rank on in ascending order, -1: none
   int q_begin[LQ_MAX_SEQS + 1], k_begin[LQ_MAX_SEQS + 1];
   int64_t cost[LQ_MAX_SEQS + 1];  // of the blocks before each sequence
 };
 
-// 64-key tiles that block blk of a sequence of R rows needs; base: row i sees keys <= base + i.
+// 64-key tiles that block blk (of ROWS rows) of a sequence of R rows needs; base: row i sees keys <= base + i.
+template <int ROWS = PROWS>
 __host__ __device__ __forceinline__ int block_tiles(int blk, int R, FastDiv g, int base) {
-  const int last = base + (int)fdiv_u((uint32_t)min(blk * PROWS + PROWS - 1, R - 1), g);
+  const int last = base + (int)fdiv_u((uint32_t)min(blk * ROWS + ROWS - 1, R - 1), g);
   return last < 0 ? 0 : last / TKEYS + 1;
 }
 
@@ -105,12 +111,13 @@ __device__ __forceinline__ Block find_block(const PromptArgs& a, int64_t u, int 
 // The block of rank x when all are in order of their tiles, most first: how many have at least n tiles is a
 // sum over the sequences, a lane each, and the largest n that more than x have is found by halving. Its cost
 // is counted from its own begin.
+template <int ROWS>
 __device__ __forceinline__ Block ranked_block(const PromptArgs& a, int x, int lane) {
   const int sl = min(lane, a.nseq - 1);
-  const int R = lane < a.nseq ? seq_rows(a, sl) : 0, base = seq_base(a, sl), nb = (R + PROWS - 1) / PROWS;
+  const int R = lane < a.nseq ? seq_rows(a, sl) : 0, base = seq_base(a, sl), nb = (R + ROWS - 1) / ROWS;
   auto from = [&](int n) {  // first block of the lane's sequence with at least n tiles (of nb: none)
     const int64_t y = a.G * ((int64_t)TKEYS * (n - 1) - base);  // the row that has to be reached
-    return n <= 0 || y <= 0 ? 0 : y > R - 1 ? nb : (int)(y / PROWS);
+    return n <= 0 || y <= 0 ? 0 : y > R - 1 ? nb : (int)(y / ROWS);
   };
   int lo = 0, hi = a.longest + 1;  // all have lo, none has hi
   int above = 0;                   // blocks with at least hi tiles
@@ -134,18 +141,25 @@ __device__ __forceinline__ int cut_tile(const Block& b, int64_t u) {
   return t >= b.tiles ? b.tiles : t < MIN_PART ? 0 : t > b.tiles - MIN_PART ? b.tiles : (int)t;
 }
 
-constexpr int STAGES = 3;  // tiles of K and of V in LDS
+template <int STAGES>  // tiles of K and of V in LDS
 struct PromptSmem {
   alignas(256) uint16_t k[STAGES][TKEYS * D];
   alignas(256) uint16_t v[STAGES][TKEYS * D];
-  uint32_t nonfinite[STAGES][2];  // keys of a masked tile whose V holds an infinity or NaN
+  uint32_t nonfinite[3][2];  // keys of tile t % 3, if masked, whose V holds an infinity or NaN
 };
 
+template <int PW>  // waves: 8, or 4 for small workgroups, two per CU
 __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArgs a) {
-  __shared__ PromptSmem sm;
+  constexpr bool HALVES = PW == 8;
+  constexpr int ROWS = 16 * NT * PW, STAGES = HALVES ? 3 : 2;
+  constexpr int CP = 16 / PW;  // copies of a wave per tile, K and V each
+  static_assert(ROWS == (HALVES ? PROWS : SROWS), "block sizes");
+  __shared__ PromptSmem<STAGES> sm;
   const int share = blockIdx.x / a.Hkv, hk = blockIdx.x - share * a.Hkv;
-  Block b = a.share ? find_block(a, a.share * share, threadIdx.x & 63)
-                    : ranked_block(a, share, threadIdx.x & 63);
+  const int blocks = gridDim.x / a.Hkv;
+  const int rank = (uint32_t)share < (uint32_t)a.paired ? share : blocks - 1 - (share - a.paired);
+  Block b = HALVES && a.share ? find_block(a, a.share * share, threadIdx.x & 63)
+                              : ranked_block<ROWS>(a, rank, threadIdx.x & 63);
   const int64_t u0 = a.share * share;  // 0 for a whole block
   const int64_t u1 = a.share ? min(u0 + a.share, a.cost[a.nseq]) : b.tiles + BLOCK_COST;
   for (bool more = true; more;) {
@@ -154,50 +168,52 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   asm volatile("" : "+v"(tid));
   const int lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const bool grp_a = wv < PW / 2;
+  const bool grp_a = HALVES && wv < PW / 2;
   const int lc = lane & 15, lq4 = lane >> 4;
   const int s = b.seq, blk = b.blk;
   const int q0 = a.q_begin[s], lq = a.q_begin[s + 1] - q0;
   const int k0 = a.k_begin[s], lk = a.k_begin[s + 1] - k0;
   const int R = lq * a.G, base = lk - lq;
   const int tiles = b.tiles;
-  const int t0 = cut_tile(b, u0), t1 = cut_tile(b, u1);
+  const int t0 = HALVES ? cut_tile(b, u0) : 0, t1 = HALVES ? cut_tile(b, u1) : tiles;
   // a block without a tile (rows without keys) belongs to the share that its begin lies in
   const bool mine = t0 < t1 || (tiles == 0 && b.begin >= u0 && b.begin < u1);
   if (mine) {
   const float scale = abs_scale(a.sl2);
   // tiles from here on are masked for some row of the block (or end behind the last key)
-  const int low = base + (int)fdiv_u((uint32_t)(blk * PROWS), a.g);
+  const int low = base + (int)fdiv_u((uint32_t)(blk * ROWS), a.g);
   const int t_masked = low < 0 ? 0 : (low + 1) / TKEYS;
 
-  // ---- copies: wave wv brings keys 8 wv .. 8 wv + 7 of every tile, K and V 1 KB (4 keys) at a time; a
+  // ---- copies: wave wv brings 4 CP keys from 4 CP wv on of every tile, K and V 1 KB (4 keys) at a time; a
   // lane's 16 bytes land at lane x 16, so the swizzle is in the chunk it reads. Keys past the last one
   // read it again.
-  const int krow = 8 * wv + (lane >> 4);  // and + 4
+  const int krow = 4 * CP * wv + (lane >> 4);  // and + 4, ..
   const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + (int64_t)k0 * a.k_tok + hk * a.k_head);
   const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + (int64_t)k0 * a.v_tok + hk * a.v_head);
-  const uint32_t k_at = lds_u32(sm.k) + 2048u * wv, v_at = lds_u32(sm.v) + 2048u * wv;
+  const uint32_t k_at = lds_u32(sm.k) + 1024u * CP * wv, v_at = lds_u32(sm.v) + 1024u * CP * wv;
   // A tile's base is scalar, a lane's offset in it fixed but in the tile that ends behind the last key.
-  auto copy = [&](const uint8_t* from, int64_t tok, int t, uint32_t to, const uint32_t (&at)[2], bool is_v) {
+  auto copy = [&](const uint8_t* from, int64_t tok, int t, uint32_t to, const uint32_t (&at)[CP], bool is_v) {
     const int tt = min(t, t1 - 1);
     const uint8_t* sb = from + 2 * TKEYS * tok * tt;
     const uint32_t m = __builtin_amdgcn_readfirstlane(to + (uint32_t)(t % STAGES) * (TKEYS * D * 2));
-    uint32_t o[2] = {at[0], at[1]};
+    uint32_t o[CP];
+#pragma unroll
+    for (int i = 0; i < CP; ++i) o[i] = at[i];
     if (TKEYS * tt + TKEYS > lk) {  // uniform
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < CP; ++i) {
         const int r = krow + 4 * i;
         o[i] = 2 * (uint32_t)tok * (uint32_t)min(r, lk - 1 - TKEYS * tt) + 16 * (lc ^ (is_v ? 2 * (r & 7) : r & 15));
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < CP; ++i)
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                    :: "v"(o[i]), "s"(sb), "s"(m + 1024u * i) : "memory");
   };
-  uint32_t ko[2], vo[2];
+  uint32_t ko[CP], vo[CP];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < CP; ++i) {
     const int r = krow + 4 * i;
     ko[i] = 2 * (uint32_t)a.k_tok * r + 16 * (lc ^ (r & 15));
     vo[i] = 2 * (uint32_t)a.v_tok * r + 16 * (lc ^ (2 * (r & 7)));
@@ -207,15 +223,15 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   // The wave's own V rows of tile t, in LDS: infinities and NaN become 0 and their keys are noted.
   auto scan_v = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint4* at = reinterpret_cast<uint4*>(&sm.v[t % STAGES][(8 * wv + 4 * i) * D + 8 * lane]);
+    for (int i = 0; i < CP; ++i) {
+      uint4* at = reinterpret_cast<uint4*>(&sm.v[t % STAGES][(4 * CP * wv + 4 * i) * D + 8 * lane]);
       const uint4 u = *at;
       uint32_t m = bf16x2_absmax_bits(bf16x2_absmax_bits(0, u.x), u.y);
       m = bf16x2_absmax_bits(bf16x2_absmax_bits(m, u.z), u.w);
       const int key = krow + 4 * i;
       if ((m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u) {
         *at = make_uint4(finite_bf2(u.x), finite_bf2(u.y), finite_bf2(u.z), finite_bf2(u.w));
-        atomicOr(&sm.nonfinite[t % STAGES][key >> 5], 1u << (key & 31));
+        atomicOr(&sm.nonfinite[t % 3][key >> 5], 1u << (key & 31));
       }
     }
   };
@@ -228,7 +244,7 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   }
 
   // ---- the wave's rows
-  const int f0 = blk * PROWS + 16 * NT * wv;
+  const int f0 = blk * ROWS + 16 * NT * wv;
   TileRows<NT> st;
   int lim[NT];  // last key of the lane's row, -1: none
 #pragma unroll
@@ -247,16 +263,19 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
 
   f4_t c[NT][4];
   bf16x8_t p[NT][2];
-  // V(t) of the wave's copies has landed (4 newer ones are out)
+  // V(t) of the wave's copies has landed (with 8 waves 4 newer ones are out)
   auto landed = [&](int t) {
-    asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    if constexpr (HALVES)
+      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // and K(t + 1)
     if (t >= t_masked) scan_v(t);  // workgroup-uniform
   };
   if (t0 < t1) {
-    if (tid < 2 * STAGES) sm.nonfinite[tid >> 1][tid & 1] = 0;
-    asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    if (tid < 6) sm.nonfinite[tid >> 1][tid & 1] = 0;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * CP) : "memory");  // K(t0)
     lds_barrier();
-    if (!grp_a) {  // half a tile behind
+    if (HALVES && !grp_a) {  // half a tile behind
       copy_k(t0 + 2);
       copy_v(t0 + 1);
       asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t0 + 1)
@@ -270,9 +289,9 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
         landed(t);
       lds_barrier();
       // vector phase
-      __builtin_amdgcn_s_setprio(1);
-      copy_k(t + (grp_a ? 2 : 3));
-      copy_v(t + (grp_a ? 1 : 2));
+      __builtin_amdgcn_s_setprio(HALVES);
+      copy_k(t + (grp_a || !HALVES ? 2 : 3));
+      copy_v(t + (grp_a || !HALVES ? 1 : 2));
       if (TKEYS * t + TKEYS - 1 > lim_lo) {  // wave-uniform: masked for some row
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -282,35 +301,40 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
             for (int r = 0; r < 4; ++r)
               c[nt][mt][r] = TKEYS * t + 16 * mt + 4 * lq4 + r <= lim[nt] ? c[nt][mt][r] : -INFINITY;
       }
-      tile_softmax<NT>(c, st, scale, p);
       Ahead ahead;
-      tile_ahead(sm.k[(t + 1) % STAGES], lane, ahead);
-      if (grp_a)
-        landed(t);
-      else
-        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t + 2)
-      lds_barrier();
+      if constexpr (HALVES) {
+        tile_softmax<NT>(c, st, scale, p);
+        tile_ahead(sm.k[(t + 1) % STAGES], lane, ahead);
+        if (grp_a)
+          landed(t);
+        else
+          asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t + 2)
+        lds_barrier();
+      } else {
+        tile_ahead(sm.k[(t + 1) % STAGES], lane, ahead);
+        tile_softmax<NT>(c, st, scale, p);
+      }
       // matrix phase: Q.K^T of tile t + 1 (behind the last one, of a copy nobody reads), P.V of tile t
-      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_s_setprio(!HALVES);
       tile_matrix<NT>(sm.k[(t + 1) % STAGES], sm.v[t % STAGES], st, lane, c, p, ahead);
       if (t >= t_masked) {
-        uint64_t nf = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % STAGES][0]) |
-                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % STAGES][1]) << 32;
+        uint64_t nf = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % 3][0]) |
+                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % 3][1]) << 32;
         for (; nf; nf &= nf - 1) {  // rare
           const int key = __builtin_ctzll(nf), at = TKEYS * t + key;
           if (at < lk) tile_nonfinite<NT>(vbase + 2 * a.v_tok * at, key, at, st, lane, p, lim);
         }
       }
-      // read by the other half for the last time a slot ago: group A clears what tile t + 2 will note
-      if (tid < 2) sm.nonfinite[(t + 2) % STAGES][tid] = 0;
+      // last read before the barrier ahead of this phase: what tile t + 2 will note
+      if (tid < 2) sm.nonfinite[(t + 2) % 3][tid] = 0;
     }
-    if (grp_a) lds_barrier();
+    if (HALVES && grp_a) lds_barrier();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies past the last tile
   }
 
   // ---- rows out: dims 16 w + 4 lq4 + r
-  const bool part = t1 - t0 < tiles;
-  const int64_t prow = ((int64_t)(2 * share + (t0 == 0)) * a.Hkv + hk) * PROWS;
+  const bool part = HALVES && t1 - t0 < tiles;
+  const int64_t prow = ((int64_t)(2 * share + (t0 == 0)) * a.Hkv + hk) * ROWS;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int f = f0 + 16 * nt + lc;
@@ -335,7 +359,7 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   }
   // the next block
   const int64_t next = b.begin + b.tiles + BLOCK_COST;
-  more = next < u1;
+  more = HALVES && next < u1;
   if (more) {
     int ns = b.seq, place = b.place + 1;
     if (place * PROWS >= R) {
@@ -404,21 +428,36 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptArgs a) {
   }
 }
 
-// Cost of the blocks of every sequence, and the share of a workgroup: one per CU. Where there are
-// WHOLE_ROUNDS blocks and more for each CU they are taken whole instead, longest first: then the last
-// round evens itself out, nothing is merged, and the workgroups of a head walk its keys together, which the
-// L2 likes (16,384 rows, 32/8 heads, 8 blocks per CU: 1,825 us whole, 2,040 in shares; 2,048 rows, one
-// block per CU: see above).
+// How the work is dealt out, with the cost of the blocks of every sequence. Three ways (us at 32/8 heads but
+// where said; on gfx950, 256 CUs):
+//
+//  - whole blocks of 256 rows, longest first, where there are WHOLE_ROUNDS and more for each CU and they are
+//    long: the last round evens itself out, nothing is merged, and the workgroups of a head walk its keys
+//    together, which the L2 likes (16,384 rows: 1,840, in shares 2,040, small 1,905).
+//  - small workgroups, whole blocks of 128 rows, two per CU: nothing is merged either, a block's start and end
+//    lie beside the other workgroup's tiles, and the rows that a short sequence leaves unused in its last block
+//    are fewer (128 rows: 12.9, in shares 17.0; 2,048: 51.4 and 59.0; 5,000: 200 and 214; 64 prompts of 400
+//    rows: 198, as whole blocks of 256 rows 241).
+//  - shares of equal cost, one per CU, where the blocks are few and long, so that whole ones would leave CUs
+//    idle (512 rows on 7,681: 82, small 169).
+//
+// Small workgroups are taken where their time comes out lower, in units of 0.03 us: 40 per tile of the longest
+// block (alone on its CU), 31 per tile of all and 31 per tile that a CU with fewer blocks has to wait (counted
+// as the shortest; 40 where the last block is alone), against 60 per tile of a share and 240 for parts and
+// merge. Over 170 shapes of 1 to 64 sequences and 8 to 64 heads the choice was the faster by up to 45%, and
+// the slower by more than 2% in one (8 prompts of 1,000 rows: 95.4, in shares 92.6).
 constexpr int64_t WHOLE_ROUNDS = 6;
+constexpr int64_t WHOLE_TILES = 48;  // per block of 128 rows
 struct PromptPlan {
   int64_t cost[LQ_MAX_SEQS + 1], share, shares;  // share 0: whole blocks, `shares` of them
-  int longest;
+  int longest, paired;
+  bool small;  // whole blocks of SROWS rows
 };
 PromptPlan prompt_plan(const int32_t* q_lens, const int32_t* k_lens, int64_t nseq, int64_t Hkv, int64_t G,
                        int cus) {
   PromptPlan p{};
   const FastDiv g = make_fastdiv((uint32_t)G);
-  int64_t blocks = 0;
+  int64_t blocks = 0, sblocks = 0, stiles = 0, shortest = INT64_MAX;
   for (int s = 0; s < LQ_MAX_SEQS; ++s) {
     int64_t c = 0;
     const int R = s < nseq ? (int)(q_lens[s] * G) : 0;
@@ -427,16 +466,30 @@ PromptPlan prompt_plan(const int32_t* q_lens, const int32_t* k_lens, int64_t nse
       p.longest = std::max(p.longest, t);
       c += t + BLOCK_COST;
       ++blocks;
+      const int ts = block_tiles<SROWS>(2 * b, R, g, k_lens[s] - q_lens[s]);
+      const bool two = b * PROWS + SROWS < R;
+      sblocks += 1 + two;
+      stiles += ts + (two ? t : 0);
+      shortest = std::min<int64_t>(shortest, ts);
     }
     p.cost[s + 1] = p.cost[s] + c;
   }
-  if (blocks * Hkv >= WHOLE_ROUNDS * cus) {
+  p.paired = -1;
+  if (blocks * Hkv >= WHOLE_ROUNDS * cus && stiles >= WHOLE_TILES * sblocks) {
     p.shares = blocks;
     return p;
   }
   const int64_t total = p.cost[nseq], per_head = std::max<int64_t>(1, cus / Hkv);
   p.share = std::max<int64_t>(BLOCK_COST + MIN_PART, (total + per_head - 1) / per_head);
   p.shares = (total + p.share - 1) / p.share;
+  const int64_t n = sblocks * Hkv, most = (n + cus - 1) / cus;  // small blocks, and of a CU
+  const int64_t idle = 31 * (most * cus - n) * shortest / cus + most % 2 * 9 * shortest;
+  if (std::max<int64_t>(40 * p.longest, 31 * stiles * Hkv / cus + idle) <= 60 * p.share + 240) {
+    p.small = true;
+    p.share = 0;
+    p.shares = sblocks;
+    if (n <= 2 * cus) p.paired = (int)per_head;
+  }
   return p;
 }
 
@@ -526,6 +579,7 @@ extern "C" int lq_prompt_attn(const uint16_t* q, const uint16_t* k, const uint16
   a.sl2 = scale * 1.4426950408889634f;
   a.share = plan.share;
   a.longest = plan.longest;
+  a.paired = plan.paired;
   a.q_begin[0] = a.k_begin[0] = 0;
   for (int s = 0; s < LQ_MAX_SEQS; ++s) {
     a.q_begin[s + 1] = a.q_begin[s] + (s < nseq ? q_lens_host[s] : 0);
@@ -533,7 +587,11 @@ extern "C" int lq_prompt_attn(const uint16_t* q, const uint16_t* k, const uint16
     a.cost[s] = plan.cost[s];
   }
   a.cost[LQ_MAX_SEQS] = plan.cost[LQ_MAX_SEQS];
-  prompt_attn_kernel<<<dim3((unsigned)(plan.shares * Hkv)), dim3(64 * PW), 0, (hipStream_t)stream>>>(a);
+  const dim3 grid((unsigned)(plan.shares * Hkv));
+  if (plan.small)
+    prompt_attn_kernel<4><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a);
+  else
+    prompt_attn_kernel<8><<<grid, dim3(512), 0, (hipStream_t)stream>>>(a);
   LQ_CHECK_LAUNCH("prompt_attn_kernel");
   if (need > 0) {
     prompt_merge_kernel<<<dim3((unsigned)((plan.shares - 1) * Hkv), PROWS / MERGE_ROWS), dim3(256), 0,

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from lagunalab_amd import _lib
 from lagunalab_amd.paged import (copy_pages, page_pool, paged_append, paged_decode_attention,
                                  paged_gather)
 from lagunalab_amd.prompt_attn import prompt_attention
@@ -518,6 +519,33 @@ def test_prompt_heads_first_layout(dev):
     g = gen(24)
     q, k, v = (randn(g, h, 90, D).to(dev).transpose(0, 1) for h in (6, 2, 2))
     check_prompt(prompt_attention(q, k, v, [90], SCALE), q, k, v, [90], [90])
+
+
+@pytest.mark.parametrize("hq,kv,q_lens,k_lens,parts", [
+    (8, 2, [700, 0, 1, 130, 64, 40], [700, 9, 1, 130, 190, 33], False),  # small blocks, all resident
+    (64, 8, [900] * 3 + [77], [900] * 3 + [600], False),                  # small blocks, several rounds
+    (8, 2, [260, 33], [9000, 4444], True),                                # shares that end inside blocks
+    (256, 4, [1600], [7000], False),                                      # large blocks, several rounds
+])
+def test_prompt_ways_of_dealing_out(dev, hq, kv, q_lens, k_lens, parts):
+    """Every way of dealing out the blocks, without and with an infinity in a V row that some rows see."""
+    from array import array
+    g = gen(31)
+    lq, lk = array("i", q_lens), array("i", k_lens)
+    need = _lib.load().lq_prompt_workspace_bytes(lq.buffer_info()[0], lk.buffer_info()[0], len(lq), hq, kv)
+    assert (need > 0) == parts
+    q = randn(g, sum(q_lens), hq, D)
+    k, v = randn(g, sum(k_lens), kv, D), randn(g, sum(k_lens), kv, D)
+    out = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens)
+    check_prompt(out, q, k, v, q_lens, k_lens, some=4)
+    G, row = hq // kv, q_lens[0] // 2  # the first row of the first sequence that sees the key
+    key = k_lens[0] - q_lens[0] + row
+    v[key, 1, 7] = float("inf")
+    hit = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens)
+    same = torch.ones(hit.shape, dtype=torch.bool)
+    same[row:q_lens[0], G:2 * G, 7] = False
+    assert (bits(hit) == bits(out)).cpu()[same].all()
+    assert not hit[row:q_lens[0], G:2 * G, 7].isfinite().any()
 
 
 @pytest.mark.parametrize("what", ["k nan", "k inf", "v nan", "v inf"])
