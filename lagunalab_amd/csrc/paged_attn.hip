@@ -8,7 +8,8 @@
 // for the G <= 16 rows, one page per wave at a time, through the wave's own LDS (no barriers), the next
 // page's loads out while it computes. With up to 16 query rows in the batch the shared pages are dealt out
 // with the own ones, in front of them, as those of one sequence with all the rows. Both kinds write
-// partial rows (max, sum, weighted values), which a second launch merges.
+// partial rows (max, sum, weighted values), which a second launch merges. Where table rows list few pages a
+// workgroup takes a whole sequence instead, and writes its output rows (short_waves has the rule).
 //
 // Lengths are read on the device, so one recorded launch serves every step of a growing batch: every
 // workgroup adds up the sequences' own pages and finds its share of them. Workgroups without one leave at
@@ -94,11 +95,12 @@ __device__ __forceinline__ const int32_t* shared_ids(const PagedArgs& a, int lan
   return nullptr;
 }
 
+template <int WV>  // waves
 struct OwnSmem {
   // a page's codes, per wave: 16-byte chunk c of row r of K at c ^ kswz(r), of V at c ^ vswz(r)
-  alignas(16) uint8_t k[DW][PAGE * D], v[DW][PAGE * D];
-  uint32_t w[DW][4][PAGE];  // its K scale, K bias, V scale, V bias words
-  float2 ml[DW][16];
+  alignas(16) uint8_t k[WV][PAGE * D], v[WV][PAGE * D];
+  uint32_t w[WV][4][PAGE];  // its K scale, K bias, V scale, V bias words
+  float2 ml[WV][16];
 };
 // A page on its way: rows 8 i + lane / 8 of K and V, the words of row `lane`. Read once: non-temporal (8
 // sessions of 42,771 to 82,671 rows 244 -> 229 us), in whole lines (K as MFMA operands straight from memory
@@ -131,8 +133,9 @@ __device__ __forceinline__ void wave_fence() {  // LDS of the wave's own: order 
 }
 
 // Pages [p0, p1) listed at ids, of a sequence of len positions, for R <= 16 query rows (row lane % 16 of them
-// at qrow).
-__device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, const int32_t* ids, int R,
+// at qrow): partial rows to slot .., or with WHOLE output rows from slot on.
+template <int WV, bool WHOLE>
+__device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, const int32_t* ids, int R,
                                          int64_t qrow, int hk, int p0, int p1, int len, int64_t slot) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -164,7 +167,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, const 
   PageRegs cur;
   int p = p0 + wv;
   if (p < p1) load_page(a, page_row(p), lane, cur);
-  for (; p < p1; p += DW) {
+  for (; p < p1; p += WV) {
     const int limit = min(PAGE, len - p * PAGE);  // keys of the page that are the sequence's
     // to LDS, and the next page's loads out at once; V words of keys past the length 0, so that their
     // slots' contents reach nothing
@@ -177,7 +180,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, const 
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) sm.w[wv][i][lane] = i < 2 || lane < limit ? cur.w[i] : 0u;
-    if (p + DW < p1) load_page(a, page_row(p + DW), lane, cur);
+    if (p + WV < p1) load_page(a, page_row(p + WV), lane, cur);
     wave_fence();
     // scores
     f4_t c[4];
@@ -280,16 +283,16 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, const 
     if (lq4 == 0) sm.ml[wv][lc] = make_float2(m, bad ? NAN : l);
   }
   __syncthreads();
-  for (int i = tid; i < R * (D / 4); i += 64 * DW) {
+  for (int i = tid; i < R * (D / 4); i += 64 * WV) {
     const int row = i >> 5, d = 4 * (i & 31);
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < DW; ++w) M = max_ieee(M, sm.ml[w][row].x);
+    for (int w = 0; w < WV; ++w) M = max_ieee(M, sm.ml[w][row].x);
     const float Mr = M == -INFINITY ? 0.0f : M;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     float L = 0.0f;
 #pragma unroll
-    for (int w = 0; w < DW; ++w) {
+    for (int w = 0; w < WV; ++w) {
       const float2 ml = sm.ml[w][row];
       const float e = ml.x == -INFINITY ? 0.0f : exp2_nonpos(ml.x - Mr);
       const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.v[w]) + row * D + d);
@@ -298,6 +301,12 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem& sm, const 
       s.z = fmaf(e, x.z, s.z);
       s.w = fmaf(e, x.w, s.w);
       L = fmaf(ml.x == -INFINITY ? 1.0f : e, ml.y, L);
+    }
+    if constexpr (WHOLE) {
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // no keys: 0; a sum that is NaN stays
+      *reinterpret_cast<uint2*>(a.out + (slot + row) * D + d) =
+          make_uint2(pack_bf2(s.x * inv, s.y * inv), pack_bf2(s.z * inv, s.w * inv));
+      continue;
     }
     *reinterpret_cast<float4*>(a.part_acc + (slot + row) * D + d) = s;
     if (d == 0) a.part_ml[slot + row] = make_float2(M, L);
@@ -412,7 +421,7 @@ __device__ __forceinline__ int64_t head_slots(const PagedArgs& a) {
 template <int NT>  // 16-row tiles of a wave in the shared part; 0: nothing is shared
 __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
   __shared__ union Smem {
-    OwnSmem own;
+    OwnSmem<DW> own;
     KvTile tile[NT ? 2 : 1];
     __device__ Smem() {}
   } sm;
@@ -440,7 +449,7 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
   int u = u0;
   if (u < deal.lead) {  // shared pages, for all rows of the batch
     const int e = min(u1, deal.lead), b = lc / a.G;
-    own_part(a, sm.own, shared_ids(a, lane), a.B * a.G, ((int64_t)b * a.Hkv + hk) * a.G + (lc - b * a.G), hk, u, e,
+    own_part<DW, false>(a, sm.own, shared_ids(a, lane), a.B * a.G, ((int64_t)b * a.Hkv + hk) * a.G + (lc - b * a.G), hk, u, e,
              a.shared * PAGE, slot0 + shared_slots(a) + (int64_t)x * a.B * a.G);
     u = e;
   }
@@ -464,11 +473,26 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
     begin += SEQ_COST;
     const int p0 = max(u - begin, 0), p1 = min(u1 - begin, n), first = own_first(a, len);
     if (p0 < p1)
-      own_part(a, sm.own, a.tab.ids + b * a.tab.stride, a.G, ((int64_t)b * a.Hkv + hk) * a.G + lc, hk, first + p0,
+      own_part<DW, false>(a, sm.own, a.tab.ids + b * a.tab.stride, a.G, ((int64_t)b * a.Hkv + hk) * a.G + lc, hk, first + p0,
                first + p1, len, slot0 + (int64_t)(x + b) * a.G);
     begin += n;
     u = begin;
   }
+}
+
+// A whole sequence per workgroup, by 4 or 8 waves: nothing to merge.
+template <int WV>
+__global__ __launch_bounds__(64 * WV, 2) void paged_short_kernel(PagedArgs a) {
+  __shared__ OwnSmem<WV> sm;
+  const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv;
+  const int len = a.lens[b];
+  const int64_t row = ((int64_t)b * a.Hkv + hk) * a.G;
+  if (!len_ok(a, len)) {
+    for (int i = threadIdx.x; i < a.G * D; i += 64 * WV) a.out[row * D + i] = 0x7fc0;
+    return;
+  }
+  own_part<WV, true>(a, sm, a.tab.ids + b * a.tab.stride, a.G, row + (threadIdx.x & 15), hk, 0,
+                     (len + PAGE - 1) / PAGE, len, row);
 }
 
 // Adds a partial (maximum m, sum l, values x) to another; one without keys (m = -infinity) has x = 0.
@@ -564,6 +588,21 @@ DecodeShape decode_shape(int64_t B, int64_t Hkv, int64_t G, int64_t shared, int 
   return s;
 }
 
+// Waves of a workgroup that takes a whole sequence, 0: the work is dealt out. Sequences of few pages are
+// taken whole, with one launch and nothing to merge; 8 waves where each has a CU of its own. us, dealt out /
+// whole, with the launch of the host and on the GPU alone:
+//   1 sequence of 1,000 positions, 8 KV heads   14.3 / 12.2, 10.1 / 11.8 (of 500 9.9 / 7.6, 2,000 10.1 / 19.5)
+//   16 of 1,000                                 16.0 / 13.8  64 of 1,000 32 / 29  256 of 300 53 / 42
+//   64 of 10 to 500                             20.0 / 14.2 (with 8 waves 16.9)
+//   64 of 100 to 2,000                          38.5 / 39.3
+// A shared part that is nearly all there is is read once all the same where workgroups are many (512
+// sequences that share 12 of 16 pages: 117 / 131; 64 of them: 20.4 / 20.6).
+constexpr int64_t SHORT_PAGES = 16;
+int short_waves(const DecodeShape& s, int64_t B, int64_t Hkv, int64_t width, int64_t cus) {
+  if (width > SHORT_PAGES || (4 * s.shared >= 3 * width && B * Hkv >= 4 * cus)) return 0;
+  return B * Hkv <= cus ? 8 : 4;
+}
+
 int64_t decode_bytes(const DecodeShape& s) { return s.slots * (int64_t)(D * sizeof(float) + sizeof(float2)); }
 
 int check_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t shared_pages) {
@@ -629,6 +668,12 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
   a.rb = s.rb;
   a.shares = s.shares;
   a.sl2 = scale * 1.4426950408889634f;
+  if (const int waves = short_waves(s, B, Hkv, table_width, device_cu_count())) {
+    auto* kern = waves == 8 ? paged_short_kernel<8> : paged_short_kernel<4>;
+    kern<<<dim3((unsigned)(B * Hkv)), dim3(64 * waves), 0, (hipStream_t)stream>>>(a);
+    LQ_CHECK_LAUNCH("paged_short_kernel");
+    return LQ_OK;
+  }
   auto* kern = s.nt == 2 ? paged_decode_kernel<2> : s.nt == 1 ? paged_decode_kernel<1> : paged_decode_kernel<0>;
   kern<<<dim3((unsigned)wgs), dim3(64 * DW), 0, (hipStream_t)stream>>>(a);
   LQ_CHECK_LAUNCH("paged_decode_kernel");

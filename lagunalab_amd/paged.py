@@ -18,7 +18,6 @@ from __future__ import annotations
 import functools
 import heapq
 from array import array
-import heapq
 
 import torch
 

@@ -402,6 +402,51 @@ def test_decode_on_two_streams_at_once(dev):
             assert torch.equal(bits(x), bits(y))
 
 
+@pytest.mark.parametrize("hq,kv,lens,shared", [
+    (12, 4, [0, 1, 63, 64, 65, 300, 1024], 64), (32, 8, [130] * 33 + [1000], 128), (16, 1, [1024, 1023, 577], 0),
+    (128, 16, [64, 1, 200] * 7, 64),
+])
+def test_decode_in_whole_sequences_and_dealt_out(dev, hq, kv, lens, shared):
+    """Sequences of few pages, as a table of their width (a workgroup per sequence and head) and a wider one
+    (pages dealt out) have them: the same to the roundings of both, bad lengths and pages NaN in both, captured
+    calls that follow the lengths."""
+    q, pool, table = decode_case(36, hq, kv, lens, shared, dev)
+    wide = torch.full((len(lens), 40), -7, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    args = [(q.to(dev), *pool, t.to(dev), n_d, SCALE, shared) for t in (table, wide)]
+    outs = [paged_decode_attention(*a) for a in args]
+    for out in outs:
+        check_decode(out, q, pool, table, lens)
+    assert (outs[0].float() - outs[1].float()).abs().max() < 2 ** -5
+    stream = torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            held = [paged_decode_attention(*a) for a in args]
+    torch.cuda.synchronize(dev)
+    for step in range(3):
+        now = [max(0, n - 29 * step) for n in lens]
+        now[0], now[1] = (-1, 64 * 40 + 1) if step == 2 else now[:2]
+        n_d.copy_(torch.tensor(now, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        for out, a in zip(held, args):
+            if step == 2:
+                assert torch.isnan(out[:2]).all()
+            check_decode(out, q, pool, table, now, rows=list(range(2 * (step == 2), len(lens))))
+            assert torch.equal(bits(out), bits(paged_decode_attention(*a)))
+    n_d.copy_(torch.tensor(lens, dtype=torch.int32))
+    last = len(lens) - 1
+    for t, a in zip((table, wide), args):
+        bad = t.clone()
+        bad[last, (lens[last] - 1) // PAGE] = pool[0][0].shape[0]
+        out = paged_decode_attention(*a[:3], bad.to(dev), n_d, SCALE, 0)
+        assert torch.isnan(out[last]).all()
+        check_decode(out, q, pool, table, lens, rows=[0, 1, last - 1])
+
+
 def test_pool_beyond_32_bit_offsets(dev):
     """Pages whose codes lie more than 4 GB into the pool: appended, attended, copied and read back."""
     pages, kv = 67000, 8
