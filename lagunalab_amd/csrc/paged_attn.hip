@@ -31,8 +31,8 @@ using namespace attn;
 constexpr int DW = 4;         // waves per workgroup
 constexpr int SHARE_MIN = 4;  // pages of a share: one per wave
 // Cost of starting on a sequence, in pages: shares of many short ones would end last. us at 0 / 2 / 4 / 8: 64
-// sessions of 10 to 500 positions, 32/8 heads 26.9 / 21.7 / 20.8 / 20.8, 8 of 100 to 4,000 21.8 / 19.2 / 17.8 /
-// 19.6, 4 of 100 to 300 behind 65,536 50.2 / 42.0 / 40.2 / 39.8.
+// sessions of 10 to 500 positions (in wider tables than those of short_waves), 32/8 heads 26.9 / 21.7 / 20.8 /
+// 20.8, 8 of 100 to 4,000 21.8 / 19.2 / 17.8 / 19.6, 4 of 100 to 300 behind 65,536 50.2 / 42.0 / 40.2 / 39.8.
 constexpr int SEQ_COST = 4;
 
 struct PagedArgs {
@@ -568,8 +568,8 @@ struct DecodeShape {
 };
 
 // Reading the shared pages once saves B - 1 readings of them; where these are fewer than SHARED_MIN pages of
-// a head, the sequences are attended on their own. (us, shared / each on its own, 8 KV heads: 512 positions
-// of 16 sequences 20.6 / 17.2, 4,096 of 3 18.7 / 17.3, of 6 17.6 / 21.9, 16,384 of 2 22.0 / 23.3.)
+// a head, the sequences are attended on their own. (us, shared / each on its own, 8 KV heads: 4,096 positions
+// of 3 sequences 18.7 / 17.3, of 6 17.6 / 21.9, 16,384 of 2 22.0 / 23.3.)
 constexpr int64_t SHARED_MIN = 1024;
 DecodeShape decode_shape(int64_t B, int64_t Hkv, int64_t G, int64_t shared, int cus) {
   DecodeShape s{0, 0, 1, 0, 0, 0};
