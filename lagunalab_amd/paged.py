@@ -39,19 +39,28 @@ def page_pool(pages: int, n_kv_heads: int, device="cuda"):
                  for _ in range(2))
 
 
+_CODES, _WORDS = torch.uint8, torch.bfloat16
+
+
 def _pool(keys, values):
     """(pages, Hkv, device, the six buffers' pointers) of a checked pool."""
     if len(keys) != 3 or len(values) != 3:
         raise ValueError("a pool's keys and values are (codes, scales, biases)")
-    bufs = (*keys, *values)
-    lead = keys[0].shape[:2]
-    wide, narrow = (*lead, PAGE, HEAD_DIM), (*lead, PAGE, HEAD_DIM // 64)
-    for i, t in enumerate(bufs):
-        want, dtype = (narrow, torch.bfloat16) if i % 3 else (wide, torch.uint8)
-        if t.shape != want or t.dtype != dtype or not t.is_contiguous():
-            raise ValueError(f"pool buffer {tuple(t.shape)} {t.dtype} is not contiguous {want} {dtype}")
-    dev = _lib.require_device(*bufs)
-    return lead[0], lead[1], dev, [t.data_ptr() for t in bufs]
+    codes = keys[0]
+    at, shape = codes.get_device(), codes.shape
+    P, H = shape[:2]
+    wide, narrow = (P, H, PAGE, HEAD_DIM), (P, H, PAGE, HEAD_DIM // 64)
+    ptrs = []
+    for buf in (keys, values):
+        want, dtype = wide, _CODES
+        for t in buf:
+            if t.shape != want or t.dtype is not dtype or not t.is_contiguous():
+                raise ValueError(f"pool buffer {tuple(t.shape)} {t.dtype} is not contiguous {want} {dtype}")
+            if at < 0 or t.get_device() != at:
+                _lib.require_device(*keys, *values)
+            ptrs.append(t.data_ptr())
+            want, dtype = narrow, _WORDS
+    return P, H, codes.device, ptrs
 
 
 def _length(table):
