@@ -89,17 +89,17 @@ struct TileRows {
 
 // Raw scores of the tile's keys. K fragments are read one key tile ahead of the MFMAs that use them (the
 // scheduling barriers keep it so).
-template <int NT>
+template <int NT, int MT>
 __device__ __forceinline__ void tile_scores(const uint16_t* kt, const TileRows<NT>& st, int lane,
-                                            f4_t (&c)[NT][4]) {
+                                            f4_t (&c)[NT][MT]) {
   const int lc = lane & 15, lq4 = lane >> 4;
   const bf16x8_t* k = reinterpret_cast<const bf16x8_t*>(kt) + 16 * lc;
   bf16x8_t f[2][4];
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) f[0][kk] = k[(4 * kk + lq4) ^ lc];
 #pragma unroll
-  for (int mt = 0; mt < 4; ++mt) {
-    if (mt + 1 < 4) {
+  for (int mt = 0; mt < MT; ++mt) {
+    if (mt + 1 < MT) {
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) f[(mt + 1) & 1][kk] = k[256 * (mt + 1) + ((4 * kk + lq4) ^ lc)];
     }
@@ -116,19 +116,20 @@ __device__ __forceinline__ void tile_scores(const uint16_t* kt, const TileRows<N
 
 // Scores to weights: raises the running maximum where needed (and rescales the row), P in bf16 as the
 // B operands of the two k-steps.
-template <int NT>
-__device__ __forceinline__ void tile_softmax(f4_t (&c)[NT][4], TileRows<NT>& st, float scale,
-                                             bf16x8_t (&p)[NT][2]) {
+template <int NT, int MT>
+__device__ __forceinline__ void tile_softmax(f4_t (&c)[NT][MT], TileRows<NT>& st, float scale,
+                                             bf16x8_t (&p)[NT][MT / 2]) {
   float t[NT];
   bool bump[NT], any = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     // four chains
-    float x[4];
+    float x[MT];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+    for (int mt = 0; mt < MT; ++mt)
       x[mt] = max_ieee(max_ieee(max_ieee(c[nt][mt][0], c[nt][mt][1]), c[nt][mt][2]), c[nt][mt][3]);
-    t[nt] = max_ieee(max_ieee(x[0], x[1]), max_ieee(x[2], x[3]));
+    t[nt] = max_ieee(x[0], x[1]);
+    if constexpr (MT == 4) t[nt] = max_ieee(t[nt], max_ieee(x[2], x[3]));
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) t[nt] = max_xor16(t[nt]);
@@ -149,9 +150,9 @@ __device__ __forceinline__ void tile_softmax(f4_t (&c)[NT][4], TileRows<NT>& st,
       for (int w = 0; w < 8; ++w) st.o[nt][w] *= alpha;
     }
   }
-  uint32_t w[NT][8];
+  uint32_t w[NT][2 * MT];
 #pragma unroll
-  for (int mt = 0; mt < 4; ++mt)
+  for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float off = st.m[nt] == -INFINITY ? 0.0f : -st.m[nt];
@@ -163,10 +164,11 @@ __device__ __forceinline__ void tile_softmax(f4_t (&c)[NT][4], TileRows<NT>& st,
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     // made here, not sunk into the product's phase
-    asm volatile("" : "+v"(w[nt][0]), "+v"(w[nt][1]), "+v"(w[nt][2]), "+v"(w[nt][3]), "+v"(w[nt][4]),
-                      "+v"(w[nt][5]), "+v"(w[nt][6]), "+v"(w[nt][7]));
-    p[nt][0] = words_as_bf8(w[nt][0], w[nt][1], w[nt][2], w[nt][3]);
-    p[nt][1] = words_as_bf8(w[nt][4], w[nt][5], w[nt][6], w[nt][7]);
+#pragma unroll
+    for (int e = 0; e < MT / 2; ++e) {
+      asm volatile("" : "+v"(w[nt][4 * e]), "+v"(w[nt][4 * e + 1]), "+v"(w[nt][4 * e + 2]), "+v"(w[nt][4 * e + 3]));
+      p[nt][e] = words_as_bf8(w[nt][4 * e], w[nt][4 * e + 1], w[nt][4 * e + 2], w[nt][4 * e + 3]);
+    }
   }
 }
 
@@ -193,16 +195,16 @@ __device__ __forceinline__ uint32_t finite_bf2(uint32_t u) {
 
 // O^T += V^T P^T. Fragments of half a k-step (four windows of 16 dims) are read ahead of the MFMAs, as in
 // tile_scores.
-template <int NT>
+template <int NT, int E>
 __device__ __forceinline__ void tile_values(const uint16_t* v, TileRows<NT>& st, int lane,
-                                            const bf16x8_t (&p)[NT][2]) {
+                                            const bf16x8_t (&p)[NT][E]) {
   const uint32_t vl = v_lane(v, lane);
   bf16x8_t f[2][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) f[0][j] = v_operand(vl, j, 0);
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {  // k-step u / 2, windows 4 (u % 2) ..
-    if (u + 1 < 4) {
+  for (int u = 0; u < 2 * E; ++u) {  // k-step u / 2, windows 4 (u % 2) ..
+    if (u + 1 < 2 * E) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[(u + 1) & 1][j] = v_operand(vl, 4 * ((u + 1) & 1) + j, (u + 1) >> 1);
     }

@@ -1,9 +1,10 @@
 // Attention of one new token per sequence over a paged 8-bit cache, the pages that all sequences share
 // read once for the batch (a prompt and the answers sampled from it, a long system prompt).
 //
-// Work. A KV head's shared pages are cut into np parts; a workgroup takes one part for a block of 64 or
+// Work. A KV head's shared pages are cut into np parts; a workgroup takes one part for a block of 32, 64 or
 // 128 query rows (the G rows of each sequence, one sequence behind the other), dequantizes each page
-// once into LDS and runs the matrix-core tile of attn_tile.h on it. The sequences' own pages, one sequence
+// once into LDS and runs the matrix-core tile of attn_tile.h on it; of long parts the workgroup of own pages
+// beside it takes the last pages (late_pages). The sequences' own pages, one sequence
 // behind the other, are dealt out to the workgroups in equal shares; a workgroup runs its pages of a sequence
 // for the G <= 16 rows, one page per wave at a time, through the wave's own LDS (no barriers), the next
 // page's loads out while it computes. With up to 16 query rows in the batch the shared pages are dealt out
@@ -46,6 +47,7 @@ struct PagedArgs {
   int B, Hkv, G;
   int shared;         // pages that all sequences share
   int np, rb;         // their parts, blocks of query rows; 0: dealt out with the own pages
+  bool late;          // parts long enough for late_pages
   int shares;         // workgroups for the own pages of a KV head
   float sl2;          // softmax scale, log2 units
 };
@@ -83,6 +85,17 @@ __device__ __forceinline__ Deal deal_out(const PagedArgs& a, int lane) {
   const int lead = a.np == 0 && __builtin_amdgcn_ballot_w64(joins) ? a.shared : 0;
   total = wave_sum_i(total) + lead;
   return {lead, total, max(SHARE_MIN, (total + a.shares - 1) / a.shares)};
+}
+// Pages of each shared part that are left to the workgroup of own pages beside it on the CU, so that both end
+// together: a share takes about OWN_START and 2/3 per page in times of a shared page, with the start on the part.
+// LATE_MIN: fewer do not pay for the partials. us without and with, 8 KV heads, own pages of 1 to 64 / 1,500 to
+// 2,500 positions: 82,688 shared positions of 5 sequences, 32 heads 64.0 / 65.7 -> 44.1 / 48.2, of 16 66.5 / 71.3 ->
+// 54.3 / 66.0, of 48, 48 heads 232 / 242 -> 172 / 194 (together with SPLIT); 16,384 of 48, which leave none, alike.
+constexpr int OWN_START = 10, LATE_MIN = 8;
+__device__ __forceinline__ int late_pages(const PagedArgs& a, const Deal& deal) {
+  const int own = deal.total ? OWN_START + 2 * deal.share / 3 : 0;
+  const int left = (a.shared / a.np - own) / 2;
+  return left < LATE_MIN ? 0 : left;
 }
 // The table row that lists the shared pages: of the first sequence that is long enough (a shorter one's may
 // end before them); null: there is none.
@@ -313,34 +326,46 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
   }
 }
 
-// A part [p0, p1) of the shared pages (listed in the table at ids) for query rows f0 .. f0 + 64 NT - 1 of
-// a KV head.
-struct RawPage {  // keys tid / 8 and tid / 8 + 32, codes 16 (tid % 8) ..
-  uint4 k[2], v[2];
-  uint32_t ks[2], kb[2], vs[2], vb[2];
+// Shared pages [p0, p1) (listed in the table at ids) for the query rows of block `block` of a KV head. Each page
+// is dequantized once into one of two tiles, the next one's codes on their way. With SPLIT (up to 32 rows) the two
+// halves of the waves take the same rows, and half of a page's keys each, and meet in LDS at the end.
+constexpr int CH = 8 / DW;  // chunks of a thread
+template <int NT, bool SPLIT>
+constexpr int block_rows() {
+  return 16 * NT * (SPLIT ? DW / 2 : DW);
+}
+struct RawPage {  // key tid / 8 + 8 DW i, codes 16 (tid % 8) ..
+  uint4 k[CH], v[CH];
+  uint32_t ks[CH], kb[CH], vs[CH], vb[CH];
+};
+struct SharedSmem {
+  KvTile tile[2];
 };
 
-template <int NT>
-__device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2], const int32_t* ids, int hk,
-                                            int p0, int p1, int f0, int64_t slot) {
+template <int NT, bool SPLIT>
+__device__ __forceinline__ void shared_part(const PagedArgs& a, SharedSmem& sm, const int32_t* ids, int hk,
+                                            int p0, int p1, int block, int64_t slot) {
+  constexpr int MT = SPLIT ? 2 : 4;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool upper = wv >= DW / 2;
   const int lc = lane & 15, lq4 = lane >> 4;
   const int rows = a.B * a.G;
+  const int f0 = block * block_rows<NT, SPLIT>() + 16 * NT * (SPLIT ? wv % (DW / 2) : wv);
   const float scale = abs_scale(a.sl2);
   const int key0 = tid >> 3, chunk = tid & 7;
   bool bad = false;
   RawPage pre[2];  // pages p + 1 and p + 2
   auto load = [&](int p, RawPage& raw) {
-    const int id = __builtin_amdgcn_readfirstlane(ids[p]);
+    const int id = __builtin_amdgcn_readfirstlane(ids[min(p, p1 - 1)]);
     const bool ok = id >= 0 && id < a.tab.pages;
     bad |= !ok;
     const int64_t row = ((int64_t)(ok ? id : 0) * a.Hkv + hk) * PAGE;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      raw.k[i] = *reinterpret_cast<const uint4*>(a.buf.kc + row * D + 4096 * i + 16 * tid);
-      raw.v[i] = *reinterpret_cast<const uint4*>(a.buf.vc + row * D + 4096 * i + 16 * tid);
-      const int64_t r = row + key0 + 32 * i;
+    for (int i = 0; i < CH; ++i) {
+      raw.k[i] = *reinterpret_cast<const uint4*>(a.buf.kc + row * D + 1024 * DW * i + 16 * tid);
+      raw.v[i] = *reinterpret_cast<const uint4*>(a.buf.vc + row * D + 1024 * DW * i + 16 * tid);
+      const int64_t r = row + key0 + 8 * DW * i;
       raw.ks[i] = reinterpret_cast<const uint32_t*>(a.buf.ks)[r];
       raw.kb[i] = reinterpret_cast<const uint32_t*>(a.buf.kb)[r];
       raw.vs[i] = reinterpret_cast<const uint32_t*>(a.buf.vs)[r];
@@ -350,8 +375,8 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
   auto pick = [&](uint32_t w) { return chunk < 4 ? bf16_lo(w) : bf16_hi(w); };
   auto stage = [&](KvTile& t, const RawPage& raw) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int key = key0 + 32 * i;
+    for (int i = 0; i < CH; ++i) {
+      const int key = key0 + 8 * DW * i;
       const float s = pick(raw.ks[i]), z = pick(raw.kb[i]);
       const uint2 k0 = dequant4(raw.k[i].x, s, z), k1 = dequant4(raw.k[i].y, s, z);
       const uint2 k2 = dequant4(raw.k[i].z, s, z), k3 = dequant4(raw.k[i].w, s, z);
@@ -365,12 +390,12 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
     }
   };
   load(p0, pre[0]);
-  load(min(p0 + 1, p1 - 1), pre[1]);
+  load(p0 + 1, pre[1]);
   TileRows<NT> st;
   st.clear();
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int f = f0 + 16 * (NT * wv + nt) + lc;
+    const int f = f0 + 16 * nt + lc;
     const int b = f / a.G;
     const int64_t row = ((int64_t)b * a.Hkv + hk) * a.G + (f - b * a.G);
 #pragma unroll
@@ -380,28 +405,47 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
       st.q[nt][kk] = u4_as_bf8(signed_q(u, a.sl2));
     }
   }
-  stage(sm[0], pre[0]);
-  load(min(p0 + 2, p1 - 1), pre[0]);
+  stage(sm.tile[0], pre[0]);
+  load(p0 + 2, pre[0]);
   __syncthreads();
+  const int part = SPLIT && upper ? 32 * D : 0;  // the wave's keys of a tile
   for (int p = p0; p < p1; p += 2) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {  // page p + s in tile s
       if (p + s >= p1) break;
-      f4_t c[NT][4];
-      bf16x8_t pr[NT][2];
-      tile_scores<NT>(sm[s].k, st, lane, c);
+      f4_t c[NT][MT];
+      bf16x8_t pr[NT][MT / 2];
+      tile_scores<NT>(sm.tile[s].k + part, st, lane, c);
       tile_softmax<NT>(c, st, scale, pr);
-      tile_values<NT>(sm[s].v, st, lane, pr);
+      tile_values<NT>(sm.tile[s].v + part, st, lane, pr);
       if (p + s + 1 < p1) {
-        stage(sm[s ^ 1], pre[s ^ 1]);
-        load(min(p + s + 3, p1 - 1), pre[s ^ 1]);
+        stage(sm.tile[s ^ 1], pre[s ^ 1]);
+        load(p + s + 3, pre[s ^ 1]);
       }
       __syncthreads();
     }
   }
+  if constexpr (SPLIT) {  // the upper half's rows to the lower's: a row of 132 floats, its maximum and sum
+    float* at = reinterpret_cast<float*>(&sm) + (16 * (wv % (DW / 2)) + lc) * 132;
+    if (upper) {
+#pragma unroll
+      for (int w = 0; w < 8; ++w) *reinterpret_cast<f4_t*>(at + 16 * w + 4 * lq4) = st.o[0][w];
+      if (lq4 == 0) *reinterpret_cast<float2*>(at + 128) = make_float2(st.m[0], st.l[0][0]);
+    }
+    __syncthreads();
+    if (upper) return;
+    const float2 ml = *reinterpret_cast<const float2*>(at + 128);
+    const float m = max_ieee(st.m[0], ml.x), mr = m == -INFINITY ? 0.0f : m;
+    const float e0 = exp2_nonpos(st.m[0] - mr), e1 = exp2_nonpos(ml.x - mr);
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+      st.o[0][w] = st.o[0][w] * e0 + *reinterpret_cast<const f4_t*>(at + 16 * w + 4 * lq4) * e1;
+    st.l[0] = st.l[0] * e0 + ml.y * e1;
+    st.m[0] = m;
+  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int f = f0 + 16 * (NT * wv + nt) + lc;
+    const int f = f0 + 16 * nt + lc;
     if (f >= rows) continue;
 #pragma unroll
     for (int w = 0; w < 8; ++w)
@@ -415,42 +459,22 @@ __device__ __forceinline__ void shared_part(const PagedArgs& a, KvTile (&sm)[2],
 // sum), then those of the shared pages, by part or by share.
 __device__ __forceinline__ int64_t shared_slots(const PagedArgs& a) { return (int64_t)(a.shares + a.B) * a.G; }
 __device__ __forceinline__ int64_t head_slots(const PagedArgs& a) {
-  return shared_slots(a) + (int64_t)(a.np ? a.np : a.shared ? a.shares : 0) * a.B * a.G;
+  return shared_slots(a) + (int64_t)(a.np ? a.np << a.late : a.shared ? a.shares : 0) * a.B * a.G;
 }
 
-template <int NT>  // 16-row tiles of a wave in the shared part; 0: nothing is shared
-__global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
-  __shared__ union Smem {
-    OwnSmem<DW> own;
-    KvTile tile[NT ? 2 : 1];
-    __device__ Smem() {}
-  } sm;
+// Share x of the pages that are dealt out for a KV head.
+template <int WV>
+__device__ __forceinline__ void own_share(const PagedArgs& a, const Deal& deal, OwnSmem<WV>& sm, int hk, int x,
+                                          int64_t slot0) {
   const int lane = threadIdx.x & 63;
-  const int hk = blockIdx.x % a.Hkv;
-  int x = blockIdx.x / a.Hkv;
-  const int64_t slot0 = hk * head_slots(a);
-  if constexpr (NT > 0) {
-    if (x < a.np * a.rb) {  // the shared parts first: they take longest
-      const int part = x / a.rb, block = x - part * a.rb;
-      const int p0 = (int)((int64_t)a.shared * part / a.np);
-      const int p1 = (int)((int64_t)a.shared * (part + 1) / a.np);
-      if (const int32_t* ids = shared_ids(a, lane))
-        shared_part<NT>(a, sm.tile, ids, hk, p0, p1, block * 64 * NT,
-                        slot0 + shared_slots(a) + (int64_t)part * a.B * a.G);
-      return;
-    }
-    x -= a.np * a.rb;
-  }
-  // share x of the pages of this KV head
-  const Deal deal = deal_out(a, lane);
   const int u0 = x * deal.share, u1 = min(u0 + deal.share, deal.total);
   if (u0 >= u1) return;
   const int lc = lane & 15;
   int u = u0;
   if (u < deal.lead) {  // shared pages, for all rows of the batch
     const int e = min(u1, deal.lead), b = lc / a.G;
-    own_part<DW, false>(a, sm.own, shared_ids(a, lane), a.B * a.G, ((int64_t)b * a.Hkv + hk) * a.G + (lc - b * a.G), hk, u, e,
-             a.shared * PAGE, slot0 + shared_slots(a) + (int64_t)x * a.B * a.G);
+    own_part<WV, false>(a, sm, shared_ids(a, lane), a.B * a.G, ((int64_t)b * a.Hkv + hk) * a.G + (lc - b * a.G), hk,
+                        u, e, a.shared * PAGE, slot0 + shared_slots(a) + (int64_t)x * a.B * a.G);
     u = e;
   }
   if (u == u1) return;
@@ -473,11 +497,45 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
     begin += SEQ_COST;
     const int p0 = max(u - begin, 0), p1 = min(u1 - begin, n), first = own_first(a, len);
     if (p0 < p1)
-      own_part<DW, false>(a, sm.own, a.tab.ids + b * a.tab.stride, a.G, ((int64_t)b * a.Hkv + hk) * a.G + lc, hk, first + p0,
-               first + p1, len, slot0 + (int64_t)(x + b) * a.G);
+      own_part<WV, false>(a, sm, a.tab.ids + b * a.tab.stride, a.G, ((int64_t)b * a.Hkv + hk) * a.G + lc, hk,
+                          first + p0, first + p1, len, slot0 + (int64_t)(x + b) * a.G);
     begin += n;
     u = begin;
   }
+}
+
+__global__ __launch_bounds__(64 * DW, 2) void paged_decode_kernel(PagedArgs a) {
+  __shared__ OwnSmem<DW> sm;
+  const int hk = blockIdx.x % a.Hkv;
+  own_share<DW>(a, deal_out(a, threadIdx.x & 63), sm, hk, blockIdx.x / a.Hkv, hk * head_slots(a));
+}
+
+// Two workgroups per CU: one takes a shared part for a block of rows, the other a share of the own pages, then, of
+// a long part, the last pages.
+template <int NT, bool SPLIT>
+__global__ __launch_bounds__(64 * DW, 2) void paged_shared_kernel(PagedArgs a) {
+  __shared__ union Smem {
+    OwnSmem<DW> own;
+    SharedSmem shared;
+    __device__ Smem() {}
+  } sm;
+  const int hk = blockIdx.x % a.Hkv, n = a.np * a.rb;
+  int x = blockIdx.x / a.Hkv;
+  const bool late = x >= n;
+  if (late) x -= n;
+  const int64_t slot0 = hk * head_slots(a);
+  const int lane = threadIdx.x & 63;
+  if (late && x < a.shares) own_share<DW>(a, deal_out(a, lane), sm.own, hk, x, slot0);
+  if (x >= n || (late && !a.late)) return;
+  const int32_t* ids = shared_ids(a, lane);
+  const int left = a.late ? late_pages(a, deal_out(a, lane)) : 0;
+  if (!ids || (late && left == 0)) return;
+  const int part = x / a.rb, block = x - part * a.rb;
+  const int p0 = (int)((int64_t)a.shared * part / a.np);
+  const int p1 = (int)((int64_t)a.shared * (part + 1) / a.np);
+  __syncthreads();  // the share is written
+  shared_part<NT, SPLIT>(a, sm.shared, ids, hk, late ? p1 - left : p0, late ? p1 : p1 - left, block,
+                         slot0 + shared_slots(a) + (int64_t)(late ? a.np + part : part) * a.B * a.G);
 }
 
 // A whole sequence per workgroup, by 4 or 8 waves: nothing to merge.
@@ -529,7 +587,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   const int64_t slot0 = hk * head_slots(a);
   const int64_t own0 = slot0 + (int64_t)(first + b) * a.G + g;
   const int64_t sh0 = slot0 + shared_slots(a) + (int64_t)b * a.G + g;
-  const int parts = n + (!joins ? 0 : a.np ? a.np : (deal.lead - 1) / S + 1);
+  const int parts = n + (!joins ? 0 : a.np ? a.np << (a.late && late_pages(a, deal)) : (deal.lead - 1) / S + 1);
   const int grp = (threadIdx.x >> 5) % GR, ln = threadIdx.x & 31;
   float M = -INFINITY, den = 0.0f;
   f4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -564,6 +622,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 
 struct DecodeShape {
   int np, rb, shares, nt, shared;
+  bool split, late;
   int64_t slots;  // partial rows, all heads
 };
 
@@ -572,19 +631,18 @@ struct DecodeShape {
 // of 3 sequences 18.7 / 17.3, of 6 17.6 / 21.9, 16,384 of 2 22.0 / 23.3.)
 constexpr int64_t SHARED_MIN = 1024;
 DecodeShape decode_shape(int64_t B, int64_t Hkv, int64_t G, int64_t shared, int cus) {
-  DecodeShape s{0, 0, 1, 0, 0, 0};
+  DecodeShape s{0, 0, 1, 0, 0, false, false, 0};
   if ((B - 1) * shared * Hkv >= SHARED_MIN) s.shared = (int)shared;
-  const int64_t fill = 2 * cus;  // workgroups that the GPU holds at once
   const bool blocks = s.shared > 0 && B * G > 16;
   if (blocks) {
-    s.nt = B * G > 64 ? 2 : 1;
-    s.rb = (int)((B * G + 64 * s.nt - 1) / (64 * s.nt));
-    s.np = (int)std::min<int64_t>((shared + 3) / 4, std::max<int64_t>(1, fill / 2 / (Hkv * s.rb)));
+    s.nt = B * G > 16 * DW ? 2 : 1;
+    s.split = B * G <= 8 * DW;
+    s.rb = (int)((B * G + 16 * DW * s.nt - 1) / (16 * DW * s.nt));
+    s.np = (int)std::min<int64_t>((shared + 3) / 4, std::max<int64_t>(1, cus / (Hkv * s.rb)));
+    s.late = shared / s.np >= 2 * LATE_MIN + OWN_START;
   }
-  // beside a shared part's workgroup a CU holds one of the own pages': all run at once (48 sessions behind
-  // 16,384 rows 70 -> 65 us, against twice as many in two rounds)
-  s.shares = (int)std::max<int64_t>(1, (blocks ? fill / 2 : fill) / Hkv);
-  s.slots = Hkv * G * (s.shares + B + (s.np ? s.np : s.shared ? s.shares : 0) * B);
+  s.shares = (int)std::max<int64_t>(1, (blocks ? cus : 2 * cus) / Hkv);
+  s.slots = Hkv * G * (s.shares + B + (s.np ? s.np << s.late : s.shared ? s.shares : 0) * B);
   return s;
 }
 
@@ -654,7 +712,8 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
     return LQ_EWORKSPACE;
   }
   LQ_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
-  const int64_t wgs = Hkv * ((int64_t)s.np * s.rb + s.shares);
+  const int64_t parts = (int64_t)s.np * s.rb;
+  const int64_t wgs = Hkv * (parts + std::max<int64_t>(s.late ? parts : 0, s.shares));
   LQ_CHECK_ARG(wgs < (1 << 23), "too many workgroups");
   a.lens = lens;
   a.part_acc = (float*)workspace;
@@ -665,6 +724,7 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
   a.G = (int)G;
   a.shared = s.shared;
   a.np = s.np;
+  a.late = s.late;
   a.rb = s.rb;
   a.shares = s.shares;
   a.sl2 = scale * 1.4426950408889634f;
@@ -674,11 +734,14 @@ extern "C" int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const 
     LQ_CHECK_LAUNCH("paged_short_kernel");
     return LQ_OK;
   }
-  auto* kern = s.nt == 2 ? paged_decode_kernel<2> : s.nt == 1 ? paged_decode_kernel<1> : paged_decode_kernel<0>;
+  auto* kern = s.nt == 2   ? paged_shared_kernel<2, false>
+               : s.split   ? paged_shared_kernel<1, true>
+               : s.nt == 1 ? paged_shared_kernel<1, false>
+                           : paged_decode_kernel;
   kern<<<dim3((unsigned)wgs), dim3(64 * DW), 0, (hipStream_t)stream>>>(a);
   LQ_CHECK_LAUNCH("paged_decode_kernel");
   // a row's partials: the shared parts and its share of the own ones
-  if (s.np + s.shares / std::min<int64_t>(B, 4) > 16)
+  if ((s.np << s.late) + s.shares / std::min<int64_t>(B, 4) > 16)
     paged_merge_kernel<8><<<dim3((unsigned)(B * Hq)), dim3(256), 0, (hipStream_t)stream>>>(a);
   else
     paged_merge_kernel<2><<<dim3((unsigned)((B * Hq + 3) / 4)), dim3(256), 0, (hipStream_t)stream>>>(a);

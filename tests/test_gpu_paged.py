@@ -402,6 +402,28 @@ def test_decode_on_two_streams_at_once(dev):
             assert torch.equal(bits(x), bits(y))
 
 
+@pytest.mark.parametrize("hq,B", [(128, 9), (256, 10), (512, 12), (1024, 10)])
+@pytest.mark.parametrize("heavy", [False, True])
+def test_long_shared_parts(dev, hq, B, heavy):
+    """Shared parts of 32 pages and more, with few own pages (the parts' last pages are then taken by the workgroups
+    of the own ones) and with many; row blocks of 32, 64 and 128 rows, one and two."""
+    kv, shared = 64, 8192
+    lens = [shared + (70 * b if heavy else b % 2) for b in range(B)]
+    lens[2], lens[B - 1] = shared - 1, 0
+    q, pool, table = decode_case(37, hq, kv, lens, shared, dev)
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    args = (q.to(dev), *pool, table.to(dev), n_d, SCALE)
+    out = paged_decode_attention(*args, shared=shared)
+    check_decode(out, q, pool, table, lens, rows=[1, 2])
+    assert (out[B - 1] == 0).all()
+    assert (out.float() - paged_decode_attention(*args).float()).abs().max() < 2 ** -5
+    assert torch.equal(bits(out), bits(paged_decode_attention(*args, shared=shared)))
+    bad = table.clone()
+    bad[:, shared // PAGE - 1] = -1  # the last shared page
+    out = paged_decode_attention(q.to(dev), *pool, bad.to(dev), n_d, SCALE, shared=shared)
+    assert torch.isnan(out[:B - 1]).all() and (out[B - 1] == 0).all()
+
+
 @pytest.mark.parametrize("hq,kv,lens,shared", [
     (12, 4, [0, 1, 63, 64, 65, 300, 1024], 64), (32, 8, [130] * 33 + [1000], 128), (16, 1, [1024, 1023, 577], 0),
     (128, 16, [64, 1, 200] * 7, 64),
