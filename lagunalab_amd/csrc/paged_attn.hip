@@ -89,8 +89,8 @@ __device__ __forceinline__ Deal deal_out(const PagedArgs& a, int lane) {
 // Pages of each shared part that are left to the workgroup of own pages beside it on the CU, so that both end
 // together: a share takes about OWN_START and 2/3 per page in times of a shared page, with the start on the part.
 // LATE_MIN: fewer do not pay for the partials. us without and with, 8 KV heads, own pages of 1 to 64 / 1,500 to
-// 2,500 positions: 82,688 shared positions of 5 sequences, 32 heads 64.0 / 65.7 -> 44.1 / 48.2, of 16 66.5 / 71.3 ->
-// 54.3 / 66.0, of 48, 48 heads 232 / 242 -> 172 / 194 (together with SPLIT); 16,384 of 48, which leave none, alike.
+// 2,500 positions: 82,688 shared positions of 5 sequences, 32 heads 64.1 / 65.9 -> 44.7 / 48.6, of 16 66.5 / 71.6 ->
+// 54.2 / 65.3, of 48, 48 heads 232 / 242 -> 176 / 200 (together with SPLIT); 16,384 of 48, which leave none, alike.
 constexpr int OWN_START = 10, LATE_MIN = 8;
 __device__ __forceinline__ int late_pages(const PagedArgs& a, const Deal& deal) {
   const int own = deal.total ? OWN_START + 2 * deal.share / 3 : 0;
