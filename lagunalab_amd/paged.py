@@ -237,9 +237,10 @@ class PagedKVCache:
 
     A session (an int) is opened empty, adopted from a contiguous 8-bit cache, or forked from another,
     whose pages it then shares; a shared page is copied when one of its sessions is about to write to
-    it. Pages go back to the pool when their last session is closed or trimmed below them. The lists
-    live on the host; device work runs on the current stream, and calls on one cache belong on one
-    stream (a page given back may be taken by the next call)."""
+    it. Pages go back to the pool when their last session is closed or trimmed below them; an append that
+    raises leaves its sessions as they were. The lists live on the host; device work runs on the current
+    stream, and calls on one cache belong on one stream (a page given back may be taken by the next
+    call)."""
 
     def __init__(self, pages: int, n_kv_heads: int, device="cuda"):
         self.keys, self.values = page_pool(pages, n_kv_heads, device)
@@ -365,22 +366,22 @@ class PagedKVCache:
         copies, fresh = [], 0
         for (pages, rows), c in zip(states, counts):
             if c and rows % PAGE:
-                p = pages[-1]
+                p = pages[rows // PAGE]
                 written[p] = written.get(p, 0) + 1
                 if written[p] < self._uses[p]:  # someone keeps it: another session, or a later writer
-                    copies.append((pages, p))
+                    copies.append((pages, rows // PAGE, p))
             if c:
                 fresh += max(0, -(-(rows + c) // PAGE) - len(pages))
         new = self._take(len(copies) + fresh)
         if copies:
             dst = new[:len(copies)]
             try:
-                copy_pages(self.keys, self.values, [p for _, p in copies], dst)
-            except Exception:
+                copy_pages(self.keys, self.values, [p for _, _, p in copies], dst)
+            except BaseException:
                 self._give(new)
                 raise
-            for (pages, p), q in zip(copies, dst):
-                pages[-1] = q
+            for (pages, i, p), q in zip(copies, dst):
+                pages[i] = q
                 self._uses[p] -= 1
         at = len(copies)
         for (pages, rows), c in zip(states, counts):
@@ -389,6 +390,15 @@ class PagedKVCache:
                 pages.extend(new[at:at + n])
                 at += n
         return bool(new)
+
+    def _undo_room(self, states):
+        """After rows that were not appended: the pages made for them go back (a page copied for its
+        writer stays its own)."""
+        for pages, rows in states:
+            keep = -(-rows // PAGE)
+            self._give(pages[keep:])
+            del pages[keep:]
+        self._version += 1
 
     def _tables(self, states):
         """(table, lens) of the sessions on the device."""
@@ -435,8 +445,12 @@ class PagedKVCache:
         _lib.require_device(k, v, self.keys[0])
         self._make_room(states, counts)
         self._version += 1
-        table, starts = self._tables(states)
-        paged_append(k, v, self.keys, self.values, table, starts, counts)
+        try:
+            table, starts = self._tables(states)
+            paged_append(k, v, self.keys, self.values, table, starts, counts)
+        except BaseException:
+            self._undo_room(states)
+            raise
         for s, c in zip(states, counts):
             s[1] += c
 
@@ -529,12 +543,17 @@ class PagedBatch:
         states = self._states()
         if self.cache._make_room(states, [L] * B):
             self.cache._version += 1
-        self._refresh(states)
-        k, v = (t.transpose(1, 2).reshape(B * L, H, D) for t in (keys, values))
-        paged_append(k, v, self.cache.keys, self.cache.values, self._table, self._lens, [L] * B)
+        try:
+            self._refresh(states)
+            k, v = (t.transpose(1, 2).reshape(B * L, H, D) for t in (keys, values))
+            paged_append(k, v, self.cache.keys, self.cache.values, self._table, self._lens, [L] * B)
+            lens = self._lens + L
+        except BaseException:
+            self.cache._undo_room(states)
+            raise
         for s in states:
             s[1] += L
-        self._lens = self._lens + L
+        self._lens = lens
         self.cache._version += 1  # other batches of these sessions hold old lengths
         self._seen = self.cache._version
         return keys, values

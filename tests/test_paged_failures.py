@@ -1,0 +1,83 @@
+"""PagedKVCache when a call fails on the way, on the CPU: nothing of it stays, and what is forked and written
+afterwards is each session's own."""
+import pytest
+import torch
+
+from lagunalab_amd import paged
+from lagunalab_amd.paged import PagedKVCache
+from test_paged_sessions import D, H, check, plain, rows  # noqa: F401
+
+
+class Lost(Exception):
+    pass
+
+
+def fail_once(monkeypatch, owner, name):
+    """owner.name raises at its next call and works again afterwards."""
+    real = getattr(owner, name)
+
+    def broken(*args, **kwargs):
+        monkeypatch.setattr(owner, name, real)
+        raise Lost(name)
+    monkeypatch.setattr(owner, name, broken)
+
+
+def step(tag, B, L):
+    return torch.full((B, H, L, D), tag, dtype=torch.bfloat16)
+
+
+# what raises: the rows' launch, the upload of the tables, the copy of a page that is shared; the row goes to a
+# new page or to a part-filled one
+@pytest.mark.parametrize("what,had", [("paged_append", 64), ("paged_append", 100), ("_tables", 64),
+                                      ("_tables", 100), ("copy_pages", 100)])
+@pytest.mark.parametrize("through", ["append", "batch"])
+def test_an_append_that_fails_leaves_no_pages_behind(plain, monkeypatch, what, had, through):  # noqa: F811
+    cache = PagedKVCache(12, H, device="cpu")
+    a = cache.open()
+    cache.append([a], rows([1] * had), rows([1] * had))
+    if what == "copy_pages":
+        keep = cache.fork(a)
+    batch = cache.batch([a])
+    free = cache.free_pages
+    fail_once(monkeypatch, PagedKVCache if what == "_tables" else paged, what)
+    with pytest.raises(Lost):
+        if through == "append":
+            cache.append([a], rows([9] * 140), rows([9] * 140))
+        else:
+            batch.update_and_fetch(step(9, 1, 140), step(9, 1, 140))
+    want = {a: [1] * had}
+    if what == "copy_pages":
+        want[keep] = [1] * had
+        assert cache.free_pages == free
+    check(cache, want)
+    # forks of it write to pages of their own, also through the batch made before
+    b = cache.fork(a)
+    cache.append([b], rows([3]), rows([3]))
+    batch.update_and_fetch(step(2, 1, 1), step(2, 1, 1))
+    want[a], want[b] = want[a] + [2], want[a] + [3]
+    check(cache, want)
+    batch._refresh(batch._states())
+    assert batch._lens.tolist() == [had + 1]
+    assert batch._table[0, :len(cache.pages(a))].tolist() == cache.pages(a)
+
+
+def test_lengths_that_cannot_be_made_leave_a_batch_as_it_was(plain, monkeypatch):  # noqa: F811
+    """The step's new lengths are a device tensor: if there is none, the step did not happen."""
+    cache = PagedKVCache(6, H, device="cpu")
+    a, b = cache.open(), cache.open()
+    batch = cache.batch([a, b])
+    batch.update_and_fetch(step(1, 2, 63), step(1, 2, 63))
+
+    class Full:
+        def __add__(self, n):
+            raise Lost("out of memory")
+
+        def tolist(self):
+            return [63, 63]
+    batch._lens = Full()
+    with pytest.raises(Lost):
+        batch.update_and_fetch(step(9, 2, 1), step(9, 2, 1))
+    check(cache, {a: [1] * 63, b: [1] * 63})
+    batch.update_and_fetch(step(2, 2, 2), step(2, 2, 2))
+    check(cache, {a: [1] * 63 + [2] * 2, b: [1] * 63 + [2] * 2})
+    assert batch._lens.tolist() == [65, 65]
