@@ -286,13 +286,17 @@ class PagedKVCache:
         _lib.require_device(*keys, *values, *self.keys)
         pages = self._take(-(-n // PAGE))
         whole = n // PAGE
-        at = torch.tensor(pages, device=self.keys[0].device)
-        for buf, rows in ((self.keys, keys), (self.values, values)):
-            for t, x in zip(buf, rows):
-                if whole:
-                    t[at[:whole]] = x[0, :, :whole * PAGE].unflatten(1, (whole, PAGE)).transpose(0, 1)
-                if n % PAGE:
-                    t[pages[-1], :, :n % PAGE] = x[0, :, whole * PAGE:]
+        try:
+            at = torch.tensor(pages, device=self.keys[0].device)
+            for buf, rows in ((self.keys, keys), (self.values, values)):
+                for t, x in zip(buf, rows):
+                    if whole:
+                        t[at[:whole]] = x[0, :, :whole * PAGE].unflatten(1, (whole, PAGE)).transpose(0, 1)
+                    if n % PAGE:
+                        t[pages[-1], :, :n % PAGE] = x[0, :, whole * PAGE:]
+        except BaseException:
+            self._give(pages)
+            raise
         new = self.open()
         self._sessions[new] = [pages, n]
         return new

@@ -81,3 +81,30 @@ def test_lengths_that_cannot_be_made_leave_a_batch_as_it_was(plain, monkeypatch)
     batch.update_and_fetch(step(2, 2, 2), step(2, 2, 2))
     check(cache, {a: [1] * 63 + [2] * 2, b: [1] * 63 + [2] * 2})
     assert batch._lens.tolist() == [65, 65]
+
+
+class Stored:
+    """A contiguous cache of n rows, as adopt reads one."""
+
+    def __init__(self, n, words=torch.bfloat16):
+        def buf():
+            return (torch.ones(1, H, n, D, dtype=torch.uint8), torch.ones(1, H, n, 2, dtype=words),
+                    torch.zeros(1, H, n, 2, dtype=words))
+        self.state = buf(), buf()
+
+
+class Unreadable(torch.Tensor):
+    def __getitem__(self, i):
+        raise Lost("copy")
+
+
+@pytest.mark.parametrize("n", [200, 128, 10])
+def test_a_cache_that_cannot_be_copied_takes_no_pages(plain, n):  # noqa: F811
+    cache = PagedKVCache(6, H, device="cpu")
+    src = Stored(n)
+    src.state[1][2].__class__ = Unreadable  # the last of the copies
+    with pytest.raises(Lost):
+        cache.adopt(src)
+    assert cache.free_pages == 6 and not cache._sessions
+    s = cache.adopt(Stored(n))
+    check(cache, {s: [1] * n})
