@@ -281,8 +281,8 @@ class PagedKVCache:
                 raise ValueError(f"codes {tuple(t.shape)} {t.dtype} are not those of one sequence of "
                                  f"{H} heads in 8 bits")
         for t in (*keys[1:], *values[1:]):
-            if t.shape != (1, H, n, HEAD_DIM // 64):
-                raise ValueError(f"scales or biases {tuple(t.shape)} are not of groups of 64")
+            if t.shape != (1, H, n, HEAD_DIM // 64) or t.dtype != torch.bfloat16:
+                raise ValueError(f"scales or biases {tuple(t.shape)} {t.dtype} are not bfloat16 of groups of 64")
         _lib.require_device(*keys, *values, *self.keys)
         pages = self._take(-(-n // PAGE))
         whole = n // PAGE

@@ -108,3 +108,15 @@ def test_a_cache_that_cannot_be_copied_takes_no_pages(plain, n):  # noqa: F811
     assert cache.free_pages == 6 and not cache._sessions
     s = cache.adopt(Stored(n))
     check(cache, {s: [1] * n})
+
+
+@pytest.mark.parametrize("words", [torch.float16, torch.float32])
+@pytest.mark.parametrize("part", [0, 1])
+def test_a_cache_of_other_scales_is_not_adopted(plain, words, part):  # noqa: F811
+    """Its scales or biases would be rounded to bf16: other values than the cache holds."""
+    cache = PagedKVCache(6, H, device="cpu")
+    src = Stored(70)
+    src.state = tuple(Stored(70, words).state[i] if i == part else src.state[i] for i in range(2))
+    with pytest.raises(ValueError, match="bfloat16"):
+        cache.adopt(src)
+    assert cache.free_pages == 6 and not cache._sessions
