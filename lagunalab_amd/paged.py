@@ -499,10 +499,10 @@ class PagedKVCache:
         if pages < max(used, 1):
             raise ValueError(f"{used} pages are in use: the pool cannot have {pages}")
         self.compact()
-        old = (*self.keys, *self.values)
-        self.keys, self.values = page_pool(pages, self.keys[0].shape[1], self.keys[0].device)
-        for t, x in zip((*self.keys, *self.values), old):
+        keys, values = page_pool(pages, self.keys[0].shape[1], self.keys[0].device)
+        for t, x in zip((*keys, *values), (*self.keys, *self.values)):
             t[:used] = x[:used]
+        self.keys, self.values = keys, values
         self._uses = self._uses[:used] + [0] * (pages - used)
         self._free = list(range(used, pages))
         self._version += 1

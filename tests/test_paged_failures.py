@@ -120,3 +120,28 @@ def test_a_cache_of_other_scales_is_not_adopted(plain, words, part):  # noqa: F8
     with pytest.raises(ValueError, match="bfloat16"):
         cache.adopt(src)
     assert cache.free_pages == 6 and not cache._sessions
+
+
+def test_a_resize_that_fails_keeps_the_pool(plain, monkeypatch):  # noqa: F811
+    cache = PagedKVCache(6, H, device="cpu")
+    s = cache.open()
+    cache.append([s], rows([7] * 100), rows([7] * 100))
+
+    class NoStores(torch.Tensor):
+        def __setitem__(self, i, x):
+            raise Lost("copy")
+    real = paged.page_pool
+
+    def broken(*args):
+        made = real(*args)
+        made[1][0].__class__ = NoStores
+        return made
+    monkeypatch.setattr(paged, "page_pool", broken)
+    with pytest.raises(Lost):
+        cache.resize(9)
+    check(cache, {s: [7] * 100})
+    assert cache.keys[0].shape[0] == 6 and cache.free_pages == 4
+    monkeypatch.setattr(paged, "page_pool", real)
+    cache.resize(9)
+    check(cache, {s: [7] * 100})
+    assert cache.keys[0].shape[0] == 9 and cache.free_pages == 7
