@@ -591,8 +591,14 @@ class PagedBatch:
         return lens.pop() if lens else 0
 
     def make_mask(self, N, return_array=False, window_size=None):
+        """The mask of a step of ``N`` rows. :meth:`attend` is causal over all rows whatever the mask: a
+        window that would leave some of them out is refused."""
         from .cache import create_attention_mask
-        return create_attention_mask(N, offset=self.offset, return_array=return_array, window_size=window_size)
+        offset = self.offset
+        if window_size is not None and offset + N > window_size:
+            raise ValueError(f"a window of {window_size} positions ends before the {offset + N} rows: paged "
+                             "batches are for full-attention layers")
+        return create_attention_mask(N, offset=offset, return_array=return_array, window_size=window_size)
 
     def is_trimmable(self):
         return True

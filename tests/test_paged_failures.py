@@ -145,3 +145,31 @@ def test_a_resize_that_fails_keeps_the_pool(plain, monkeypatch):  # noqa: F811
     cache.resize(9)
     check(cache, {s: [7] * 100})
     assert cache.keys[0].shape[0] == 9 and cache.free_pages == 7
+
+
+def test_masks_of_a_window_that_ends_before_the_rows_are_refused(plain):  # noqa: F811
+    """attend() is causal over all rows: a sliding-window layer gets that only while its window covers them."""
+    cache = PagedKVCache(6, H, device="cpu")
+    batch = cache.batch([cache.open(), cache.open()])
+    batch.update_and_fetch(step(1, 2, 60), step(1, 2, 60))
+    with pytest.raises(ValueError, match="window"):
+        batch.make_mask(1, window_size=60)
+    with pytest.raises(ValueError, match="window"):
+        batch.make_mask(8, window_size=67)
+    with pytest.raises(ValueError, match="window"):
+        batch.make_mask(1, window_size=0)
+    for n, window in ((1, 61), (8, 68), (8, 500)):  # the whole of what the rows see
+        q, k = torch.arange(60, 60 + n)[:, None], torch.arange(60 + n)[None]
+        assert torch.equal(batch.make_mask(n, window_size=window), k <= q)
+    assert batch.make_mask(8) == "causal" and batch.make_mask(1) is None
+    assert torch.equal(batch.make_mask(8, return_array=True), batch.make_mask(8, window_size=68))
+
+
+def test_a_model_with_a_sliding_window_layer_is_refused(plain):  # noqa: F811
+    from tiny_model import TinyArgs, TinyLM
+    model = TinyLM(TinyArgs(layer_types=["sliding_attention"]))
+    cache = PagedKVCache(6, H, device="cpu")
+    s = cache.open()
+    with pytest.raises(ValueError, match="window"), torch.no_grad():
+        model(torch.tensor([[1, 2, 3, 4, 5, 6, 7, 8, 9]]), cache=[cache.batch([s])])
+    assert cache.length(s) == 0 and cache.free_pages == 6
