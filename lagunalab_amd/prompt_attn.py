@@ -7,6 +7,7 @@ from __future__ import annotations
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -16,6 +17,8 @@ HEAD_DIM = 128
 def _refuse_grad(*tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError("this attention has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("this attention has no forward derivative: its inputs have tangents")
 
 
 def _lens(lens, what):

@@ -155,3 +155,31 @@ def test_arguments_that_do_not_fit():
         paged.paged_gather((keys[0].transpose(0, 1), *keys[1:]), values, torch.zeros(1, 1), None, [1])
     with pytest.raises(ValueError, match="contiguous"):
         paged.paged_gather((keys[0].int(), *keys[1:]), values, torch.zeros(1, 1), None, [1])
+
+
+def test_gradients_and_tangents_are_refused(monkeypatch):
+    """Neither attention has a backward or a forward derivative: a call that would need one raises, before any
+    work (what follows the check is left out here)."""
+    from torch.autograd import forward_ad
+    monkeypatch.setattr(_lib, "require_device", lambda *t: t[0].device)
+    x = torch.zeros((2, 2, 128), dtype=torch.bfloat16)
+    grad = x.clone().requires_grad_()
+    for args in ((grad, x, x), (x, grad, x), (x, x, grad)):
+        with pytest.raises(ValueError, match="backward"):
+            prompt_attn.prompt_attention(*args, [2], 0.1)
+    monkeypatch.setattr(paged, "_pool", lambda k, v: (4, 2, x.device, [0] * 6))
+    keys, values = paged.page_pool(4, 2, device="cpu")
+    decode = lambda q: paged.paged_decode_attention(q.unsqueeze(2), keys, values, None, None, 0.1)  # noqa: E731
+    with pytest.raises(ValueError, match="backward"):
+        decode(grad)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for no_grad in (False, True):  # which does not stop forward mode
+            with torch.set_grad_enabled(not no_grad):
+                for args in ((dual, x, x), (x, dual, x), (x, x, dual)):
+                    with pytest.raises(ValueError, match="tangent"):
+                        prompt_attn.prompt_attention(*args, [2], 0.1)
+                with pytest.raises(ValueError, match="tangent"):
+                    decode(dual)
+        with pytest.raises(ValueError, match="table"):  # plain tensors beside it go on
+            decode(x)
