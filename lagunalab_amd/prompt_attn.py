@@ -35,7 +35,7 @@ def _rows(x, heads, total, what):
         raise ValueError(f"{what} {tuple(x.shape)} does not have {total} rows"
                          + (f" of {heads} heads" if heads else ""))
     st = x.stride()
-    if st[2] != 1 or st[0] % 8 or st[1] % 8 or x.data_ptr() % 16:
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or st[0] >= 1 << 24 or x.data_ptr() % 16:  # the kernel's limits
         x = x.clone(memory_format=torch.contiguous_format)
         st = x.stride()
     return x, st[0], st[1]

@@ -898,3 +898,15 @@ def test_attention_block_over_a_paged_batch(dev):
         mask = None if L == 1 else "causal"
         got, want = block(x, mask, batch), block(x, mask, wide)
         assert (got.float() - want.float()).abs().max() < 3e-2 * want.float().abs().max()
+
+
+def test_prompt_rows_far_apart(dev):
+    """Keys, values and queries 2^24 values apart, as rows of a wide buffer are."""
+    g = gen(38)
+    q, k, v = randn(g, 3, 4, D), randn(g, 5, 2, D), randn(g, 5, 2, D)
+    wide = torch.zeros((5, 1 << 24), dtype=torch.bfloat16, device=dev)
+    views = []
+    for at, x in ((0, q), (1024, k), (2048, v)):
+        views.append(wide[:x.shape[0], at:at + x[0].numel()].unflatten(1, x.shape[1:]))
+        views[-1].copy_(x)
+    check_prompt(prompt_attention(*views, [1, 2], SCALE, k_lens=[3, 2]), q, k, v, [1, 2], [3, 2])

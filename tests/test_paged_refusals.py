@@ -183,3 +183,14 @@ def test_gradients_and_tangents_are_refused(monkeypatch):
                     decode(dual)
         with pytest.raises(ValueError, match="table"):  # plain tensors beside it go on
             decode(x)
+
+
+def test_prompt_rows_far_apart_are_copied():
+    """Any token and head strides: the kernel takes rows less than 2^24 values apart as they lie, others are
+    copied, and so is a single row whatever its stride."""
+    far = 1 << 24
+    store = torch.zeros(far + 300, dtype=torch.bfloat16)
+    for rows, stride, copied in ((2, far, True), (2, far - 8, False), (1, 1 << 40, True), (1, 256, False)):
+        x = store.as_strided((rows, 2, 128), (stride, 128, 1))
+        got, tok, head = prompt_attn._rows(x, 2, rows, "k")
+        assert (got is not x) == copied and (tok, head) == ((256 if copied else stride), 128)
