@@ -147,6 +147,14 @@ def raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def capturing(device: torch.device) -> bool:
+    """Whether work on the device's current stream is recorded into a graph instead of done."""
+    if device.type != "cuda":
+        return False
+    with on_device(device):
+        return torch._C._cuda_isCurrentStreamCapturing()
+
+
 def require_device(*tensors: torch.Tensor):
     """All tensors on one ROCm device; returns it."""
     dev = None

@@ -240,7 +240,8 @@ class PagedKVCache:
     it. Pages go back to the pool when their last session is closed or trimmed below them; an append that
     raises leaves its sessions as they were. The lists live on the host; device work runs on the current
     stream, and calls on one cache belong on one stream (a page given back may be taken by the next
-    call)."""
+    call), outside of captured graphs: a replay would repeat the recorded step on the recorded rows
+    (:func:`paged_append` and :func:`paged_decode_attention` can be captured)."""
 
     def __init__(self, pages: int, n_kv_heads: int, device="cuda"):
         self.keys, self.values = page_pool(pages, n_kv_heads, device)
@@ -271,6 +272,7 @@ class PagedKVCache:
         """A session of the rows of a contiguous 8-bit cache of one sequence (a ``DequantKVCache`` or
         ``QuantizedKVCache`` of group 64, loaded from a prompt cache for instance): its codes, scales and
         biases are copied as they are."""
+        self._outside_graphs()
         keys, values = cache.state
         if keys is None:
             return self.open()
@@ -335,6 +337,10 @@ class PagedKVCache:
     @property
     def nbytes(self):
         return sum(t.numel() * t.element_size() for t in (*self.keys, *self.values))
+
+    def _outside_graphs(self):
+        if _lib.capturing(self.keys[0].device):
+            raise RuntimeError("sessions move on the host: calls on them cannot be captured into a graph")
 
     def _session(self, session):
         if session not in self._sessions:
@@ -432,6 +438,7 @@ class PagedKVCache:
     def append(self, sessions, k, v, counts=None):
         """Appends rows ``k``, ``v`` (bf16 ``[T, Hkv, 128]``, packed one session behind the other,
         ``counts[i]`` each or as many each) to the sessions."""
+        self._outside_graphs()
         sessions, states = self._distinct(sessions)
         if not states:
             return
@@ -460,12 +467,14 @@ class PagedKVCache:
 
     def rows(self, sessions):
         """All rows of the sessions as bf16, packed: ``(k, v)``, each ``[sum of lengths, Hkv, 128]``."""
+        self._outside_graphs()
         _, states = self._distinct(sessions)
         table, lens = self._tables(states)
         return paged_gather(self.keys, self.values, table, torch.zeros_like(lens), [n for _, n in states])
 
     def attention(self, sessions, q, scale):
         """Attention of one new token per session over its rows: ``q`` bf16 ``[B, Hq, 1, 128]``."""
+        self._outside_graphs()
         _, states = self._distinct(sessions)
         table, lens = self._tables(states)
         return paged_decode_attention(q, self.keys, self.values, table, lens, scale,
@@ -479,6 +488,7 @@ class PagedKVCache:
 
     def compact(self) -> int:
         """Moves pages in use to the front of the pool; returns how many there are."""
+        self._outside_graphs()
         live = [p for p, n in enumerate(self._uses) if n]
         n = len(live)
         holes = [p for p in range(n) if not self._uses[p]]
@@ -495,6 +505,7 @@ class PagedKVCache:
 
     def resize(self, pages: int):
         """A pool of ``pages`` pages: compacted, then copied into new buffers."""
+        self._outside_graphs()
         used = len(self._uses) - len(self._free)
         if pages < max(used, 1):
             raise ValueError(f"{used} pages are in use: the pool cannot have {pages}")
@@ -536,6 +547,7 @@ class PagedBatch:
     def update_and_fetch(self, keys, values):
         """Appends ``keys``, ``values`` (bf16 ``[B, Hkv, L, 128]``) to the sessions; returns them (attention
         goes through :meth:`attend`)."""
+        self.cache._outside_graphs()
         B, H, L, D = keys.shape
         if B != len(self.sessions) or (H, D) != (self.cache.keys[0].shape[1], HEAD_DIM) \
                 or values.shape != keys.shape:
@@ -565,6 +577,7 @@ class PagedBatch:
     def attend(self, queries, scale):
         """Attention of the step's rows, ``queries`` bf16 ``[B, Hq, L, 128]``: the last ``L`` positions of
         each session, causal."""
+        self.cache._outside_graphs()
         B, Hq, L, D = queries.shape
         if B != len(self.sessions):
             raise ValueError(f"{B} rows of queries for {len(self.sessions)} sessions")

@@ -910,3 +910,37 @@ def test_prompt_rows_far_apart(dev):
         views.append(wide[:x.shape[0], at:at + x[0].numel()].unflatten(1, x.shape[1:]))
         views[-1].copy_(x)
     check_prompt(prompt_attention(*views, [1, 2], SCALE, k_lens=[3, 2]), q, k, v, [1, 2], [3, 2])
+
+
+def test_sessions_are_not_captured(dev):
+    """A step of a batch inside a capture is refused before anything is recorded or moved; the graph goes on
+    without it, and the sessions step outside."""
+    from lagunalab_amd.paged import PagedKVCache
+    g = gen(39)
+    cache = PagedKVCache(8, 2, dev)
+    batch = cache.batch([cache.open(), cache.open()])
+    rows = lambda L: randn(g, 2, 2, L, D).to(dev)  # noqa: E731
+    batch.update_and_fetch(rows(70), rows(70))
+    k, q = rows(1), randn(g, 2, 4, 1, D).to(dev)
+    batch.attend(q, SCALE)
+    before = [t.clone() for t in (*cache.keys, *cache.values)]
+    x = torch.zeros(4, device=dev)
+    stream = torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            x += 1
+            for call in (lambda: batch.update_and_fetch(k, k), lambda: batch.attend(q, SCALE),
+                         lambda: cache.attention(batch.sessions, q, SCALE)):
+                with pytest.raises(RuntimeError, match="captured"):
+                    call()
+    torch.cuda.current_stream(dev).wait_stream(stream)
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        assert (x == i + 1).all() and batch.offset == 70
+        for t, o in zip((*cache.keys, *cache.values), before):
+            assert torch.equal(bits(t), bits(o))
+    batch.update_and_fetch(k, k)
+    assert batch.offset == 71 and batch.attend(q, SCALE).isfinite().all()

@@ -173,3 +173,23 @@ def test_a_model_with_a_sliding_window_layer_is_refused(plain):  # noqa: F811
     with pytest.raises(ValueError, match="window"), torch.no_grad():
         model(torch.tensor([[1, 2, 3, 4, 5, 6, 7, 8, 9]]), cache=[cache.batch([s])])
     assert cache.length(s) == 0 and cache.free_pages == 6
+
+
+def test_nothing_of_the_session_layer_runs_in_a_captured_graph(plain, monkeypatch):  # noqa: F811
+    """Its lists and lengths move on the host, once: a replay would write the same rows again."""
+    cache = PagedKVCache(8, H, device="cpu")
+    a, b = cache.open(), cache.open()
+    cache.append([a, b], rows([1] * 80), rows([1] * 80))
+    cache.close(cache.fork(a))
+    batch = cache.batch([a, b])
+    q = torch.zeros(2, 4, 1, D, dtype=torch.bfloat16)
+    monkeypatch.setattr(paged._lib, "capturing", lambda dev: True)
+    for call in (lambda: cache.append([a], rows([2]), rows([2])), lambda: cache.rows([a]),
+                 lambda: cache.attention([a, b], q, 0.1), lambda: cache.compact(), lambda: cache.resize(9),
+                 lambda: cache.adopt(Stored(70)), lambda: batch.update_and_fetch(step(2, 2, 1), step(2, 2, 1)),
+                 lambda: batch.attend(q, 0.1)):
+        with pytest.raises(RuntimeError, match="captured"):
+            call()
+    check(cache, {a: [1] * 40, b: [1] * 40})
+    monkeypatch.undo()
+    assert paged._lib.capturing(torch.device("cpu")) is False
