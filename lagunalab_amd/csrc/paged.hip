@@ -231,7 +231,7 @@ extern "C" int lq_paged_append(const uint16_t* k, const uint16_t* v, int64_t k_t
                    ((k_tok | k_head | v_tok | v_head) & 7) == 0,
                "rows must be 16-byte aligned (strides a multiple of 8)");
   const int64_t units = T * Hkv;
-  LQ_CHECK_ARG(units < (int64_t)1 << 28, "an append of %lld rows is too large for one call",
+  LQ_CHECK_ARG((units + 15) / 16 < 1 << 24, "an append of %lld rows is too large for one call",
                (long long)T);
   paged_append_kernel<<<dim3((unsigned)((units + 15) / 16), 2), dim3(256), 0, (hipStream_t)stream>>>(
       k, v, k_tok, k_head, v_tok, v_head, buf, tab, starts, rows, (uint32_t)units,

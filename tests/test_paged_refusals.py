@@ -194,3 +194,10 @@ def test_prompt_rows_far_apart_are_copied():
         x = store.as_strided((rows, 2, 128), (stride, 128, 1))
         got, tok, head = prompt_attn._rows(x, 2, rows, "k")
         assert (got is not x) == copied and (tok, head) == ((256 if copied else stride), 128)
+
+
+def test_appends_of_a_full_grid_are_refused(lib):
+    """16 rows per workgroup of 256 threads: 2^32 threads are more than a launch may have."""
+    for kv, rows in ((8, (1 << 25) - 1), (1, (1 << 28) - 14)):
+        assert append(lib, kv=kv, counts=ints(rows), n=1) == _lib.LQ_EINVAL
+        assert b"too large" in lib.lq_last_error()
