@@ -1,0 +1,263 @@
+"""Every form of the paged decode kernel and every way of dealing out prompts, on values that name their page or
+their key (one lost, doubled or taken from elsewhere shows at any length), at the scales and magnitudes where a
+form's own arithmetic could go wrong, and on pages beyond 4 GB. Which form a call takes follows from its shape;
+the tests check that the shapes here take the one they mean."""
+import ctypes as C
+
+import pytest
+import torch
+
+from lagunalab_amd import _lib
+from lagunalab_amd.paged import copy_pages, paged_append, paged_decode_attention, paged_gather
+from lagunalab_amd.prompt_attn import prompt_attention
+from paged_util import D, PAGE, assert_within, exact_attention, make_table, randn, read_rows, write_rows
+
+pytestmark = pytest.mark.gpu
+SCALE = D ** -0.5
+
+# (query heads, KV heads, sequences, shared positions): pages dealt out; the shared ones with them (9 query rows);
+# shared parts for blocks of 32, 64 and 128 rows, for two blocks; parts of 32 pages, whose last ones are left
+# to the workgroups of own pages
+FORMS = {
+    "dealt out": (8, 2, 9, 0), "dealt out, 16 rows": (32, 2, 9, 0), "shared dealt out": (16, 16, 9, 512),
+    "blocks of 32": (32, 16, 9, 512), "blocks of 64": (64, 16, 9, 512), "blocks of 128": (64, 8, 9, 1024),
+    "two blocks": (128, 8, 9, 1024), "late pages": (128, 64, 9, 8192),
+}
+SPARE = 17  # pages that a table row has beyond the longest: tables of up to 16 take whole sequences
+
+
+def gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def workspace(B, hq, kv, pages):
+    return _lib.load().lq_paged_decode_workspace_bytes(B, hq, kv, pages)
+
+
+def lengths(B, shared, most=300):
+    """Own positions from none to several pages, sequences that end before the shared part, with it, and in it."""
+    g = gen(shared + B)
+    lens = [shared + int(n) for n in torch.randint(1, most, (B,), generator=g)]
+    if shared:
+        lens[0], lens[1], lens[2], lens[3] = shared - 1, shared, 1, shared // 2 + 5
+    else:
+        lens[0], lens[1], lens[2], lens[3] = 63, 64, 1, 0
+    return lens
+
+
+def check_form(form, table):
+    hq, kv, B, shared = FORMS[form]
+    assert table.shape[1] > 16
+    # read once: with rows of partial results for them
+    once = workspace(B, hq, kv, shared // PAGE) > workspace(B, hq, kv, 0)
+    assert once == (shared > 0)
+
+
+def names(pages, kv, by):
+    """The dim that names a pool's slot [pages, kv, 64]: by its page or by its key."""
+    at, heads = torch.arange(pages)[:, None, None], torch.arange(kv)[:, None]
+    return ((5 * at + 3 * heads + (37 * torch.arange(PAGE) if by == "key" else 0)) % D).expand(pages, kv, PAGE)
+
+
+def wanted(dim, table, lens):
+    """What every sequence and KV head gets of rows that are 1 in their dim, under equal weights."""
+    kv = dim.shape[1]
+    want = torch.zeros((len(lens), kv, D), dtype=torch.float64)
+    for b, n in enumerate(lens):
+        if n:
+            p, slot = table[b, torch.arange(n) // PAGE].long(), torch.arange(n) % PAGE
+            want[b].scatter_add_(1, dim[p, :, slot].T, torch.ones((kv, n), dtype=torch.float64))
+            want[b] /= n
+    return want
+
+
+def named(seed, dim, table, lens, dev):
+    """A pool whose V rows are 1 in their dim; slots that no sequence has hold NaN scales."""
+    pages, kv, _ = dim.shape
+    used = torch.zeros((pages, PAGE), dtype=torch.bool)
+    for b, n in enumerate(lens):
+        used[table[b, torch.arange(n) // PAGE].long(), torch.arange(n) % PAGE] = True
+    v = torch.zeros((pages, kv, PAGE, D), dtype=torch.uint8).scatter_(3, dim[..., None], 1)
+    k = torch.randint(0, 256, (pages, kv, PAGE, D), generator=gen(seed), dtype=torch.uint8)
+    scales, biases = (torch.where(used, x, float("nan"))[:, None, :, None].expand(-1, kv, -1, 2)
+                      .to(torch.bfloat16) for x in (1.0, 0.0))
+    return [tuple(t.contiguous().to(dev) for t in (codes, scales, biases)) for codes in (k, v)]
+
+
+def assert_named(out, want, what):
+    """Equal weights: sums and their quotient of whole numbers below 2^24, exact but for the reciprocal and the
+    product (2^-24 each, with room), rounded to bf16 (2^-8)."""
+    got = out.double().cpu()
+    off = (got - want).abs() - want * (2.0 ** -8 + 2.0 ** -20)
+    assert (off <= 0).all(), f"{what}: {int((off > 0).sum())} values, by up to {off.max().item():.3g}"
+
+
+@pytest.mark.parametrize("by", ["page", "key"])
+@pytest.mark.parametrize("form", FORMS)
+def test_every_page_and_key_counts_once(dev, form, by):
+    hq, kv, B, shared = FORMS[form]
+    lens = lengths(B, shared)
+    table, pages = make_table(gen(1), lens, shared, width_spare=SPARE)
+    check_form(form, table)
+    dim = names(pages, kv, by)
+    pool = named(2, dim, table, lens, dev)
+    q = randn(gen(3), B, hq, 1, D).to(dev)
+    n_d = torch.zeros(B, dtype=torch.int32, device=dev)
+    # shorter by up to two pages and a part: the shared part's end passes through the lengths
+    for less in (0, 1, 64, 150):
+        now = [max(0, n - less) for n in lens]
+        n_d.copy_(torch.tensor(now, dtype=torch.int32))
+        out = paged_decode_attention(q, *pool, table.to(dev), n_d, 0.0, shared=shared)
+        want = wanted(dim, table, now).repeat_interleave(hq // kv, 1)[:, :, None]
+        assert_named(out, want, f"{form}, {less} fewer")
+
+
+@pytest.mark.parametrize("by", ["page", "key"])
+@pytest.mark.parametrize("hq,kv,lens,spare", [
+    (4, 1, [16390, 5], 0), (32, 8, [16001], 0), (16, 1, [1024, 1023, 577], 0), (32, 8, [130] * 33 + [1000], 0),
+    (6, 2, list(range(0, 640, 7)), 9), (3, 3, [2, 9000, 1, 700], 0),
+])
+def test_every_page_and_key_of_single_sequences(dev, hq, kv, lens, spare, by):
+    table, pages = make_table(gen(4), lens, 0, width_spare=spare)
+    dim = names(pages, kv, by)
+    pool, want = named(5, dim, table, lens, dev), wanted(dim, table, lens)
+    q = randn(gen(6), len(lens), hq, 1, D).to(dev)
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    out = paged_decode_attention(q, *pool, table.to(dev), n_d, 0.0)
+    assert_named(out, want.repeat_interleave(hq // kv, 1)[:, :, None], "single")
+
+
+def rows_case(form, dev, vstd=1.0, own=90):
+    """Quantized rows of a form's sequences: (pool, table, lens)."""
+    hq, kv, B, shared = FORMS[form]
+    lens = lengths(B, shared, own if shared else 1500)
+    g = gen(7)
+    table, pages = make_table(g, lens, shared, width_spare=SPARE)
+    check_form(form, table)
+    pool = []
+    for _ in range(2):  # what no sequence has: NaN
+        codes = torch.randint(0, 256, (pages, kv, PAGE, D), generator=g, dtype=torch.uint8)
+        words = torch.full((pages, kv, PAGE, 2), float("nan"), dtype=torch.bfloat16)
+        pool.append((codes.to(dev), words.to(dev), words.to(dev)))
+    if shared:
+        longest = max(range(B), key=lambda b: lens[b])
+        write_rows(pool, table[longest], randn(g, shared, kv, D), randn(g, shared, kv, D, std=vstd))
+    for b, n in enumerate(lens):
+        if n > shared:
+            write_rows(pool, table[b], randn(g, n - shared, kv, D), randn(g, n - shared, kv, D, std=vstd), shared)
+    return pool, table, lens
+
+
+def check_rows(out, q, pool, table, lens, scale, rows):
+    hq, kv = q.shape[1], pool[0][0].shape[1]
+    G = hq // kv
+    for b in rows:
+        k, v = (read_rows(buf, table[b], lens[b]) for buf in pool)
+        for h in range(kv):
+            want, bound = exact_attention(q[b, h * G:(h + 1) * G, 0].double(), k[:, h], v[:, h],
+                                          [lens[b] - 1] * G, scale)
+            assert_within(out[b, h * G:(h + 1) * G, 0], want, bound, f"sequence {b} head {h}")
+
+
+SMALLER = [f for f in FORMS if f != "late pages"]
+
+
+@pytest.mark.parametrize("form", SMALLER)
+def test_forms_at_other_scales(dev, form):
+    hq, kv, B, shared = FORMS[form]
+    pool, table, lens = rows_case(form, dev)
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    for scale, std in ((-SCALE, 1.0), (0.0, 1.0), (1.0, 1.0), (SCALE, 30.0), (SCALE, 1e-6)):
+        q = randn(gen(8), B, hq, 1, D, std=std)
+        out = paged_decode_attention(q.to(dev), *pool, table.to(dev), n_d, scale, shared=shared)
+        check_rows(out, q, pool, table, lens, scale, [0, 4, B - 1])
+
+
+@pytest.mark.parametrize("vstd", [1e20, 1e-20])
+@pytest.mark.parametrize("form", SMALLER)
+def test_forms_at_large_and_tiny_values(dev, form, vstd):
+    hq, kv, B, shared = FORMS[form]
+    pool, table, lens = rows_case(form, dev, vstd=vstd)
+    q = randn(gen(9), B, hq, 1, D)
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    out = paged_decode_attention(q.to(dev), *pool, table.to(dev), n_d, SCALE, shared=shared)
+    check_rows(out, q, pool, table, lens, SCALE, [0, 1, B - 1])
+
+
+def test_late_pages_at_other_scales(dev):
+    hq, kv, B, shared = FORMS["late pages"]
+    pool, table, lens = rows_case("late pages", dev, own=30)
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    for scale, std in ((-SCALE, 1.0), (SCALE, 30.0)):
+        q = randn(gen(10), B, hq, 1, D, std=std)
+        out = paged_decode_attention(q.to(dev), *pool, table.to(dev), n_d, scale, shared=shared)
+        check_rows(out, q, pool, table, lens, scale, [B - 1])
+
+
+FAR = {"dealt out": (16, 8, 3, 0), "shared dealt out": (8, 8, 9, 1024), "blocks of 32": (8, 8, 17, 512),
+       "blocks of 64": (16, 8, 17, 512), "blocks of 128": (64, 8, 17, 512)}
+
+
+def test_forms_on_pages_beyond_32_bit_offsets(dev):
+    """Pages whose codes lie more than 4 GB into the pool, in the tables of every form: appended, attended to,
+    copied and read back."""
+    pages, kv = 67000, 8
+    pool = [(torch.empty((pages, kv, PAGE, D), dtype=torch.uint8, device=dev),
+             torch.empty((pages, kv, PAGE, 2), dtype=torch.bfloat16, device=dev),
+             torch.empty((pages, kv, PAGE, 2), dtype=torch.bfloat16, device=dev)) for _ in range(2)]
+    g = gen(11)
+    for form, (hq, kv, B, shared) in FAR.items():
+        lens = [(shared or 1000) + 10 + 37 * b for b in range(B)]
+        low, count = make_table(g, lens, shared, spare=0, width_spare=SPARE)
+        assert low.shape[1] > 16
+        assert (workspace(B, hq, kv, shared // PAGE) > workspace(B, hq, kv, 0)) == (shared > 0), form
+        ids = 66000 + torch.randperm(1000, generator=g)[:count].to(torch.int32)
+        far = ids[low.long()]
+        # the shared rows through the first sequence, its own and the others' behind them
+        counts = [lens[0]] + [n - shared for n in lens[1:]]
+        k, v = randn(g, sum(counts), kv, D).to(dev), randn(g, sum(counts), kv, D).to(dev)
+        starts = torch.tensor([0] + [shared] * (B - 1), dtype=torch.int32, device=dev)
+        paged_append(k, v, *pool, far.to(dev), starts, counts)
+        near = [tuple(t[ids.long().to(dev)].cpu() for t in buf) for buf in pool]
+        q = randn(g, B, hq, 1, D)
+        n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+        out = paged_decode_attention(q.to(dev), *pool, far.to(dev), n_d, SCALE, shared=shared)
+        check_rows(out, q, near, low, lens, SCALE, [0, B // 2, B - 1])
+        rows = paged_gather(*pool, far.to(dev), torch.zeros_like(n_d), lens)
+        for x, buf in zip(rows, near):
+            want = torch.cat([read_rows(buf, low[b], lens[b]) for b in range(B)])
+            assert torch.equal(x.cpu().double(), want), form
+        there = 65000 + torch.arange(count)
+        copy_pages(*pool, ids, there)
+        for buf in pool:
+            for t in buf:
+                same = t[ids.long().to(dev)].view(torch.uint8) == t[there.to(dev)].view(torch.uint8)
+                assert same.all(), form
+
+
+# -------------------------------------------------------------------------------- packed prompts
+
+@pytest.mark.parametrize("hq,kv,q_lens,k_lens,parts", [
+    (8, 2, [700, 0, 1, 130, 64, 40], [700, 9, 1, 130, 190, 33], False),  # small blocks, all resident
+    (64, 8, [900] * 3 + [77], [900] * 3 + [600], False),                  # small blocks, several rounds
+    (8, 2, [260, 33], [9000, 4444], True),                                # shares that end inside blocks
+    (12, 2, [512], [8193], True), (5, 1, [1000, 1, 700], [5001, 8000, 700], True),
+    (256, 4, [1600], [7000], False),                                      # large blocks, several rounds
+])
+def test_every_key_of_a_prompt_counts_once(dev, hq, kv, q_lens, k_lens, parts):
+    """Equal weights over V rows that are 1 in the dim of their key: row i gets the shares of the keys it sees."""
+    lq, lk = ((C.c_int32 * len(x))(*x) for x in (q_lens, k_lens))
+    assert (_lib.load().lq_prompt_workspace_bytes(lq, lk, len(q_lens), hq, kv) > 0) == parts
+    g = gen(12)
+    q, k = randn(g, sum(q_lens), hq, D), randn(g, sum(k_lens), kv, D)
+    for by in (1, 64):  # every key, every tile of keys
+        dim = (5 * (torch.arange(sum(k_lens))[:, None] // by) + 3 * torch.arange(kv)) % D
+        v = torch.nn.functional.one_hot(dim, D)
+        out = prompt_attention(q.to(dev), k.to(dev), v.to(torch.bfloat16).to(dev), q_lens, 0.0, k_lens=k_lens)
+        a = c = 0
+        for n, m in zip(q_lens, k_lens):
+            seen = torch.arange(m - n, m).clamp(min=-1) + 1  # keys of each row
+            upto = torch.cat([torch.zeros((1, kv, D)), v[c:c + m].double().cumsum(0)])  # [m + 1, kv, 128]
+            want = upto[seen] / seen.clamp(min=1)[:, None, None]
+            assert_named(out[a:a + n], want.repeat_interleave(hq // kv, 1), f"{n} rows on {m}")
+            a, c = a + n, c + m
