@@ -227,8 +227,9 @@ __device__ __forceinline__ void tile_values(const uint16_t* v, TileRows<NT>& st,
 }
 
 // Q.K^T of one tile, then P.V of another, in eight steps of 4 NT MFMAs: two key tiles of K by half the
-// dims (so that an MFMA's accumulator was last written 2 NT MFMAs before), then half a k-step of V. A step's four fragments are read two steps ahead (tile_ahead: the first two, which may
-// lie in the phase before), so that no MFMA waits for LDS.
+// dims (so that an MFMA's accumulator was last written 2 NT MFMAs before), then half a k-step of V. A step's
+// four fragments are read two steps ahead (tile_ahead: the first two, which may lie in the phase before), so
+// that no MFMA waits for LDS.
 struct Ahead {
   bf16x8_t f[3][4];
 };

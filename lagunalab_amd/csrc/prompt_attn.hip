@@ -5,12 +5,12 @@
 // without a key are 0.
 //
 // Work: a workgroup of 8 waves (or 4, see below) takes 256 query rows (128) of a KV head, numbered
-// position-major (row f is position f / G of query head f % G), so that any grouping fills the matrix cores
-// and a block's rows see nearly the same keys; a wave has 32 of them. It walks the 64-key tiles up to its last row's bound, each
-// copied into LDS once for all waves (three buffers of K and of V, copies two tiles ahead) and run through
-// attn_tile.h. A SIMD holds one wave of each half of the workgroup, and the halves run one phase apart, so
-// that one's matrix phase (P.V of a tile, Q.K^T of the next) lies beside the other's vector phase (softmax,
-// copies), with a barrier after each:
+// position-major (row f is position f / G of query head f % G), so that any grouping fills the matrix
+// cores and a block's rows see nearly the same keys; a wave has 32 of them. It walks the 64-key tiles up
+// to its last row's bound, each copied into LDS once for all waves (three buffers of K and of V, copies
+// two tiles ahead) and run through attn_tile.h. A SIMD holds one wave of each half of the workgroup, and
+// the halves run one phase apart, so that one's matrix phase (P.V of a tile, Q.K^T of the next) lies
+// beside the other's vector phase (softmax, copies), with a barrier after each:
 //
 //   slot    group A                   group B
 //   2t      Q.K^T(t), P.V(t-1)        softmax(t-1), copies K(t+2) V(t+1)
@@ -163,213 +163,215 @@ __global__ __launch_bounds__(64 * PW, 2) void prompt_attn_kernel(const PromptArg
   const int64_t u0 = a.share * share;  // 0 for a whole block
   const int64_t u1 = a.share ? min(u0 + a.share, a.cost[a.nseq]) : b.tiles + BLOCK_COST;
   for (bool more = true; more;) {
-  // re-read per block, so that no lane value made of it is kept across blocks
-  int tid = threadIdx.x;
-  asm volatile("" : "+v"(tid));
-  const int lane = tid & 63;
-  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const bool grp_a = HALVES && wv < PW / 2;
-  const int lc = lane & 15, lq4 = lane >> 4;
-  const int s = b.seq, blk = b.blk;
-  const int q0 = a.q_begin[s], lq = a.q_begin[s + 1] - q0;
-  const int k0 = a.k_begin[s], lk = a.k_begin[s + 1] - k0;
-  const int R = lq * a.G, base = lk - lq;
-  const int tiles = b.tiles;
-  const int t0 = HALVES ? cut_tile(b, u0) : 0, t1 = HALVES ? cut_tile(b, u1) : tiles;
-  // a block without a tile (rows without keys) belongs to the share that its begin lies in
-  const bool mine = t0 < t1 || (tiles == 0 && b.begin >= u0 && b.begin < u1);
-  if (mine) {
-  const float scale = abs_scale(a.sl2);
-  // tiles from here on are masked for some row of the block (or end behind the last key)
-  const int low = base + (int)fdiv_u((uint32_t)(blk * ROWS), a.g);
-  const int t_masked = low < 0 ? 0 : (low + 1) / TKEYS;
+    // re-read per block, so that no lane value made of it is kept across blocks
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool grp_a = HALVES && wv < PW / 2;
+    const int lc = lane & 15, lq4 = lane >> 4;
+    const int s = b.seq, blk = b.blk;
+    const int q0 = a.q_begin[s], lq = a.q_begin[s + 1] - q0;
+    const int k0 = a.k_begin[s], lk = a.k_begin[s + 1] - k0;
+    const int R = lq * a.G, base = lk - lq;
+    const int tiles = b.tiles;
+    const int t0 = HALVES ? cut_tile(b, u0) : 0, t1 = HALVES ? cut_tile(b, u1) : tiles;
+    // a block without a tile (rows without keys) belongs to the share that its begin lies in
+    const bool mine = t0 < t1 || (tiles == 0 && b.begin >= u0 && b.begin < u1);
+    if (mine) {
+      const float scale = abs_scale(a.sl2);
+      // tiles from here on are masked for some row of the block (or end behind the last key)
+      const int low = base + (int)fdiv_u((uint32_t)(blk * ROWS), a.g);
+      const int t_masked = low < 0 ? 0 : (low + 1) / TKEYS;
 
-  // ---- copies: wave wv brings 4 CP keys from 4 CP wv on of every tile, K and V 1 KB (4 keys) at a time; a
-  // lane's 16 bytes land at lane x 16, so the swizzle is in the chunk it reads. Keys past the last one
-  // read it again.
-  const int krow = 4 * CP * wv + (lane >> 4);  // and + 4, ..
-  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + (int64_t)k0 * a.k_tok + hk * a.k_head);
-  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + (int64_t)k0 * a.v_tok + hk * a.v_head);
-  const uint32_t k_at = lds_u32(sm.k) + 1024u * CP * wv, v_at = lds_u32(sm.v) + 1024u * CP * wv;
-  // A tile's base is scalar, a lane's offset in it fixed but in the tile that ends behind the last key.
-  auto copy = [&](const uint8_t* from, int64_t tok, int t, uint32_t to, const uint32_t (&at)[CP], bool is_v) {
-    const int tt = min(t, t1 - 1);
-    const uint8_t* sb = from + 2 * TKEYS * tok * tt;
-    const uint32_t m = __builtin_amdgcn_readfirstlane(to + (uint32_t)(t % STAGES) * (TKEYS * D * 2));
-    uint32_t o[CP];
+      // ---- copies: wave wv brings 4 CP keys from 4 CP wv on of every tile, K and V 1 KB (4 keys) at a
+      // time; a lane's 16 bytes land at lane x 16, so the swizzle is in the chunk it reads. Keys past the
+      // last one read it again.
+      const int krow = 4 * CP * wv + (lane >> 4);  // and + 4, ..
+      const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + (int64_t)k0 * a.k_tok + hk * a.k_head);
+      const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + (int64_t)k0 * a.v_tok + hk * a.v_head);
+      const uint32_t k_at = lds_u32(sm.k) + 1024u * CP * wv, v_at = lds_u32(sm.v) + 1024u * CP * wv;
+      // A tile's base is scalar, a lane's offset in it fixed but in the tile that ends behind the last key.
+      auto copy = [&](const uint8_t* from, int64_t tok, int t, uint32_t to, const uint32_t (&at)[CP],
+                      bool is_v) {
+        const int tt = min(t, t1 - 1);
+        const uint8_t* sb = from + 2 * TKEYS * tok * tt;
+        const uint32_t m = __builtin_amdgcn_readfirstlane(to + (uint32_t)(t % STAGES) * (TKEYS * D * 2));
+        uint32_t o[CP];
 #pragma unroll
-    for (int i = 0; i < CP; ++i) o[i] = at[i];
-    if (TKEYS * tt + TKEYS > lk) {  // uniform
+        for (int i = 0; i < CP; ++i) o[i] = at[i];
+        if (TKEYS * tt + TKEYS > lk) {  // uniform
+#pragma unroll
+          for (int i = 0; i < CP; ++i) {
+            const int r = krow + 4 * i;
+            o[i] = 2 * (uint32_t)tok * (uint32_t)min(r, lk - 1 - TKEYS * tt) +
+                   16 * (lc ^ (is_v ? 2 * (r & 7) : r & 15));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < CP; ++i)
+          asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                       :: "v"(o[i]), "s"(sb), "s"(m + 1024u * i) : "memory");
+      };
+      uint32_t ko[CP], vo[CP];
 #pragma unroll
       for (int i = 0; i < CP; ++i) {
         const int r = krow + 4 * i;
-        o[i] = 2 * (uint32_t)tok * (uint32_t)min(r, lk - 1 - TKEYS * tt) + 16 * (lc ^ (is_v ? 2 * (r & 7) : r & 15));
+        ko[i] = 2 * (uint32_t)a.k_tok * r + 16 * (lc ^ (r & 15));
+        vo[i] = 2 * (uint32_t)a.v_tok * r + 16 * (lc ^ (2 * (r & 7)));
       }
-    }
+      auto copy_k = [&](int t) { copy(kbase, a.k_tok, t, k_at, ko, false); };
+      auto copy_v = [&](int t) { copy(vbase, a.v_tok, t, v_at, vo, true); };
+      // The wave's own V rows of tile t, in LDS: infinities and NaN become 0 and their keys are noted.
+      auto scan_v = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < CP; ++i)
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                   :: "v"(o[i]), "s"(sb), "s"(m + 1024u * i) : "memory");
-  };
-  uint32_t ko[CP], vo[CP];
-#pragma unroll
-  for (int i = 0; i < CP; ++i) {
-    const int r = krow + 4 * i;
-    ko[i] = 2 * (uint32_t)a.k_tok * r + 16 * (lc ^ (r & 15));
-    vo[i] = 2 * (uint32_t)a.v_tok * r + 16 * (lc ^ (2 * (r & 7)));
-  }
-  auto copy_k = [&](int t) { copy(kbase, a.k_tok, t, k_at, ko, false); };
-  auto copy_v = [&](int t) { copy(vbase, a.v_tok, t, v_at, vo, true); };
-  // The wave's own V rows of tile t, in LDS: infinities and NaN become 0 and their keys are noted.
-  auto scan_v = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < CP; ++i) {
-      uint4* at = reinterpret_cast<uint4*>(&sm.v[t % STAGES][(4 * CP * wv + 4 * i) * D + 8 * lane]);
-      const uint4 u = *at;
-      uint32_t m = bf16x2_absmax_bits(bf16x2_absmax_bits(0, u.x), u.y);
-      m = bf16x2_absmax_bits(bf16x2_absmax_bits(m, u.z), u.w);
-      const int key = krow + 4 * i;
-      if ((m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u) {
-        *at = make_uint4(finite_bf2(u.x), finite_bf2(u.y), finite_bf2(u.z), finite_bf2(u.w));
-        atomicOr(&sm.nonfinite[t % 3][key >> 5], 1u << (key & 31));
-      }
-    }
-  };
-
-  lds_barrier();  // the other half is done with the block before
-  if (t0 < t1) {  // out before the rows of q are asked for
-    copy_k(t0);
-    copy_k(t0 + 1);
-    copy_v(t0);
-  }
-
-  // ---- the wave's rows
-  const int f0 = blk * ROWS + 16 * NT * wv;
-  TileRows<NT> st;
-  int lim[NT];  // last key of the lane's row, -1: none
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int f = f0 + 16 * nt + lc;
-    const int i = (int)fdiv_u((uint32_t)min(f, R - 1), a.g);
-    const int head = min(f, R - 1) - i * a.G;
-    lim[nt] = f < R ? base + i : -1;
-    const uint16_t* qr = a.q + (int64_t)(q0 + i) * a.q_tok + (hk * a.G + head) * a.q_head + 8 * lq4;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
-      st.q[nt][kk] = u4_as_bf8(signed_q(*reinterpret_cast<const uint4*>(qr + 32 * kk), a.sl2));
-  }
-  st.clear();
-  const int lim_lo = f0 < R ? base + (int)fdiv_u((uint32_t)f0, a.g) : -1;
-
-  f4_t c[NT][4];
-  bf16x8_t p[NT][2];
-  // V(t) of the wave's copies has landed (with 8 waves 4 newer ones are out)
-  auto landed = [&](int t) {
-    if constexpr (HALVES)
-      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // and K(t + 1)
-    if (t >= t_masked) scan_v(t);  // workgroup-uniform
-  };
-  if (t0 < t1) {
-    if (tid < 6) sm.nonfinite[tid >> 1][tid & 1] = 0;
-    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * CP) : "memory");  // K(t0)
-    lds_barrier();
-    if (HALVES && !grp_a) {  // half a tile behind
-      copy_k(t0 + 2);
-      copy_v(t0 + 1);
-      asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t0 + 1)
-      lds_barrier();
-    }
-    tile_scores<NT>(sm.k[t0 % STAGES], st, lane, c);
-    for (int t = t0; t < t1; ++t) {
-      if (grp_a)
-        asm volatile("s_waitcnt vmcnt(2)" ::: "memory");  // K(t + 1)
-      else
-        landed(t);
-      lds_barrier();
-      // vector phase
-      __builtin_amdgcn_s_setprio(HALVES);
-      copy_k(t + (grp_a || !HALVES ? 2 : 3));
-      copy_v(t + (grp_a || !HALVES ? 1 : 2));
-      if (TKEYS * t + TKEYS - 1 > lim_lo) {  // wave-uniform: masked for some row
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              c[nt][mt][r] = TKEYS * t + 16 * mt + 4 * lq4 + r <= lim[nt] ? c[nt][mt][r] : -INFINITY;
-      }
-      Ahead ahead;
-      if constexpr (HALVES) {
-        tile_softmax<NT>(c, st, scale, p);
-        tile_ahead(sm.k[(t + 1) % STAGES], lane, ahead);
-        if (grp_a)
-          landed(t);
-        else
-          asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t + 2)
-        lds_barrier();
-      } else {
-        tile_ahead(sm.k[(t + 1) % STAGES], lane, ahead);
-        tile_softmax<NT>(c, st, scale, p);
-      }
-      // matrix phase: Q.K^T of tile t + 1 (behind the last one, of a copy nobody reads), P.V of tile t
-      __builtin_amdgcn_s_setprio(!HALVES);
-      tile_matrix<NT>(sm.k[(t + 1) % STAGES], sm.v[t % STAGES], st, lane, c, p, ahead);
-      if (t >= t_masked) {
-        uint64_t nf = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % 3][0]) |
-                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % 3][1]) << 32;
-        for (; nf; nf &= nf - 1) {  // rare
-          const int key = __builtin_ctzll(nf), at = TKEYS * t + key;
-          if (at < lk) tile_nonfinite<NT>(vbase + 2 * a.v_tok * at, key, at, st, lane, p, lim);
+        for (int i = 0; i < CP; ++i) {
+          uint4* at = reinterpret_cast<uint4*>(&sm.v[t % STAGES][(4 * CP * wv + 4 * i) * D + 8 * lane]);
+          const uint4 u = *at;
+          uint32_t m = bf16x2_absmax_bits(bf16x2_absmax_bits(0, u.x), u.y);
+          m = bf16x2_absmax_bits(bf16x2_absmax_bits(m, u.z), u.w);
+          const int key = krow + 4 * i;
+          if ((m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u) {
+            *at = make_uint4(finite_bf2(u.x), finite_bf2(u.y), finite_bf2(u.z), finite_bf2(u.w));
+            atomicOr(&sm.nonfinite[t % 3][key >> 5], 1u << (key & 31));
+          }
         }
-      }
-      // last read before the barrier ahead of this phase: what tile t + 2 will note
-      if (tid < 2) sm.nonfinite[(t + 2) % 3][tid] = 0;
-    }
-    if (HALVES && grp_a) lds_barrier();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies past the last tile
-  }
+      };
 
-  // ---- rows out: dims 16 w + 4 lq4 + r
-  const bool part = HALVES && t1 - t0 < tiles;
-  const int64_t prow = ((int64_t)(2 * share + (t0 == 0)) * a.Hkv + hk) * ROWS;
+      lds_barrier();  // the other half is done with the block before
+      if (t0 < t1) {  // out before the rows of q are asked for
+        copy_k(t0);
+        copy_k(t0 + 1);
+        copy_v(t0);
+      }
+
+      // ---- the wave's rows
+      const int f0 = blk * ROWS + 16 * NT * wv;
+      TileRows<NT> st;
+      int lim[NT];  // last key of the lane's row, -1: none
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int f = f0 + 16 * nt + lc;
-    if (f >= R) continue;
-    if (part) {
-      const int64_t pr = prow + 16 * (NT * wv + nt) + lc;
+      for (int nt = 0; nt < NT; ++nt) {
+        const int f = f0 + 16 * nt + lc;
+        const int i = (int)fdiv_u((uint32_t)min(f, R - 1), a.g);
+        const int head = min(f, R - 1) - i * a.G;
+        lim[nt] = f < R ? base + i : -1;
+        const uint16_t* qr = a.q + (int64_t)(q0 + i) * a.q_tok + (hk * a.G + head) * a.q_head + 8 * lq4;
 #pragma unroll
-      for (int w = 0; w < 8; ++w)
-        *reinterpret_cast<f4_t*>(a.part_acc + pr * D + 16 * w + 4 * lq4) = st.o[nt][w];
-      if (lq4 == 0) a.part_ml[pr] = make_float2(st.m[nt], st.l[nt][0]);
-      continue;
+        for (int kk = 0; kk < 4; ++kk)
+          st.q[nt][kk] = u4_as_bf8(signed_q(*reinterpret_cast<const uint4*>(qr + 32 * kk), a.sl2));
+      }
+      st.clear();
+      const int lim_lo = f0 < R ? base + (int)fdiv_u((uint32_t)f0, a.g) : -1;
+
+      f4_t c[NT][4];
+      bf16x8_t p[NT][2];
+      // V(t) of the wave's copies has landed (with 8 waves 4 newer ones are out)
+      auto landed = [&](int t) {
+        if constexpr (HALVES)
+          asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // and K(t + 1)
+        if (t >= t_masked) scan_v(t);  // workgroup-uniform
+      };
+      if (t0 < t1) {
+        if (tid < 6) sm.nonfinite[tid >> 1][tid & 1] = 0;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * CP) : "memory");  // K(t0)
+        lds_barrier();
+        if (HALVES && !grp_a) {  // half a tile behind
+          copy_k(t0 + 2);
+          copy_v(t0 + 1);
+          asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t0 + 1)
+          lds_barrier();
+        }
+        tile_scores<NT>(sm.k[t0 % STAGES], st, lane, c);
+        for (int t = t0; t < t1; ++t) {
+          if (grp_a)
+            asm volatile("s_waitcnt vmcnt(2)" ::: "memory");  // K(t + 1)
+          else
+            landed(t);
+          lds_barrier();
+          // vector phase
+          __builtin_amdgcn_s_setprio(HALVES);
+          copy_k(t + (grp_a || !HALVES ? 2 : 3));
+          copy_v(t + (grp_a || !HALVES ? 1 : 2));
+          if (TKEYS * t + TKEYS - 1 > lim_lo) {  // wave-uniform: masked for some row
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  c[nt][mt][r] = TKEYS * t + 16 * mt + 4 * lq4 + r <= lim[nt] ? c[nt][mt][r] : -INFINITY;
+          }
+          Ahead ahead;
+          if constexpr (HALVES) {
+            tile_softmax<NT>(c, st, scale, p);
+            tile_ahead(sm.k[(t + 1) % STAGES], lane, ahead);
+            if (grp_a)
+              landed(t);
+            else
+              asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // K(t + 2)
+            lds_barrier();
+          } else {
+            tile_ahead(sm.k[(t + 1) % STAGES], lane, ahead);
+            tile_softmax<NT>(c, st, scale, p);
+          }
+          // matrix phase: Q.K^T of tile t + 1 (behind the last one, of a copy nobody reads), P.V of tile t
+          __builtin_amdgcn_s_setprio(!HALVES);
+          tile_matrix<NT>(sm.k[(t + 1) % STAGES], sm.v[t % STAGES], st, lane, c, p, ahead);
+          if (t >= t_masked) {
+            uint64_t nf = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % 3][0]) |
+                          (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.nonfinite[t % 3][1]) << 32;
+            for (; nf; nf &= nf - 1) {  // rare
+              const int key = __builtin_ctzll(nf), at = TKEYS * t + key;
+              if (at < lk) tile_nonfinite<NT>(vbase + 2 * a.v_tok * at, key, at, st, lane, p, lim);
+            }
+          }
+          // last read before the barrier ahead of this phase: what tile t + 2 will note
+          if (tid < 2) sm.nonfinite[(t + 2) % 3][tid] = 0;
+        }
+        if (HALVES && grp_a) lds_barrier();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies past the last tile
+      }
+
+      // ---- rows out: dims 16 w + 4 lq4 + r
+      const bool part = HALVES && t1 - t0 < tiles;
+      const int64_t prow = ((int64_t)(2 * share + (t0 == 0)) * a.Hkv + hk) * ROWS;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int f = f0 + 16 * nt + lc;
+        if (f >= R) continue;
+        if (part) {
+          const int64_t pr = prow + 16 * (NT * wv + nt) + lc;
+#pragma unroll
+          for (int w = 0; w < 8; ++w)
+            *reinterpret_cast<f4_t*>(a.part_acc + pr * D + 16 * w + 4 * lq4) = st.o[nt][w];
+          if (lq4 == 0) a.part_ml[pr] = make_float2(st.m[nt], st.l[nt][0]);
+          continue;
+        }
+        const int i = (int)fdiv_u((uint32_t)f, a.g), head = f - i * a.G;
+        uint16_t* o = a.out + ((int64_t)(q0 + i) * a.Hkv * a.G + hk * a.G + head) * D + 4 * lq4;
+        const float inv = st.l[nt][0] == 0.0f ? 0.0f : 1.0f / st.l[nt][0];
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          *reinterpret_cast<uint2*>(o + 16 * w) =
+              make_uint2(pack_bf2(st.o[nt][w][0] * inv, st.o[nt][w][1] * inv),
+                         pack_bf2(st.o[nt][w][2] * inv, st.o[nt][w][3] * inv));
+      }
     }
-    const int i = (int)fdiv_u((uint32_t)f, a.g), head = f - i * a.G;
-    uint16_t* o = a.out + ((int64_t)(q0 + i) * a.Hkv * a.G + hk * a.G + head) * D + 4 * lq4;
-    const float inv = st.l[nt][0] == 0.0f ? 0.0f : 1.0f / st.l[nt][0];
-#pragma unroll
-    for (int w = 0; w < 8; ++w)
-      *reinterpret_cast<uint2*>(o + 16 * w) =
-          make_uint2(pack_bf2(st.o[nt][w][0] * inv, st.o[nt][w][1] * inv),
-                     pack_bf2(st.o[nt][w][2] * inv, st.o[nt][w][3] * inv));
-  }
-  }
-  // the next block
-  const int64_t next = b.begin + b.tiles + BLOCK_COST;
-  more = HALVES && next < u1;
-  if (more) {
-    int ns = b.seq, place = b.place + 1;
-    if (place * PROWS >= R) {
-      place = 0;
-      do ++ns;
-      while (a.cost[ns + 1] == a.cost[ns]);  // sequences without rows cost nothing
+    // the next block
+    const int64_t next = b.begin + b.tiles + BLOCK_COST;
+    more = HALVES && next < u1;
+    if (more) {
+      int ns = b.seq, place = b.place + 1;
+      if (place * PROWS >= R) {
+        place = 0;
+        do ++ns;
+        while (a.cost[ns + 1] == a.cost[ns]);  // sequences without rows cost nothing
+      }
+      const int nr = seq_rows(a, ns), nblk = block_at(place, (nr + PROWS - 1) / PROWS);
+      b = Block{ns, nblk, block_tiles(nblk, nr, a.g, seq_base(a, ns)), next, place};
     }
-    const int nr = seq_rows(a, ns), nblk = block_at(place, (nr + PROWS - 1) / PROWS);
-    b = Block{ns, nblk, block_tiles(nblk, nr, a.g, seq_base(a, ns)), next, place};
-  }
   }
 }
 
