@@ -17,7 +17,8 @@
 // once.
 //
 // Values: an attended K or V is bf16(scale * code + bias), what dequantizing the page gives; products on
-// bf16 operands with fp32 sums, P rounded to bf16. Positions past a length are not attended whatever
+// bf16 operands with fp32 sums, P rounded to bf16 (in the values and in its sum alike, so that a row that one
+// key rules keeps that key's V). Positions past a length are not attended whatever
 // their slots hold: their scores are -infinity and their V terms 0. A length outside [0, 64 width] or a
 // page outside the pool makes the sequence's rows NaN; length 0 makes them 0. A sequence shorter than the
 // shared part takes no part in it: its own parts cover it whole.
@@ -167,7 +168,8 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
   f4_t o[8];
 #pragma unroll
   for (int w = 0; w < 8; ++w) o[w] = f4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY;
+  f4_t l = {0.f, 0.f, 0.f, 0.f};  // sums of the rounded weights, the same in all four (a product with ones)
   bool bad = false;
 
   auto page_row = [&](int p) {
@@ -243,10 +245,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
     for (int mt = 0; mt < 4; ++mt) {
       float e[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        e[r] = __builtin_amdgcn_exp2f(fmaf(c[mt][r], scale, off));
-        l += e[r];
-      }
+      for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(c[mt][r], scale, off));
       pw[2 * mt] = pack_bf2(e[0], e[1]);
       pw[2 * mt + 1] = pack_bf2(e[2], e[3]);
     }
@@ -257,6 +256,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const bf16x8_t pe = words_as_bf8(pw[4 * e], pw[4 * e + 1], pw[4 * e + 2], pw[4 * e + 3]);
+      l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_ones(), pe, l, 0, 0, 0);
       const uint4 s0 = *reinterpret_cast<const uint4*>(&sm.w[wv][2][32 * e + 4 * lq4]);
       const uint4 s1 = *reinterpret_cast<const uint4*>(&sm.w[wv][2][32 * e + 4 * lq4 + 16]);
       const uint4 z0 = *reinterpret_cast<const uint4*>(&sm.w[wv][3][32 * e + 4 * lq4]);
@@ -285,7 +285,6 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
   }
 
   // ---- the waves' rows meet in LDS (wave wv's in its own V area: 16 rows of 128 floats)
-  l = sum_xor32(sum_xor16(l));
   wave_fence();
   float* acc = reinterpret_cast<float*>(sm.v[wv]);
   if (lc < R) {
@@ -293,7 +292,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
     for (int w = 0; w < 8; ++w)
       *reinterpret_cast<float4*>(acc + lc * D + 16 * w + 4 * lq4) =
           make_float4(o[w][0], o[w][1], o[w][2], o[w][3]);
-    if (lq4 == 0) sm.ml[wv][lc] = make_float2(m, bad ? NAN : l);
+    if (lq4 == 0) sm.ml[wv][lc] = make_float2(m, bad ? NAN : l[0]);
   }
   __syncthreads();
   for (int i = tid; i < R * (D / 4); i += 64 * WV) {

@@ -3,6 +3,7 @@ their key (one lost, doubled or taken from elsewhere shows at any length), at th
 form's own arithmetic could go wrong, and on pages beyond 4 GB. Which form a call takes follows from its shape;
 the tests check that the shapes here take the one they mean."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -192,6 +193,42 @@ def test_late_pages_at_other_scales(dev):
         q = randn(gen(10), B, hq, 1, D, std=std)
         out = paged_decode_attention(q.to(dev), *pool, table.to(dev), n_d, scale, shared=shared)
         check_rows(out, q, pool, table, lens, scale, [B - 1])
+
+
+@pytest.mark.parametrize("kv,pages,second", [
+    (2, 16, 8),    # whole sequences, 8 waves: a wave takes every eighth page
+    (300, 9, 4),   # 4 waves
+    (64, 200, 4),  # dealt out in 8 shares of 26 pages, a wave's every fourth
+])
+def test_a_weight_counts_the_same_in_values_and_sum(dev, kv, pages, second):
+    """Two keys that one wave meets in turn, the second's weight 128.4 times the first's (below the 2^8 at which
+    a running maximum moves), the others' 2^-93. 128.4 rounds to 128 in bf16. In the values and in the sum alike
+    that moves the result by 0.4 / 128.4 of 128.4 / 129.4^2 of the two values' difference, 2.4e-5; in one of
+    them by 0.3%, which shows beside a bf16 result's half step in half of the dims."""
+    g = gen(13)
+    steps = 15
+    scale = math.log(128.4) / steps
+    k = torch.zeros((pages, kv, PAGE, D), dtype=torch.uint8)
+    first, last = (0, 5), (second, 33)  # page, slot
+    k[first[0], :, first[1], 0], k[last[0], :, last[1], 0] = 200, 200 + steps
+    v = torch.randint(0, 256, (pages, kv, PAGE, D), generator=g, dtype=torch.uint8)
+    word = lambda x: torch.full((pages, kv, PAGE, 2), x, dtype=torch.bfloat16, device=dev)  # noqa: E731
+    pool = (k.to(dev), word(1.0), word(0.0)), (v.to(dev), word(2.0 ** -6), word(-2.0))
+    q = torch.zeros((1, kv, 1, D), dtype=torch.bfloat16)
+    q[..., 0] = 1
+    table = torch.arange(pages, dtype=torch.int32)[None].to(dev)
+    n_d = torch.tensor([64 * pages], dtype=torch.int32, device=dev)
+    out = paged_decode_attention(q.to(dev), *pool, table, n_d, scale)
+    a, b = (v[p, :, s].double() * 2.0 ** -6 - 2 for p, s in (first, last))
+    want = (a + 128.4 * b) / 129.4
+    # and fp32: the scale, scores of 93 log2 units, exp2, sums (2^-24 each, 100-fold through the exponential)
+    slack = (a - b).abs() * 2.5e-5 + (a.abs() + b.abs()) * 200 * 2.0 ** -24
+    # the other keys: 2^-93.4 of the first's weight each (200 codes of log2(128.4) / 15), values up to 2; where
+    # both of the two are 0 they are what the row has (a first run showed 1e-29 there)
+    slack = slack + 64 * pages * 2 * 2.0 ** -93
+    half = torch.exp2(torch.floor(torch.log2(want.abs() + slack)) - 8)
+    off = (out[0, :, 0].double().cpu() - want).abs() - half - slack
+    assert (off <= 0).all(), f"{int((off > 0).sum())} of {off.numel()}, by up to {off.max().item():.3g}"
 
 
 FAR = {"dealt out": (16, 8, 3, 0), "shared dealt out": (8, 8, 9, 1024), "blocks of 32": (8, 8, 17, 512),
