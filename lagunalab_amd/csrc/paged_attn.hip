@@ -239,7 +239,8 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
 #pragma unroll
       for (int w = 0; w < 8; ++w) o[w] *= alpha;
     }
-    const float off = m == -INFINITY ? 0.0f : -m;
+    float off = m == -INFINITY ? 0.0f : -m;
+    if (__builtin_amdgcn_ballot_w64(is_huge(off))) settle_huge(c, off, scale);
     uint32_t pw[8];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {

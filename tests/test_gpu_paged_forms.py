@@ -231,6 +231,71 @@ def test_a_weight_counts_the_same_in_values_and_sum(dev, kv, pages, second):
     assert (off <= 0).all(), f"{int((off > 0).sum())} of {off.numel()}, by up to {off.max().item():.3g}"
 
 
+HUGE = [3e8, 1e10, 3e12, -1e10, 1e20]  # queries whose scores pass 2^31
+
+
+@pytest.mark.parametrize("form", [*FORMS, "whole sequences"])
+def test_huge_queries_take_the_key_of_the_largest_score(dev, form):
+    """Scores of any finite size: a query along one dim, keys of small whole numbers in it, so that products are
+    exact and a step between two keys is 2^22 and more; the row is the V of its one largest key, bit for bit."""
+    hq, kv, B, shared = FORMS.get(form, (16, 2, 3, 0))
+    spare = 0 if form == "whole sequences" else SPARE
+    lens = [shared + 130 + 61 * b for b in range(B)]
+    g = gen(14)
+    table, pages = make_table(g, lens, shared, width_spare=spare)
+    assert (table.shape[1] > 16) == (spare > 0)
+    k = torch.randint(100, 120, (pages, kv, PAGE, D), generator=g, dtype=torch.uint8)
+    v = torch.randint(0, 256, (pages, kv, PAGE, D), generator=g, dtype=torch.uint8)
+    tops, lows = [], []  # positions of the largest and the smallest key: in the shared part and in the own one
+    for b, n in enumerate(lens):
+        tops.append((7 * b) % shared if shared and b % 2 else n - 1 - 5 * b)
+        lows.append(n - 70 - b)
+    if shared:  # one key of the shared part for all that have theirs there
+        tops = [77 if b % 2 else t for b, t in enumerate(tops)]
+    for b in range(B):
+        for at, code in ((tops[b], 200 if b % 2 else 255), (lows[b], 3)):
+            k[table[b, at // PAGE].long(), :, at % PAGE, 0] = code
+    word = lambda x: torch.full((pages, kv, PAGE, 2), x, dtype=torch.bfloat16, device=dev)  # noqa: E731
+    pool = (k.to(dev), word(1.0), word(0.0)), (v.to(dev), word(2.0 ** -6), word(-2.0))
+    n_d = torch.tensor(lens, dtype=torch.int32, device=dev)
+    for size in HUGE:
+        q = torch.zeros((B, hq, 1, D), dtype=torch.bfloat16)
+        q[..., 0] = size
+        out = paged_decode_attention(q.to(dev), *pool, table.to(dev), n_d, SCALE, shared=shared)
+        for b in range(B):
+            at = tops[b] if size > 0 else lows[b]
+            want = v[table[b, at // PAGE].long(), :, at % PAGE].double() * 2.0 ** -6 - 2
+            want = want.repeat_interleave(hq // kv, 0)
+            assert torch.equal(out[b, :, 0].double().cpu(), want), f"sequence {b}, queries of {size}"
+
+
+@pytest.mark.parametrize("hq,kv,q_lens,k_lens", [
+    (8, 2, [256, 100], [256, 256]),   # small blocks
+    (8, 2, [256, 31], [9000, 4444]),  # shares that end inside blocks
+    (256, 8, [256] * 64, [4400] * 64),  # large blocks, several rounds
+])
+def test_huge_queries_of_prompts(dev, hq, kv, q_lens, k_lens):
+    """The last keys' numbers rise: every row takes the V of its own position, or with a negative query of the
+    first key, whose number is the smallest."""
+    g = gen(15)
+    k = torch.zeros((sum(k_lens), kv, D), dtype=torch.bfloat16)
+    at = 0
+    for n, m in zip(q_lens, k_lens):
+        k[at:at + m, :, 0] = (torch.arange(m) - (m - 256)).clamp(min=-1)[:, None].to(torch.bfloat16)
+        k[at, :, 0] = -5
+        at += m
+    v = randn(g, sum(k_lens), kv, D)
+    for size in HUGE:
+        q = torch.zeros((sum(q_lens), hq, D), dtype=torch.bfloat16)
+        q[..., 0] = size
+        out = prompt_attention(q.to(dev), k.to(dev), v.to(dev), q_lens, SCALE, k_lens=k_lens).cpu()
+        a = c = 0
+        for n, m in zip(q_lens, k_lens):
+            own = v[c + m - n:c + m] if size > 0 else v[c:c + 1].expand(n, -1, -1)
+            assert torch.equal(out[a:a + n], own.repeat_interleave(hq // kv, 1)), f"{n} on {m}, queries of {size}"
+            a, c = a + n, c + m
+
+
 FAR = {"dealt out": (16, 8, 3, 0), "shared dealt out": (8, 8, 9, 1024), "blocks of 32": (8, 8, 17, 512),
        "blocks of 64": (16, 8, 17, 512), "blocks of 128": (64, 8, 17, 512)}
 
