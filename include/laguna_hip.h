@@ -430,7 +430,7 @@ int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const uint16_t* k
  * sequence behind the other; its row i sees keys 0 .. k_lens - q_lens + i (a prompt has as many of
  * both, a later chunk more keys). Rows that see no key are 0.
  *   q bf16: row t of head h at q + t q_tok + h q_head; k, v alike (elements; strides multiples of 8,
- *   rows 16-byte aligned); out bf16 [rows, Hq, 128] contiguous. Hq / Hkv <= 64.
+ *   rows 16-byte aligned, 0 <= k_tok, v_tok < 2^24); out bf16 [rows, Hq, 128] contiguous. Hq / Hkv <= 64.
  * Workspace: lq_prompt_workspace_bytes (0 for many calls), any contents.
  */
 int64_t lq_prompt_workspace_bytes(const int32_t* q_lens_host, const int32_t* k_lens_host,

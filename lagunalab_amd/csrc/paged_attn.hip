@@ -17,11 +17,11 @@
 // once.
 //
 // Values: an attended K or V is bf16(scale * code + bias), what dequantizing the page gives; products on
-// bf16 operands with fp32 sums, P rounded to bf16 (in the values and in its sum alike, so that a row that one
-// key rules keeps that key's V). Positions past a length are not attended whatever
-// their slots hold: their scores are -infinity and their V terms 0. A length outside [0, 64 width] or a
-// page outside the pool makes the sequence's rows NaN; length 0 makes them 0. A sequence shorter than the
-// shared part takes no part in it: its own parts cover it whole.
+// bf16 operands with fp32 sums, P rounded to bf16 (in the values and in its sum alike, so that a row that
+// one key rules keeps that key's V). Positions past a length are not attended whatever their slots hold:
+// their scores are -infinity and their V terms 0. A length outside [0, 64 width] or a page outside the
+// pool makes the sequence's rows NaN; length 0 makes them 0. A sequence shorter than the shared part takes
+// no part in it: its own parts cover it whole.
 #include "attn_tile.h"
 #include "paged.h"
 
@@ -648,7 +648,8 @@ DecodeShape decode_shape(int64_t B, int64_t Hkv, int64_t G, int64_t shared, int 
 
 // Waves of a workgroup that takes a whole sequence, 0: the work is dealt out. Sequences of few pages are
 // taken whole, with one launch and nothing to merge; 8 waves where each has a CU of its own. us, dealt out /
-// whole, with the launch of the host and on the GPU alone:
+// whole, with the launch of the host and on the GPU alone (the rule goes by the first: in a captured graph one
+// sequence of 1,000 positions is the faster dealt out, and a table with room to grow is never taken whole):
 //   1 sequence of 1,000 positions, 8 KV heads   14.3 / 12.2, 10.1 / 11.8 (of 500 9.9 / 7.6, 2,000 10.1 / 19.5)
 //   16 of 1,000                                 16.0 / 13.8  64 of 1,000 32 / 29  256 of 300 53 / 42
 //   64 of 10 to 500                             20.0 / 14.2 (with 8 waves 16.9)
