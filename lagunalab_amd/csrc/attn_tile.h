@@ -69,12 +69,12 @@ __device__ __forceinline__ uint4 signed_q(uint4 u, float sl2) {
   return make_uint4(u.x ^ x, u.y ^ x, u.z ^ x, u.w ^ x);
 }
 
-// A weight is exp2(fma(score, scale, off)) with off = -m, the running maximum rounded to fp32; the product is
-// not rounded, so that the largest key's exponent is not 0 but off's rounding, up to 2^-24 of it: a common
-// factor of the row as long as it is small, 2^128 and beyond fp32 at a maximum of 2^31. From HUGE_LOG2 on, where
-// it is up to 2^(1/2), the scores of a row are made differences to the maximum first, of rounded products, in raw units, and off 0.
-// The test costs 0 to 1% (7 prompts of 1 to 4,099 rows 545 -> 551 us, 2,048 rows 51.7 -> 51.9, 16,384 rows
-// 1,870 -> 1,865, 48 sessions behind 16,384 64.8 -> 64.7).
+// A weight is exp2(fma(score, scale, off)) with off = -m, the running maximum rounded to fp32; the product
+// is not rounded, so that the largest key's exponent is not 0 but off's rounding, up to 2^-24 of it: a
+// common factor of the row as long as it is small, 2^128 and beyond fp32 at a maximum of 2^31. From
+// HUGE_LOG2 on, where it is up to 2^(1/2), the scores of a row are made differences to the maximum first,
+// of rounded products, in raw units, and off 0. The test costs 0 to 1% (7 prompts of 1 to 4,099 rows 545
+// -> 551 us, 2,048 rows 51.7 -> 51.9, 16,384 rows 1,870 -> 1,865, 48 sessions behind 16,384 64.8 -> 64.7).
 constexpr float HUGE_LOG2 = 8388608.0f;  // 2^23
 __device__ __forceinline__ bool is_huge(float off) { return fabsf(off) >= HUGE_LOG2; }
 template <int MT>
