@@ -388,6 +388,28 @@ int lq_paged_append(const uint16_t* k, const uint16_t* v, int64_t k_tok, int64_t
                     const int32_t* starts, const int32_t* counts_host, int64_t nseq, void* stream);
 
 /*
+ * lq_paged_append with what a layer does to its projections on the way, for sequences that are each at
+ * a position of their own: row t of sequence b is at position p = starts[b] + its number in the
+ * sequence. Query and key heads (q bf16, row t of head h at q + t q_tok + h q_head, k alike) are
+ *   y = x / sqrt(mean(x^2) + eps) * norm weight   (bf16 [128]; a null weight: y = x), then
+ *   each pair (a, c) of the first rot_dims dims turned by p * inv_freq[i] (fp32 [rot_dims / 2], radians) and
+ *   scaled by mscale: dims i and i + rot_dims / 2, or with interleaved != 0 dims 2 i and 2 i + 1,
+ * in fp32 (the angle in 64 bits) and rounded once: queries to bf16 (q_out [rows, Hq, 128]), keys, like
+ * values as they are, to 8 bits, into the pages as lq_paged_append stores rows. k_out, v_out (bf16 [rows, Hkv, 128],
+ * or both null): the keys and values as the pages hold them, what lq_paged_gather reads. Hq may be 0. rot_dims a
+ * multiple of 4 (interleaved: of 2) in [0, 128]. Rows that are not stored are still written to q_out, k_out, v_out.
+ */
+int lq_paged_append_rotated(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t q_tok,
+                            int64_t q_head, int64_t k_tok, int64_t k_head, int64_t v_tok, int64_t v_head,
+                            const uint16_t* q_norm_w, const uint16_t* k_norm_w, float eps,
+                            const float* inv_freq, int64_t rot_dims, float mscale, int interleaved,
+                            uint8_t* kc, uint16_t* ks, uint16_t* kb, uint8_t* vc, uint16_t* vs,
+                            uint16_t* vb, int64_t pages, int64_t Hq, int64_t Hkv, int64_t D,
+                            const int32_t* table, int64_t table_stride, int64_t table_width,
+                            const int32_t* starts, const int32_t* counts_host, int64_t nseq,
+                            uint16_t* q_out, uint16_t* k_out, uint16_t* v_out, void* stream);
+
+/*
  * Positions starts[b] .. starts[b] + counts_host[b] - 1 of each sequence as bf16 rows, dequantized
  * as lq_dequantize, packed one sequence behind the other: k_out, v_out bf16 [rows, Hkv, 128].
  * Positions whose page does not exist read as NaN.
@@ -423,6 +445,26 @@ int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const uint16_t* k
                          int64_t D, const int32_t* table, int64_t table_stride, int64_t table_width,
                          const int32_t* lens, int64_t shared_pages, float scale, uint16_t* out,
                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention of the last rows of up to LQ_MAX_SEQS sequences over a paged cache: sequence b has
+ * counts_host[b] query rows (host), packed one sequence behind the other, and lens[b] positions (int32,
+ * device; read by the kernel, so a captured call follows them), its own rows the last of them. Row i, at
+ * position p = lens[b] - counts_host[b] + i, sees positions max(0, p - window + 1) .. p (window 0: 0 .. p), values
+ * as lq_paged_gather reads them. Pages that no row sees are not read. Rows at negative positions are 0; a
+ * length outside [0, 64 table_width] makes the sequence's rows NaN, a page outside the pool the rows that
+ * see one of its positions.
+ *   q bf16: row t of head h at q + t q_tok + h q_head (elements; strides multiples of 8, rows 16-byte
+ *   aligned); out bf16 [rows, Hq, 128] contiguous. Hq / Hkv <= 64.
+ * Workspace: lq_paged_chunk_workspace_bytes, any contents; calls that may overlap need their own.
+ */
+int64_t lq_paged_chunk_workspace_bytes(const int32_t* counts_host, int64_t nseq, int64_t Hq, int64_t Hkv);
+int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_head, const uint8_t* kc,
+                        const uint16_t* ks, const uint16_t* kb, const uint8_t* vc, const uint16_t* vs,
+                        const uint16_t* vb, int64_t pages, int64_t Hq, int64_t Hkv, int64_t D,
+                        const int32_t* table, int64_t table_stride, int64_t table_width,
+                        const int32_t* lens, const int32_t* counts_host, int64_t nseq, int64_t window,
+                        float scale, uint16_t* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Causal attention of packed prompts (bf16), without padding or a score matrix: sequence s has

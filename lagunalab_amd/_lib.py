@@ -69,12 +69,18 @@ SIGNATURES = {
                                            i64, i64, vp, f32, vp, vp, i64, vp]),
     "lq_paged_append": (i32, [vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp,
                               i64, i64, vp, vp, i64, vp]),
+    "lq_paged_append_rotated": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i64, vp, vp, f32, vp, i64, f32,
+                                      i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp, i64, i64, vp, vp,
+                                      i64, vp, vp, vp, vp]),
     "lq_paged_gather": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, i64, i64, vp, vp, i64, vp, vp,
                               vp]),
     "lq_copy_pages": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, vp, i64, vp]),
     "lq_paged_decode_workspace_bytes": (i64, [i64, i64, i64, i64]),
     "lq_paged_decode_attn": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, i64, i64, vp,
                                    i64, f32, vp, vp, i64, vp]),
+    "lq_paged_chunk_workspace_bytes": (i64, [vp, i64, i64, i64]),
+    "lq_paged_chunk_attn": (i32, [vp, i64, i64, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp, i64, i64, vp,
+                                  vp, i64, i64, f32, vp, vp, i64, vp]),
     "lq_prompt_workspace_bytes": (i64, [vp, vp, i64, i64, i64]),
     "lq_prompt_attn": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i64, vp, vp, i64, i64, i64, i64, f32,
                              vp, vp, i64, vp]),

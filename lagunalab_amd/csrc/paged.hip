@@ -1,9 +1,10 @@
 // Rows into and out of a paged 8-bit cache, and pages copied within it.
 //
 // lq_paged_append quantizes K/V rows (bf16, any token and head strides) into the pages of several
-// sequences, with the arithmetic of the contiguous cache's append; lq_paged_gather reads positions back
+// sequences, with the arithmetic of the contiguous cache's append; lq_paged_append_rotated norms and rotates
+// queries and keys on the way; lq_paged_gather reads positions back
 // as bf16 rows, packed one sequence behind the other, as the contiguous cache's dequantize; lq_copy_pages
-// copies pages of all heads. All three are bound by their traffic (append 512 B read and 272 B written
+// copies pages of all heads. All are bound by their traffic (append 512 B read and 272 B written
 // per row and head, gather 272 and 512, copy 17,408 each way per page and head).
 #include <algorithm>
 #include <vector>
@@ -40,36 +41,8 @@ __device__ __forceinline__ float max8(float x) {
   return fmaxf(x, dpp<DPP_ROW_HALF_MIRROR>(x));
 }
 
-__global__ __launch_bounds__(256) void paged_append_kernel(
-    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t k_tok, int64_t k_head,
-    int64_t v_tok, int64_t v_head, PagedBufs buf, PageTable tab, const int32_t* __restrict__ starts,
-    PackedRows rows, uint32_t units, FastDiv per_tok, int Hkv) {
-  const int lane = threadIdx.x & 63;
-  const int sub = lane & 15;
-  const uint32_t u = blockIdx.x * 16 + (threadIdx.x >> 4);  // (token, head)
-  const bool is_v = blockIdx.y != 0;
-  const uint32_t uc = min(u, units - 1);
-  const int t = (int)fdiv_u(uc, per_tok);
-  const int h = (int)(uc - (uint32_t)t * (uint32_t)Hkv);
-  const int end = lane < rows.nseq ? rows.begin[lane + 1] : INT32_MAX;
-  int b = 0;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {  // the four rows of the wave
-    const int bs = find_packed(end, __builtin_amdgcn_readlane(t, 16 * r));
-    b = (lane >> 4) == r ? bs : b;
-  }
-  const int64_t pos = (int64_t)starts[b] + (t - rows.begin[b]);
-  const bool inside = u < units && pos >= 0 && pos < (int64_t)tab.width * PAGE;
-  const int id = inside ? tab.ids[b * tab.stride + (pos >> 6)] : -1;
-  const uint16_t* src = is_v ? v + t * v_tok + h * v_head : k + t * k_tok + h * k_head;
-  const uint4 x4 = *reinterpret_cast<const uint4*>(src + 8 * sub);
-  const uint32_t xw[4] = {x4.x, x4.y, x4.z, x4.w};
-  float x[8];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[2 * j] = bf16_lo(xw[j]);
-    x[2 * j + 1] = bf16_hi(xw[j]);
-  }
+// Codes of a lane's 8 values (8 lanes hold a group of 64) and the group's parameters.
+__device__ __forceinline__ AffineParams quantize8(const float (&x)[8], uint2& codes) {
   float lo = x[0], hi = x[0];
 #pragma unroll
   for (int j = 1; j < 8; ++j) {
@@ -94,15 +67,219 @@ __global__ __launch_bounds__(256) void paged_append_kernel(
       if (slow) c[j] = affine_code<8>(x[j], p);
     }
   }
+  codes = make_uint2(c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24),
+                     c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24));
+  return p;
+}
+__device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = bf16_lo(w[j]);
+    x[2 * j + 1] = bf16_hi(w[j]);
+  }
+}
+
+__global__ __launch_bounds__(256) void paged_append_kernel(
+    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t k_tok, int64_t k_head,
+    int64_t v_tok, int64_t v_head, PagedBufs buf, PageTable tab, const int32_t* __restrict__ starts,
+    PackedRows rows, uint32_t units, FastDiv per_tok, int Hkv) {
+  const int lane = threadIdx.x & 63;
+  const int sub = lane & 15;
+  const uint32_t u = blockIdx.x * 16 + (threadIdx.x >> 4);  // (token, head)
+  const bool is_v = blockIdx.y != 0;
+  const uint32_t uc = min(u, units - 1);
+  const int t = (int)fdiv_u(uc, per_tok);
+  const int h = (int)(uc - (uint32_t)t * (uint32_t)Hkv);
+  const int end = lane < rows.nseq ? rows.begin[lane + 1] : INT32_MAX;
+  int b = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {  // the four rows of the wave
+    const int bs = find_packed(end, __builtin_amdgcn_readlane(t, 16 * r));
+    b = (lane >> 4) == r ? bs : b;
+  }
+  const int64_t pos = (int64_t)starts[b] + (t - rows.begin[b]);
+  const bool inside = u < units && pos >= 0 && pos < (int64_t)tab.width * PAGE;
+  const int id = inside ? tab.ids[b * tab.stride + (pos >> 6)] : -1;
+  const uint16_t* src = is_v ? v + t * v_tok + h * v_head : k + t * k_tok + h * k_head;
+  float x[8];
+  unpack8(*reinterpret_cast<const uint4*>(src + 8 * sub), x);
+  uint2 c;
+  const AffineParams p = quantize8(x, c);
   if (id < 0 || id >= tab.pages) return;
   const int64_t row = ((int64_t)id * Hkv + h) * PAGE + (pos & (PAGE - 1));
   uint8_t* codes = is_v ? buf.vc : buf.kc;
-  *reinterpret_cast<uint2*>(codes + row * D + 8 * sub) =
-      make_uint2(c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24),
-                 c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24));
+  *reinterpret_cast<uint2*>(codes + row * D + 8 * sub) = c;
   if ((sub & 7) == 0) {
     (is_v ? buf.vs : buf.ks)[2 * row + (sub >> 3)] = f32_to_bf16(p.scale);
     (is_v ? buf.vb : buf.kb)[2 * row + (sub >> 3)] = f32_to_bf16(p.bias);
+  }
+}
+
+// ---- append with the norm and the rotation on the way: the heads of a token are its queries', keys' and values',
+// 16 lanes per head (8 dims each), 4 heads per wave at a time and RT times that many in turn, so that a wave
+// finds its token's angles once. A rotated dim's partner (half layout) comes by a load of its own, out with the
+// lane's own values, rather than from another lane behind them.
+struct RotateArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  const uint16_t* q_w;  // norm weights; null: no norm
+  const uint16_t* k_w;
+  float eps;
+  const float* freq;  // radians per position [dims / 2]
+  int dims;           // rotated dims of a head
+  float mscale;       // factor on rotated dims
+  PagedBufs buf;
+  PageTable tab;
+  const int32_t* starts;
+  uint16_t* q_out;  // [T, Hq, 128]
+  uint16_t* k_out;  // the stored rows as they read, [T, Hkv, 128]; null: not asked for
+  uint16_t* v_out;
+  int T, Hq, Hkv;
+  int per_tok;  // waves of a token
+  FastDiv tok;
+};
+
+// cos and sin (times mscale) of a lane's 8 dims at a position. The angle is a product in 64 bits, reduced to a
+// turn there: in 32 it would be off by 0.004 radians at position 82,671, two steps of a bf16 sine.
+template <bool PAIRS>
+__device__ __forceinline__ void rotation8(const RotateArgs& a, int64_t pos, int d0, float (&c)[8], float (&s)[8]) {
+  const int half = a.dims >> 1;
+#pragma unroll
+  for (int j = 0; j < 8; j += PAIRS ? 2 : 1) {
+    const int d = d0 + j;
+    c[j] = 1.0f;
+    s[j] = 0.0f;
+    if (d < a.dims) {
+      const double turns = (double)pos * (double)a.freq[PAIRS ? d >> 1 : d < half ? d : d - half] * 0.15915494309189535;
+      float sn, cs;
+      sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
+      c[j] = cs * a.mscale;
+      s[j] = sn * a.mscale;
+      if (!PAIRS && d < half) s[j] = -s[j];  // first half: x c - partner s
+    }
+    if (PAIRS) {
+      c[j + 1] = c[j];
+      s[j + 1] = s[j];
+      s[j] = -s[j];
+    }
+  }
+}
+// The 8 values at a lane's partner dims (half layout). WIDE: dims / 2 is a multiple of 8, they lie together.
+template <bool WIDE>
+__device__ __forceinline__ uint4 partner8(const uint16_t* row, int d0, int dims) {
+  const int half = dims >> 1;
+  if constexpr (WIDE) {
+    const int d = d0 < half ? d0 + half : d0 < dims ? d0 - half : d0;
+    return *reinterpret_cast<const uint4*>(row + d);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // half is even
+      const int d = d0 + 2 * j;
+      w[j] = *reinterpret_cast<const uint32_t*>(row + (d < half ? d + half : d < dims ? d - half : d));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+// Sum over the 16 lanes of a head.
+__device__ __forceinline__ float sum16(float x) {
+  x += dpp<DPP_QUAD_XOR1>(x);
+  x += dpp<DPP_QUAD_XOR2>(x);
+  x += dpp<DPP_ROW_ROR4>(x);
+  return x + dpp<DPP_ROW_ROR8>(x);
+}
+
+// Turns of a wave where the heads of all tokens fill this many waves per CU.
+constexpr int ROTATE_TURNS = 4, ROTATE_MANY = 32;
+
+template <bool PAIRS, bool WIDE, int RT>
+__global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateArgs a, const PackedRows rows) {
+  const int lane = threadIdx.x & 63, sub = lane & 15, d0 = 8 * sub;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const int t = (int)fdiv_u((uint32_t)wave, a.tok);
+  if (t >= a.T) return;
+  const int h0 = 4 * RT * (wave - t * a.per_tok) + (lane >> 4);
+  const int heads = a.Hq + 2 * a.Hkv;
+  // a head's row; past the last head the last one's, not stored
+  auto row_of = [&](int h) {
+    h = min(h, heads - 1);
+    return h < a.Hq             ? a.q + t * a.q_tok + h * a.q_head
+           : h < a.Hq + a.Hkv ? a.k + t * a.k_tok + (h - a.Hq) * a.k_head
+                              : a.v + t * a.v_tok + (h - a.Hq - a.Hkv) * a.v_head;
+  };
+  uint4 own[RT], other[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const uint16_t* row = row_of(h0 + 4 * i);
+    own[i] = *reinterpret_cast<const uint4*>(row + d0);
+    if constexpr (!PAIRS) other[i] = partner8<WIDE>(row, d0, a.dims);
+  }
+  const int end = lane < rows.nseq ? rows.begin[lane + 1] : INT32_MAX;
+  const int b = __builtin_amdgcn_readfirstlane(find_packed(end, t));
+  const int64_t pos = (int64_t)a.starts[b] + (t - rows.begin[b]);
+  const bool inside = pos >= 0 && pos < (int64_t)a.tab.width * PAGE;
+  const int id = inside ? a.tab.ids[b * a.tab.stride + (pos >> 6)] : -1;
+  const bool stored = id >= 0 && id < a.tab.pages;
+  float c[8], s[8];
+  rotation8<PAIRS>(a, pos, d0, c, s);
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int h = h0 + 4 * i;
+    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
+    const uint16_t* w = is_q ? a.q_w : a.k_w;
+    float x[8], y[8];
+    unpack8(own[i], x);
+    if constexpr (!PAIRS) unpack8(other[i], y);
+    if (w) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+      const float inv = rsqrtf(sum16(ss) * (1.0f / D) + a.eps);
+      float g[8];
+      unpack8(*reinterpret_cast<const uint4*>(w + d0), g);
+      if (!is_v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= inv * g[j];
+      }
+      if constexpr (!PAIRS) {
+        unpack8(partner8<WIDE>(w, d0, a.dims), g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] *= inv * g[j];
+      }
+    }
+    if (!is_v) {
+      float r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = fmaf(PAIRS ? x[j ^ 1] : y[j], s[j], x[j] * c[j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.dims ? r[j] : x[j];
+    }
+    if (is_q)  // rounded here and nowhere before
+      *reinterpret_cast<uint4*>(a.q_out + ((int64_t)t * a.Hq + h) * D + d0) =
+          make_uint4(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));
+    if (!__builtin_amdgcn_ballot_w64(!is_q)) continue;  // queries alone
+    uint2 codes;
+    const AffineParams p = quantize8(x, codes);
+    if (is_q || h >= heads) continue;
+    const int hk = is_v ? h - a.Hq - a.Hkv : h - a.Hq;
+    const uint16_t sb = f32_to_bf16(p.scale), zb = f32_to_bf16(p.bias);
+    if (stored) {
+      const int64_t row = ((int64_t)id * a.Hkv + hk) * PAGE + (pos & (PAGE - 1));
+      *reinterpret_cast<uint2*>((is_v ? a.buf.vc : a.buf.kc) + row * D + d0) = codes;
+      if ((sub & 7) == 0) {
+        (is_v ? a.buf.vs : a.buf.ks)[2 * row + (sub >> 3)] = sb;
+        (is_v ? a.buf.vb : a.buf.kb)[2 * row + (sub >> 3)] = zb;
+      }
+    }
+    if (a.k_out) {
+      const uint2 lo = dequant4(codes.x, bf16_to_f32(sb), bf16_to_f32(zb));
+      const uint2 hi = dequant4(codes.y, bf16_to_f32(sb), bf16_to_f32(zb));
+      *reinterpret_cast<uint4*>((is_v ? a.v_out : a.k_out) + ((int64_t)t * a.Hkv + hk) * D + d0) =
+          make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
   }
 }
 
@@ -237,6 +414,51 @@ extern "C" int lq_paged_append(const uint16_t* k, const uint16_t* v, int64_t k_t
       k, v, k_tok, k_head, v_tok, v_head, buf, tab, starts, rows, (uint32_t)units,
       make_fastdiv((uint32_t)Hkv), (int)Hkv);
   LQ_CHECK_LAUNCH("paged_append_kernel");
+  return LQ_OK;
+}
+
+extern "C" int lq_paged_append_rotated(
+    const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t q_tok, int64_t q_head, int64_t k_tok,
+    int64_t k_head, int64_t v_tok, int64_t v_head, const uint16_t* q_norm_w, const uint16_t* k_norm_w, float eps,
+    const float* inv_freq, int64_t rot_dims, float mscale, int interleaved, uint8_t* kc, uint16_t* ks, uint16_t* kb,
+    uint8_t* vc, uint16_t* vs, uint16_t* vb, int64_t pages, int64_t Hq, int64_t Hkv, int64_t D,
+    const int32_t* table, int64_t table_stride, int64_t table_width, const int32_t* starts,
+    const int32_t* counts_host, int64_t nseq, uint16_t* q_out, uint16_t* k_out, uint16_t* v_out, void* stream) {
+  using namespace lq;
+  clear_error();
+  const PagedBufs buf{kc, ks, kb, vc, vs, vb};
+  const PageTable tab{table, table_stride, (int)table_width, (int)pages};
+  if (const int st = check_pool(buf, tab, table_stride, table_width, pages, Hkv, D)) return st;
+  LQ_CHECK_ARG(Hq >= 0 && Hq <= (1 << 16), "%lld query heads are not in [0, 2^16]", (long long)Hq);
+  LQ_CHECK_ARG(rot_dims >= 0 && rot_dims <= D && rot_dims % (interleaved ? 2 : 4) == 0,
+               "%lld rotated dims are not a multiple of %d in [0, %lld]", (long long)rot_dims, interleaved ? 2 : 4,
+               (long long)D);
+  LQ_CHECK_ARG(rot_dims == 0 || inv_freq, "no frequencies for %lld rotated dims", (long long)rot_dims);
+  LQ_CHECK_ARG(std::isfinite(mscale) && eps >= 0.0f && std::isfinite(eps), "mscale or eps out of range");
+  PackedRows rows;
+  const int64_t T = pack_rows(counts_host, nseq, &rows);
+  if (T < 0) return LQ_EINVAL;
+  if (T == 0) return LQ_OK;
+  LQ_CHECK_ARG((Hq == 0 || (q && q_out)) && k && v && starts, "null pointer");
+  LQ_CHECK_ARG((k_out == nullptr) == (v_out == nullptr), "one of k_out and v_out alone");
+  LQ_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)k_out |
+                 (uintptr_t)v_out | (uintptr_t)q_norm_w | (uintptr_t)k_norm_w) & 15) == 0 &&
+                   ((q_tok | q_head | k_tok | k_head | v_tok | v_head) & 7) == 0,
+               "rows and norm weights must be 16-byte aligned (strides a multiple of 8)");
+  RotateArgs a{q, k, v, q_tok, q_head, k_tok, k_head, v_tok, v_head, q_norm_w, k_norm_w, eps, inv_freq, (int)rot_dims,
+               mscale, buf, tab, starts, q_out, k_out, v_out, (int)T, (int)Hq, (int)Hkv, 0, {}};
+  const int64_t heads = Hq + 2 * Hkv;
+  const bool wide = rot_dims % 16 == 0, many = T * ((heads + 3) / 4) >= ROTATE_MANY * (int64_t)device_cu_count();
+  a.per_tok = (int)((heads + 3) / 4);
+  if (many) a.per_tok = (a.per_tok + ROTATE_TURNS - 1) / ROTATE_TURNS;
+  a.tok = make_fastdiv((uint32_t)a.per_tok);
+  const int64_t waves = T * a.per_tok;
+  LQ_CHECK_ARG(waves < (int64_t)1 << 26, "an append of %lld rows is too large for one call", (long long)T);
+  auto* kern = interleaved ? (many ? paged_rotate_kernel<true, true, ROTATE_TURNS> : paged_rotate_kernel<true, true, 1>)
+               : wide      ? (many ? paged_rotate_kernel<false, true, ROTATE_TURNS> : paged_rotate_kernel<false, true, 1>)
+                      : (many ? paged_rotate_kernel<false, false, ROTATE_TURNS> : paged_rotate_kernel<false, false, 1>);
+  kern<<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, (hipStream_t)stream>>>(a, rows);
+  LQ_CHECK_LAUNCH("paged_rotate_kernel");
   return LQ_OK;
 }
 

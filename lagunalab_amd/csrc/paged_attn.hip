@@ -22,8 +22,7 @@
 // their scores are -infinity and their V terms 0. A length outside [0, 64 width] or a page outside the
 // pool makes the sequence's rows NaN; length 0 makes them 0. A sequence shorter than the shared part takes
 // no part in it: its own parts cover it whole.
-#include "attn_tile.h"
-#include "paged.h"
+#include "paged_tile.h"
 
 namespace lq {
 namespace {
@@ -116,36 +115,6 @@ struct OwnSmem {
   uint32_t w[WV][4][PAGE];  // its K scale, K bias, V scale, V bias words
   float2 ml[WV][16];
 };
-// A page on its way: rows 8 i + lane / 8 of K and V, the words of row `lane`. Read once: non-temporal (8
-// sessions of 42,771 to 82,671 rows 244 -> 229 us), in whole lines (K as MFMA operands straight from memory
-// takes half lines: 220 -> 238).
-struct PageRegs {
-  u4_t k[8], v[8];
-  uint32_t w[4];
-};
-
-__device__ __forceinline__ void load_page(const PagedArgs& a, int64_t row, int lane, PageRegs& p) {
-  const u4_t* k = reinterpret_cast<const u4_t*>(a.buf.kc + row * D) + lane;
-  const u4_t* v = reinterpret_cast<const u4_t*>(a.buf.vc + row * D) + lane;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) p.k[i] = __builtin_nontemporal_load(k + 64 * i);
-  p.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(a.buf.ks) + row + lane);
-  p.w[1] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(a.buf.kb) + row + lane);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) p.v[i] = __builtin_nontemporal_load(v + 64 * i);
-  p.w[2] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(a.buf.vs) + row + lane);
-  p.w[3] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(a.buf.vb) + row + lane);
-}
-
-__device__ __forceinline__ int kswz(int r) { return (r >> 1) & 7; }
-__device__ __forceinline__ int vswz(int r) { return (r & 3) | ((r >> 2) & 4); }
-
-__device__ __forceinline__ void wave_fence() {  // LDS of the wave's own: order across its lanes
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Pages [p0, p1) listed at ids, of a sequence of len positions, for R <= 16 query rows (row lane % 16 of them
 // at qrow): partial rows to slot .., or with WHOLE output rows from slot on.
 template <int WV, bool WHOLE>
@@ -181,7 +150,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
 
   PageRegs cur;
   int p = p0 + wv;
-  if (p < p1) load_page(a, page_row(p), lane, cur);
+  if (p < p1) load_page(a.buf, page_row(p), lane, cur);
   for (; p < p1; p += WV) {
     const int limit = min(PAGE, len - p * PAGE);  // keys of the page that are the sequence's
     // to LDS, and the next page's loads out at once; V words of keys past the length 0, so that their
@@ -195,7 +164,7 @@ __device__ __forceinline__ void own_part(const PagedArgs& a, OwnSmem<WV>& sm, co
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) sm.w[wv][i][lane] = i < 2 || lane < limit ? cur.w[i] : 0u;
-    if (p + WV < p1) load_page(a, page_row(p + WV), lane, cur);
+    if (p + WV < p1) load_page(a.buf, page_row(p + WV), lane, cur);
     wave_fence();
     // scores
     f4_t c[4];
@@ -551,16 +520,6 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_short_kernel(PagedArgs a) {
   }
   own_part<WV, true>(a, sm, a.tab.ids + b * a.tab.stride, a.G, row + (threadIdx.x & 15), hk, 0,
                      (len + PAGE - 1) / PAGE, len, row);
-}
-
-// Adds a partial (maximum m, sum l, values x) to another; one without keys (m = -infinity) has x = 0.
-__device__ __forceinline__ void merge_into(float& M, float& den, f4_t& acc, float m, float l, f4_t x) {
-  const float mn = max_ieee(M, m);
-  const float mr = mn == -INFINITY ? 0.0f : mn;
-  const float e0 = exp2_nonpos(M - mr), e1 = exp2_nonpos(m - mr);
-  acc = acc * e0 + x * e1;
-  den = den * e0 + l * e1;
-  M = mn;
 }
 
 // An output row by GR groups of 32 lanes (4 dims each), 8 / GR rows per workgroup: group g takes every GR-th

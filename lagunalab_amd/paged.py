@@ -7,7 +7,10 @@ layout of 64 rows. Row ``b`` of a table (int32 ``[B, width]``, on the device) li
 sequence ``b`` in order; position ``p`` is slot ``p % 64`` of page ``table[b, p // 64]``.
 
 * :func:`paged_append`, :func:`paged_gather`: rows quantized into the pages, positions read back as bf16;
+* :func:`paged_append_rotated`: the same from projected rows, queries and keys normed and rotated on the way;
 * :func:`paged_decode_attention`: one new token per sequence, pages that all sequences share read once;
+* :func:`paged_chunk_attention`: the last rows of each sequence (a token, a verified block, a chunk), over all
+  that is before them or within a window;
 * :func:`copy_pages`: pages copied within the pool;
 * :class:`PagedKVCache`: the pool with its page lists -- sequences opened, forked (their pages shared until
   one is written to), trimmed, closed, the pool compacted -- and :class:`PagedBatch`, some of its
@@ -149,6 +152,66 @@ def paged_append(k, v, keys, values, table, starts, counts=None):
                                            _lib.raw_stream(dev)), "lq_paged_append")
 
 
+def _norm_weight(w, what):
+    if w is None:
+        return None
+    if w.dtype != torch.bfloat16 or w.shape != (HEAD_DIM,):
+        raise ValueError(f"{what} must be bfloat16 [{HEAD_DIM}], got {tuple(w.shape)} {w.dtype}")
+    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+
+
+def paged_append_rotated(q, k, v, keys, values, table, starts, rotary, counts=None, q_norm=None, k_norm=None,
+                         eps=1e-6, fetch=False):
+    """:func:`paged_append` of projected rows, with what a layer does to them on the way, for sequences at
+    positions of their own: the heads of ``q`` (bf16 ``[T, Hq, 128]``) and ``k`` (``[T, Hkv, 128]``) get their
+    RMSNorm (weights bf16 ``[128]``; None: no norm) and the rotation of their positions ``starts[b]``, ``starts[b]
+    + 1``, .. (``rotary`` a :class:`lagunalab_amd.rotary.Rotary`, or None), ``v`` is stored as it is. ``q``, ``k``
+    and ``v`` may be views into the rows of one projection. Returns the queries (bf16 ``[T, Hq, 128]``); with
+    ``fetch`` also the new keys and values as the pages hold them, ``(q, k, v)``.
+
+    Norm, rotation and quantization are in fp32, the angles in 64 bits, with one rounding at the end: queries to
+    bf16, keys to 8 bits. (The attention block's own norm and rotation round the normed row to bf16 in between
+    and take angles in fp32, off by up to 0.004 radians at 82,671 positions.)"""
+    P, H, dev, ptrs = _pool(keys, values)
+    B, T = _length(table), k.shape[0]
+    if counts is None:
+        if B == 0 or T % B:
+            raise ValueError(f"{T} rows are not the same number for each of {B} sequences")
+        counts = [T // B] * B
+    counts = _counts(counts, B)
+    if sum(counts) != T:
+        raise ValueError(f"counts add up to {sum(counts)}, not to the {T} rows")
+    _lib.require_device(q, k, v, keys[0], q_norm, k_norm)
+    _refuse_grad(q, k, v, *(w for w in (q_norm, k_norm) if w is not None))
+    Hq = q.shape[1] if q.dim() == 3 else -1
+    q, qt, qh = _rows(q, T, Hq, "q")
+    k, kt, kh = _rows(k, T, H, "k")
+    v, vt, vh = _rows(v, T, H, "v")
+    q_norm, k_norm = _norm_weight(q_norm, "q_norm"), _norm_weight(k_norm, "k_norm")
+    freq, dims, mscale, pairs = None, 0, 1.0, False
+    if rotary is not None:
+        freq, dims, mscale, pairs = rotary.inv_freq, rotary.dims, rotary.mscale, rotary.interleaved
+        _lib.require_device(freq, keys[0])
+    table, ts, width = _table(table, B, dev)
+    starts = _ints(starts, B, "starts", dev)
+    out = torch.empty((T, Hq, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    got = torch.empty((2, T, H, HEAD_DIM), dtype=torch.bfloat16, device=dev) if fetch else None
+    qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    gp = got.data_ptr() if fetch else None
+    tp, sp = table.data_ptr(), starts.data_ptr()
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        for a, n, at, cp in _launches(counts):
+            g = 2 * at * H * HEAD_DIM
+            _lib.check(lib.lq_paged_append_rotated(
+                qp + 2 * at * qt, kp + 2 * at * kt, vp + 2 * at * vt, qt, qh, kt, kh, vt, vh, _lib.ptr(q_norm),
+                _lib.ptr(k_norm), eps, _lib.ptr(freq), dims, mscale, pairs, *ptrs, P, Hq, H, HEAD_DIM,
+                tp + 4 * a * ts, ts, width, sp + 4 * a, cp, n, op + 2 * at * Hq * HEAD_DIM,
+                gp + g if fetch else None, gp + g + 2 * T * H * HEAD_DIM if fetch else None,
+                _lib.raw_stream(dev)), "lq_paged_append_rotated")
+    return (out, *got.unbind()) if fetch else out
+
+
 def paged_gather(keys, values, table, starts, counts):
     """Positions ``starts[b] .. starts[b] + counts[b] - 1`` of each sequence as bf16 rows, packed one
     sequence behind the other: ``(k, v)``, each ``[sum(counts), Hkv, 128]``, as
@@ -214,6 +277,50 @@ def paged_decode_attention(q, keys, values, table, lens, scale, shared: int = 0)
                                             width, lens.data_ptr(), pages, scale, out.data_ptr(),
                                             ws.data_ptr(), need, _lib.raw_stream(dev)),
                    "lq_paged_decode_attn")
+    return out
+
+
+def paged_chunk_attention(q, keys, values, table, lens, scale, counts=None, window=None):
+    """Attention of the last rows of each sequence: ``q`` bf16 ``[T, Hq, 128]`` (any token and head strides), packed
+    one sequence behind the other, ``counts[b]`` rows of sequence ``b`` (host integers; None: as many each), which
+    are the last of its ``lens[b]`` positions (int32 ``[B]`` on the device). A row at position ``p`` sees positions
+    ``0 .. p``, or with a ``window`` the last ``window`` of them, itself among them. Returns ``[T, Hq, 128]``. Rows
+    at negative positions are 0; a length beyond the table's row makes NaN of its sequence, a page outside the
+    pool of the rows that see it. Pages before the window are not read. The table and the lengths are read by the
+    kernel: a captured call follows them. K and V are the rows that :func:`paged_gather` reads."""
+    P, H, dev, ptrs = _pool(keys, values)
+    B = _length(table)
+    if q.dim() != 3:
+        raise ValueError(f"q must be bfloat16 [T, Hq, {HEAD_DIM}], got {tuple(q.shape)}")
+    T, Hq = q.shape[:2]
+    if counts is None:
+        if B == 0 or T % B:
+            raise ValueError(f"{T} rows are not the same number for each of {B} sequences")
+        counts = [T // B] * B
+    counts = _counts(counts, B)
+    if sum(counts) != T:
+        raise ValueError(f"counts add up to {sum(counts)}, not to the {T} rows")
+    if window is not None and window < 1:
+        raise ValueError(f"a window of {window} positions")
+    _lib.require_device(q, keys[0])
+    _refuse_grad(q)
+    q, qt, qh = _rows(q, T, Hq, "q")
+    if H < 1 or Hq % H or not 1 <= Hq // H <= 64:
+        raise ValueError(f"{Hq} query heads are not 1 to 64 per KV head ({H})")
+    table, ts, width = _table(table, B, dev)
+    lens = _ints(lens, B, "lens", dev)
+    out = torch.empty((T, Hq, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        for a, n, at, cp in _launches(counts):
+            need = lib.lq_paged_chunk_workspace_bytes(cp, n, Hq, H)
+            if need < 0:
+                _lib.check(_lib.LQ_EINVAL, "lq_paged_chunk_workspace_bytes")
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            _lib.check(lib.lq_paged_chunk_attn(
+                q.data_ptr() + 2 * at * qt, qt, qh, *ptrs, P, Hq, H, HEAD_DIM, table.data_ptr() + 4 * a * ts, ts, width,
+                lens.data_ptr() + 4 * a, cp, n, window or 0, scale, out.data_ptr() + 2 * at * Hq * HEAD_DIM,
+                ws.data_ptr(), need, _lib.raw_stream(dev)), "lq_paged_chunk_attn")
     return out
 
 
