@@ -20,6 +20,7 @@
 // the rows that see one of its positions, a length outside the table to all rows of the sequence.
 #include <algorithm>
 
+#include "attn_tile32.h"
 #include "paged_tile.h"
 
 namespace lq {
@@ -132,47 +133,62 @@ __device__ __forceinline__ int cut_tile(const Block& b, int u) {
 // Whether a V scale and bias may give something that is no finite bf16.
 __device__ __forceinline__ bool wild(float s, float z) { return !(fabsf(s) * 255.0f + fabsf(z) < 3.3e38f); }
 
-// The wild groups of one V row (key `key` of a tile whose P is p, position `at`, row `row` of the pool), for the
-// rows that see it: O^T took 0 in their place.
-template <int NT>
-__device__ __forceinline__ void add_wild(const PagedBufs& buf, int64_t row, int key, int at, TileRows<NT>& st,
-                                         int lane, const bf16x8_t (&p)[NT][2], const int (&lim)[NT], int window) {
-  const int lc = lane & 15, lq4 = lane >> 4;
-  const int word = 2 * ((key >> 4) & 1) + ((key >> 1) & 1);
-  float pk[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const u4_t p0 = __builtin_bit_cast(u4_t, p[nt][0]), p1 = __builtin_bit_cast(u4_t, p[nt][1]);
-    uint32_t mine = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) mine = j == word ? (key < 32 ? p0[j] : p1[j]) : mine;
-    const uint32_t w = __shfl(mine, 16 * ((key >> 2) & 3) + lc, 64);
-    pk[nt] = key & 1 ? bf16_hi(w) : bf16_lo(w);
-  }
+// The wild groups of one V row (key `key` of a tile whose P is p, `rel` behind the lane's row, row `row` of the
+// pool), for the rows that see it: O^T took 0 in their place.
+__device__ __forceinline__ void add_wild(const PagedBufs& buf, int64_t row, int key, int rel, Rows32& st, int lane,
+                                         const bf16x8_t (&p)[4], int window) {
+  const float pk = weight32(p, key, lane);
+  const bool sees = (uint32_t)rel < (uint32_t)window;
   const uint32_t sw = reinterpret_cast<const uint32_t*>(buf.vs)[row], zw = reinterpret_cast<const uint32_t*>(buf.vb)[row];
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float s = w < 4 ? bf16_lo(sw) : bf16_hi(sw), z = w < 4 ? bf16_lo(zw) : bf16_hi(zw);
-    const uint2 v2 = dequant4(*reinterpret_cast<const uint32_t*>(buf.vc + row * D + 16 * w + 4 * lq4), s, z);
-    const float v[4] = {bf16_lo(v2.x), bf16_hi(v2.x), bf16_lo(v2.y), bf16_hi(v2.y)};
+  for (int g = 0; g < 2; ++g) {
+    const float s = g ? bf16_hi(sw) : bf16_lo(sw), z = g ? bf16_hi(zw) : bf16_lo(zw);
+    if (!wild(s, z)) continue;  // uniform
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int w = 2 * g; w < 2 * g + 2; ++w)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (wild(s, z) && at <= lim[nt] && at > lim[nt] - window) st.o[nt][w][r] = fmaf(pk[nt], v[r], st.o[nt][w][r]);
+      for (int j = 0; j < 4; ++j) {
+        const uint2 v2 = dequant4(
+            *reinterpret_cast<const uint32_t*>(buf.vc + row * D + 32 * w + 8 * j + 4 * (lane >> 5)), s, z);
+        const float v[4] = {bf16_lo(v2.x), bf16_hi(v2.x), bf16_lo(v2.y), bf16_hi(v2.y)};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (sees) st.o[w][4 * j + r] = fmaf(pk, v[r], st.o[w][4 * j + r]);
+      }
   }
 }
 
+// An entry of an array at a wave-uniform place, by the scalar cache: nothing of a call writes what it reads.
+__device__ __forceinline__ int scalar(const int32_t* p, int i) {
+  return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p)[i];
+}
+// A wave-uniform pointer into global memory, kept apart from the lanes' offsets: loads take it as a scalar base.
+template <typename T>
+using global_ptr = const __attribute__((address_space(1))) T*;
+template <typename T>
+__device__ __forceinline__ global_ptr<T> uniform(const T* p) {
+  global_ptr<T> g = (global_ptr<T>)p;
+  asm volatile("" : "+s"(g));
+  return g;
+}
+
+__device__ __forceinline__ uint32_t lane_offset(uint32_t o) {
+  asm volatile("" : "+v"(o));
+  return o;
+}
+
+template <int STAGES>
 struct ChunkSmem {
-  KvTile tile[2];            // K of tile t in tile[t % 2], V likewise
+  KvTile tile[STAGES];       // K of tile t in tile[t % STAGES], V likewise
   uint32_t wild[3][2];       // keys of tile t % 3, if masked, whose V is wild
 };
 
-template <int PW, int NT>  // waves, 16-row tiles of each
+template <int PW>  // waves, of 32 rows each: 8 or 4
 __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
-  constexpr int ROWS = 16 * NT * PW;
+  constexpr bool HALVES = PW == 8;
+  constexpr int ROWS = 32 * PW, STAGES = HALVES ? 3 : 2;
   constexpr int C = 8 / PW;  // 16-byte chunks of K (of V) that a thread brings per tile
-  __shared__ ChunkSmem sm;
+  __shared__ ChunkSmem<STAGES> sm;
   const int share = blockIdx.x / a.Hkv, hk = blockIdx.x - share * a.Hkv;
   const Deal deal = deal_out<ROWS>(a, threadIdx.x & 63);
   const int u0 = deal.share * share, u1 = min(u0 + deal.share, deal.total);
@@ -184,7 +200,8 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
     asm volatile("" : "+v"(tid));
     const int lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lc = lane & 15, lq4 = lane >> 4;
+    const bool grp_a = HALVES && wv < PW / 2;
+    const int ln = lane & 31, h = lane >> 5;
     const Seq sq = seq_of(a, b.seq);
     const int q0 = a.row0[b.seq];
     const int c0 = cut_tile(b, u0), c1 = cut_tile(b, u1);
@@ -202,36 +219,48 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
       // ---- a tile: thread tid brings 16 codes (chunk tid % 8) of key tid / 8 (and + 8 PW)
       const int32_t* ids = a.tab.ids + (int64_t)a.seq[b.seq] * a.tab.stride;
       const int key0 = tid >> 3, chunk = tid & 7;
-      uint4 rk[C], rv[C];
-      uint32_t ks[C], kb[C], vs[C], vb[C];
-      bool k_ok = true, v_ok = true;
-      int id_k = 0, id_next = t0 < t1 ? ids[t0] : 0;  // of the last K loaded, of the next
-      auto pool_row = [&](int id, bool& ok) {
-        ok = id >= 0 && id < a.tab.pages;
-        return ((int64_t)(ok ? id : 0) * a.Hkv + hk) * PAGE;
-      };
-      auto load_k = [&](int t) {  // tile t, in order
-        id_k = __builtin_amdgcn_readfirstlane(id_next);
-        id_next = ids[min(t + 1, t1 - 1)];
-        const int64_t row = pool_row(id_k, k_ok);
+      u4_t rk[C], rv[C];
+      uint32_t ks[C], kb[C], vs[C], vb[C];  // words of both groups
+      // whether there are such pages, and their rows: of the K loaded last, of the one before it, the V loaded last,
+      // the K loaded next
+      bool k_ok = true, before_ok = true, v_ok = true, next_ok = true;
+      int64_t row_k = 0, row_before = 0, row_next = 0;
+      int id_next = t0 < t1 ? scalar(ids, t0) : 0;
+      const uint32_t group = chunk < 4 ? SEL_LO : SEL_HI;  // of the thread's codes
+      auto load_codes = [&](const uint8_t* codes, int64_t row, u4_t (&c)[C]) {
+        const global_ptr<uint8_t> cp = uniform(codes + row * D);
+        const uint32_t o = lane_offset(16u * tid);
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-          rk[i] = *reinterpret_cast<const uint4*>(a.buf.kc + row * D + 1024 * PW * i + 16 * tid);
-          ks[i] = reinterpret_cast<const uint32_t*>(a.buf.ks)[row + key0 + 8 * PW * i];
-          kb[i] = reinterpret_cast<const uint32_t*>(a.buf.kb)[row + key0 + 8 * PW * i];
-        }
+        for (int i = 0; i < C; ++i) c[i] = *(global_ptr<u4_t>)(cp + (o + 1024 * PW * i));
       };
-      auto load_v = [&](int id) {
-        const int64_t row = pool_row(id, v_ok);
+      auto load_words = [&](const uint16_t* words, int64_t row, uint32_t (&w)[C]) {
+        const global_ptr<uint8_t> p = uniform(reinterpret_cast<const uint8_t*>(words + 2 * row));
+        const uint32_t o = lane_offset(4u * key0);
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-          rv[i] = *reinterpret_cast<const uint4*>(a.buf.vc + row * D + 1024 * PW * i + 16 * tid);
-          vs[i] = reinterpret_cast<const uint32_t*>(a.buf.vs)[row + key0 + 8 * PW * i];
-          vb[i] = reinterpret_cast<const uint32_t*>(a.buf.vb)[row + key0 + 8 * PW * i];
-        }
+        for (int i = 0; i < C; ++i) w[i] = *(global_ptr<uint32_t>)(p + (o + 32 * PW * i));
       };
-      auto pick = [&](uint32_t w) { return chunk < 4 ? bf16_lo(w) : bf16_hi(w); };
-      auto put = [&](uint4* lo, uint4* hi, uint4 c, float s, float z) {
+      // K of the tiles in order, V of each one behind
+      auto next_row = [&](int t) {  // of tile t, behind the last loaded
+        next_ok = id_next >= 0 && id_next < a.tab.pages;
+        row_next = ((int64_t)(next_ok ? id_next : 0) * a.Hkv + hk) * PAGE;
+        id_next = scalar(ids, min(t + 1, t1 - 1));
+      };
+      auto load_k = [&]() {
+        row_before = row_k;
+        before_ok = k_ok;
+        row_k = row_next;
+        k_ok = next_ok;
+        load_codes(a.buf.kc, row_k, rk);
+        load_words(a.buf.ks, row_k, ks);
+        load_words(a.buf.kb, row_k, kb);
+      };
+      auto load_v = [&]() {
+        v_ok = before_ok;
+        load_codes(a.buf.vc, row_before, rv);
+        load_words(a.buf.vs, row_before, vs);
+        load_words(a.buf.vb, row_before, vb);
+      };
+      auto put = [&](uint4* lo, uint4* hi, u4_t c, float s, float z) {
         const uint2 d0 = dequant4(c.x, s, z), d1 = dequant4(c.y, s, z);
         const uint2 d2 = dequant4(c.z, s, z), d3 = dequant4(c.w, s, z);
         *lo = make_uint4(d0.x, d0.y, d1.x, d1.y);
@@ -239,131 +268,165 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
       };
       auto stage_k = [&](int t) {
         if (t >= t1) return;  // uniform
-        KvTile& to = sm.tile[t & 1];
+        KvTile& to = sm.tile[t % STAGES];
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           const int key = key0 + 8 * PW * i;
-          put(k_chunk(to, key, 2 * chunk), k_chunk(to, key, 2 * chunk + 1), rk[i], k_ok ? pick(ks[i]) : NAN, pick(kb[i]));
+          put(k_chunk(to, key, 2 * chunk), k_chunk(to, key, 2 * chunk + 1), rk[i], bf16_pick(k_ok ? ks[i] : 0x7fc07fc0u, group), bf16_pick(kb[i], group));
         }
       };
-      auto stage_v = [&](int t) {
-        if (t >= t1) return;
-        KvTile& to = sm.tile[t & 1];
-        const bool masked = t >= t_masked || t < t_open;
+      // V of tile t (of no tile behind the last: its place is free) in steps: its words settled, then a chunk's halves.
+      auto settle_v = [&](int t) {
+        if (!v_ok || t >= t_masked || t < t_open) {  // uniform
+#pragma unroll
+          for (int i = 0; i < C; ++i) {
+            const int key = key0 + 8 * PW * i;
+            const bool none = !v_ok || TKEYS * t + key >= sq.len;  // no such position
+            const bool w = !none && wild(bf16_pick(vs[i], group), bf16_pick(vb[i], group));
+            if (w && t < t1) atomicOr(&sm.wild[t % 3][key >> 5], 1u << (key & 31));
+            if (none || w) vs[i] = vb[i] = 0;
+          }
+        }
+      };
+      // two codes of each chunk per step, eight steps
+      uint32_t vd[C][4];
+      auto stage_v = [&](int t, int step) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-          const int key = key0 + 8 * PW * i;
-          float s = pick(vs[i]), z = pick(vb[i]);
-          if (masked || !v_ok) {  // uniform
-            const bool none = !v_ok || TKEYS * t + key >= sq.len;  // no such position
-            const bool w = !none && wild(s, z);
-            if (w) atomicOr(&sm.wild[t % 3][key >> 5], 1u << (key & 31));
-            if (none || w) s = z = 0.0f;
-          }
-          put(v_chunk(to, key, 2 * chunk), v_chunk(to, key, 2 * chunk + 1), rv[i], s, z);
+          const uint32_t w = rv[i][step >> 1] >> (16 * (step & 1));
+          const float sc = bf16_pick(vs[i], group), z = bf16_pick(vb[i], group);
+          vd[i][step & 3] = pack_bf2(fmaf(sc, (float)(w & 0xffu), z), fmaf(sc, (float)((w >> 8) & 0xffu), z));
+          if ((step & 3) == 3)
+            *v_chunk32(sm.tile[t % STAGES], key0 + 8 * PW * i, 2 * chunk + (step >> 2)) =
+                make_uint4(vd[i][0], vd[i][1], vd[i][2], vd[i][3]);
         }
       };
 
       lds_barrier();  // the block before is done with LDS
-      if (t0 < t1) load_k(t0);
+      if (t0 < t1) {
+        next_row(t0);
+        load_k();
+      }
 
       // ---- the wave's rows
-      const int f0 = b.blk * ROWS + 16 * NT * wv;
-      TileRows<NT> st;
-      int lim[NT];  // last key of the lane's row, -1: none
+      const int f0 = b.blk * ROWS + 32 * wv, f = f0 + ln;
+      const int i = (int)fdiv_u((uint32_t)min(f, sq.R - 1), a.g);
+      const int head = min(f, sq.R - 1) - i * a.G;
+      const int lim = f < sq.R ? sq.base + i : -1;  // last key of the lane's row, below 0: none
+      const uint16_t* qr = a.q + (int64_t)(q0 + i) * a.q_tok + (hk * a.G + head) * a.q_head + 8 * h;
+      Rows32 st;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int f = f0 + 16 * nt + lc;
-        const int i = (int)fdiv_u((uint32_t)min(f, sq.R - 1), a.g);
-        const int head = min(f, sq.R - 1) - i * a.G;
-        lim[nt] = f < sq.R ? sq.base + i : -1;
-        const uint16_t* qr = a.q + (int64_t)(q0 + i) * a.q_tok + (hk * a.G + head) * a.q_head + 8 * lq4;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          st.q[nt][kk] = u4_as_bf8(signed_q(*reinterpret_cast<const uint4*>(qr + 32 * kk), a.sl2));
-      }
+      for (int kk = 0; kk < 8; ++kk)
+        st.q[kk] = u4_as_bf8(signed_q(*reinterpret_cast<const uint4*>(qr + 16 * kk), a.sl2));
       st.clear();
-      // keys that all, and that some, of the wave's rows see
+      // keys up to here, and from there on, are seen by all of the wave's rows
       const int lim_lo = f0 < sq.R ? sq.base + (int)fdiv_u((uint32_t)f0, a.g) : -1;
       const int open_from =
-          f0 < sq.R ? sq.base + (int)fdiv_u((uint32_t)min(f0 + 16 * NT - 1, sq.R - 1), a.g) - a.window + 1 : 0;
+          f0 < sq.R ? sq.base + (int)fdiv_u((uint32_t)min(f0 + 31, sq.R - 1), a.g) - a.window + 1 : 0;
 
-      f4_t c[NT][4];
-      bf16x8_t p[NT][2];
+      f16v_t c[2];
+      bf16x8_t p[4];
+      const uint32_t k_at = k_lane32(sm.tile[0], lane), v_at = v_lane32(sm.tile[0], lane);
+      auto tile_at = [](int t) { return (uint32_t)(t % STAGES) * (uint32_t)sizeof(KvTile); };
       if (t0 < t1) {
         if (tid < 6) sm.wild[tid >> 1][tid & 1] = 0;
         stage_k(t0);
-        int id_v = id_k;
-        load_k(t0 + 1);
-        load_v(id_v);
+        next_row(t0 + 1);
+        load_k();
+        load_v();
+        next_row(t0 + 2);
+        auto begin = [&]() {  // K of the second tile, V of the first; the next ones loaded
+          stage_k(t0 + 1);
+          settle_v(t0);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) stage_v(t0, i);
+          load_k();
+          load_v();
+          next_row(t0 + 3);
+        };
         lds_barrier();
-        tile_scores<NT>(sm.tile[t0 & 1].k, st, lane, c);
-        stage_k(t0 + 1);
-        stage_v(t0);
-        id_v = id_k;
-        load_k(t0 + 2);
-        load_v(id_v);
+        if (HALVES && !grp_a) {  // half a tile behind
+          begin();
+          lds_barrier();
+        }
+        scores32(k_at + tile_at(t0), st, c);
+        if (!HALVES || grp_a) begin();
         for (int t = t0; t < t1; ++t) {
           lds_barrier();
+          // vector phase
+          __builtin_amdgcn_s_setprio(0);
           stage_k(t + 2);
-          stage_v(t + 1);
-          id_v = id_k;
-          load_k(t + 3);
-          load_v(id_v);
+          load_k();
           if (TKEYS * t + TKEYS - 1 > lim_lo || TKEYS * t < open_from) {  // wave-uniform: masked for some row
+            const int rel = lim - TKEYS * t - 4 * h;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-              for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const int key = TKEYS * t + 16 * mt + 4 * lq4 + r;
-                  c[nt][mt][r] = key <= lim[nt] && key > lim[nt] - a.window ? c[nt][mt][r] : -INFINITY;
-                }
+              for (int r = 0; r < 16; ++r)
+                c[mt][r] = (uint32_t)(rel - (32 * mt + 8 * (r >> 2) + (r & 3))) < (uint32_t)a.window ? c[mt][r]
+                                                                                                 : -INFINITY;
           }
-          Ahead ahead;
-          tile_ahead(sm.tile[(t + 1) & 1].k, lane, ahead);
-          tile_softmax<NT>(c, st, scale, p);
-          // Q.K^T of tile t + 1 (behind the last one, of a tile nobody uses), P.V of tile t
-          tile_matrix<NT>(sm.tile[(t + 1) & 1].k, sm.tile[t & 1].v, st, lane, c, p, ahead);
+          Ahead32 ahead;
+          const uint32_t kt = k_at + tile_at(t + 1);
+          if constexpr (HALVES) {
+            softmax32(c, st, scale, p);
+            ahead32(kt, ahead);
+            lds_barrier();
+          } else {
+            ahead32(kt, ahead);
+            softmax32(c, st, scale, p);
+          }
+          // matrix phase: Q.K^T of tile t + 1 (behind the last one, of a tile nobody uses), P.V of tile t
+          __builtin_amdgcn_s_setprio(1);
+          // between them V of tile t + 1 is staged, and the tiles behind are loaded
+          settle_v(t + 1);
+          matrix32(kt, v_at + tile_at(t), st, c, p, ahead, [&](int u) {
+            if (u < 8) stage_v(t + 1, u);
+            if (u == 8) load_v();
+            if (u == 12) {
+              next_row(t + 4);
+              asm volatile("" : "+s"(row_next));  // here, not behind the last step
+            }
+          });
           if (t >= t_masked || t < t_open) {
             uint64_t w = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.wild[t % 3][0]) |
                          (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.wild[t % 3][1]) << 32;
             for (; w; w &= w - 1) {  // rare
               const int key = __builtin_ctzll(w);
-              bool ok;
-              const int64_t row = pool_row(__builtin_amdgcn_readfirstlane(ids[t]), ok);
-              add_wild<NT>(a.buf, row + key, key, TKEYS * t + key, st, lane, p, lim, a.window);
+              const int64_t row = ((int64_t)scalar(ids, t) * a.Hkv + hk) * PAGE + key;  // a page of the pool
+              add_wild(a.buf, row, key, lim - TKEYS * t - key, st, lane, p, a.window);
             }
           }
           // last read before the barrier ahead of this phase: what tile t + 2 will note
           if (tid < 2) sm.wild[(t + 2) % 3][tid] = 0;
         }
+        if (HALVES && grp_a) lds_barrier();
       }
 
-      // ---- rows out: dims 16 w + 4 lq4 + r
+      // ---- rows out: dims 32 w + 8 j + 4 h ..
       const bool part = c1 - c0 < b.tiles;
-      const int64_t prow = ((int64_t)(2 * share + (c0 == 0)) * a.Hkv + hk) * ROWS;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int f = f0 + 16 * nt + lc;
-        if (f >= sq.R) continue;
+      st.l = sum_xor32(st.l);
+      if (f < sq.R) {
         if (part) {
-          const int64_t pr = prow + 16 * (NT * wv + nt) + lc;
+          const int64_t pr = ((int64_t)(2 * share + (c0 == 0)) * a.Hkv + hk) * ROWS + 32 * wv + ln;
 #pragma unroll
-          for (int w = 0; w < 8; ++w)
-            *reinterpret_cast<f4_t*>(a.part_acc + pr * D + 16 * w + 4 * lq4) = st.o[nt][w];
-          if (lq4 == 0) a.part_ml[pr] = make_float2(st.m[nt], st.l[nt][0]);
-          continue;
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<f4_t*>(a.part_acc + pr * D + 32 * w + 8 * j + 4 * h) =
+                  f4_t{st.o[w][4 * j], st.o[w][4 * j + 1], st.o[w][4 * j + 2], st.o[w][4 * j + 3]};
+          if (h == 0) a.part_ml[pr] = make_float2(st.m, st.l);
+        } else {
+          uint16_t* o = a.out + ((int64_t)(q0 + i) * a.Hkv * a.G + hk * a.G + head) * D + 4 * h;
+          const float inv = sq.len < 0 ? NAN : st.l == 0.0f ? 0.0f : 1.0f / st.l;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<uint2*>(o + 32 * w + 8 * j) =
+                  make_uint2(pack_bf2(st.o[w][4 * j] * inv, st.o[w][4 * j + 1] * inv),
+                             pack_bf2(st.o[w][4 * j + 2] * inv, st.o[w][4 * j + 3] * inv));
         }
-        const int i = (int)fdiv_u((uint32_t)f, a.g), head = f - i * a.G;
-        uint16_t* o = a.out + ((int64_t)(q0 + i) * a.Hkv * a.G + hk * a.G + head) * D + 4 * lq4;
-        const float inv = sq.len < 0 ? NAN : st.l[nt][0] == 0.0f ? 0.0f : 1.0f / st.l[nt][0];
-#pragma unroll
-        for (int w = 0; w < 8; ++w)
-          *reinterpret_cast<uint2*>(o + 16 * w) =
-              make_uint2(pack_bf2(st.o[nt][w][0] * inv, st.o[nt][w][1] * inv),
-                         pack_bf2(st.o[nt][w][2] * inv, st.o[nt][w][3] * inv));
       }
     }
     // the next block
@@ -436,28 +499,30 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkArgs a) {
 
 // How a call's sequences are dealt out.
 struct ChunkPlan {
-  int nseq, lanes, shares;
+  int nseq, lanes, shares, rows_of;
   int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];
 };
-constexpr int ROWS = 64;
 ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G, int cus) {
   ChunkPlan p{};
   int at = 0;
+  int64_t most = 0;  // query rows of a sequence
   for (int s = 0; s < nseq; ++s) {
     if (counts[s]) {
       p.seq[p.nseq] = s;
       p.row0[p.nseq] = at;
       p.rows[p.nseq++] = counts[s];
+      most = std::max<int64_t>(most, counts[s] * G);
     }
     at += counts[s];
   }
   p.lanes = 6;
   while ((p.nseq << p.lanes) > 64) --p.lanes;
-  p.shares = (int)std::max<int64_t>(1, 2 * cus / Hkv);
+  p.rows_of = most > 128 ? 256 : 128;
+  p.shares = (int)std::max<int64_t>(1, (p.rows_of == 256 ? 1 : 2) * cus / Hkv);
   return p;
 }
 int64_t chunk_bytes(const ChunkPlan& p, int64_t Hkv) {
-  return 2 * p.shares * Hkv * ROWS * (int64_t)(D * sizeof(float) + sizeof(float2));
+  return 2 * p.shares * Hkv * p.rows_of * (int64_t)(D * sizeof(float) + sizeof(float2));
 }
 
 int check_chunk(int64_t Hq, int64_t Hkv, const int32_t* counts, int64_t nseq) {
@@ -510,7 +575,7 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
                "rows must be 16-byte aligned (strides a multiple of 8)");
   int64_t most = 0;  // cost, if every block sees the whole table
   for (int s = 0; s < plan.nseq; ++s)
-    most += (plan.rows[s] * G + lq::ROWS - 1) / lq::ROWS * (table_width + lq::BLOCK_COST);
+    most += (plan.rows[s] * G + plan.rows_of - 1) / plan.rows_of * (table_width + lq::BLOCK_COST);
   LQ_CHECK_ARG(most < (1ll << 31) - (1 << 20), "too many rows for table rows of %lld pages", (long long)table_width);
   const int64_t need = chunk_bytes(plan, Hkv);
   if (!workspace || workspace_bytes < need) {
@@ -524,7 +589,7 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
   a.lens = lens;
   a.out = out;
   a.part_acc = (float*)workspace;
-  a.part_ml = (float2*)(a.part_acc + 2 * plan.shares * Hkv * lq::ROWS * 128);
+  a.part_ml = (float2*)(a.part_acc + 2 * plan.shares * Hkv * plan.rows_of * 128);
   a.Hkv = (int)Hkv;
   a.G = (int)G;
   a.g = make_fastdiv((uint32_t)G);
@@ -536,11 +601,15 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
   std::copy(plan.seq, plan.seq + LQ_MAX_SEQS, a.seq);
   std::copy(plan.row0, plan.row0 + LQ_MAX_SEQS, a.row0);
   std::copy(plan.rows, plan.rows + LQ_MAX_SEQS, a.rows);
-  chunk_kernel<4, 1><<<dim3((unsigned)(plan.shares * Hkv)), dim3(256), 0, (hipStream_t)stream>>>(a);
+  const dim3 grid((unsigned)(plan.shares * Hkv));
+  if (plan.rows_of == 256)
+    chunk_kernel<8><<<grid, dim3(512), 0, (hipStream_t)stream>>>(a);
+  else
+    chunk_kernel<4><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a);
   LQ_CHECK_LAUNCH("chunk_kernel");
   if (plan.shares > 1) {
-    chunk_merge_kernel<lq::ROWS><<<dim3((unsigned)((plan.shares - 1) * Hkv), lq::ROWS / MERGE_ROWS), dim3(256), 0,
-                                   (hipStream_t)stream>>>(a);
+    auto* merge = plan.rows_of == 256 ? chunk_merge_kernel<256> : chunk_merge_kernel<128>;
+    merge<<<dim3((unsigned)((plan.shares - 1) * Hkv), plan.rows_of / MERGE_ROWS), dim3(256), 0, (hipStream_t)stream>>>(a);
     LQ_CHECK_LAUNCH("chunk_merge_kernel");
   }
   return LQ_OK;
