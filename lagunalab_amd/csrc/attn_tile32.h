@@ -96,6 +96,24 @@ __device__ __forceinline__ void softmax32(f16v_t (&c)[2], Rows32& st, float scal
   }
 }
 
+// Adds the rounded weights to the row sums.
+__device__ __forceinline__ void sums32(Rows32& st, const bf16x8_t (&p)[4]) {
+  typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+  const bf2_t ones = __builtin_bit_cast(bf2_t, 0x3f803f80u);
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const u4_t w = __builtin_bit_cast(u4_t, p[e]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = w[j];
+      float& l = j & 1 ? sum : st.l;
+      l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2_t, x), ones, l, false);
+    }
+  }
+  st.l += sum;
+}
+
 // A wave's place in a tile: byte addresses of its operands' first fragments. The tile is 256-byte aligned, so that
 // the bits that choose among a row's chunks and windows are the lane's alone.
 __device__ __forceinline__ uint32_t k_lane32(const KvTile& t, int lane) {
@@ -141,9 +159,6 @@ __device__ __forceinline__ void ahead32(uint32_t k, Ahead32& a) {
 template <typename Work>
 __device__ __forceinline__ void matrix32(uint32_t k, uint32_t v, Rows32& st, f16v_t (&c)[2],
                                          const bf16x8_t (&p)[4], Ahead32& a, Work work) {
-  typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
-  const bf2_t ones = __builtin_bit_cast(bf2_t, 0x3f803f80u);
-  float sum = 0.0f;
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
     if (u + AHEAD < 16) fetch32(k, v, u + AHEAD, a.f[(u + AHEAD) % (AHEAD + 1)]);
@@ -167,18 +182,8 @@ __device__ __forceinline__ void matrix32(uint32_t k, uint32_t v, Rows32& st, f16
     __builtin_amdgcn_sched_barrier(0);
   }
   // behind the last MFMA: beside MFMAs, of either wave of the SIMD, v_dot2 stalls both (2,048 rows behind 32,771
-  // positions, 32/8 heads: 1,100 us here, 1,212 between the steps, 1,135 in the softmax)
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const u4_t w = __builtin_bit_cast(u4_t, p[e]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t x = w[j];
-      float& l = j & 1 ? sum : st.l;
-      l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2_t, x), ones, l, false);
-    }
-  }
-  st.l += sum;
+  // positions, 32/8 heads: 1,113 us here, 1,212 between the steps, 1,135 in the softmax)
+  sums32(st, p);
 }
 // Raw scores of one tile.
 __device__ __forceinline__ void scores32(uint32_t k, const Rows32& st, f16v_t (&c)[2]) {

@@ -31,6 +31,9 @@ using namespace attn;
 constexpr int BLOCK_COST = 4;  // of a block's start and end, in tiles
 constexpr int MIN_PART = 2;    // tiles of a block's part: nearer cuts move to the block's end
 constexpr int NO_WINDOW = 1 << 25;
+constexpr int FEW_WAVES = 4;
+constexpr int SHARE_MIN = 4;  // pages of a share of few rows: one per wave
+constexpr int SEQ_COST = 4;   // of starting on a sequence, in pages
 
 struct ChunkArgs {
   const uint16_t* q;
@@ -46,6 +49,7 @@ struct ChunkArgs {
   float sl2;
   int window;          // positions a row sees, NO_WINDOW: all
   int shares;          // per KV head
+  int blocks;          // of 32 rows, of the sequence with the most (few rows)
   int nseq, lanes;     // sequences, log2 of the lanes that add up the blocks of one
   int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];  // table row, first row of q, rows (not 0)
 };
@@ -497,32 +501,338 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkArgs a) {
   }
 }
 
-// How a call's sequences are dealt out.
-struct ChunkPlan {
-  int nseq, lanes, shares, rows_of;
-  int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];
+// ---- sequences of few rows (single tokens, verified blocks): up to 32 query rows per workgroup, all of them in
+// every wave, which takes a page at a time through LDS of its own (no barriers), dequantized on its way into the
+// matrix cores, the next page's loads out. What bounds these calls is reading the pages.
+
+template <int WV>  // waves
+struct FewSmem {
+  // a wave's page: 16-byte chunk c of row r of K at c ^ kswz(r), of V at c ^ vfew(r); at the end its rows' values,
+  // 16-byte chunk c of row r at c ^ r
+  alignas(256) uint8_t page[WV][2][PAGE * D];
+  alignas(16) uint32_t w[WV][4][PAGE];  // its K scale, K bias, V scale, V bias words
+  uint4 q[8][64];               // the rows of q as B operands, a lane's place in each: not kept in registers
+  float2 ml[WV][32];
 };
+// Rows of V that a transposed read takes together, 4 h + 8 i + r: in different banks.
+__device__ __forceinline__ int vfew(int r) { return (r & 3) | ((r >> 1) & 4); }
+
+// First page that the rows of a sequence see, and how many.
+struct Pages {
+  int lo, n;
+};
+__device__ __forceinline__ Pages few_pages(const ChunkArgs& a, const Seq& q) {
+  const int lo = max(0, q.base - a.window + 1) / PAGE;
+  return {lo, q.len <= 0 ? 0 : (q.len + PAGE - 1) / PAGE - lo};
+}
+__device__ __forceinline__ int few_cost(const ChunkArgs& a, int s) {
+  if (s >= a.nseq) return 0;
+  const int n = few_pages(a, seq_of(a, s)).n;
+  return n ? n + SEQ_COST : 0;
+}
+__device__ __forceinline__ Deal few_deal(const ChunkArgs& a, int lane) {
+  const int upto = wave_scan_i(few_cost(a, lane));
+  const int total = __builtin_amdgcn_readlane(upto, 63);
+  return {upto, total, max(SHARE_MIN, (total + a.shares - 1) / a.shares)};
+}
+
+// Pages [p0, p1) of sequence s for the rows of block rb: partial rows to slot .., or with WHOLE output rows.
+template <int WV, bool WHOLE>
+__device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, int s, const Seq& sq, int rb, int hk,
+                                         int p0, int p1, int64_t slot) {
+  int tid = threadIdx.x;  // re-read, so that no lane value made of it is kept across sequences
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 31, h = lane >> 5;
+  __syncthreads();  // the sequence before is written
+  const float scale = abs_scale(a.sl2);
+  const int f0 = 32 * rb, f = f0 + ln;
+  const int i = (int)fdiv_u((uint32_t)min(f, sq.R - 1), a.g);
+  const int head = min(f, sq.R - 1) - i * a.G;
+  const int lim = f < sq.R ? sq.base + i : -1;
+  const uint16_t* qr = a.q + (int64_t)(a.row0[s] + i) * a.q_tok + (hk * a.G + head) * a.q_head + 16 * h;
+  // q in K's order of dims: step 2 j + x holds dims 16 (2 j + h) + 8 x .. + 7
+#pragma unroll
+  for (int kk = wv; kk < 8; kk += WV)
+    sm.q[kk][lane] = signed_q(*reinterpret_cast<const uint4*>(qr + 32 * (kk >> 1) + 8 * (kk & 1)), a.sl2);
+  Rows32 st;
+  st.clear();
+  const int lim_lo = sq.base + (int)fdiv_u((uint32_t)f0, a.g);
+  const int open_from = sq.base + (int)fdiv_u((uint32_t)min(f0 + 31, sq.R - 1), a.g) - a.window + 1;
+
+  const int32_t* ids = a.tab.ids + (int64_t)a.seq[s] * a.tab.stride;
+  uint8_t* const kp = sm.page[wv][0];
+  uint8_t* const vp = sm.page[wv][1];
+  PageRegs cur;
+  bool next_ok = true;
+  int64_t row_next = 0;
+  auto load = [&](int p) {
+    const int id = scalar(ids, p);
+    next_ok = id >= 0 && id < a.tab.pages;
+    row_next = ((int64_t)(next_ok ? id : 0) * a.Hkv + hk) * PAGE;
+    load_page(a.buf, row_next, lane, cur);
+  };
+  int p = p0 + wv;
+  if (p < p1) load(p);
+  __syncthreads();  // q
+  for (; p < p1; p += WV) {
+    const int64_t row = row_next;
+    const bool ok = next_ok;
+    const bool masked = PAGE * p + PAGE - 1 > lim_lo || PAGE * p < open_from;
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 8 * i + (lane >> 3), c = lane & 7;
+      reinterpret_cast<u4_t*>(kp)[8 * r + (c ^ kswz(r))] = cur.k[i];
+      reinterpret_cast<u4_t*>(vp)[8 * r + (c ^ vfew(r))] = cur.v[i];
+    }
+    // no V of positions that are not there, nor of those that are not finite where some row does not see them
+    const bool none = !ok || PAGE * p + lane >= sq.len;
+    uint32_t keep = none ? 0u : 0xffffffffu;
+    uint64_t wilds = 0;
+    if (masked) {  // uniform
+      if (wild(bf16_lo(cur.w[2]), bf16_lo(cur.w[3]))) keep &= 0xffff0000u;
+      if (wild(bf16_hi(cur.w[2]), bf16_hi(cur.w[3]))) keep &= 0x0000ffffu;
+      wilds = __builtin_amdgcn_ballot_w64(!none && keep != 0xffffffffu);
+    }
+    sm.w[wv][0][lane] = ok ? cur.w[0] : 0x7fc07fc0u;
+    sm.w[wv][1][lane] = cur.w[1];
+    sm.w[wv][2][lane] = cur.w[2] & keep;
+    sm.w[wv][3][lane] = cur.w[3] & keep;
+    if (p + WV < p1) load(p + WV);
+    wave_fence();
+    // scores
+    f16v_t c[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[mt][i] = 0.0f;
+      const int key = 32 * mt + ln;
+      const uint32_t sw = sm.w[wv][0][key], zw = sm.w[wv][1][key];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float s = j < 2 ? bf16_lo(sw) : bf16_hi(sw), z = j < 2 ? bf16_lo(zw) : bf16_hi(zw);
+        const u4_t w = reinterpret_cast<const u4_t*>(kp)[8 * key + ((2 * j + h) ^ kswz(key))];
+        const uint2 d0 = dequant4(w[0], s, z), d1 = dequant4(w[1], s, z);
+        const uint2 d2 = dequant4(w[2], s, z), d3 = dequant4(w[3], s, z);
+        c[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d0.x, d0.y, d1.x, d1.y),
+                                                        u4_as_bf8(sm.q[2 * j][lane]), c[mt], 0, 0, 0);
+        c[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d2.x, d2.y, d3.x, d3.y),
+                                                        u4_as_bf8(sm.q[2 * j + 1][lane]), c[mt], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (masked) {  // uniform
+      const int rel = lim - PAGE * p - 4 * h;
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          c[mt][r] = (uint32_t)(rel - (32 * mt + 8 * (r >> 2) + (r & 3))) < (uint32_t)a.window ? c[mt][r] : -INFINITY;
+    }
+    bf16x8_t pr[4];
+    softmax32(c, st, scale, pr);
+    sums32(st, pr);
+    // values: of keys 16 e + 8 (j / 4) + 4 h + j % 4, j < 8, this lane's dim of each window of 32
+    const int r8 = (lane >> 1) & 7, src = 4 * h + 8 * (r8 >> 2) + (r8 & 3);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint4 s0 = *reinterpret_cast<const uint4*>(&sm.w[wv][2][16 * e + 4 * h]);
+      const uint4 s1 = *reinterpret_cast<const uint4*>(&sm.w[wv][2][16 * e + 8 + 4 * h]);
+      const uint4 z0 = *reinterpret_cast<const uint4*>(&sm.w[wv][3][16 * e + 4 * h]);
+      const uint4 z1 = *reinterpret_cast<const uint4*>(&sm.w[wv][3][16 * e + 8 + 4 * h]);
+      const uint32_t sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+      const uint32_t zw[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int chunk = 2 * w + ((lane >> 4) & 1);
+        const v2i_t raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_v2i_t*)(vp + (16 * e + src) * D + 16 * (chunk ^ vfew(src)) + 8 * (lane & 1)));
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float s = w < 2 ? bf16_lo(sw[j]) : bf16_hi(sw[j]), z = w < 2 ? bf16_lo(zw[j]) : bf16_hi(zw[j]);
+          v[j] = fmaf(s, (float)(((uint32_t)(j < 4 ? raw.x : raw.y) >> (8 * (j & 3))) & 0xffu), z);
+        }
+        st.o[w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            words_as_bf8(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])), pr[e],
+            st.o[w], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    for (; wilds; wilds &= wilds - 1) {  // rare
+      const int key = __builtin_ctzll(wilds);
+      add_wild(a.buf, row + key, key, lim - PAGE * p - key, st, lane, pr, a.window);
+    }
+  }
+
+  // ---- the waves' rows meet in LDS
+  wave_fence();
+  f4_t* acc = reinterpret_cast<f4_t*>(sm.page[wv]);
+  st.l = sum_xor32(st.l);
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      acc[32 * ln + ((8 * w + 2 * j + h) ^ ln)] = f4_t{st.o[w][4 * j], st.o[w][4 * j + 1], st.o[w][4 * j + 2], st.o[w][4 * j + 3]};
+  if (h == 0) sm.ml[wv][ln] = make_float2(st.m, st.l);
+  __syncthreads();
+  const int R = min(32, sq.R - f0);
+  for (int x = tid; x < 32 * R; x += 64 * WV) {
+    const int r = x >> 5, ch = x & 31;
+    float M = -INFINITY, L = 0.0f;
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WV; ++w) M = max_ieee(M, sm.ml[w][r].x);
+    const float Mr = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int w = 0; w < WV; ++w) {
+      const float2 ml = sm.ml[w][r];
+      const float e = exp2_nonpos(ml.x - Mr);  // of no keys: 0, and a sum that is NaN stays
+      o += reinterpret_cast<const f4_t*>(sm.page[w])[32 * r + (ch ^ r)] * e;
+      L += ml.y * e;
+    }
+    if constexpr (WHOLE) {
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      const int p = (int)fdiv_u((uint32_t)(f0 + r), a.g), head = f0 + r - p * a.G;
+      *reinterpret_cast<uint2*>(a.out + ((int64_t)(a.row0[s] + p) * a.Hkv * a.G + hk * a.G + head) * D + 4 * ch) =
+          make_uint2(pack_bf2(o[0] * inv, o[1] * inv), pack_bf2(o[2] * inv, o[3] * inv));
+    } else {
+      *reinterpret_cast<f4_t*>(a.part_acc + (slot + r) * D + 4 * ch) = o;
+      if (ch == 0) a.part_ml[slot + r] = make_float2(M, L);
+    }
+  }
+}
+
+// Partial rows of a KV head and row block: 32 for each share and sequence (along both each part adds one to their sum).
+__device__ __forceinline__ int64_t few_slot(const ChunkArgs& a, int hk, int rb, int x) {
+  return ((int64_t)(hk * a.blocks + rb) * (a.shares + a.nseq) + x) * 32;
+}
+
+// A share of the sequences' pages, dealt out one sequence behind the other.
+__global__ __launch_bounds__(64 * FEW_WAVES, 2) void few_kernel(const ChunkArgs a) {
+  __shared__ FewSmem<FEW_WAVES> sm;
+  const int hk = blockIdx.x % a.Hkv, y = blockIdx.x / a.Hkv, x = y / a.blocks, rb = y - x * a.blocks;
+  const int lane = threadIdx.x & 63;
+  const Deal deal = few_deal(a, lane);
+  const int u0 = x * deal.share, u1 = min(u0 + deal.share, deal.total);
+  if (u0 >= u1) return;
+  int s = __builtin_popcountll(__builtin_amdgcn_ballot_w64(deal.upto <= u0));
+  int begin = s ? __builtin_amdgcn_readlane(deal.upto, s - 1) : 0;
+  for (int u = u0; u < u1; ++s) {
+    const Seq sq = seq_of(a, s);
+    const Pages pg = few_pages(a, sq);
+    if (pg.n == 0) continue;
+    begin += SEQ_COST;
+    const int p0 = max(u - begin, 0), p1 = min(u1 - begin, pg.n);
+    if (p0 < p1 && 32 * rb < sq.R) few_part<FEW_WAVES, false>(a, sm, s, sq, rb, hk, pg.lo + p0, pg.lo + p1, few_slot(a, hk, rb, x + s));
+    begin += pg.n;
+    u = begin;
+  }
+}
+
+// A whole sequence per workgroup: nothing to merge.
+template <int WV>
+__global__ __launch_bounds__(64 * WV, 2) void few_whole_kernel(const ChunkArgs a) {
+  __shared__ FewSmem<WV> sm;
+  const int hk = blockIdx.x % a.Hkv, y = blockIdx.x / a.Hkv, s = y / a.blocks, rb = y - s * a.blocks;
+  const Seq sq = seq_of(a, s);
+  const int R = min(32, sq.R - 32 * rb);
+  if (sq.len < 0) {
+    for (int x = threadIdx.x; x < R * D; x += 64 * WV) {
+      const int f = 32 * rb + x / D, p = (int)fdiv_u((uint32_t)f, a.g);
+      a.out[((int64_t)(a.row0[s] + p) * a.Hkv * a.G + hk * a.G + f - p * a.G) * D + x % D] = 0x7fc0;
+    }
+    return;
+  }
+  const Pages pg = few_pages(a, sq);
+  if (R > 0) few_part<WV, true>(a, sm, s, sq, rb, hk, pg.lo, pg.lo + pg.n, 0);
+}
+
+// An output row by GR groups of 32 lanes (4 dims each), 8 / GR rows per workgroup: group g takes every GR-th
+// partial, four at a time, and the groups meet in LDS.
+template <int GR>
+__global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
+  __shared__ float2 sh_ml[8];
+  __shared__ f4_t sh_acc[8][32];
+  const int lane = threadIdx.x & 63;
+  // wave-uniform: a row has at least a wave. Rows of a sequence and KV head: 32 per block
+  const int row = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (8 / GR) + threadIdx.x / (32 * GR)));
+  const int per = 32 * a.blocks, y = row / per, f = row - y * per, s = min(y / a.Hkv, a.nseq - 1), hk = y % a.Hkv;
+  const Deal deal = few_deal(a, lane);
+  const Seq sq = seq_of(a, s);
+  const int pages = few_pages(a, sq).n;
+  const int before = (s ? __builtin_amdgcn_readlane(deal.upto, s - 1) : 0) + SEQ_COST;
+  const int first = before / deal.share;
+  const bool mine = f < sq.R;
+  const int parts = mine && pages ? (before + pages - 1) / deal.share - first + 1 : 0;
+  const int64_t slot = few_slot(a, hk, f >> 5, first + s) + (f & 31);
+  const int grp = (threadIdx.x >> 5) % GR, ch = threadIdx.x & 31;
+  float M = -INFINITY, den = 0.0f;
+  f4_t acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = grp; i0 < parts; i0 += 4 * GR) {
+    float2 ml[4];
+    f4_t x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = slot + 32 * (int64_t)min(i0 + GR * j, parts - 1);
+      ml[j] = a.part_ml[at];
+      x[j] = *reinterpret_cast<const f4_t*>(a.part_acc + at * D + 4 * ch);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + GR * j < parts) merge_into(M, den, acc, ml[j].x, ml[j].y, x[j]);
+  }
+  const int at = threadIdx.x >> 5;
+  sh_acc[at][ch] = acc;
+  if (ch == 0) sh_ml[at] = make_float2(M, den);
+  __syncthreads();
+  if (grp != 0 || !mine) return;
+#pragma unroll
+  for (int j = 1; j < GR; ++j) merge_into(M, den, acc, sh_ml[at + j].x, sh_ml[at + j].y, sh_acc[at + j][ch]);
+  const float inv = sq.len < 0 ? NAN : den == 0.0f ? 0.0f : 1.0f / den;
+  const int p = (int)fdiv_u((uint32_t)f, a.g);
+  *reinterpret_cast<uint2*>(a.out + ((int64_t)(a.row0[s] + p) * a.Hkv * a.G + hk * a.G + f - p * a.G) * D + 4 * ch) =
+      make_uint2(pack_bf2(acc[0] * inv, acc[1] * inv), pack_bf2(acc[2] * inv, acc[3] * inv));
+}
+
+// How a call's sequences are dealt out.
+struct ChunkPart {  // the sequences of few rows, or of many
+  int nseq, rows_of, shares, blocks;  // rows of a block, shares per KV head
+  int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];
+  int64_t slots;  // partial rows, all heads
+};
+struct ChunkPlan {
+  ChunkPart few, many;
+};
+constexpr int64_t FEW_ROWS = 32;
 ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G, int cus) {
   ChunkPlan p{};
   int at = 0;
-  int64_t most = 0;  // query rows of a sequence
+  int64_t most = 0, few = 0;  // query rows of a sequence
   for (int s = 0; s < nseq; ++s) {
     if (counts[s]) {
-      p.seq[p.nseq] = s;
-      p.row0[p.nseq] = at;
-      p.rows[p.nseq++] = counts[s];
-      most = std::max<int64_t>(most, counts[s] * G);
+      const int64_t R = counts[s] * G;
+      ChunkPart& c = R <= FEW_ROWS ? p.few : p.many;
+      c.seq[c.nseq] = s;
+      c.row0[c.nseq] = at;
+      c.rows[c.nseq++] = counts[s];
+      (R <= FEW_ROWS ? few : most) = std::max(R <= FEW_ROWS ? few : most, R);
     }
     at += counts[s];
   }
-  p.lanes = 6;
-  while ((p.nseq << p.lanes) > 64) --p.lanes;
-  p.rows_of = most > 128 ? 256 : 128;
-  p.shares = (int)std::max<int64_t>(1, (p.rows_of == 256 ? 1 : 2) * cus / Hkv);
+  p.many.rows_of = most > 128 ? 256 : 128;
+  p.many.shares = (int)std::max<int64_t>(1, (p.many.rows_of == 256 ? 1 : 2) * cus / Hkv);
+  p.many.slots = p.many.nseq ? 2 * p.many.shares * Hkv * p.many.rows_of : 0;
+  p.few.rows_of = 32;
+  p.few.blocks = (int)((few + 31) / 32);
+  p.few.shares = (int)std::max<int64_t>(1, 2 * cus / Hkv);
+  p.few.slots = Hkv * p.few.blocks * (int64_t)(p.few.shares + p.few.nseq) * 32;
   return p;
 }
-int64_t chunk_bytes(const ChunkPlan& p, int64_t Hkv) {
-  return 2 * p.shares * Hkv * p.rows_of * (int64_t)(D * sizeof(float) + sizeof(float2));
+int64_t chunk_bytes(const ChunkPlan& p) {
+  return std::max(p.few.slots, p.many.slots) * (int64_t)(D * sizeof(float) + sizeof(float2));
 }
 
 int check_chunk(int64_t Hq, int64_t Hkv, const int32_t* counts, int64_t nseq) {
@@ -540,6 +850,48 @@ int check_chunk(int64_t Hq, int64_t Hkv, const int32_t* counts, int64_t nseq) {
   return LQ_OK;
 }
 
+int launch_many(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
+  const dim3 grid((unsigned)(a.shares * a.Hkv));
+  if (c.rows_of == 256)
+    chunk_kernel<8><<<grid, dim3(512), 0, st>>>(a);
+  else
+    chunk_kernel<4><<<grid, dim3(256), 0, st>>>(a);
+  LQ_CHECK_LAUNCH("chunk_kernel");
+  if (a.shares > 1) {
+    auto* merge = c.rows_of == 256 ? chunk_merge_kernel<256> : chunk_merge_kernel<128>;
+    merge<<<dim3((unsigned)((a.shares - 1) * a.Hkv), c.rows_of / MERGE_ROWS), dim3(256), 0, st>>>(a);
+    LQ_CHECK_LAUNCH("chunk_merge_kernel");
+  }
+  return LQ_OK;
+}
+
+// A call of few pages per sequence takes each whole.
+constexpr int64_t WHOLE_PAGES = 16;
+int launch_few(const ChunkArgs& a, const ChunkPart& c, int64_t window, hipStream_t st) {
+  int rows = 0;
+  for (int s = 0; s < c.nseq; ++s) rows = std::max(rows, c.rows[s]);
+  // pages that rows at `rows` positions see of a window each
+  const int64_t seen = window == 0 ? a.tab.width : std::min<int64_t>(a.tab.width, (window + rows - 2 + PAGE - 1) / PAGE + 1);
+  if (seen <= WHOLE_PAGES) {
+    const int64_t wgs = (int64_t)c.nseq * c.blocks * a.Hkv;
+    if (wgs <= device_cu_count())
+      few_whole_kernel<8><<<dim3((unsigned)wgs), dim3(512), 0, st>>>(a);
+    else
+      few_whole_kernel<4><<<dim3((unsigned)wgs), dim3(256), 0, st>>>(a);
+    LQ_CHECK_LAUNCH("few_whole_kernel");
+    return LQ_OK;
+  }
+  few_kernel<<<dim3((unsigned)(a.shares * c.blocks * a.Hkv)), dim3(64 * FEW_WAVES), 0, st>>>(a);
+  LQ_CHECK_LAUNCH("few_kernel");
+  const int64_t n = (int64_t)c.nseq * a.Hkv * 32 * c.blocks;
+  if (a.shares / std::min(c.nseq, 4) > 16)
+    few_merge_kernel<8><<<dim3((unsigned)n), dim3(256), 0, st>>>(a);
+  else
+    few_merge_kernel<2><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(a);
+  LQ_CHECK_LAUNCH("few_merge_kernel");
+  return LQ_OK;
+}
+
 }  // namespace
 }  // namespace lq
 
@@ -547,7 +899,7 @@ extern "C" int64_t lq_paged_chunk_workspace_bytes(const int32_t* counts_host, in
   using namespace lq;
   clear_error();
   if (check_chunk(Hq, Hkv, counts_host, nseq)) return -1;
-  return chunk_bytes(chunk_plan(counts_host, nseq, Hkv, Hq / Hkv, device_cu_count()), Hkv);
+  return chunk_bytes(chunk_plan(counts_host, nseq, Hkv, Hq / Hkv, device_cu_count()));
 }
 
 extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_head, const uint8_t* kc,
@@ -569,16 +921,17 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
   LQ_CHECK_ARG(std::isfinite(scale), "the softmax scale is not finite");
   const int64_t G = Hq / Hkv;
   const ChunkPlan plan = chunk_plan(counts_host, nseq, Hkv, G, device_cu_count());
-  if (plan.nseq == 0) return LQ_OK;
+  if (plan.few.nseq + plan.many.nseq == 0) return LQ_OK;
   LQ_CHECK_ARG(q && lens && out, "null pointer");
   LQ_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0 && ((q_tok | q_head) & 7) == 0,
                "rows must be 16-byte aligned (strides a multiple of 8)");
   int64_t most = 0;  // cost, if every block sees the whole table
-  for (int s = 0; s < plan.nseq; ++s)
-    most += (plan.rows[s] * G + plan.rows_of - 1) / plan.rows_of * (table_width + lq::BLOCK_COST);
+  for (int s = 0; s < plan.many.nseq; ++s)
+    most += (plan.many.rows[s] * G + plan.many.rows_of - 1) / plan.many.rows_of * (table_width + lq::BLOCK_COST);
+  most = std::max<int64_t>(most, plan.few.nseq * (table_width + lq::SEQ_COST));
   LQ_CHECK_ARG(most < (1ll << 31) - (1 << 20), "too many rows for table rows of %lld pages", (long long)table_width);
-  const int64_t need = chunk_bytes(plan, Hkv);
-  if (!workspace || workspace_bytes < need) {
+  const int64_t need = chunk_bytes(plan);
+  if (need > 0 && (!workspace || workspace_bytes < need)) {
     set_error("workspace of %lld bytes is smaller than the %lld needed", (long long)workspace_bytes, (long long)need);
     return LQ_EWORKSPACE;
   }
@@ -588,29 +941,26 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
   a.q_head = q_head;
   a.lens = lens;
   a.out = out;
-  a.part_acc = (float*)workspace;
-  a.part_ml = (float2*)(a.part_acc + 2 * plan.shares * Hkv * plan.rows_of * 128);
   a.Hkv = (int)Hkv;
   a.G = (int)G;
   a.g = make_fastdiv((uint32_t)G);
   a.sl2 = scale * 1.4426950408889634f;
   a.window = window == 0 ? NO_WINDOW : (int)std::min<int64_t>(window, NO_WINDOW);
-  a.shares = plan.shares;
-  a.nseq = plan.nseq;
-  a.lanes = plan.lanes;
-  std::copy(plan.seq, plan.seq + LQ_MAX_SEQS, a.seq);
-  std::copy(plan.row0, plan.row0 + LQ_MAX_SEQS, a.row0);
-  std::copy(plan.rows, plan.rows + LQ_MAX_SEQS, a.rows);
-  const dim3 grid((unsigned)(plan.shares * Hkv));
-  if (plan.rows_of == 256)
-    chunk_kernel<8><<<grid, dim3(512), 0, (hipStream_t)stream>>>(a);
-  else
-    chunk_kernel<4><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a);
-  LQ_CHECK_LAUNCH("chunk_kernel");
-  if (plan.shares > 1) {
-    auto* merge = plan.rows_of == 256 ? chunk_merge_kernel<256> : chunk_merge_kernel<128>;
-    merge<<<dim3((unsigned)((plan.shares - 1) * Hkv), plan.rows_of / MERGE_ROWS), dim3(256), 0, (hipStream_t)stream>>>(a);
-    LQ_CHECK_LAUNCH("chunk_merge_kernel");
+  const hipStream_t st = (hipStream_t)stream;
+  for (const ChunkPart* c : {&plan.many, &plan.few}) {
+    if (c->nseq == 0) continue;
+    a.part_acc = (float*)workspace;
+    a.part_ml = (float2*)(a.part_acc + c->slots * 128);
+    a.shares = c->shares;
+    a.blocks = c->blocks;
+    a.nseq = c->nseq;
+    a.lanes = 6;
+    while ((c->nseq << a.lanes) > 64) --a.lanes;
+    std::copy(c->seq, c->seq + LQ_MAX_SEQS, a.seq);
+    std::copy(c->row0, c->row0 + LQ_MAX_SEQS, a.row0);
+    std::copy(c->rows, c->rows + LQ_MAX_SEQS, a.rows);
+    const int status = c == &plan.many ? launch_many(a, *c, st) : launch_few(a, *c, window, st);
+    if (status) return status;
   }
   return LQ_OK;
 }
