@@ -55,6 +55,23 @@ __device__ __forceinline__ void settle_huge32(f16v_t (&c)[2], float& off, float 
   off = huge ? 0.0f : off;
 }
 
+// Scores of keys that the lane's row does not see to -infinity: it sees the `window` keys up to key `rel` of those
+// from 4 h on. By bits: a key's bit spread over a word chooses between the score and -infinity.
+__device__ __forceinline__ void mask32(f16v_t (&c)[2], int rel, int window) {
+  uint64_t seen = rel < 0 ? 0 : ~0ull >> (63 - min(rel, 63));
+  const int out = rel - window;  // the last key before the window
+  if (out >= 0) seen = out >= 63 ? 0 : seen >> (out + 1) << (out + 1);
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) {
+    const int w = (int)(seen >> (32 * mt));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t on = (uint32_t)((w << (31 - 8 * (i >> 2) - (i & 3))) >> 31);
+      c[mt][i] = __uint_as_float((__float_as_uint(c[mt][i]) & on) | (0xff800000u & ~on));
+    }
+  }
+}
+
 // Scores to weights: raises the running maximum where needed (and rescales the row), P in bf16 as the B operands
 // of the four 16-key steps.
 __device__ __forceinline__ void softmax32(f16v_t (&c)[2], Rows32& st, float scale, bf16x8_t (&p)[4]) {

@@ -48,7 +48,7 @@ struct ChunkArgs {
   FastDiv g;
   float sl2;
   int window;          // positions a row sees, NO_WINDOW: all
-  int shares;          // per KV head
+  int shares;          // per KV head; 0: a workgroup takes a whole block
   int blocks;          // of 32 rows, of the sequence with the most (few rows)
   int nseq, lanes;     // sequences, log2 of the lanes that add up the blocks of one
   int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];  // table row, first row of q, rows (not 0)
@@ -79,6 +79,7 @@ __device__ __forceinline__ Span block_span(const ChunkArgs& a, const Seq& q, int
 // A block, its tiles, its place among its sequence's blocks and where its cost begins.
 struct Block {
   int seq, blk, lo, tiles, begin, place;
+  Seq q;
 };
 // The block at a place among nb: the last, the first, the last but one, .., so that two neighbours cost about
 // the same and cuts are few.
@@ -86,22 +87,31 @@ __device__ __forceinline__ int block_at(int place, int nb) {
   return place & 1 ? place >> 1 : nb - 1 - (place >> 1);
 }
 
-// What the call deals out: a lane's inclusive sum of costs (2^lanes of them per sequence), the whole and a share.
+// What the call deals out: a lane's inclusive sum of costs (2^lanes of them per sequence) and its sequence, the whole
+// and a share.
 struct Deal {
-  int upto, total, share;
+  int upto;
+  Seq q;
+  int total, share;
 };
+// The sequence of a lane.
+__device__ __forceinline__ Seq seq_at(const Deal& d, int lane) {
+  return {__builtin_amdgcn_readlane(d.q.R, lane), __builtin_amdgcn_readlane(d.q.len, lane),
+          __builtin_amdgcn_readlane(d.q.base, lane)};
+}
 template <int ROWS>
 __device__ __forceinline__ Deal deal_out(const ChunkArgs& a, int lane) {
   const int s = lane >> a.lanes;
   int cost = 0;
+  Seq q{0, 0, 0};
   if (s < a.nseq) {
-    const Seq q = seq_of(a, s);
+    q = seq_of(a, s);
     for (int b = lane & ((1 << a.lanes) - 1); b * ROWS < q.R; b += 1 << a.lanes)
       cost += block_span<ROWS>(a, q, b).n + BLOCK_COST;
   }
   const int upto = wave_scan_i(cost);
   const int total = __builtin_amdgcn_readlane(upto, 63);
-  return {upto, total, max(BLOCK_COST + MIN_PART, (total + a.shares - 1) / a.shares)};
+  return {upto, q, total, max(BLOCK_COST + MIN_PART, (total + a.shares - 1) / a.shares)};
 }
 // The block that holds cost u (below the total).
 template <int ROWS>
@@ -109,7 +119,7 @@ __device__ __forceinline__ Block find_block(const ChunkArgs& a, const Deal& d, i
   const int last = (1 << a.lanes) - 1;  // a sequence's last lane has its end
   const int s = __builtin_popcountll(__builtin_amdgcn_ballot_w64((lane & last) == last && d.upto <= u));
   int before = s ? __builtin_amdgcn_readlane(d.upto, (s << a.lanes) - 1) : 0;
-  const Seq q = seq_of(a, s);
+  const Seq q = seq_at(d, s << a.lanes);
   const int nb = (q.R + ROWS - 1) / ROWS;
   for (int i = 0;; i += 64) {
     Span sp{0, 0};
@@ -123,7 +133,7 @@ __device__ __forceinline__ Block find_block(const ChunkArgs& a, const Deal& d, i
     if (past || i + 64 >= nb) {
       const int l = past ? __builtin_ctzll(past) : 0;
       return {s, block_at(i + l, nb), __builtin_amdgcn_readlane(sp.lo, l), __builtin_amdgcn_readlane(sp.n, l),
-              before + __builtin_amdgcn_readlane(upto - c, l), i + l};
+              before + __builtin_amdgcn_readlane(upto - c, l), i + l, q};
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
@@ -132,6 +142,44 @@ __device__ __forceinline__ Block find_block(const ChunkArgs& a, const Deal& d, i
 __device__ __forceinline__ int cut_tile(const Block& b, int u) {
   const int t = u - b.begin - BLOCK_COST;
   return t >= b.tiles ? b.tiles : t < MIN_PART ? 0 : t > b.tiles - MIN_PART ? b.tiles : t;
+}
+
+// The block of rank x when all are in order of their tiles, most first: how many have at least n tiles is a sum over
+// the sequences, a lane each, and the largest n that more than x have is found by halving. Behind a window all cost
+// about the same and stand one sequence behind the other. Its cost is counted from its own begin.
+template <int ROWS>
+__device__ __forceinline__ Block ranked_block(const ChunkArgs& a, int x, int lane) {
+  const Seq q = lane < a.nseq ? seq_of(a, lane) : Seq{0, 0, 0};
+  const int nb = (q.R + ROWS - 1) / ROWS;
+  Deal d{0, q, 0, 0};
+  int s, blk;
+  if (a.window < NO_WINDOW) {
+    const int upto = wave_scan_i(nb);
+    s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > x));
+    blk = __builtin_amdgcn_readlane(upto, s) - 1 - x;
+  } else {
+    auto from = [&](int n) {  // first block of the lane's sequence with at least n tiles (of nb: none)
+      const int64_t y = (int64_t)a.G * ((int64_t)TKEYS * (n - 1) - q.base);  // the row that has to be reached
+      return n <= 0 || y <= 0 ? 0 : y > q.R - 1 ? nb : (int)(y / ROWS);
+    };
+    int lo = 0, hi = a.tab.width + 1;  // all have lo, none has hi
+    int above = 0;                     // blocks with at least hi tiles
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1, n = __builtin_amdgcn_readfirstlane(wave_sum_i(nb - from(mid)));
+      if (n > x) {
+        lo = mid;
+      } else {
+        hi = mid;
+        above = n;
+      }
+    }
+    const int n = from(lo + 1) - from(lo), upto = wave_scan_i(n);
+    s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > x - above));
+    blk = __builtin_amdgcn_readlane(from(lo), s) + x - above - __builtin_amdgcn_readlane(upto - n, s);
+  }
+  const Seq sq = seq_at(d, s);
+  const Span sp = block_span<ROWS>(a, sq, blk);
+  return {s, blk, sp.lo, sp.n, 0, 0, sq};
 }
 
 // Whether a V scale and bias may give something that is no finite bf16.
@@ -194,10 +242,18 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
   constexpr int C = 8 / PW;  // 16-byte chunks of K (of V) that a thread brings per tile
   __shared__ ChunkSmem<STAGES> sm;
   const int share = blockIdx.x / a.Hkv, hk = blockIdx.x - share * a.Hkv;
-  const Deal deal = deal_out<ROWS>(a, threadIdx.x & 63);
-  const int u0 = deal.share * share, u1 = min(u0 + deal.share, deal.total);
-  if (u0 >= u1) return;
-  Block b = find_block<ROWS>(a, deal, u0, threadIdx.x & 63);
+  int u0 = 0, u1;
+  Block b;
+  if (a.shares) {
+    const Deal deal = deal_out<ROWS>(a, threadIdx.x & 63);
+    u0 = deal.share * share;
+    u1 = min(u0 + deal.share, deal.total);
+    if (u0 >= u1) return;
+    b = find_block<ROWS>(a, deal, u0, threadIdx.x & 63);
+  } else {  // a whole block
+    b = ranked_block<ROWS>(a, share, threadIdx.x & 63);
+    u1 = b.tiles + BLOCK_COST;
+  }
   for (bool more = true; more;) {
     // re-read per block, so that no lane value made of it is kept across blocks
     int tid = threadIdx.x;
@@ -206,7 +262,7 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const bool grp_a = HALVES && wv < PW / 2;
     const int ln = lane & 31, h = lane >> 5;
-    const Seq sq = seq_of(a, b.seq);
+    const Seq sq = b.q;
     const int q0 = a.row0[b.seq];
     const int c0 = cut_tile(b, u0), c1 = cut_tile(b, u1);
     const int t0 = b.lo + c0, t1 = b.lo + c1;
@@ -270,7 +326,7 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
         *lo = make_uint4(d0.x, d0.y, d1.x, d1.y);
         *hi = make_uint4(d2.x, d2.y, d3.x, d3.y);
       };
-      auto stage_k = [&](int t) {
+      auto stage_k = [&](int t, const u4_t (&rk)[C], const uint32_t (&ks)[C], const uint32_t (&kb)[C], bool k_ok) {
         if (t >= t1) return;  // uniform
         KvTile& to = sm.tile[t % STAGES];
 #pragma unroll
@@ -306,10 +362,24 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
         }
       };
 
-      lds_barrier();  // the block before is done with LDS
+      // the first tile's K, the second's and the first's V are all out before any is waited for
+      u4_t fk[C];
+      uint32_t fs[C], fb[C];
+      bool f_ok = true;
       if (t0 < t1) {
         next_row(t0);
         load_k();
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          fk[i] = rk[i];
+          fs[i] = ks[i];
+          fb[i] = kb[i];
+        }
+        f_ok = k_ok;
+        next_row(t0 + 1);
+        load_k();
+        load_v();
+        next_row(t0 + 2);
       }
 
       // ---- the wave's rows
@@ -332,15 +402,12 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
       bf16x8_t p[4];
       const uint32_t k_at = k_lane32(sm.tile[0], lane), v_at = v_lane32(sm.tile[0], lane);
       auto tile_at = [](int t) { return (uint32_t)(t % STAGES) * (uint32_t)sizeof(KvTile); };
+      lds_barrier();  // the block before is done with LDS
       if (t0 < t1) {
         if (tid < 6) sm.wild[tid >> 1][tid & 1] = 0;
-        stage_k(t0);
-        next_row(t0 + 1);
-        load_k();
-        load_v();
-        next_row(t0 + 2);
+        stage_k(t0, fk, fs, fb, f_ok);
         auto begin = [&]() {  // K of the second tile, V of the first; the next ones loaded
-          stage_k(t0 + 1);
+          stage_k(t0 + 1, rk, ks, kb, k_ok);
           settle_v(t0);
 #pragma unroll
           for (int i = 0; i < 8; ++i) stage_v(t0, i);
@@ -359,16 +426,10 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
           lds_barrier();
           // vector phase
           __builtin_amdgcn_s_setprio(0);
-          stage_k(t + 2);
+          stage_k(t + 2, rk, ks, kb, k_ok);
           load_k();
           if (TKEYS * t + TKEYS - 1 > lim_lo || TKEYS * t < open_from) {  // wave-uniform: masked for some row
-            const int rel = lim - TKEYS * t - 4 * h;
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-              for (int r = 0; r < 16; ++r)
-                c[mt][r] = (uint32_t)(rel - (32 * mt + 8 * (r >> 2) + (r & 3))) < (uint32_t)a.window ? c[mt][r]
-                                                                                                 : -INFINITY;
+            mask32(c, lim - TKEYS * t - 4 * h, a.window);
           }
           Ahead32 ahead;
           const uint32_t kt = k_at + tile_at(t + 1);
@@ -442,10 +503,10 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
         place = 0;
         ++ns;
       }
-      const Seq nq = seq_of(a, ns);
-      const int blk = block_at(place, (nq.R + ROWS - 1) / ROWS);
-      const Span sp = block_span<ROWS>(a, nq, blk);
-      b = Block{ns, blk, sp.lo, sp.n, next, place};
+      if (ns != b.seq) b.q = seq_of(a, ns);
+      const int blk = block_at(place, (b.q.R + ROWS - 1) / ROWS);
+      const Span sp = block_span<ROWS>(a, b.q, blk);
+      b = Block{ns, blk, sp.lo, sp.n, next, place, b.q};
     }
   }
 }
@@ -462,7 +523,7 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkArgs a) {
   const Block b = find_block<ROWS>(a, deal, u, lane);
   const int t = cut_tile(b, u);
   if (t == 0 || t == b.tiles || cut_tile(b, u - deal.share) != 0) return;  // no cut, or not its first
-  const Seq sq = seq_of(a, b.seq);
+  const Seq sq = b.q;
   const int d = 4 * (threadIdx.x & 31);
   int n = 1;  // parts
   while (cut_tile(b, u + n * deal.share - deal.share) < b.tiles) ++n;
@@ -525,15 +586,12 @@ __device__ __forceinline__ Pages few_pages(const ChunkArgs& a, const Seq& q) {
   const int lo = max(0, q.base - a.window + 1) / PAGE;
   return {lo, q.len <= 0 ? 0 : (q.len + PAGE - 1) / PAGE - lo};
 }
-__device__ __forceinline__ int few_cost(const ChunkArgs& a, int s) {
-  if (s >= a.nseq) return 0;
-  const int n = few_pages(a, seq_of(a, s)).n;
-  return n ? n + SEQ_COST : 0;
-}
 __device__ __forceinline__ Deal few_deal(const ChunkArgs& a, int lane) {
-  const int upto = wave_scan_i(few_cost(a, lane));
+  const Seq q = lane < a.nseq ? seq_of(a, lane) : Seq{0, 0, 0};
+  const int n = few_pages(a, q).n;
+  const int upto = wave_scan_i(n ? n + SEQ_COST : 0);
   const int total = __builtin_amdgcn_readlane(upto, 63);
-  return {upto, total, max(SHARE_MIN, (total + a.shares - 1) / a.shares)};
+  return {upto, q, total, max(SHARE_MIN, (total + a.shares - 1) / a.shares)};
 }
 
 // Pages [p0, p1) of sequence s for the rows of block rb: partial rows to slot .., or with WHOLE output rows.
@@ -553,7 +611,6 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
   const int lim = f < sq.R ? sq.base + i : -1;
   const uint16_t* qr = a.q + (int64_t)(a.row0[s] + i) * a.q_tok + (hk * a.G + head) * a.q_head + 16 * h;
   // q in K's order of dims: step 2 j + x holds dims 16 (2 j + h) + 8 x .. + 7
-#pragma unroll
   for (int kk = wv; kk < 8; kk += WV)
     sm.q[kk][lane] = signed_q(*reinterpret_cast<const uint4*>(qr + 32 * (kk >> 1) + 8 * (kk & 1)), a.sl2);
   Rows32 st;
@@ -624,12 +681,7 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
       __builtin_amdgcn_sched_barrier(0);
     }
     if (masked) {  // uniform
-      const int rel = lim - PAGE * p - 4 * h;
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          c[mt][r] = (uint32_t)(rel - (32 * mt + 8 * (r >> 2) + (r & 3))) < (uint32_t)a.window ? c[mt][r] : -INFINITY;
+      mask32(c, lim - PAGE * p - 4 * h, a.window);
     }
     bf16x8_t pr[4];
     softmax32(c, st, scale, pr);
@@ -721,7 +773,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void few_kernel(const ChunkArgs 
   int s = __builtin_popcountll(__builtin_amdgcn_ballot_w64(deal.upto <= u0));
   int begin = s ? __builtin_amdgcn_readlane(deal.upto, s - 1) : 0;
   for (int u = u0; u < u1; ++s) {
-    const Seq sq = seq_of(a, s);
+    const Seq sq = seq_at(deal, s);
     const Pages pg = few_pages(a, sq);
     if (pg.n == 0) continue;
     begin += SEQ_COST;
@@ -761,7 +813,7 @@ __global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
   const int row = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (8 / GR) + threadIdx.x / (32 * GR)));
   const int per = 32 * a.blocks, y = row / per, f = row - y * per, s = min(y / a.Hkv, a.nseq - 1), hk = y % a.Hkv;
   const Deal deal = few_deal(a, lane);
-  const Seq sq = seq_of(a, s);
+  const Seq sq = seq_at(deal, s);
   const int pages = few_pages(a, sq).n;
   const int before = (s ? __builtin_amdgcn_readlane(deal.upto, s - 1) : 0) + SEQ_COST;
   const int first = before / deal.share;
@@ -799,7 +851,7 @@ __global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
 
 // How a call's sequences are dealt out.
 struct ChunkPart {  // the sequences of few rows, or of many
-  int nseq, rows_of, shares, blocks;  // rows of a block, shares per KV head
+  int nseq, rows_of, shares, blocks;  // rows of a block, shares (0: whole blocks) and blocks per KV head
   int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];
   int64_t slots;  // partial rows, all heads
 };
@@ -807,6 +859,7 @@ struct ChunkPlan {
   ChunkPart few, many;
 };
 constexpr int64_t FEW_ROWS = 32;
+constexpr int64_t WHOLE_ROUNDS = 6, SMALL_ROUNDS = 3;
 ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G, int cus) {
   ChunkPlan p{};
   int at = 0;
@@ -822,8 +875,14 @@ ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G
     }
     at += counts[s];
   }
-  p.many.rows_of = most > 128 ? 256 : 128;
-  p.many.shares = (int)std::max<int64_t>(1, (p.many.rows_of == 256 ? 1 : 2) * cus / Hkv);
+  int64_t blocks[2] = {0, 0};  // of 128 and of 256 rows
+  for (int s = 0; s < p.many.nseq; ++s)
+    for (int i = 0; i < 2; ++i) blocks[i] += (p.many.rows[s] * G + (128 << i) - 1) / (128 << i);
+  const bool large = blocks[1] * Hkv >= WHOLE_ROUNDS * cus;
+  const bool small = !large && blocks[0] * Hkv >= SMALL_ROUNDS * cus;
+  p.many.rows_of = !small && most > 128 ? 256 : 128;
+  p.many.blocks = (int)blocks[!small && most > 128];
+  p.many.shares = large || small ? 0 : (int)std::max<int64_t>(1, (p.many.rows_of == 256 ? 1 : 2) * cus / Hkv);
   p.many.slots = p.many.nseq ? 2 * p.many.shares * Hkv * p.many.rows_of : 0;
   p.few.rows_of = 32;
   p.few.blocks = (int)((few + 31) / 32);
@@ -851,7 +910,7 @@ int check_chunk(int64_t Hq, int64_t Hkv, const int32_t* counts, int64_t nseq) {
 }
 
 int launch_many(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
-  const dim3 grid((unsigned)(a.shares * a.Hkv));
+  const dim3 grid((unsigned)((a.shares ? a.shares : c.blocks) * a.Hkv));
   if (c.rows_of == 256)
     chunk_kernel<8><<<grid, dim3(512), 0, st>>>(a);
   else
