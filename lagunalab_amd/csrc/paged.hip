@@ -117,9 +117,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(
 }
 
 // ---- append with the norm and the rotation on the way: the heads of a token are its queries', keys' and values',
-// 16 lanes per head (8 dims each), 4 heads per wave at a time and RT times that many in turn, so that a wave
-// finds its token's angles once. A rotated dim's partner (half layout) comes by a load of its own, out with the
-// lane's own values, rather than from another lane behind them.
+// 16 lanes per head (8 dims each), 4 heads per wave at a time and RT times that many in turn. A wave finds its
+// token's angles, one per lane, and hands them round through LDS (8 per lane in registers, as the lanes need them:
+// 2,048 rows of 48/8 heads 27.6 us, VALU-bound). A rotated dim's partner (half layout) comes by a load of its own,
+// out with the lane's own values, rather than from another lane behind them.
 struct RotateArgs {
   const uint16_t* q;
   const uint16_t* k;
@@ -142,44 +143,51 @@ struct RotateArgs {
   FastDiv tok;
 };
 
-// cos and sin (times mscale) of a lane's 8 dims at a position. The angle is a product in 64 bits, reduced to a
-// turn there: in 32 it would be off by 0.004 radians at position 82,671, two steps of a bf16 sine.
+// cos and sin (times mscale) of a pair's angle at a position. The angle is a product in 64 bits, reduced to a turn
+// there: in 32 it would be off by 0.004 radians at position 82,671, two steps of a bf16 sine.
+__device__ __forceinline__ float2 rotation(const RotateArgs& a, int64_t pos, int pair) {
+  const double turns = (double)pos * (double)a.freq[pair] * 0.15915494309189535;
+  float sn, cs;
+  sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
+  return make_float2(cs * a.mscale, sn * a.mscale);
+}
+// Those of a lane's 8 dims, the sine with the sign that its partner takes; 1 and 0 of dims that stay.
 template <bool PAIRS>
-__device__ __forceinline__ void rotation8(const RotateArgs& a, int64_t pos, int d0, float (&c)[8], float (&s)[8]) {
-  const int half = a.dims >> 1;
+__device__ __forceinline__ void rotation8(const float2* pairs, int d0, int dims, float (&c)[8], float (&s)[8]) {
+  const int half = dims >> 1;
 #pragma unroll
-  for (int j = 0; j < 8; j += PAIRS ? 2 : 1) {
+  for (int j = 0; j < 8; j += 2) {
     const int d = d0 + j;
-    c[j] = 1.0f;
-    s[j] = 0.0f;
-    if (d < a.dims) {
-      const double turns = (double)pos * (double)a.freq[PAIRS ? d >> 1 : d < half ? d : d - half] * 0.15915494309189535;
-      float sn, cs;
-      sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
-      c[j] = cs * a.mscale;
-      s[j] = sn * a.mscale;
-      if (!PAIRS && d < half) s[j] = -s[j];  // first half: x c - partner s
-    }
     if (PAIRS) {
-      c[j + 1] = c[j];
-      s[j + 1] = s[j];
-      s[j] = -s[j];
+      const float2 p = d < dims ? pairs[d >> 1] : make_float2(1.0f, 0.0f);
+      c[j] = c[j + 1] = p.x;
+      s[j] = -p.y;
+      s[j + 1] = p.y;
+    } else {  // half is even: two dims are of one side
+      const int at = d < half ? d : d - half;
+      const float4 p = d < dims ? *reinterpret_cast<const float4*>(pairs + at) : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
+      c[j] = p.x;
+      s[j] = d < half ? -p.y : p.y;
+      c[j + 1] = p.z;
+      s[j + 1] = d < half ? -p.w : p.w;
     }
   }
 }
-// The 8 values at a lane's partner dims (half layout). WIDE: dims / 2 is a multiple of 8, they lie together.
+// The 8 values at a lane's partner dims (half layout), 0 for dims that stay. WIDE: dims / 2 is a multiple of 8, they
+// lie together.
 template <bool WIDE>
 __device__ __forceinline__ uint4 partner8(const uint16_t* row, int d0, int dims) {
   const int half = dims >> 1;
   if constexpr (WIDE) {
-    const int d = d0 < half ? d0 + half : d0 < dims ? d0 - half : d0;
-    return *reinterpret_cast<const uint4*>(row + d);
+    const uint4 u = *reinterpret_cast<const uint4*>(row + (d0 < half ? d0 + half : d0 < dims ? d0 - half : d0));
+    return d0 < dims ? u : make_uint4(0, 0, 0, 0);
   } else {
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {  // half is even
       const int d = d0 + 2 * j;
-      w[j] = *reinterpret_cast<const uint32_t*>(row + (d < half ? d + half : d < dims ? d - half : d));
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(row + (d < half ? d + half : d < dims ? d - half : d));
+      w[j] = d < dims ? u : 0;
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -197,6 +205,7 @@ constexpr int ROTATE_TURNS = 4, ROTATE_MANY = 32;
 
 template <bool PAIRS, bool WIDE, int RT>
 __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateArgs a, const PackedRows rows) {
+  __shared__ alignas(16) float2 sh_pairs[4][D / 2];
   const int lane = threadIdx.x & 63, sub = lane & 15, d0 = 8 * sub;
   const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
   const int t = (int)fdiv_u((uint32_t)wave, a.tok);
@@ -223,39 +232,56 @@ __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateArgs a, c
   const bool inside = pos >= 0 && pos < (int64_t)a.tab.width * PAGE;
   const int id = inside ? a.tab.ids[b * a.tab.stride + (pos >> 6)] : -1;
   const bool stored = id >= 0 && id < a.tab.pages;
+  float2* pairs = sh_pairs[threadIdx.x >> 6];
+  if (2 * lane < a.dims) pairs[lane] = rotation(a, pos, lane);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   float c[8], s[8];
-  rotation8<PAIRS>(a, pos, d0, c, s);
+  rotation8<PAIRS>(pairs, d0, a.dims, c, s);
+  float cw[8], sw[8];  // with the norm weights of the dim and of its partner
+  const uint16_t* of = nullptr;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    cw[j] = c[j];
+    sw[j] = s[j];
+  }
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     const int h = h0 + 4 * i;
     const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
-    const uint16_t* w = is_q ? a.q_w : a.k_w;
+    const uint16_t* w = is_v ? of : is_q ? a.q_w : a.k_w;
+    if (w != of) {  // a lane's first head, and where its queries end
+      of = w;
+      float g[8], o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = o[j] = 1.0f;
+      if (w) {
+        unpack8(*reinterpret_cast<const uint4*>(w + d0), g);
+        if constexpr (!PAIRS) unpack8(partner8<WIDE>(w, d0, a.dims), o);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        cw[j] = c[j] * g[j];
+        sw[j] = s[j] * (PAIRS ? g[j ^ 1] : o[j]);
+      }
+    }
     float x[8], y[8];
     unpack8(own[i], x);
     if constexpr (!PAIRS) unpack8(other[i], y);
-    if (w) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
-      const float inv = rsqrtf(sum16(ss) * (1.0f / D) + a.eps);
-      float g[8];
-      unpack8(*reinterpret_cast<const uint4*>(w + d0), g);
-      if (!is_v) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= inv * g[j];
-      }
-      if constexpr (!PAIRS) {
-        unpack8(partner8<WIDE>(w, d0, a.dims), g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] *= inv * g[j];
-      }
-    }
     if (!is_v) {
+      float inv = 1.0f;
+      if (w) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+        inv = rsqrtf(sum16(ss) * (1.0f / D) + a.eps);
+      }
       float r[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = fmaf(PAIRS ? x[j ^ 1] : y[j], s[j], x[j] * c[j]);
+      for (int j = 0; j < 8; ++j) r[j] = fmaf(PAIRS ? x[j ^ 1] : y[j], sw[j], x[j] * cw[j]) * inv;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.dims ? r[j] : x[j];
+      for (int j = 0; j < 8; ++j) x[j] = r[j];
     }
     if (is_q)  // rounded here and nowhere before
       *reinterpret_cast<uint4*>(a.q_out + ((int64_t)t * a.Hq + h) * D + d0) =
