@@ -41,12 +41,13 @@ struct Rows32 {
 };
 
 // As settle_huge of attn_tile.h.
-__device__ __forceinline__ void settle_huge32(f16v_t (&c)[2], float& off, float scale) {
+template <int MT>
+__device__ __forceinline__ void settle_huge32(f16v_t (&c)[MT], float& off, float scale) {
 #pragma clang fp contract(off)
   const bool huge = is_huge(off);
   const float inv = 1.0f / scale;
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt)
+  for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float x = c[mt][i] * scale;  // rounded as the maximum was
@@ -57,12 +58,13 @@ __device__ __forceinline__ void settle_huge32(f16v_t (&c)[2], float& off, float 
 
 // Scores of keys that the lane's row does not see to -infinity: it sees the `window` keys up to key `rel` of those
 // from 4 h on. By bits: a key's bit spread over a word chooses between the score and -infinity.
-__device__ __forceinline__ void mask32(f16v_t (&c)[2], int rel, int window) {
+template <int MT>
+__device__ __forceinline__ void mask32(f16v_t (&c)[MT], int rel, int window) {
   uint64_t seen = rel < 0 ? 0 : ~0ull >> (63 - min(rel, 63));
   const int out = rel - window;  // the last key before the window
   if (out >= 0) seen = out >= 63 ? 0 : seen >> (out + 1) << (out + 1);
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt) {
+  for (int mt = 0; mt < MT; ++mt) {
     const int w = (int)(seen >> (32 * mt));
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -72,12 +74,13 @@ __device__ __forceinline__ void mask32(f16v_t (&c)[2], int rel, int window) {
   }
 }
 
-// Scores to weights: raises the running maximum where needed (and rescales the row), P in bf16 as the B operands
-// of the four 16-key steps.
-__device__ __forceinline__ void softmax32(f16v_t (&c)[2], Rows32& st, float scale, bf16x8_t (&p)[4]) {
-  float x[4];
+// Scores of MT key tiles to weights: raises the running maximum where needed (and rescales the row), P in bf16 as the
+// B operands of the 16-key steps.
+template <int MT>
+__device__ __forceinline__ void softmax32(f16v_t (&c)[MT], Rows32& st, float scale, bf16x8_t (&p)[2 * MT]) {
+  float x[2 * MT];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {  // four chains
+  for (int j = 0; j < 2 * MT; ++j) {  // chains
     const f16v_t& s = c[j >> 1];
     const int i = 8 * (j & 1);
     x[j] = max_ieee(max_ieee(s[i], s[i + 1]), s[i + 2]);
@@ -85,7 +88,9 @@ __device__ __forceinline__ void softmax32(f16v_t (&c)[2], Rows32& st, float scal
     for (int k = 3; k < 7; k += 2) x[j] = max_ieee(max_ieee(x[j], s[i + k]), s[i + k + 1]);
     x[j] = max_ieee(x[j], s[i + 7]);
   }
-  const float t = max_xor32(max_ieee(max_ieee(x[0], x[1]), max_ieee(x[2], x[3]))) * scale;
+  float top = max_ieee(x[0], x[1]);
+  if constexpr (MT == 2) top = max_ieee(top, max_ieee(x[2], x[3]));
+  const float t = max_xor32(top) * scale;
   const bool bump = t > (st.m == -INFINITY ? -INFINITY : st.m + RESCALE_LOG2);
   float off = st.m == -INFINITY ? 0.0f : -st.m;
   if (__builtin_amdgcn_ballot_w64(bump | is_huge(off))) {
@@ -99,7 +104,7 @@ __device__ __forceinline__ void softmax32(f16v_t (&c)[2], Rows32& st, float scal
     if (__builtin_amdgcn_ballot_w64(is_huge(off))) settle_huge32(c, off, scale);
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 2 * MT; ++e) {
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -114,12 +119,13 @@ __device__ __forceinline__ void softmax32(f16v_t (&c)[2], Rows32& st, float scal
 }
 
 // Adds the rounded weights to the row sums.
-__device__ __forceinline__ void sums32(Rows32& st, const bf16x8_t (&p)[4]) {
+template <int E>
+__device__ __forceinline__ void sums32(Rows32& st, const bf16x8_t (&p)[E]) {
   typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
   const bf2_t ones = __builtin_bit_cast(bf2_t, 0x3f803f80u);
   float sum = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < E; ++e) {
     const u4_t w = __builtin_bit_cast(u4_t, p[e]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -215,11 +221,12 @@ __device__ __forceinline__ void scores32(uint32_t k, const Rows32& st, f16v_t (&
 }
 
 // The weight of key `key` (of the tile) for the lane's row.
-__device__ __forceinline__ float weight32(const bf16x8_t (&p)[4], int key, int lane) {
+template <int E>
+__device__ __forceinline__ float weight32(const bf16x8_t (&p)[E], int key, int lane) {
   const int word = 2 * ((key >> 3) & 1) + ((key & 3) >> 1);
   uint32_t mine = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < E; ++e) {
     const u4_t w = __builtin_bit_cast(u4_t, p[e]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) mine = e == (key >> 4) && j == word ? w[j] : mine;

@@ -32,8 +32,8 @@ constexpr int BLOCK_COST = 4;  // of a block's start and end, in tiles
 constexpr int MIN_PART = 2;    // tiles of a block's part: nearer cuts move to the block's end
 constexpr int NO_WINDOW = 1 << 25;
 constexpr int FEW_WAVES = 4;
-constexpr int SHARE_MIN = 4;  // pages of a share of few rows: one per wave
-constexpr int SEQ_COST = 4;   // of starting on a sequence, in pages
+constexpr int SHARE_MIN = 4;  // half pages of a share of few rows: one per wave
+constexpr int SEQ_COST = 8;   // of starting on a sequence, in half pages
 
 struct ChunkArgs {
   const uint16_t* q;
@@ -187,8 +187,9 @@ __device__ __forceinline__ bool wild(float s, float z) { return !(fabsf(s) * 255
 
 // The wild groups of one V row (key `key` of a tile whose P is p, `rel` behind the lane's row, row `row` of the
 // pool), for the rows that see it: O^T took 0 in their place.
+template <int E>
 __device__ __forceinline__ void add_wild(const PagedBufs& buf, int64_t row, int key, int rel, Rows32& st, int lane,
-                                         const bf16x8_t (&p)[4], int window) {
+                                         const bf16x8_t (&p)[E], int window) {
   const float pk = weight32(p, key, lane);
   const bool sees = (uint32_t)rel < (uint32_t)window;
   const uint32_t sw = reinterpret_cast<const uint32_t*>(buf.vs)[row], zw = reinterpret_cast<const uint32_t*>(buf.vb)[row];
@@ -563,38 +564,41 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkArgs a) {
 }
 
 // ---- sequences of few rows (single tokens, verified blocks): up to 32 query rows per workgroup, all of them in
-// every wave, which takes a page at a time through LDS of its own (no barriers), dequantized on its way into the
-// matrix cores, the next page's loads out. What bounds these calls is reading the pages.
+// every wave, which takes half a page (32 keys) at a time through LDS of its own (no barriers), dequantized on its way
+// into the matrix cores, the next one's loads out. Reading the pages bounds long calls, a wave's way through a half
+// page short ones: with whole pages per wave, and two waves per SIMD for it instead of three, 1,024 positions of one
+// session took 15.1 us in one launch.
+constexpr int UNIT = 32;  // keys of a wave's step
 
 template <int WV>  // waves
 struct FewSmem {
-  // a wave's page: 16-byte chunk c of row r of K at c ^ kswz(r), of V at c ^ vfew(r); at the end its rows' values,
-  // 16-byte chunk c of row r at c ^ r
-  alignas(256) uint8_t page[WV][2][PAGE * D];
-  alignas(16) uint32_t w[WV][4][PAGE];  // its K scale, K bias, V scale, V bias words
-  uint4 q[8][64];               // the rows of q as B operands, a lane's place in each: not kept in registers
+  // a wave's keys: 16-byte chunk c of row r of K at c ^ kswz(r), of V at c ^ vfew(r); at the end 16 of its rows'
+  // values, 16-byte chunk c of row r at c ^ r
+  alignas(256) uint8_t codes[WV][2][UNIT * D];
+  alignas(16) float w[WV][4][2][UNIT];  // K scales, K biases, V scales, V biases of the two groups
+  uint4 q[8][64];                       // the rows of q as B operands, a lane's place in each
   float2 ml[WV][32];
 };
 // Rows of V that a transposed read takes together, 4 h + 8 i + r: in different banks.
 __device__ __forceinline__ int vfew(int r) { return (r & 3) | ((r >> 1) & 4); }
 
-// First page that the rows of a sequence see, and how many.
-struct Pages {
+// First unit that the rows of a sequence see, and how many.
+struct Units {
   int lo, n;
 };
-__device__ __forceinline__ Pages few_pages(const ChunkArgs& a, const Seq& q) {
-  const int lo = max(0, q.base - a.window + 1) / PAGE;
-  return {lo, q.len <= 0 ? 0 : (q.len + PAGE - 1) / PAGE - lo};
+__device__ __forceinline__ Units few_units(const ChunkArgs& a, const Seq& q) {
+  const int lo = max(0, q.base - a.window + 1) / UNIT;
+  return {lo, q.len <= 0 ? 0 : (q.len + UNIT - 1) / UNIT - lo};
 }
 __device__ __forceinline__ Deal few_deal(const ChunkArgs& a, int lane) {
   const Seq q = lane < a.nseq ? seq_of(a, lane) : Seq{0, 0, 0};
-  const int n = few_pages(a, q).n;
+  const int n = few_units(a, q).n;
   const int upto = wave_scan_i(n ? n + SEQ_COST : 0);
   const int total = __builtin_amdgcn_readlane(upto, 63);
   return {upto, q, total, max(SHARE_MIN, (total + a.shares - 1) / a.shares)};
 }
 
-// Pages [p0, p1) of sequence s for the rows of block rb: partial rows to slot .., or with WHOLE output rows.
+// Units [p0, p1) of sequence s for the rows of block rb: partial rows to slot .., or with WHOLE output rows.
 template <int WV, bool WHOLE>
 __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, int s, const Seq& sq, int rb, int hk,
                                          int p0, int p1, int64_t slot) {
@@ -603,13 +607,35 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
   const int lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 31, h = lane >> 5;
-  __syncthreads();  // the sequence before is written
+
+  const int32_t* ids = a.tab.ids + (int64_t)a.seq[s] * a.tab.stride;
+  u4_t rk[4], rv[4];
+  uint32_t kw, vw;  // of key ln: scale words (h == 0) or bias words of both groups
+  bool next_ok = true;
+  int64_t row_next = 0;
+  auto load = [&](int p) {
+    const int id = scalar(ids, p / (PAGE / UNIT));
+    next_ok = id >= 0 && id < a.tab.pages;
+    row_next = ((int64_t)(next_ok ? id : 0) * a.Hkv + hk) * PAGE + p % (PAGE / UNIT) * UNIT;
+    const u4_t* k = reinterpret_cast<const u4_t*>(a.buf.kc + row_next * D) + lane;
+    const u4_t* v = reinterpret_cast<const u4_t*>(a.buf.vc + row_next * D) + lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rk[i] = __builtin_nontemporal_load(k + 64 * i);
+    kw = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(h ? a.buf.kb : a.buf.ks) + row_next + ln);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rv[i] = __builtin_nontemporal_load(v + 64 * i);
+    vw = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(h ? a.buf.vb : a.buf.vs) + row_next + ln);
+  };
+  int p = p0 + wv;
+  if (p < p1) load(p);
+
   const float scale = abs_scale(a.sl2);
   const int f0 = 32 * rb, f = f0 + ln;
   const int i = (int)fdiv_u((uint32_t)min(f, sq.R - 1), a.g);
   const int head = min(f, sq.R - 1) - i * a.G;
   const int lim = f < sq.R ? sq.base + i : -1;
   const uint16_t* qr = a.q + (int64_t)(a.row0[s] + i) * a.q_tok + (hk * a.G + head) * a.q_head + 16 * h;
+  __syncthreads();  // the sequence before is written
   // q in K's order of dims: step 2 j + x holds dims 16 (2 j + h) + 8 x .. + 7
   for (int kk = wv; kk < 8; kk += WV)
     sm.q[kk][lane] = signed_q(*reinterpret_cast<const uint4*>(qr + 32 * (kk >> 1) + 8 * (kk & 1)), a.sl2);
@@ -617,142 +643,129 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
   st.clear();
   const int lim_lo = sq.base + (int)fdiv_u((uint32_t)f0, a.g);
   const int open_from = sq.base + (int)fdiv_u((uint32_t)min(f0 + 31, sq.R - 1), a.g) - a.window + 1;
-
-  const int32_t* ids = a.tab.ids + (int64_t)a.seq[s] * a.tab.stride;
-  uint8_t* const kp = sm.page[wv][0];
-  uint8_t* const vp = sm.page[wv][1];
-  PageRegs cur;
-  bool next_ok = true;
-  int64_t row_next = 0;
-  auto load = [&](int p) {
-    const int id = scalar(ids, p);
-    next_ok = id >= 0 && id < a.tab.pages;
-    row_next = ((int64_t)(next_ok ? id : 0) * a.Hkv + hk) * PAGE;
-    load_page(a.buf, row_next, lane, cur);
-  };
-  int p = p0 + wv;
-  if (p < p1) load(p);
+  uint8_t* const kp = sm.codes[wv][0];
+  uint8_t* const vp = sm.codes[wv][1];
   __syncthreads();  // q
   for (; p < p1; p += WV) {
     const int64_t row = row_next;
     const bool ok = next_ok;
-    const bool masked = PAGE * p + PAGE - 1 > lim_lo || PAGE * p < open_from;
+    const bool masked = UNIT * p + UNIT - 1 > lim_lo || UNIT * p < open_from;
     wave_fence();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int r = 8 * i + (lane >> 3), c = lane & 7;
-      reinterpret_cast<u4_t*>(kp)[8 * r + (c ^ kswz(r))] = cur.k[i];
-      reinterpret_cast<u4_t*>(vp)[8 * r + (c ^ vfew(r))] = cur.v[i];
+      reinterpret_cast<u4_t*>(kp)[8 * r + (c ^ kswz(r))] = rk[i];
+      reinterpret_cast<u4_t*>(vp)[8 * r + (c ^ vfew(r))] = rv[i];
     }
     // no V of positions that are not there, nor of those that are not finite where some row does not see them
-    const bool none = !ok || PAGE * p + lane >= sq.len;
+    const bool none = !ok || UNIT * p + ln >= sq.len;
     uint32_t keep = none ? 0u : 0xffffffffu;
     uint64_t wilds = 0;
     if (masked) {  // uniform
-      if (wild(bf16_lo(cur.w[2]), bf16_lo(cur.w[3]))) keep &= 0xffff0000u;
-      if (wild(bf16_hi(cur.w[2]), bf16_hi(cur.w[3]))) keep &= 0x0000ffffu;
-      wilds = __builtin_amdgcn_ballot_w64(!none && keep != 0xffffffffu);
+      const uint32_t other = __shfl_xor(vw, 32, 64), sw = h ? other : vw, zw = h ? vw : other;
+      if (wild(bf16_lo(sw), bf16_lo(zw))) keep &= 0xffff0000u;
+      if (wild(bf16_hi(sw), bf16_hi(zw))) keep &= 0x0000ffffu;
+      wilds = __builtin_amdgcn_ballot_w64(!none && keep != 0xffffffffu) & 0xffffffffu;
     }
-    sm.w[wv][0][lane] = ok ? cur.w[0] : 0x7fc07fc0u;
-    sm.w[wv][1][lane] = cur.w[1];
-    sm.w[wv][2][lane] = cur.w[2] & keep;
-    sm.w[wv][3][lane] = cur.w[3] & keep;
+    if (!ok && h == 0) kw = 0x7fc07fc0u;
+    sm.w[wv][h][0][ln] = bf16_lo(kw);
+    sm.w[wv][h][1][ln] = bf16_hi(kw);
+    sm.w[wv][2 + h][0][ln] = bf16_lo(vw & keep);
+    sm.w[wv][2 + h][1][ln] = bf16_hi(vw & keep);
     if (p + WV < p1) load(p + WV);
     wave_fence();
     // scores
-    f16v_t c[2];
+    f16v_t c[1];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+    for (int i = 0; i < 16; ++i) c[0][i] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) c[mt][i] = 0.0f;
-      const int key = 32 * mt + ln;
-      const uint32_t sw = sm.w[wv][0][key], zw = sm.w[wv][1][key];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float s = j < 2 ? bf16_lo(sw) : bf16_hi(sw), z = j < 2 ? bf16_lo(zw) : bf16_hi(zw);
-        const u4_t w = reinterpret_cast<const u4_t*>(kp)[8 * key + ((2 * j + h) ^ kswz(key))];
-        const uint2 d0 = dequant4(w[0], s, z), d1 = dequant4(w[1], s, z);
-        const uint2 d2 = dequant4(w[2], s, z), d3 = dequant4(w[3], s, z);
-        c[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d0.x, d0.y, d1.x, d1.y),
-                                                        u4_as_bf8(sm.q[2 * j][lane]), c[mt], 0, 0, 0);
-        c[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d2.x, d2.y, d3.x, d3.y),
-                                                        u4_as_bf8(sm.q[2 * j + 1][lane]), c[mt], 0, 0, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+    for (int j = 0; j < 4; ++j) {
+      const float sc = sm.w[wv][0][j >> 1][ln], z = sm.w[wv][1][j >> 1][ln];
+      const u4_t w = reinterpret_cast<const u4_t*>(kp)[8 * ln + ((2 * j + h) ^ kswz(ln))];
+      const uint2 d0 = dequant4(w[0], sc, z), d1 = dequant4(w[1], sc, z);
+      const uint2 d2 = dequant4(w[2], sc, z), d3 = dequant4(w[3], sc, z);
+      c[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d0.x, d0.y, d1.x, d1.y),
+                                                     u4_as_bf8(sm.q[2 * j][lane]), c[0], 0, 0, 0);
+      c[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d2.x, d2.y, d3.x, d3.y),
+                                                     u4_as_bf8(sm.q[2 * j + 1][lane]), c[0], 0, 0, 0);
     }
-    if (masked) {  // uniform
-      mask32(c, lim - PAGE * p - 4 * h, a.window);
-    }
-    bf16x8_t pr[4];
+    if (masked) mask32(c, lim - UNIT * p - 4 * h, a.window);  // uniform
+    bf16x8_t pr[2];
     softmax32(c, st, scale, pr);
     sums32(st, pr);
     // values: of keys 16 e + 8 (j / 4) + 4 h + j % 4, j < 8, this lane's dim of each window of 32
     const int r8 = (lane >> 1) & 7, src = 4 * h + 8 * (r8 >> 2) + (r8 & 3);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint4 s0 = *reinterpret_cast<const uint4*>(&sm.w[wv][2][16 * e + 4 * h]);
-      const uint4 s1 = *reinterpret_cast<const uint4*>(&sm.w[wv][2][16 * e + 8 + 4 * h]);
-      const uint4 z0 = *reinterpret_cast<const uint4*>(&sm.w[wv][3][16 * e + 4 * h]);
-      const uint4 z1 = *reinterpret_cast<const uint4*>(&sm.w[wv][3][16 * e + 8 + 4 * h]);
-      const uint32_t sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-      const uint32_t zw[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int chunk = 2 * w + ((lane >> 4) & 1);
-        const v2i_t raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (lds_v2i_t*)(vp + (16 * e + src) * D + 16 * (chunk ^ vfew(src)) + 8 * (lane & 1)));
-        float v[8];
+      for (int g = 0; g < 2; ++g) {
+        float sc[8], z[8];
+        *reinterpret_cast<f4_t*>(sc) = *reinterpret_cast<const f4_t*>(&sm.w[wv][2][g][16 * e + 4 * h]);
+        *reinterpret_cast<f4_t*>(sc + 4) = *reinterpret_cast<const f4_t*>(&sm.w[wv][2][g][16 * e + 8 + 4 * h]);
+        *reinterpret_cast<f4_t*>(z) = *reinterpret_cast<const f4_t*>(&sm.w[wv][3][g][16 * e + 4 * h]);
+        *reinterpret_cast<f4_t*>(z + 4) = *reinterpret_cast<const f4_t*>(&sm.w[wv][3][g][16 * e + 8 + 4 * h]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float s = w < 2 ? bf16_lo(sw[j]) : bf16_hi(sw[j]), z = w < 2 ? bf16_lo(zw[j]) : bf16_hi(zw[j]);
-          v[j] = fmaf(s, (float)(((uint32_t)(j < 4 ? raw.x : raw.y) >> (8 * (j & 3))) & 0xffu), z);
+        for (int w = 2 * g; w < 2 * g + 2; ++w) {
+          const int chunk = 2 * w + ((lane >> 4) & 1);
+          const v2i_t raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (lds_v2i_t*)(vp + (16 * e + src) * D + 16 * (chunk ^ vfew(src)) + 8 * (lane & 1)));
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            v[j] = fmaf(sc[j], (float)(((uint32_t)(j < 4 ? raw.x : raw.y) >> (8 * (j & 3))) & 0xffu), z[j]);
+          st.o[w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              words_as_bf8(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])),
+              pr[e], st.o[w], 0, 0, 0);
         }
-        st.o[w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            words_as_bf8(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])), pr[e],
-            st.o[w], 0, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
     for (; wilds; wilds &= wilds - 1) {  // rare
       const int key = __builtin_ctzll(wilds);
-      add_wild(a.buf, row + key, key, lim - PAGE * p - key, st, lane, pr, a.window);
+      add_wild(a.buf, row + key, key, lim - UNIT * p - key, st, lane, pr, a.window);
     }
   }
 
-  // ---- the waves' rows meet in LDS
-  wave_fence();
-  f4_t* acc = reinterpret_cast<f4_t*>(sm.page[wv]);
-  st.l = sum_xor32(st.l);
-#pragma unroll
-  for (int w = 0; w < 4; ++w)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      acc[32 * ln + ((8 * w + 2 * j + h) ^ ln)] = f4_t{st.o[w][4 * j], st.o[w][4 * j + 1], st.o[w][4 * j + 2], st.o[w][4 * j + 3]};
-  if (h == 0) sm.ml[wv][ln] = make_float2(st.m, st.l);
-  __syncthreads();
+  // ---- the waves' rows meet in LDS, 16 at a time
   const int R = min(32, sq.R - f0);
-  for (int x = tid; x < 32 * R; x += 64 * WV) {
-    const int r = x >> 5, ch = x & 31;
-    float M = -INFINITY, L = 0.0f;
-    f4_t o = {0.f, 0.f, 0.f, 0.f};
+  f4_t* acc = reinterpret_cast<f4_t*>(sm.codes[wv]);
+  st.l = sum_xor32(st.l);
+  if (h == 0) sm.ml[wv][ln] = make_float2(st.m, st.l);
 #pragma unroll
-    for (int w = 0; w < WV; ++w) M = max_ieee(M, sm.ml[w][r].x);
-    const float Mr = M == -INFINITY ? 0.0f : M;
+  for (int part = 0; part < 2; ++part) {
+    if (16 * part >= R) break;  // uniform
+    if (part) __syncthreads();  // the 16 before are read
+    wave_fence();
+    if (ln >> 4 == part) {
 #pragma unroll
-    for (int w = 0; w < WV; ++w) {
-      const float2 ml = sm.ml[w][r];
-      const float e = exp2_nonpos(ml.x - Mr);  // of no keys: 0, and a sum that is NaN stays
-      o += reinterpret_cast<const f4_t*>(sm.page[w])[32 * r + (ch ^ r)] * e;
-      L += ml.y * e;
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[32 * (ln & 15) + ((8 * w + 2 * j + h) ^ (ln & 15))] =
+              f4_t{st.o[w][4 * j], st.o[w][4 * j + 1], st.o[w][4 * j + 2], st.o[w][4 * j + 3]};
     }
-    if constexpr (WHOLE) {
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      const int p = (int)fdiv_u((uint32_t)(f0 + r), a.g), head = f0 + r - p * a.G;
-      *reinterpret_cast<uint2*>(a.out + ((int64_t)(a.row0[s] + p) * a.Hkv * a.G + hk * a.G + head) * D + 4 * ch) =
-          make_uint2(pack_bf2(o[0] * inv, o[1] * inv), pack_bf2(o[2] * inv, o[3] * inv));
-    } else {
-      *reinterpret_cast<f4_t*>(a.part_acc + (slot + r) * D + 4 * ch) = o;
-      if (ch == 0) a.part_ml[slot + r] = make_float2(M, L);
+    __syncthreads();
+    for (int x = tid; x < 32 * min(16, R - 16 * part); x += 64 * WV) {
+      const int r = x >> 5, ch = x & 31, row = 16 * part + r;
+      float M = -INFINITY, L = 0.0f;
+      f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WV; ++w) M = max_ieee(M, sm.ml[w][row].x);
+      const float Mr = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+      for (int w = 0; w < WV; ++w) {
+        const float2 ml = sm.ml[w][row];
+        const float e = exp2_nonpos(ml.x - Mr);  // of no keys: 0, and a sum that is NaN stays
+        o += reinterpret_cast<const f4_t*>(sm.codes[w])[32 * r + (ch ^ r)] * e;
+        L += ml.y * e;
+      }
+      if constexpr (WHOLE) {
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        const int q = (int)fdiv_u((uint32_t)(f0 + row), a.g), head = f0 + row - q * a.G;
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(a.row0[s] + q) * a.Hkv * a.G + hk * a.G + head) * D + 4 * ch) =
+            make_uint2(pack_bf2(o[0] * inv, o[1] * inv), pack_bf2(o[2] * inv, o[3] * inv));
+      } else {
+        *reinterpret_cast<f4_t*>(a.part_acc + (slot + row) * D + 4 * ch) = o;
+        if (ch == 0) a.part_ml[slot + row] = make_float2(M, L);
+      }
     }
   }
 }
@@ -762,7 +775,7 @@ __device__ __forceinline__ int64_t few_slot(const ChunkArgs& a, int hk, int rb, 
   return ((int64_t)(hk * a.blocks + rb) * (a.shares + a.nseq) + x) * 32;
 }
 
-// A share of the sequences' pages, dealt out one sequence behind the other.
+// A share of the sequences' half pages, dealt out one sequence behind the other.
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void few_kernel(const ChunkArgs a) {
   __shared__ FewSmem<FEW_WAVES> sm;
   const int hk = blockIdx.x % a.Hkv, y = blockIdx.x / a.Hkv, x = y / a.blocks, rb = y - x * a.blocks;
@@ -774,7 +787,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void few_kernel(const ChunkArgs 
   int begin = s ? __builtin_amdgcn_readlane(deal.upto, s - 1) : 0;
   for (int u = u0; u < u1; ++s) {
     const Seq sq = seq_at(deal, s);
-    const Pages pg = few_pages(a, sq);
+    const Units pg = few_units(a, sq);
     if (pg.n == 0) continue;
     begin += SEQ_COST;
     const int p0 = max(u - begin, 0), p1 = min(u1 - begin, pg.n);
@@ -798,7 +811,7 @@ __global__ __launch_bounds__(64 * WV, 2) void few_whole_kernel(const ChunkArgs a
     }
     return;
   }
-  const Pages pg = few_pages(a, sq);
+  const Units pg = few_units(a, sq);
   if (R > 0) few_part<WV, true>(a, sm, s, sq, rb, hk, pg.lo, pg.lo + pg.n, 0);
 }
 
@@ -814,7 +827,7 @@ __global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
   const int per = 32 * a.blocks, y = row / per, f = row - y * per, s = min(y / a.Hkv, a.nseq - 1), hk = y % a.Hkv;
   const Deal deal = few_deal(a, lane);
   const Seq sq = seq_at(deal, s);
-  const int pages = few_pages(a, sq).n;
+  const int pages = few_units(a, sq).n;
   const int before = (s ? __builtin_amdgcn_readlane(deal.upto, s - 1) : 0) + SEQ_COST;
   const int first = before / deal.share;
   const bool mine = f < sq.R;
@@ -924,16 +937,18 @@ int launch_many(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
   return LQ_OK;
 }
 
-// A call of few pages per sequence takes each whole.
-constexpr int64_t WHOLE_PAGES = 16;
+// Calls of few pages per sequence take each whole: one launch, nothing to merge. Many sequences also where they are
+// longer. us, dealt out / whole: 1 session of 512 positions, 8 KV heads 9.9 / 9.5, of 1,024 10.0 / 13.6; 8 of 1,500
+// 16.4 / 20.3, 16 windows of 1,100 20.6 / 17.6, 32 of 1,500 32.1 / 24.3, 64 of 100 to 1,500 39.1 / 33.2.
+constexpr int64_t WHOLE_PAGES = 16, WHOLE_PAGES_MANY = 32;
 int launch_few(const ChunkArgs& a, const ChunkPart& c, int64_t window, hipStream_t st) {
   int rows = 0;
   for (int s = 0; s < c.nseq; ++s) rows = std::max(rows, c.rows[s]);
   // pages that rows at `rows` positions see of a window each
   const int64_t seen = window == 0 ? a.tab.width : std::min<int64_t>(a.tab.width, (window + rows - 2 + PAGE - 1) / PAGE + 1);
-  if (seen <= WHOLE_PAGES) {
-    const int64_t wgs = (int64_t)c.nseq * c.blocks * a.Hkv;
-    if (wgs <= device_cu_count())
+  const int64_t wgs = (int64_t)c.nseq * c.blocks * a.Hkv, cus = device_cu_count();
+  if (seen <= (2 * wgs >= cus ? WHOLE_PAGES_MANY : WHOLE_PAGES)) {
+    if (wgs <= cus)
       few_whole_kernel<8><<<dim3((unsigned)wgs), dim3(512), 0, st>>>(a);
     else
       few_whole_kernel<4><<<dim3((unsigned)wgs), dim3(256), 0, st>>>(a);
@@ -987,7 +1002,7 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
   int64_t most = 0;  // cost, if every block sees the whole table
   for (int s = 0; s < plan.many.nseq; ++s)
     most += (plan.many.rows[s] * G + plan.many.rows_of - 1) / plan.many.rows_of * (table_width + lq::BLOCK_COST);
-  most = std::max<int64_t>(most, plan.few.nseq * (table_width + lq::SEQ_COST));
+  most = std::max<int64_t>(most, plan.few.nseq * (2 * table_width + lq::SEQ_COST));
   LQ_CHECK_ARG(most < (1ll << 31) - (1 << 20), "too many rows for table rows of %lld pages", (long long)table_width);
   const int64_t need = chunk_bytes(plan);
   if (need > 0 && (!workspace || workspace_bytes < need)) {
