@@ -871,7 +871,11 @@ struct ChunkPart {  // the sequences of few rows, or of many
 struct ChunkPlan {
   ChunkPart few, many;
 };
-constexpr int64_t FEW_ROWS = 32;
+// Up to FEW_ROWS query rows of a sequence and KV head go as blocks of 32 that read the pages each, from the L2 but
+// the first, more as blocks that share a dequantized page. us, shared / each, 8 KV heads: 36 rows behind 20,000 positions
+// 54 / 27, 64 behind 65,536 87 / 60, 96 behind 5,000 27 / 22, 48 of 16 sessions of 100 to 4,100 44 / 45, 96 of 4 of
+// 9,000 51 / 53, 126 behind 65,536 90 / more.
+constexpr int64_t FEW_ROWS = 96;
 constexpr int64_t WHOLE_ROUNDS = 6, SMALL_ROUNDS = 3;
 ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G, int cus) {
   ChunkPlan p{};
@@ -899,7 +903,7 @@ ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G
   p.many.slots = p.many.nseq ? 2 * p.many.shares * Hkv * p.many.rows_of : 0;
   p.few.rows_of = 32;
   p.few.blocks = (int)((few + 31) / 32);
-  p.few.shares = (int)std::max<int64_t>(1, 2 * cus / Hkv);
+  p.few.shares = (int)std::max<int64_t>(1, 2 * cus / (Hkv * std::max(1, p.few.blocks)));
   p.few.slots = Hkv * p.few.blocks * (int64_t)(p.few.shares + p.few.nseq) * 32;
   return p;
 }
