@@ -456,9 +456,10 @@ int lq_paged_decode_attn(const uint16_t* q, const uint8_t* kc, const uint16_t* k
  * see one of its positions.
  *   q bf16: row t of head h at q + t q_tok + h q_head (elements; strides multiples of 8, rows 16-byte
  *   aligned); out bf16 [rows, Hq, 128] contiguous. Hq / Hkv <= 64.
- * Workspace: lq_paged_chunk_workspace_bytes, any contents; calls that may overlap need their own.
+ * Workspace: lq_paged_chunk_workspace_bytes (0 for many calls), any contents; calls that may overlap need their own.
  */
-int64_t lq_paged_chunk_workspace_bytes(const int32_t* counts_host, int64_t nseq, int64_t Hq, int64_t Hkv);
+int64_t lq_paged_chunk_workspace_bytes(const int32_t* counts_host, int64_t nseq, int64_t Hq, int64_t Hkv,
+                                       int64_t table_width, int64_t window);
 int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_head, const uint8_t* kc,
                         const uint16_t* ks, const uint16_t* kb, const uint8_t* vc, const uint16_t* vs,
                         const uint16_t* vb, int64_t pages, int64_t Hq, int64_t Hkv, int64_t D,

@@ -78,7 +78,7 @@ SIGNATURES = {
     "lq_paged_decode_workspace_bytes": (i64, [i64, i64, i64, i64]),
     "lq_paged_decode_attn": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, i64, i64, vp,
                                    i64, f32, vp, vp, i64, vp]),
-    "lq_paged_chunk_workspace_bytes": (i64, [vp, i64, i64, i64]),
+    "lq_paged_chunk_workspace_bytes": (i64, [vp, i64, i64, i64, i64, i64]),
     "lq_paged_chunk_attn": (i32, [vp, i64, i64, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp, i64, i64, vp,
                                   vp, i64, i64, f32, vp, vp, i64, vp]),
     "lq_prompt_workspace_bytes": (i64, [vp, vp, i64, i64, i64]),

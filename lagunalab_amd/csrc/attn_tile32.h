@@ -210,13 +210,22 @@ __device__ __forceinline__ void matrix32(uint32_t k, uint32_t v, Rows32& st, f16
 }
 // Raw scores of one tile.
 __device__ __forceinline__ void scores32(uint32_t k, const Rows32& st, f16v_t (&c)[2]) {
+  Ahead32 a;
+  ahead32(k, a);
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt) {
+  for (int u = 0; u < 8; ++u) {
+    if (u + AHEAD < 8) fetch32(k, 0, u + AHEAD, a.f[(u + AHEAD) % (AHEAD + 1)]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) c[mt][i] = 0.0f;
+    for (int j = 0; j < 2; ++j) {
+      f16v_t z;
+      if (u == 0) {
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk)
-      c[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_operand32(k, mt, kk), st.q[kk], c[mt], 0, 0, 0);
+        for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+      }
+      c[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f[u % (AHEAD + 1)][j], st.q[u], u == 0 ? z : c[j], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 

@@ -243,84 +243,123 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
   constexpr int C = 8 / PW;  // 16-byte chunks of K (of V) that a thread brings per tile
   __shared__ ChunkSmem<STAGES> sm;
   const int share = blockIdx.x / a.Hkv, hk = blockIdx.x - share * a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool grp_a = HALVES && wv < PW / 2;
+  const int ln = lane & 31, h = lane >> 5;
+  const float scale = abs_scale(a.sl2);
   int u0 = 0, u1;
   Block b;
   if (a.shares) {
-    const Deal deal = deal_out<ROWS>(a, threadIdx.x & 63);
+    const Deal deal = deal_out<ROWS>(a, lane);
     u0 = deal.share * share;
     u1 = min(u0 + deal.share, deal.total);
     if (u0 >= u1) return;
-    b = find_block<ROWS>(a, deal, u0, threadIdx.x & 63);
+    b = find_block<ROWS>(a, deal, u0, lane);
   } else {  // a whole block
-    b = ranked_block<ROWS>(a, share, threadIdx.x & 63);
+    b = ranked_block<ROWS>(a, share, lane);
     u1 = b.tiles + BLOCK_COST;
   }
-  for (bool more = true; more;) {
-    // re-read per block, so that no lane value made of it is kept across blocks
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & 63;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const bool grp_a = HALVES && wv < PW / 2;
-    const int ln = lane & 31, h = lane >> 5;
-    const Seq sq = b.q;
-    const int q0 = a.row0[b.seq];
-    const int c0 = cut_tile(b, u0), c1 = cut_tile(b, u1);
-    const int t0 = b.lo + c0, t1 = b.lo + c1;
+
+  // ---- a tile: thread tid brings 16 codes (chunk tid % 8) of key tid / 8 (and + 8 PW)
+  const int key0 = tid >> 3, chunk = tid & 7;
+  const uint32_t group = chunk < 4 ? SEL_LO : SEL_HI;  // of the thread's codes
+  int c0, c1, t0, t1;  // the share's tiles of the block, from its own first and from the sequence's
+  bool mine;
+  const int32_t* ids;
+  u4_t rk[C], rv[C], fk[C];
+  uint32_t ks[C], kb[C], vs[C], vb[C], fs[C], fb[C];  // words of both groups
+  // whether there are such pages, and their rows: of the K loaded last, of the one before it, the V loaded last, the
+  // K loaded next; the first
+  bool k_ok, before_ok, v_ok, next_ok, f_ok;
+  int64_t row_k, row_before, row_next;
+  int id_next;
+  auto load_codes = [&](const uint8_t* codes, int64_t row, u4_t (&c)[C]) {
+    const global_ptr<uint8_t> cp = uniform(codes + row * D);
+    const uint32_t o = lane_offset(16u * tid);
+#pragma unroll
+    for (int i = 0; i < C; ++i) c[i] = *(global_ptr<u4_t>)(cp + (o + 1024 * PW * i));
+  };
+  auto load_words = [&](const uint16_t* words, int64_t row, uint32_t (&w)[C]) {
+    const global_ptr<uint8_t> p = uniform(reinterpret_cast<const uint8_t*>(words + 2 * row));
+    const uint32_t o = lane_offset(4u * key0);
+#pragma unroll
+    for (int i = 0; i < C; ++i) w[i] = *(global_ptr<uint32_t>)(p + (o + 32 * PW * i));
+  };
+  // K of the tiles in order, V of each one behind
+  auto next_row = [&](int t) {  // of tile t, behind the last loaded
+    next_ok = id_next >= 0 && id_next < a.tab.pages;
+    row_next = ((int64_t)(next_ok ? id_next : 0) * a.Hkv + hk) * PAGE;
+    id_next = scalar(ids, min(t + 1, t1 - 1));
+  };
+  auto load_k = [&]() {
+    row_before = row_k;
+    before_ok = k_ok;
+    row_k = row_next;
+    k_ok = next_ok;
+    load_codes(a.buf.kc, row_k, rk);
+    load_words(a.buf.ks, row_k, ks);
+    load_words(a.buf.kb, row_k, kb);
+  };
+  auto load_v = [&]() {
+    v_ok = before_ok;
+    load_codes(a.buf.vc, row_before, rv);
+    load_words(a.buf.vs, row_before, vs);
+    load_words(a.buf.vb, row_before, vb);
+  };
+
+  // ---- a block: the wave's rows, and its first loads, out before the rows of the block before are written: the
+  // first tile's K, the second's and the first's V
+  int f, i, head;
+  Rows32 st;
+  auto open = [&]() {
+    c0 = cut_tile(b, u0);
+    c1 = cut_tile(b, u1);
+    t0 = b.lo + c0;
+    t1 = b.lo + c1;
     // a block without a tile (rows without keys) belongs to the share that its begin lies in
-    const bool mine = c0 < c1 || (b.tiles == 0 && b.begin >= u0 && b.begin < u1);
+    mine = c0 < c1 || (b.tiles == 0 && b.begin >= u0 && b.begin < u1);
+    if (!mine) return;
+    ids = a.tab.ids + (int64_t)a.seq[b.seq] * a.tab.stride;
+    if (t0 < t1) {
+      k_ok = before_ok = true;
+      row_k = row_before = 0;
+      id_next = scalar(ids, t0);
+      next_row(t0);
+      load_k();
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        fk[i] = rk[i];
+        fs[i] = ks[i];
+        fb[i] = kb[i];
+      }
+      f_ok = k_ok;
+      next_row(t0 + 1);
+      load_k();
+      load_v();
+      next_row(t0 + 2);
+    }
+    f = b.blk * ROWS + 32 * wv + ln;
+    i = (int)fdiv_u((uint32_t)min(f, b.q.R - 1), a.g);
+    head = min(f, b.q.R - 1) - i * a.G;
+    const uint16_t* qr = a.q + (int64_t)(a.row0[b.seq] + i) * a.q_tok + (hk * a.G + head) * a.q_head + 8 * h;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) st.q[kk] = u4_as_bf8(*reinterpret_cast<const uint4*>(qr + 16 * kk));
+  };
+  open();
+
+  for (bool more = true; more;) {
+    const Seq sq = b.q;
+    uint16_t* out = nullptr;  // the lane's row, or its part
+    float* part_acc = nullptr;
+    float2* part_ml = nullptr;
+    float inv = 0.0f;
     if (mine) {
-      const float scale = abs_scale(a.sl2);
       // tiles in [t_open, t_masked) are open to all rows of the block
       const int first = sq.base + (int)fdiv_u((uint32_t)(b.blk * ROWS), a.g);
       const int last = sq.base + (int)fdiv_u((uint32_t)min(b.blk * ROWS + ROWS - 1, sq.R - 1), a.g);
       const int t_masked = first < 0 ? 0 : (first + 1) / TKEYS;
       const int t_open = (max(0, last - a.window + 1) + TKEYS - 1) / TKEYS;
-
-      // ---- a tile: thread tid brings 16 codes (chunk tid % 8) of key tid / 8 (and + 8 PW)
-      const int32_t* ids = a.tab.ids + (int64_t)a.seq[b.seq] * a.tab.stride;
-      const int key0 = tid >> 3, chunk = tid & 7;
-      u4_t rk[C], rv[C];
-      uint32_t ks[C], kb[C], vs[C], vb[C];  // words of both groups
-      // whether there are such pages, and their rows: of the K loaded last, of the one before it, the V loaded last,
-      // the K loaded next
-      bool k_ok = true, before_ok = true, v_ok = true, next_ok = true;
-      int64_t row_k = 0, row_before = 0, row_next = 0;
-      int id_next = t0 < t1 ? scalar(ids, t0) : 0;
-      const uint32_t group = chunk < 4 ? SEL_LO : SEL_HI;  // of the thread's codes
-      auto load_codes = [&](const uint8_t* codes, int64_t row, u4_t (&c)[C]) {
-        const global_ptr<uint8_t> cp = uniform(codes + row * D);
-        const uint32_t o = lane_offset(16u * tid);
-#pragma unroll
-        for (int i = 0; i < C; ++i) c[i] = *(global_ptr<u4_t>)(cp + (o + 1024 * PW * i));
-      };
-      auto load_words = [&](const uint16_t* words, int64_t row, uint32_t (&w)[C]) {
-        const global_ptr<uint8_t> p = uniform(reinterpret_cast<const uint8_t*>(words + 2 * row));
-        const uint32_t o = lane_offset(4u * key0);
-#pragma unroll
-        for (int i = 0; i < C; ++i) w[i] = *(global_ptr<uint32_t>)(p + (o + 32 * PW * i));
-      };
-      // K of the tiles in order, V of each one behind
-      auto next_row = [&](int t) {  // of tile t, behind the last loaded
-        next_ok = id_next >= 0 && id_next < a.tab.pages;
-        row_next = ((int64_t)(next_ok ? id_next : 0) * a.Hkv + hk) * PAGE;
-        id_next = scalar(ids, min(t + 1, t1 - 1));
-      };
-      auto load_k = [&]() {
-        row_before = row_k;
-        before_ok = k_ok;
-        row_k = row_next;
-        k_ok = next_ok;
-        load_codes(a.buf.kc, row_k, rk);
-        load_words(a.buf.ks, row_k, ks);
-        load_words(a.buf.kb, row_k, kb);
-      };
-      auto load_v = [&]() {
-        v_ok = before_ok;
-        load_codes(a.buf.vc, row_before, rv);
-        load_words(a.buf.vs, row_before, vs);
-        load_words(a.buf.vb, row_before, vb);
-      };
       auto put = [&](uint4* lo, uint4* hi, u4_t c, float s, float z) {
         const uint2 d0 = dequant4(c.x, s, z), d1 = dequant4(c.y, s, z);
         const uint2 d2 = dequant4(c.z, s, z), d3 = dequant4(c.w, s, z);
@@ -333,7 +372,8 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           const int key = key0 + 8 * PW * i;
-          put(k_chunk(to, key, 2 * chunk), k_chunk(to, key, 2 * chunk + 1), rk[i], bf16_pick(k_ok ? ks[i] : 0x7fc07fc0u, group), bf16_pick(kb[i], group));
+          put(k_chunk(to, key, 2 * chunk), k_chunk(to, key, 2 * chunk + 1), rk[i],
+              bf16_pick(k_ok ? ks[i] : 0x7fc07fc0u, group), bf16_pick(kb[i], group));
         }
       };
       // V of tile t (of no tile behind the last: its place is free) in steps: its words settled, then a chunk's halves.
@@ -363,47 +403,22 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
         }
       };
 
-      // the first tile's K, the second's and the first's V are all out before any is waited for
-      u4_t fk[C];
-      uint32_t fs[C], fb[C];
-      bool f_ok = true;
-      if (t0 < t1) {
-        next_row(t0);
-        load_k();
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-          fk[i] = rk[i];
-          fs[i] = ks[i];
-          fb[i] = kb[i];
-        }
-        f_ok = k_ok;
-        next_row(t0 + 1);
-        load_k();
-        load_v();
-        next_row(t0 + 2);
-      }
-
-      // ---- the wave's rows
-      const int f0 = b.blk * ROWS + 32 * wv, f = f0 + ln;
-      const int i = (int)fdiv_u((uint32_t)min(f, sq.R - 1), a.g);
-      const int head = min(f, sq.R - 1) - i * a.G;
+      const int f0 = b.blk * ROWS + 32 * wv;
       const int lim = f < sq.R ? sq.base + i : -1;  // last key of the lane's row, below 0: none
-      const uint16_t* qr = a.q + (int64_t)(q0 + i) * a.q_tok + (hk * a.G + head) * a.q_head + 8 * h;
-      Rows32 st;
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-        st.q[kk] = u4_as_bf8(signed_q(*reinterpret_cast<const uint4*>(qr + 16 * kk), a.sl2));
-      st.clear();
       // keys up to here, and from there on, are seen by all of the wave's rows
       const int lim_lo = f0 < sq.R ? sq.base + (int)fdiv_u((uint32_t)f0, a.g) : -1;
       const int open_from =
           f0 < sq.R ? sq.base + (int)fdiv_u((uint32_t)min(f0 + 31, sq.R - 1), a.g) - a.window + 1 : 0;
-
       f16v_t c[2];
       bf16x8_t p[4];
       const uint32_t k_at = k_lane32(sm.tile[0], lane), v_at = v_lane32(sm.tile[0], lane);
       auto tile_at = [](int t) { return (uint32_t)(t % STAGES) * (uint32_t)sizeof(KvTile); };
       lds_barrier();  // the block before is done with LDS
+      if (a.sl2 < 0.0f) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) st.q[kk] = u4_as_bf8(signed_q(__builtin_bit_cast(uint4, st.q[kk]), a.sl2));
+      }
+      st.clear();
       if (t0 < t1) {
         if (tid < 6) sm.wild[tid >> 1][tid & 1] = 0;
         stage_k(t0, fk, fs, fb, f_ok);
@@ -470,31 +485,17 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
       }
 
       // ---- rows out: dims 32 w + 8 j + 4 h ..
-      const bool part = c1 - c0 < b.tiles;
       st.l = sum_xor32(st.l);
-      if (f < sq.R) {
-        if (part) {
-          const int64_t pr = ((int64_t)(2 * share + (c0 == 0)) * a.Hkv + hk) * ROWS + 32 * wv + ln;
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<f4_t*>(a.part_acc + pr * D + 32 * w + 8 * j + 4 * h) =
-                  f4_t{st.o[w][4 * j], st.o[w][4 * j + 1], st.o[w][4 * j + 2], st.o[w][4 * j + 3]};
-          if (h == 0) a.part_ml[pr] = make_float2(st.m, st.l);
-        } else {
-          uint16_t* o = a.out + ((int64_t)(q0 + i) * a.Hkv * a.G + hk * a.G + head) * D + 4 * h;
-          const float inv = sq.len < 0 ? NAN : st.l == 0.0f ? 0.0f : 1.0f / st.l;
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<uint2*>(o + 32 * w + 8 * j) =
-                  make_uint2(pack_bf2(st.o[w][4 * j] * inv, st.o[w][4 * j + 1] * inv),
-                             pack_bf2(st.o[w][4 * j + 2] * inv, st.o[w][4 * j + 3] * inv));
-        }
+      if (c1 - c0 < b.tiles) {
+        const int64_t pr = ((int64_t)(2 * share + (c0 == 0)) * a.Hkv + hk) * ROWS + 32 * wv + ln;
+        part_acc = a.part_acc + pr * D;
+        part_ml = a.part_ml + pr;
+      } else {
+        out = a.out + ((int64_t)(a.row0[b.seq] + i) * a.Hkv * a.G + hk * a.G + head) * D;
+        inv = sq.len < 0 ? NAN : st.l == 0.0f ? 0.0f : 1.0f / st.l;
       }
     }
+    const bool write = mine && f < sq.R;
     // the next block
     const int next = b.begin + b.tiles + BLOCK_COST;
     more = next < u1;
@@ -508,6 +509,32 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
       const int blk = block_at(place, (b.q.R + ROWS - 1) / ROWS);
       const Span sp = block_span<ROWS>(a, b.q, blk);
       b = Block{ns, blk, sp.lo, sp.n, next, place, b.q};
+      open();
+    }
+    if (part_acc) {  // uniform, as out
+      if (write) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<f4_t*>(part_acc + 32 * w + 8 * j + 4 * h) =
+                f4_t{st.o[w][4 * j], st.o[w][4 * j + 1], st.o[w][4 * j + 2], st.o[w][4 * j + 3]};
+        if (h == 0) *part_ml = make_float2(st.m, st.l);
+      }
+    } else if (out) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          // dims 8 j .. of the lower lanes' rows and 8 (j + 1) .. of the upper ones' come together: 16 bytes each
+          const auto lo = __builtin_amdgcn_permlane32_swap(pack_bf2(st.o[w][4 * j] * inv, st.o[w][4 * j + 1] * inv),
+                                                           pack_bf2(st.o[w][4 * j + 4] * inv, st.o[w][4 * j + 5] * inv),
+                                                           false, false);
+          const auto hi = __builtin_amdgcn_permlane32_swap(pack_bf2(st.o[w][4 * j + 2] * inv, st.o[w][4 * j + 3] * inv),
+                                                           pack_bf2(st.o[w][4 * j + 6] * inv, st.o[w][4 * j + 7] * inv),
+                                                           false, false);
+          if (write) *reinterpret_cast<uint4*>(out + 32 * w + 8 * (j + h)) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+        }
     }
   }
 }
@@ -866,7 +893,7 @@ __global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
 struct ChunkPart {  // the sequences of few rows, or of many
   int nseq, rows_of, shares, blocks;  // rows of a block, shares (0: whole blocks) and blocks per KV head
   int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];
-  int64_t slots;  // partial rows, all heads
+  int64_t slots;  // partial rows, all heads; 0: no parts
 };
 struct ChunkPlan {
   ChunkPart few, many;
@@ -877,7 +904,12 @@ struct ChunkPlan {
 // 9,000 51 / 53, 126 behind 65,536 90 / more.
 constexpr int64_t FEW_ROWS = 96;
 constexpr int64_t WHOLE_ROUNDS = 6, SMALL_ROUNDS = 3;
-ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G, int cus) {
+// Calls of few pages per sequence take each whole: one launch, nothing to merge. Many sequences also where they are
+// longer. us on the GPU, dealt out / whole: 1 session of 512 positions, 8 KV heads 9.9 / 9.5, of 1,038 10.0 / 13.8 (with
+// the host, whose launches bound such a call, 16.3 / 14); 8 of 1,500
+// 16.4 / 20.3, 16 windows of 1,100 20.6 / 17.6, 32 of 1,500 32.1 / 24.3, 64 of 100 to 1,500 39.1 / 33.2.
+constexpr int64_t WHOLE_PAGES = 20, WHOLE_PAGES_MANY = 32;
+ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G, int64_t width, int64_t window, int cus) {
   ChunkPlan p{};
   int at = 0;
   int64_t most = 0, few = 0;  // query rows of a sequence
@@ -903,15 +935,22 @@ ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G
   p.many.slots = p.many.nseq ? 2 * p.many.shares * Hkv * p.many.rows_of : 0;
   p.few.rows_of = 32;
   p.few.blocks = (int)((few + 31) / 32);
-  p.few.shares = (int)std::max<int64_t>(1, 2 * cus / (Hkv * std::max(1, p.few.blocks)));
-  p.few.slots = Hkv * p.few.blocks * (int64_t)(p.few.shares + p.few.nseq) * 32;
+  const int64_t wgs = p.few.nseq * p.few.blocks * Hkv;
+  int rows = 0;
+  for (int s = 0; s < p.few.nseq; ++s) rows = std::max(rows, p.few.rows[s]);
+  // pages that `rows` rows of a sequence see, a window each
+  const int64_t seen = window == 0 ? width : std::min(width, (window + rows - 2 + PAGE - 1) / PAGE + 1);
+  if (seen > (2 * wgs >= cus ? WHOLE_PAGES_MANY : WHOLE_PAGES)) {
+    p.few.shares = (int)std::max<int64_t>(1, 2 * cus / (Hkv * std::max(1, p.few.blocks)));
+    p.few.slots = Hkv * p.few.blocks * (int64_t)(p.few.shares + p.few.nseq) * 32;
+  }
   return p;
 }
 int64_t chunk_bytes(const ChunkPlan& p) {
   return std::max(p.few.slots, p.many.slots) * (int64_t)(D * sizeof(float) + sizeof(float2));
 }
 
-int check_chunk(int64_t Hq, int64_t Hkv, const int32_t* counts, int64_t nseq) {
+int check_chunk(int64_t Hq, int64_t Hkv, const int32_t* counts, int64_t nseq, int64_t width, int64_t window) {
   LQ_CHECK_ARG(Hkv >= 1 && Hkv <= 1024 && Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= 64,
                "Hq=%lld must be 1 to 64 times Hkv=%lld", (long long)Hq, (long long)Hkv);
   LQ_CHECK_ARG(nseq >= 1 && nseq <= LQ_MAX_SEQS && counts, "%lld sequences are not in [1, %d], or no counts",
@@ -923,6 +962,8 @@ int check_chunk(int64_t Hq, int64_t Hkv, const int32_t* counts, int64_t nseq) {
     rows += counts[s];
   }
   LQ_CHECK_ARG(rows < (1 << 30), "too many rows");
+  LQ_CHECK_ARG(width >= 1 && window >= 0 && window < ((int64_t)1 << 40), "a window of %lld positions, or table rows of %lld pages",
+               (long long)window, (long long)width);
   return LQ_OK;
 }
 
@@ -941,18 +982,10 @@ int launch_many(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
   return LQ_OK;
 }
 
-// Calls of few pages per sequence take each whole: one launch, nothing to merge. Many sequences also where they are
-// longer. us, dealt out / whole: 1 session of 512 positions, 8 KV heads 9.9 / 9.5, of 1,024 10.0 / 13.6; 8 of 1,500
-// 16.4 / 20.3, 16 windows of 1,100 20.6 / 17.6, 32 of 1,500 32.1 / 24.3, 64 of 100 to 1,500 39.1 / 33.2.
-constexpr int64_t WHOLE_PAGES = 16, WHOLE_PAGES_MANY = 32;
-int launch_few(const ChunkArgs& a, const ChunkPart& c, int64_t window, hipStream_t st) {
-  int rows = 0;
-  for (int s = 0; s < c.nseq; ++s) rows = std::max(rows, c.rows[s]);
-  // pages that rows at `rows` positions see of a window each
-  const int64_t seen = window == 0 ? a.tab.width : std::min<int64_t>(a.tab.width, (window + rows - 2 + PAGE - 1) / PAGE + 1);
-  const int64_t wgs = (int64_t)c.nseq * c.blocks * a.Hkv, cus = device_cu_count();
-  if (seen <= (2 * wgs >= cus ? WHOLE_PAGES_MANY : WHOLE_PAGES)) {
-    if (wgs <= cus)
+int launch_few(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
+  if (a.shares == 0) {
+    const int64_t wgs = (int64_t)c.nseq * c.blocks * a.Hkv;
+    if (wgs <= device_cu_count())
       few_whole_kernel<8><<<dim3((unsigned)wgs), dim3(512), 0, st>>>(a);
     else
       few_whole_kernel<4><<<dim3((unsigned)wgs), dim3(256), 0, st>>>(a);
@@ -973,11 +1006,12 @@ int launch_few(const ChunkArgs& a, const ChunkPart& c, int64_t window, hipStream
 }  // namespace
 }  // namespace lq
 
-extern "C" int64_t lq_paged_chunk_workspace_bytes(const int32_t* counts_host, int64_t nseq, int64_t Hq, int64_t Hkv) {
+extern "C" int64_t lq_paged_chunk_workspace_bytes(const int32_t* counts_host, int64_t nseq, int64_t Hq, int64_t Hkv,
+                                                  int64_t table_width, int64_t window) {
   using namespace lq;
   clear_error();
-  if (check_chunk(Hq, Hkv, counts_host, nseq)) return -1;
-  return chunk_bytes(chunk_plan(counts_host, nseq, Hkv, Hq / Hkv, device_cu_count()));
+  if (check_chunk(Hq, Hkv, counts_host, nseq, table_width, window)) return -1;
+  return chunk_bytes(chunk_plan(counts_host, nseq, Hkv, Hq / Hkv, table_width, window, device_cu_count()));
 }
 
 extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_head, const uint8_t* kc,
@@ -994,11 +1028,10 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
            const_cast<uint8_t*>(vc), const_cast<uint16_t*>(vs), const_cast<uint16_t*>(vb)};
   a.tab = {table, table_stride, (int)table_width, (int)pages};
   if (const int st = check_pool(a.buf, a.tab, table_stride, table_width, pages, Hkv, D)) return st;
-  if (const int st = check_chunk(Hq, Hkv, counts_host, nseq)) return st;
-  LQ_CHECK_ARG(window >= 0, "a window of %lld positions", (long long)window);
+  if (const int st = check_chunk(Hq, Hkv, counts_host, nseq, table_width, window)) return st;
   LQ_CHECK_ARG(std::isfinite(scale), "the softmax scale is not finite");
   const int64_t G = Hq / Hkv;
-  const ChunkPlan plan = chunk_plan(counts_host, nseq, Hkv, G, device_cu_count());
+  const ChunkPlan plan = chunk_plan(counts_host, nseq, Hkv, G, table_width, window, device_cu_count());
   if (plan.few.nseq + plan.many.nseq == 0) return LQ_OK;
   LQ_CHECK_ARG(q && lens && out, "null pointer");
   LQ_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0 && ((q_tok | q_head) & 7) == 0,
@@ -1037,7 +1070,7 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
     std::copy(c->seq, c->seq + LQ_MAX_SEQS, a.seq);
     std::copy(c->row0, c->row0 + LQ_MAX_SEQS, a.row0);
     std::copy(c->rows, c->rows + LQ_MAX_SEQS, a.rows);
-    const int status = c == &plan.many ? launch_many(a, *c, st) : launch_few(a, *c, window, st);
+    const int status = c == &plan.many ? launch_many(a, *c, st) : launch_few(a, *c, st);
     if (status) return status;
   }
   return LQ_OK;

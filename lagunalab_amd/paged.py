@@ -50,8 +50,8 @@ def _pool(keys, values):
     if len(keys) != 3 or len(values) != 3:
         raise ValueError("a pool's keys and values are (codes, scales, biases)")
     codes = keys[0]
-    at, shape = codes.get_device(), codes.shape
-    P, H = shape[:2]
+    at = codes.get_device()
+    P, H = codes.shape[:2]
     wide, narrow = (P, H, PAGE, HEAD_DIM), (P, H, PAGE, HEAD_DIM // 64)
     ptrs = []
     for buf in (keys, values):
@@ -102,6 +102,13 @@ def _counts(counts, B):
     return counts
 
 
+def _even(T, B):
+    """As many of T rows for each of B sequences."""
+    if B == 0 or T % B:
+        raise ValueError(f"{T} rows are not the same number for each of {B} sequences")
+    return [T // B] * B
+
+
 def _rows(x, T, H, what):
     """Rows [T, H, 128] as the kernels read them: bf16, any token and head strides of 16-byte steps."""
     if x.dtype != torch.bfloat16 or x.shape != (T, H, HEAD_DIM):
@@ -117,6 +124,13 @@ def _launches(counts):
     """The sequences of a call in launches of at most LQ_MAX_SEQS: (first, how many, rows before, its
     counts' address)."""
     at, ptr = 0, counts.buffer_info()[0]
+    if len(counts) <= _lib.LQ_MAX_SEQS:
+        return ((0, len(counts), 0, ptr),) if counts else ()
+    return _many_launches(counts, ptr)
+
+
+def _many_launches(counts, ptr):
+    at = 0
     for a in range(0, len(counts), _lib.LQ_MAX_SEQS):
         n = min(len(counts) - a, _lib.LQ_MAX_SEQS)
         yield a, n, at, ptr + 4 * a
@@ -131,11 +145,7 @@ def paged_append(k, v, keys, values, table, starts, counts=None):
     exist are not stored; no two rows may go to one slot."""
     P, H, dev, ptrs = _pool(keys, values)
     B, T = _length(table), k.shape[0]
-    if counts is None:
-        if B == 0 or T % B:
-            raise ValueError(f"{T} rows are not the same number for each of {B} sequences")
-        counts = [T // B] * B
-    counts = _counts(counts, B)
+    counts = _counts(_even(T, B) if counts is None else counts, B)
     if sum(counts) != T:
         raise ValueError(f"counts add up to {sum(counts)}, not to the {T} rows")
     _lib.require_device(k, v, keys[0])
@@ -174,41 +184,35 @@ def paged_append_rotated(q, k, v, keys, values, table, starts, rotary, counts=No
     and take angles in fp32, off by up to 0.004 radians at 82,671 positions.)"""
     P, H, dev, ptrs = _pool(keys, values)
     B, T = _length(table), k.shape[0]
-    if counts is None:
-        if B == 0 or T % B:
-            raise ValueError(f"{T} rows are not the same number for each of {B} sequences")
-        counts = [T // B] * B
-    counts = _counts(counts, B)
+    counts = _counts(_even(T, B) if counts is None else counts, B)
     if sum(counts) != T:
         raise ValueError(f"counts add up to {sum(counts)}, not to the {T} rows")
-    _lib.require_device(q, k, v, keys[0], q_norm, k_norm)
+    freq = rotary.inv_freq if rotary is not None else None
+    _lib.require_device(q, k, v, keys[0], q_norm, k_norm, freq)
     _refuse_grad(q, k, v, *(w for w in (q_norm, k_norm) if w is not None))
     Hq = q.shape[1] if q.dim() == 3 else -1
     q, qt, qh = _rows(q, T, Hq, "q")
     k, kt, kh = _rows(k, T, H, "k")
     v, vt, vh = _rows(v, T, H, "v")
     q_norm, k_norm = _norm_weight(q_norm, "q_norm"), _norm_weight(k_norm, "k_norm")
-    freq, dims, mscale, pairs = None, 0, 1.0, False
-    if rotary is not None:
-        freq, dims, mscale, pairs = rotary.inv_freq, rotary.dims, rotary.mscale, rotary.interleaved
-        _lib.require_device(freq, keys[0])
+    rope = (None, 0, 1.0, False) if freq is None else (freq.data_ptr(), rotary.dims, rotary.mscale,
+                                                       rotary.interleaved)
     table, ts, width = _table(table, B, dev)
     starts = _ints(starts, B, "starts", dev)
-    out = torch.empty((T, Hq, HEAD_DIM), dtype=torch.bfloat16, device=dev)
-    got = torch.empty((2, T, H, HEAD_DIM), dtype=torch.bfloat16, device=dev) if fetch else None
+    out = q.new_empty((T, Hq, HEAD_DIM))
+    got = q.new_empty((2, T, H, HEAD_DIM)) if fetch else None
     qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     gp = got.data_ptr() if fetch else None
     tp, sp = table.data_ptr(), starts.data_ptr()
-    lib = _lib.load()
+    run = _lib.load().lq_paged_append_rotated
     with _lib.on_device(dev):
         for a, n, at, cp in _launches(counts):
             g = 2 * at * H * HEAD_DIM
-            _lib.check(lib.lq_paged_append_rotated(
+            _lib.check(run(
                 qp + 2 * at * qt, kp + 2 * at * kt, vp + 2 * at * vt, qt, qh, kt, kh, vt, vh, _lib.ptr(q_norm),
-                _lib.ptr(k_norm), eps, _lib.ptr(freq), dims, mscale, pairs, *ptrs, P, Hq, H, HEAD_DIM,
-                tp + 4 * a * ts, ts, width, sp + 4 * a, cp, n, op + 2 * at * Hq * HEAD_DIM,
-                gp + g if fetch else None, gp + g + 2 * T * H * HEAD_DIM if fetch else None,
-                _lib.raw_stream(dev)), "lq_paged_append_rotated")
+                _lib.ptr(k_norm), eps, *rope, *ptrs, P, Hq, H, HEAD_DIM, tp + 4 * a * ts, ts, width, sp + 4 * a, cp, n,
+                op + 2 * at * Hq * HEAD_DIM, gp + g if fetch else None,
+                gp + g + 2 * T * H * HEAD_DIM if fetch else None, _lib.raw_stream(dev)), "lq_paged_append_rotated")
     return (out, *got.unbind()) if fetch else out
 
 
@@ -293,11 +297,7 @@ def paged_chunk_attention(q, keys, values, table, lens, scale, counts=None, wind
     if q.dim() != 3:
         raise ValueError(f"q must be bfloat16 [T, Hq, {HEAD_DIM}], got {tuple(q.shape)}")
     T, Hq = q.shape[:2]
-    if counts is None:
-        if B == 0 or T % B:
-            raise ValueError(f"{T} rows are not the same number for each of {B} sequences")
-        counts = [T // B] * B
-    counts = _counts(counts, B)
+    counts = _counts(_even(T, B) if counts is None else counts, B)
     if sum(counts) != T:
         raise ValueError(f"counts add up to {sum(counts)}, not to the {T} rows")
     if window is not None and window < 1:
@@ -309,18 +309,19 @@ def paged_chunk_attention(q, keys, values, table, lens, scale, counts=None, wind
         raise ValueError(f"{Hq} query heads are not 1 to 64 per KV head ({H})")
     table, ts, width = _table(table, B, dev)
     lens = _ints(lens, B, "lens", dev)
-    out = torch.empty((T, Hq, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    out = q.new_empty((T, Hq, HEAD_DIM))
+    qp, op, tp, np = q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr()
+    seen = window or 0
     lib = _lib.load()
     with _lib.on_device(dev):
         for a, n, at, cp in _launches(counts):
-            need = lib.lq_paged_chunk_workspace_bytes(cp, n, Hq, H)
+            need = lib.lq_paged_chunk_workspace_bytes(cp, n, Hq, H, width, seen)
             if need < 0:
                 _lib.check(_lib.LQ_EINVAL, "lq_paged_chunk_workspace_bytes")
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = keys[0].new_empty(need) if need else None
             _lib.check(lib.lq_paged_chunk_attn(
-                q.data_ptr() + 2 * at * qt, qt, qh, *ptrs, P, Hq, H, HEAD_DIM, table.data_ptr() + 4 * a * ts, ts, width,
-                lens.data_ptr() + 4 * a, cp, n, window or 0, scale, out.data_ptr() + 2 * at * Hq * HEAD_DIM,
-                ws.data_ptr(), need, _lib.raw_stream(dev)), "lq_paged_chunk_attn")
+                qp + 2 * at * qt, qt, qh, *ptrs, P, Hq, H, HEAD_DIM, tp + 4 * a * ts, ts, width, np + 4 * a, cp, n, seen,
+                scale, op + 2 * at * Hq * HEAD_DIM, _lib.ptr(ws), need, _lib.raw_stream(dev)), "lq_paged_chunk_attn")
     return out
 
 

@@ -14,7 +14,7 @@ class Rotary:
     inv_freq[i]`` radians (fp32, on the device) and is scaled by ``mscale``. Pairs are dims ``i`` and ``i +
     len(inv_freq)``, or with ``interleaved`` dims ``2 i`` and ``2 i + 1``; the other dims stay."""
 
-    __slots__ = ("inv_freq", "mscale", "interleaved")
+    __slots__ = ("inv_freq", "dims", "mscale", "interleaved")
 
     def __init__(self, inv_freq: torch.Tensor, mscale: float = 1.0, interleaved: bool = False):
         if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
@@ -22,14 +22,10 @@ class Rotary:
         if not math.isfinite(mscale):
             raise ValueError(f"a factor of {mscale}")
         self.inv_freq, self.mscale, self.interleaved = inv_freq.contiguous(), float(mscale), bool(interleaved)
+        self.dims = 2 * inv_freq.shape[0]  # rotated dims of a head
 
     @classmethod
     def of(cls, params: dict, device="cuda", interleaved: bool = False, head_dim: int = 128) -> "Rotary":
         """Of a rope config, as :func:`lagunalab_amd.attention.rope_frequencies` reads it."""
         inv_freq, _, mscale = rope_frequencies(head_dim, params)
         return cls(inv_freq.to(device), mscale, interleaved)
-
-    @property
-    def dims(self) -> int:
-        """Rotated dims of a head."""
-        return 2 * self.inv_freq.shape[0]

@@ -297,7 +297,7 @@ def test_nothing_behind_the_outputs_is_touched(dev):
         pool, table = sessions(g, kv, lens, dev)
         q = randn(g, T, hq, D).to(dev)
         cn = (C.c_int32 * len(counts))(*counts)
-        need = lib.lq_paged_chunk_workspace_bytes(cn, len(counts), hq, kv)
+        need = lib.lq_paged_chunk_workspace_bytes(cn, len(counts), hq, kv, table.shape[1], 0)
         ws = torch.full((need + 4096,), 0xA5, dtype=torch.uint8, device=dev)
         out = torch.full((T + 8, hq, D), 7.0, dtype=torch.bfloat16, device=dev)
         t_d, n_d = table.to(dev), ints(lens, dev)
