@@ -903,11 +903,19 @@ struct ChunkPlan {
 // 54 / 27, 64 behind 65,536 87 / 60, 96 behind 5,000 27 / 22, 48 of 16 sessions of 100 to 4,100 44 / 45, 96 of 4 of
 // 9,000 51 / 53, 126 behind 65,536 90 / more.
 constexpr int64_t FEW_ROWS = 96;
-constexpr int64_t WHOLE_ROUNDS = 6, SMALL_ROUNDS = 3;
+// Blocks of many rows are taken whole, a workgroup each and the longest first, where that leaves few compute units
+// idle: IDLE_TILES per block, were all blocks as long as the table (or window) lets them be. Else the call is dealt out
+// in shares, which end together but write, merge and start on parts. How the lengths differ is not known here, and one
+// long block among short ones would be waited for: whole blocks have at most LONGEST tiles, or those that the rows see
+// of each other alone keep the other workgroups busy for as long. us, shares / whole, 48/8 heads: 2,048 rows of a window
+// of 512 66.8 / 57.4, of 4,096 240 / 263, 1,024 behind 1,000 68.4 / 67.5, behind 8,000 235 / 258, 7 prompts of up to
+// 4,099 653 / 623, 24 chunks of up to 300 rows behind up to 5,985 365 / 348 (in shares all the same); 32/8 heads: 5
+// prompts of up to 2,049 rows 123 / 103, 4 of 500 38 / 27, one of 5,000 254 / 244, 64 of 400 220 / 234.
+constexpr int64_t IDLE_TILES = 8, LONGEST = 40;
 // Calls of few pages per sequence take each whole: one launch, nothing to merge. Many sequences also where they are
 // longer. us on the GPU, dealt out / whole: 1 session of 512 positions, 8 KV heads 9.9 / 9.5, of 1,038 10.0 / 13.8 (with
-// the host, whose launches bound such a call, 16.3 / 14); 8 of 1,500
-// 16.4 / 20.3, 16 windows of 1,100 20.6 / 17.6, 32 of 1,500 32.1 / 24.3, 64 of 100 to 1,500 39.1 / 33.2.
+// the host, whose launches bound such a call, 16.3 / 14); 8 of 1,500 16.4 / 20.3, 16 windows of 1,100 20.6 / 17.6, 32
+// of 1,500 32.1 / 24.3, 64 of 100 to 1,500 39.1 / 33.2.
 constexpr int64_t WHOLE_PAGES = 20, WHOLE_PAGES_MANY = 32;
 ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G, int64_t width, int64_t window, int cus) {
   ChunkPlan p{};
@@ -924,23 +932,28 @@ ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G
     }
     at += counts[s];
   }
-  int64_t blocks[2] = {0, 0};  // of 128 and of 256 rows
-  for (int s = 0; s < p.many.nseq; ++s)
-    for (int i = 0; i < 2; ++i) blocks[i] += (p.many.rows[s] * G + (128 << i) - 1) / (128 << i);
-  const bool large = blocks[1] * Hkv >= WHOLE_ROUNDS * cus;
-  const bool small = !large && blocks[0] * Hkv >= SMALL_ROUNDS * cus;
-  p.many.rows_of = !small && most > 128 ? 256 : 128;
-  p.many.blocks = (int)blocks[!small && most > 128];
-  p.many.shares = large || small ? 0 : (int)std::max<int64_t>(1, (p.many.rows_of == 256 ? 1 : 2) * cus / Hkv);
+  // pages that a window lets n positions see
+  auto seen = [&](int64_t n) { return window == 0 ? width : std::min(width, (window + n - 2 + PAGE - 1) / PAGE + 1); };
+  p.many.rows_of = most > 128 ? 256 : 128;
+  int64_t blocks = 0, own = 0;  // tiles that a KV head's rows see of each other
+  for (int s = 0; s < p.many.nseq; ++s) {
+    const int64_t n = (p.many.rows[s] * G + p.many.rows_of - 1) / p.many.rows_of;
+    blocks += n;
+    own += n * std::min<int64_t>(seen(1), p.many.rows[s] / (2 * PAGE));
+  }
+  p.many.blocks = (int)std::min<int64_t>(blocks, INT32_MAX);
+  const int64_t slots = p.many.rows_of == 256 ? cus : 2 * cus;  // workgroups at a time
+  const int64_t idle = (slots - blocks * Hkv % slots) % slots;
+  const int64_t tiles = seen(p.many.rows_of / G + 1);
+  if (idle * tiles > IDLE_TILES * blocks * Hkv || tiles > std::max(LONGEST, own * Hkv / slots))
+    p.many.shares = (int)std::max<int64_t>(1, slots / Hkv);
   p.many.slots = p.many.nseq ? 2 * p.many.shares * Hkv * p.many.rows_of : 0;
   p.few.rows_of = 32;
   p.few.blocks = (int)((few + 31) / 32);
   const int64_t wgs = p.few.nseq * p.few.blocks * Hkv;
   int rows = 0;
   for (int s = 0; s < p.few.nseq; ++s) rows = std::max(rows, p.few.rows[s]);
-  // pages that `rows` rows of a sequence see, a window each
-  const int64_t seen = window == 0 ? width : std::min(width, (window + rows - 2 + PAGE - 1) / PAGE + 1);
-  if (seen > (2 * wgs >= cus ? WHOLE_PAGES_MANY : WHOLE_PAGES)) {
+  if (seen(rows) > (2 * wgs >= cus ? WHOLE_PAGES_MANY : WHOLE_PAGES)) {
     p.few.shares = (int)std::max<int64_t>(1, 2 * cus / (Hkv * std::max(1, p.few.blocks)));
     p.few.slots = Hkv * p.few.blocks * (int64_t)(p.few.shares + p.few.nseq) * 32;
   }
@@ -1036,6 +1049,7 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
   LQ_CHECK_ARG(q && lens && out, "null pointer");
   LQ_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0 && ((q_tok | q_head) & 7) == 0,
                "rows must be 16-byte aligned (strides a multiple of 8)");
+  LQ_CHECK_ARG((int64_t)plan.many.blocks * Hkv <= 1 << 22, "too many rows");  // workgroups of a launch
   int64_t most = 0;  // cost, if every block sees the whole table
   for (int s = 0; s < plan.many.nseq; ++s)
     most += (plan.many.rows[s] * G + plan.many.rows_of - 1) / plan.many.rows_of * (table_width + lq::BLOCK_COST);
