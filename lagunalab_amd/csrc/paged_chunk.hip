@@ -625,8 +625,10 @@ __device__ __forceinline__ Deal few_deal(const ChunkArgs& a, int lane) {
   return {upto, q, total, max(SHARE_MIN, (total + a.shares - 1) / a.shares)};
 }
 
-// Units [p0, p1) of sequence s for the rows of block rb: partial rows to slot .., or with WHOLE output rows.
-template <int WV, bool WHOLE>
+// Units [p0, p1) of sequence s for the rows of block rb: partial rows to slot .., or with WHOLE output rows. AGAIN: the
+// other blocks read the pages too, and they stay in the L2 (streaming / staying, us: 48 rows of 16 sessions of 100 to
+// 4,100 positions 42.6 / 39.2; of one block 64 single tokens of up to 8,200 118 / 124).
+template <int WV, bool WHOLE, bool AGAIN>
 __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, int s, const Seq& sq, int rb, int hk,
                                          int p0, int p1, int64_t slot) {
   int tid = threadIdx.x;  // re-read, so that no lane value made of it is kept across sequences
@@ -640,6 +642,12 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
   uint32_t kw, vw;  // of key ln: scale words (h == 0) or bias words of both groups
   bool next_ok = true;
   int64_t row_next = 0;
+  auto read = [](const auto* from) {
+    if constexpr (AGAIN)
+      return *from;
+    else
+      return __builtin_nontemporal_load(from);
+  };
   auto load = [&](int p) {
     const int id = scalar(ids, p / (PAGE / UNIT));
     next_ok = id >= 0 && id < a.tab.pages;
@@ -647,11 +655,11 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
     const u4_t* k = reinterpret_cast<const u4_t*>(a.buf.kc + row_next * D) + lane;
     const u4_t* v = reinterpret_cast<const u4_t*>(a.buf.vc + row_next * D) + lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) rk[i] = __builtin_nontemporal_load(k + 64 * i);
-    kw = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(h ? a.buf.kb : a.buf.ks) + row_next + ln);
+    for (int i = 0; i < 4; ++i) rk[i] = read(k + 64 * i);
+    kw = read(reinterpret_cast<const uint32_t*>(h ? a.buf.kb : a.buf.ks) + row_next + ln);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) rv[i] = __builtin_nontemporal_load(v + 64 * i);
-    vw = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(h ? a.buf.vb : a.buf.vs) + row_next + ln);
+    for (int i = 0; i < 4; ++i) rv[i] = read(v + 64 * i);
+    vw = read(reinterpret_cast<const uint32_t*>(h ? a.buf.vb : a.buf.vs) + row_next + ln);
   };
   int p = p0 + wv;
   if (p < p1) load(p);
@@ -803,6 +811,7 @@ __device__ __forceinline__ int64_t few_slot(const ChunkArgs& a, int hk, int rb, 
 }
 
 // A share of the sequences' half pages, dealt out one sequence behind the other.
+template <bool AGAIN>
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void few_kernel(const ChunkArgs a) {
   __shared__ FewSmem<FEW_WAVES> sm;
   const int hk = blockIdx.x % a.Hkv, y = blockIdx.x / a.Hkv, x = y / a.blocks, rb = y - x * a.blocks;
@@ -818,14 +827,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void few_kernel(const ChunkArgs 
     if (pg.n == 0) continue;
     begin += SEQ_COST;
     const int p0 = max(u - begin, 0), p1 = min(u1 - begin, pg.n);
-    if (p0 < p1 && 32 * rb < sq.R) few_part<FEW_WAVES, false>(a, sm, s, sq, rb, hk, pg.lo + p0, pg.lo + p1, few_slot(a, hk, rb, x + s));
+    if (p0 < p1 && 32 * rb < sq.R)
+      few_part<FEW_WAVES, false, AGAIN>(a, sm, s, sq, rb, hk, pg.lo + p0, pg.lo + p1, few_slot(a, hk, rb, x + s));
     begin += pg.n;
     u = begin;
   }
 }
 
 // A whole sequence per workgroup: nothing to merge.
-template <int WV>
+template <int WV, bool AGAIN>
 __global__ __launch_bounds__(64 * WV, 2) void few_whole_kernel(const ChunkArgs a) {
   __shared__ FewSmem<WV> sm;
   const int hk = blockIdx.x % a.Hkv, y = blockIdx.x / a.Hkv, s = y / a.blocks, rb = y - s * a.blocks;
@@ -839,7 +849,7 @@ __global__ __launch_bounds__(64 * WV, 2) void few_whole_kernel(const ChunkArgs a
     return;
   }
   const Units pg = few_units(a, sq);
-  if (R > 0) few_part<WV, true>(a, sm, s, sq, rb, hk, pg.lo, pg.lo + pg.n, 0);
+  if (R > 0) few_part<WV, true, AGAIN>(a, sm, s, sq, rb, hk, pg.lo, pg.lo + pg.n, 0);
 }
 
 // An output row by GR groups of 32 lanes (4 dims each), 8 / GR rows per workgroup: group g takes every GR-th
@@ -998,14 +1008,15 @@ int launch_many(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
 int launch_few(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
   if (a.shares == 0) {
     const int64_t wgs = (int64_t)c.nseq * c.blocks * a.Hkv;
-    if (wgs <= device_cu_count())
-      few_whole_kernel<8><<<dim3((unsigned)wgs), dim3(512), 0, st>>>(a);
-    else
-      few_whole_kernel<4><<<dim3((unsigned)wgs), dim3(256), 0, st>>>(a);
+    const bool wide = wgs <= device_cu_count();
+    auto* whole = c.blocks > 1 ? wide ? few_whole_kernel<8, true> : few_whole_kernel<4, true>
+                               : wide ? few_whole_kernel<8, false> : few_whole_kernel<4, false>;
+    whole<<<dim3((unsigned)wgs), dim3(wide ? 512 : 256), 0, st>>>(a);
     LQ_CHECK_LAUNCH("few_whole_kernel");
     return LQ_OK;
   }
-  few_kernel<<<dim3((unsigned)(a.shares * c.blocks * a.Hkv)), dim3(64 * FEW_WAVES), 0, st>>>(a);
+  auto* few = c.blocks > 1 ? few_kernel<true> : few_kernel<false>;
+  few<<<dim3((unsigned)(a.shares * c.blocks * a.Hkv)), dim3(64 * FEW_WAVES), 0, st>>>(a);
   LQ_CHECK_LAUNCH("few_kernel");
   const int64_t n = (int64_t)c.nseq * a.Hkv * 32 * c.blocks;
   if (a.shares / std::min(c.nseq, 4) > 16)
