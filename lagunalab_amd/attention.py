@@ -13,6 +13,8 @@ mlx-lm's SDPA routes it), SDPA over the returned K/V otherwise, then the softplu
 * ``lq_qkv_norm_rope``: the projection taken apart, the q and k RMSNorms and the rotary embedding
   of both in one launch
   (frequencies from :func:`rope_frequencies`: mlx-lm's default or YaRN RoPE, partial rotary);
+* in place of that launch, over a cache that ``rotates`` (a paged batch of sessions at positions of their own):
+  the cache's ``append_rotated``, which does it on the way into the pages;
 * the cache: the fused decode / verify kernels, or dequantized K/V for the unfused path;
 * ``lq_gate_heads_strided``: softplus gate times the attention output, written in ``o_proj``'s layout.
 
@@ -188,6 +190,8 @@ class Attention:
         self.k_norm = k_norm.to(device=dev, dtype=torch.bfloat16).contiguous()
         inv, self.rot_dims, self.mscale = rope_frequencies(head_dim, rope)
         self.inv_freq = inv.to(dev)
+        from .rotary import Rotary
+        self.rotary = Rotary(self.inv_freq, self.mscale)
         H, Hkv, D = n_heads, n_kv_heads, head_dim
         self._splits = [H * D, Hkv * D, Hkv * D, wg.shape[0]]
 
@@ -199,17 +203,21 @@ class Attention:
         x = x.to(torch.bfloat16)
         proj = linear(x, self.w_in)  # [B, L, (H + 2 Hkv) D + gate]
         N = proj.shape[-1]
-        q = torch.empty((B, H, L, D), dtype=torch.bfloat16, device=dev)
-        k = torch.empty((B, Hkv, L, D), dtype=torch.bfloat16, device=dev)
-        v = torch.empty((B, Hkv, L, D), dtype=torch.bfloat16, device=dev)
-        offset = cache.offset if cache is not None else 0
-        _lib.check(lib.lq_qkv_norm_rope(proj.data_ptr(), N, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                        self.q_norm.data_ptr(), self.k_norm.data_ptr(), B, H, Hkv,
-                                        L, D, self.eps, self.inv_freq.data_ptr(), self.rot_dims,
-                                        self.mscale, int(offset), _lib.stream_ptr(dev)),
-                   "lq_qkv_norm_rope")
-        if cache is not None:
-            k, v = cache.update_and_fetch(k, v)
+        if getattr(cache, "rotates", False):
+            q, k, v = proj[..., :(H + 2 * Hkv) * D].unflatten(-1, (-1, D)).split([H, Hkv, Hkv], dim=2)
+            q = cache.append_rotated(q, k, v, self.rotary, self.q_norm, self.k_norm, self.eps)
+        else:
+            q = torch.empty((B, H, L, D), dtype=torch.bfloat16, device=dev)
+            k = torch.empty((B, Hkv, L, D), dtype=torch.bfloat16, device=dev)
+            v = torch.empty((B, Hkv, L, D), dtype=torch.bfloat16, device=dev)
+            offset = cache.offset if cache is not None else 0
+            _lib.check(lib.lq_qkv_norm_rope(proj.data_ptr(), N, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                            self.q_norm.data_ptr(), self.k_norm.data_ptr(), B, H, Hkv,
+                                            L, D, self.eps, self.inv_freq.data_ptr(), self.rot_dims,
+                                            self.mscale, int(offset), _lib.stream_ptr(dev)),
+                       "lq_qkv_norm_rope")
+            if cache is not None:
+                k, v = cache.update_and_fetch(k, v)
         if getattr(cache, "fused_step", False):
             out = cache.attend(q, self.scale)
         elif hasattr(cache, "bits"):  # quantized_decode step: packed K/V, quantized attention

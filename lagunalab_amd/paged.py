@@ -189,7 +189,7 @@ def paged_append_rotated(q, k, v, keys, values, table, starts, rotary, counts=No
         raise ValueError(f"counts add up to {sum(counts)}, not to the {T} rows")
     freq = rotary.inv_freq if rotary is not None else None
     _lib.require_device(q, k, v, keys[0], q_norm, k_norm, freq)
-    _refuse_grad(q, k, v, *(w for w in (q_norm, k_norm) if w is not None))
+    _refuse_grad(q, k, v, *(w for w in (q_norm, k_norm, freq) if w is not None), what="append")
     Hq = q.shape[1] if q.dim() == 3 else -1
     q, qt, qh = _rows(q, T, Hq, "q")
     k, kt, kh = _rows(k, T, H, "k")
@@ -545,13 +545,8 @@ class PagedKVCache:
                 n = next(i for i in range(n) if pages[i] != first[i])
         return n * PAGE
 
-    def append(self, sessions, k, v, counts=None):
-        """Appends rows ``k``, ``v`` (bf16 ``[T, Hkv, 128]``, packed one session behind the other,
-        ``counts[i]`` each or as many each) to the sessions."""
-        self._outside_graphs()
-        sessions, states = self._distinct(sessions)
-        if not states:
-            return
+    def _new_rows(self, states, k, v, counts):
+        """Host counts of checked rows."""
         T = k.shape[0]
         if counts is None:
             if T % len(states):
@@ -564,16 +559,42 @@ class PagedKVCache:
         if not k.dtype == v.dtype == torch.bfloat16:
             raise ValueError(f"K/V rows must be bfloat16, got {k.dtype} and {v.dtype}")
         _lib.require_device(k, v, self.keys[0])
+        return counts
+
+    def _write(self, states, counts, write):
+        """What ``write(table, starts)`` gives, which stores ``counts`` new rows of the sessions."""
         self._make_room(states, counts)
         self._version += 1
         try:
-            table, starts = self._tables(states)
-            paged_append(k, v, self.keys, self.values, table, starts, counts)
+            got = write(*self._tables(states))
         except BaseException:
             self._undo_room(states)
             raise
         for s, c in zip(states, counts):
             s[1] += c
+        return got
+
+    def append(self, sessions, k, v, counts=None):
+        """Appends rows ``k``, ``v`` (bf16 ``[T, Hkv, 128]``, packed one session behind the other,
+        ``counts[i]`` each or as many each) to the sessions."""
+        self._outside_graphs()
+        sessions, states = self._distinct(sessions)
+        if not states:
+            return
+        counts = self._new_rows(states, k, v, counts)
+        self._write(states, counts, lambda table, starts: paged_append(k, v, self.keys, self.values, table, starts,
+                                                                       counts))
+
+    def append_rotated(self, sessions, q, k, v, rotary, counts=None, q_norm=None, k_norm=None, eps=1e-6, fetch=False):
+        """:meth:`append` of projected rows: their heads get norm and rotation at their sessions' positions on the
+        way (:func:`paged_append_rotated`). Returns the queries (bf16 ``[T, Hq, 128]``); with ``fetch`` ``(q, k, v)``."""
+        self._outside_graphs()
+        sessions, states = self._distinct(sessions)
+        if not states:
+            raise ValueError("no sessions")
+        counts = self._new_rows(states, k, v, counts)
+        return self._write(states, counts, lambda table, starts: paged_append_rotated(
+            q, k, v, self.keys, self.values, table, starts, rotary, counts, q_norm, k_norm, eps, fetch))
 
     def rows(self, sessions):
         """All rows of the sessions as bf16, packed: ``(k, v)``, each ``[sum of lengths, Hkv, 128]``."""
@@ -590,9 +611,23 @@ class PagedKVCache:
         return paged_decode_attention(q, self.keys, self.values, table, lens, scale,
                                       shared=self._common(states))
 
-    def batch(self, sessions) -> "PagedBatch":
-        """The sessions as the cache of a model call with one row of the batch for each."""
-        return PagedBatch(self, sessions)
+    def chunk_attention(self, sessions, q, scale, counts=None, window=None):
+        """Attention of the last rows of each session, ``q`` bf16 ``[T, Hq, 128]`` packed one session behind the
+        other, ``counts[i]`` each or as many each, over all before them or a window (:func:`paged_chunk_attention`)."""
+        self._outside_graphs()
+        sessions, states = self._distinct(sessions)
+        counts = _counts(_even(q.shape[0], len(states)) if counts is None else counts, len(states)).tolist()
+        for s, (_, rows), c in zip(sessions, states, counts):
+            if rows < c:
+                raise ValueError(f"session {s} of {rows} rows is shorter than its {c} queries")
+        table, lens = self._tables(states)
+        return paged_chunk_attention(q, self.keys, self.values, table, lens, scale, counts, window)
+
+    def batch(self, sessions, window=None, rotates=False) -> "PagedBatch":
+        """The sessions as the cache of a model call with one row of the batch for each. ``window``: of a
+        sliding-window layer, whose rows see that many positions, themselves among them. ``rotates``: the attention
+        block leaves norm and rotation to the append, and the sessions may be of different lengths."""
+        return PagedBatch(self, sessions, window, rotates)
 
     # ---- pages
 
@@ -636,13 +671,20 @@ class PagedBatch:
     sessions share read once; longer ones (prompts, chunks) read the sessions' rows back and run
     :func:`lagunalab_amd.prompt_attn.prompt_attention`, causal. What is attended are the quantized rows,
     as with ``DequantKVCache``. ``offset`` needs sessions of one length (the block's rotary embedding has
-    one position per call); the layers are full-attention ones (:meth:`make_mask`)."""
+    one position per call); the layers are full-attention ones (:meth:`make_mask`).
+
+    With a ``window`` the layers are sliding-window ones: every step runs :func:`paged_chunk_attention`. With
+    ``rotates`` the block hands its projections to :meth:`append_rotated`, each session is at a position of its own,
+    and steps of more than one row run :func:`paged_chunk_attention` too, which copies nothing."""
 
     fused_step = True
 
-    def __init__(self, cache: PagedKVCache, sessions):
+    def __init__(self, cache: PagedKVCache, sessions, window=None, rotates=False):
+        if window is not None and window < 1:
+            raise ValueError(f"a window of {window} positions")
         self.cache = cache
         self.sessions, _ = cache._distinct(sessions)
+        self.window, self.rotates = window, bool(rotates)
         self._seen = -1
 
     def _states(self):
@@ -666,13 +708,37 @@ class PagedBatch:
         if not keys.dtype == values.dtype == torch.bfloat16:
             raise ValueError(f"K/V rows must be bfloat16, got {keys.dtype} and {values.dtype}")
         _lib.require_device(keys, values, self.cache.keys[0])
+        k, v = (t.transpose(1, 2).reshape(B * L, H, D) for t in (keys, values))
+        self._write(L, lambda: paged_append(k, v, self.cache.keys, self.cache.values, self._table, self._lens, [L] * B))
+        return keys, values
+
+    def append_rotated(self, queries, keys, values, rotary, q_norm=None, k_norm=None, eps=1e-6):
+        """Appends projected rows (bf16 ``[B, L, heads, 128]``, any strides) to the sessions, queries and keys normed
+        and rotated at each session's positions on the way (:func:`paged_append_rotated`); returns the queries
+        ``[B, Hq, L, 128]`` for :meth:`attend`."""
+        self.cache._outside_graphs()
+        B, L, H, D = keys.shape
+        if B != len(self.sessions) or (H, D) != (self.cache.keys[0].shape[1], HEAD_DIM) \
+                or values.shape != keys.shape or queries.shape[:2] != (B, L):
+            raise ValueError(f"queries {tuple(queries.shape)}, keys {tuple(keys.shape)} and values "
+                             f"{tuple(values.shape)} are not rows of {len(self.sessions)} sessions of "
+                             f"{self.cache.keys[0].shape[1]} heads")
+        if not queries.dtype == keys.dtype == values.dtype == torch.bfloat16:
+            raise ValueError(f"rows must be bfloat16, got {queries.dtype}, {keys.dtype} and {values.dtype}")
+        _lib.require_device(queries, keys, values, self.cache.keys[0])
+        q, k, v = (t.flatten(0, 1) for t in (queries, keys, values))
+        got = self._write(L, lambda: paged_append_rotated(
+            q, k, v, self.cache.keys, self.cache.values, self._table, self._lens, rotary, [L] * B, q_norm, k_norm, eps))
+        return got.view(queries.shape).transpose(1, 2)
+
+    def _write(self, L, write):
+        """What ``write()`` gives, which stores L new rows of each session."""
         states = self._states()
-        if self.cache._make_room(states, [L] * B):
+        if self.cache._make_room(states, [L] * len(states)):
             self.cache._version += 1
         try:
             self._refresh(states)
-            k, v = (t.transpose(1, 2).reshape(B * L, H, D) for t in (keys, values))
-            paged_append(k, v, self.cache.keys, self.cache.values, self._table, self._lens, [L] * B)
+            got = write()
             lens = self._lens + L
         except BaseException:
             self.cache._undo_room(states)
@@ -682,11 +748,11 @@ class PagedBatch:
         self._lens = lens
         self.cache._version += 1  # other batches of these sessions hold old lengths
         self._seen = self.cache._version
-        return keys, values
+        return got
 
     def attend(self, queries, scale):
         """Attention of the step's rows, ``queries`` bf16 ``[B, Hq, L, 128]``: the last ``L`` positions of
-        each session, causal."""
+        each session, causal, within the window."""
         self.cache._outside_graphs()
         B, Hq, L, D = queries.shape
         if B != len(self.sessions):
@@ -697,7 +763,11 @@ class PagedBatch:
         self._refresh(states)
         q = queries.to(torch.bfloat16)
         keys, values = self.cache.keys, self.cache.values
-        if L == 1:
+        if self.window is not None or (self.rotates and L > 1):
+            out = paged_chunk_attention(q.transpose(1, 2).reshape(B * L, Hq, D), keys, values, self._table, self._lens,
+                                        scale, [L] * B, self.window)
+            out = out.view(B, L, Hq, D).transpose(1, 2)
+        elif L == 1:
             out = paged_decode_attention(q, keys, values, self._table, self._lens, scale, shared=self._shared)
         else:
             lens = [n for _, n in states]
@@ -714,14 +784,20 @@ class PagedBatch:
         return lens.pop() if lens else 0
 
     def make_mask(self, N, return_array=False, window_size=None):
-        """The mask of a step of ``N`` rows. :meth:`attend` is causal over all rows whatever the mask: a
-        window that would leave some of them out is refused."""
+        """The mask of a step of ``N`` rows. :meth:`attend` is causal over all rows, or those of the batch's
+        window, whatever the mask: another window is refused, unless neither leaves out any of the rows. Sessions of
+        different lengths have no array for a mask: "causal" stands for it, of a single row None."""
         from .cache import create_attention_mask
-        offset = self.offset
-        if window_size is not None and offset + N > window_size:
-            raise ValueError(f"a window of {window_size} positions ends before the {offset + N} rows: paged "
+        lens = [n for _, n in self._states()] if self.rotates else [self.offset]
+        rows = max(lens, default=0) + N
+        if min(rows, rows if window_size is None else window_size) != min(rows, self.window or rows):
+            if self.window is not None:
+                raise ValueError(f"the batch has a window of {self.window} positions, its layer one of {window_size}")
+            raise ValueError(f"a window of {window_size} positions ends before the {rows} rows: paged "
                              "batches are for full-attention layers")
-        return create_attention_mask(N, offset=offset, return_array=return_array, window_size=window_size)
+        if self.rotates and not return_array:
+            return None if N == 1 else "causal"
+        return create_attention_mask(N, offset=self.offset, return_array=return_array, window_size=window_size)
 
     def is_trimmable(self):
         return True

@@ -14,11 +14,11 @@ from . import _lib
 HEAD_DIM = 128
 
 
-def _refuse_grad(*tensors):
+def _refuse_grad(*tensors, what="attention"):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError("this attention has no backward pass: call it under torch.no_grad()")
+        raise ValueError(f"this {what} has no backward pass: call it under torch.no_grad()")
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-        raise ValueError("this attention has no forward derivative: its inputs have tangents")
+        raise ValueError(f"this {what} has no forward derivative: its inputs have tangents")
 
 
 def _lens(lens, what):
