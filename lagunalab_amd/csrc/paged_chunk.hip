@@ -49,7 +49,8 @@ struct ChunkArgs {
   float sl2;
   int window;          // positions a row sees, NO_WINDOW: all
   int shares;          // per KV head; 0: a workgroup takes a whole block
-  int blocks;          // of 32 rows, of the sequence with the most (few rows)
+  int blocks;          // of the sequence with the most rows (few rows)
+  int row_bits;        // log2 of a block's rows (few rows)
   int nseq, lanes;     // sequences, log2 of the lanes that add up the blocks of one
   int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];  // table row, first row of q, rows (not 0)
 };
@@ -597,14 +598,14 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkArgs a) {
 // session took 15.1 us in one launch.
 constexpr int UNIT = 32;  // keys of a wave's step
 
-template <int WV>  // waves
+template <int WV, int NB>  // waves, 32 rows each of a block
 struct FewSmem {
   // a wave's keys: 16-byte chunk c of row r of K at c ^ kswz(r), of V at c ^ vfew(r); at the end 16 of its rows'
   // values, 16-byte chunk c of row r at c ^ r
   alignas(256) uint8_t codes[WV][2][UNIT * D];
   alignas(16) float w[WV][4][2][UNIT];  // K scales, K biases, V scales, V biases of the two groups
-  uint4 q[8][64];                       // the rows of q as B operands, a lane's place in each
-  float2 ml[WV][32];
+  uint4 q[NB][8][64];                   // the rows of q as B operands, a lane's place in each
+  float2 ml[WV][32 * NB];
 };
 // Rows of V that a transposed read takes together, 4 h + 8 i + r: in different banks.
 __device__ __forceinline__ int vfew(int r) { return (r & 3) | ((r >> 1) & 4); }
@@ -625,11 +626,11 @@ __device__ __forceinline__ Deal few_deal(const ChunkArgs& a, int lane) {
   return {upto, q, total, max(SHARE_MIN, (total + a.shares - 1) / a.shares)};
 }
 
-// Units [p0, p1) of sequence s for the rows of block rb: partial rows to slot .., or with WHOLE output rows. AGAIN: the
-// other blocks read the pages too, and they stay in the L2 (streaming / staying, us: 48 rows of 16 sessions of 100 to
-// 4,100 positions 42.6 / 39.2; of one block 64 single tokens of up to 8,200 118 / 124).
-template <int WV, bool WHOLE, bool AGAIN>
-__device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, int s, const Seq& sq, int rb, int hk,
+// Units [p0, p1) of sequence s for its rows f0 .. f0 + 32 NB - 1: partial rows to slot .., or with WHOLE output rows.
+// AGAIN: other blocks read the pages too, and they stay in the L2 (streaming / staying, us: 48 rows of 16
+// sessions of 100 to 4,100 positions 42.6 / 39.2; of one block 64 single tokens of up to 8,200 118 / 124).
+template <int NB, bool WHOLE, bool AGAIN, int WV, int MB>
+__device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV, MB>& sm, int s, const Seq& sq, int f0, int hk,
                                          int p0, int p1, int64_t slot) {
   int tid = threadIdx.x;  // re-read, so that no lane value made of it is kept across sequences
   asm volatile("" : "+v"(tid));
@@ -665,19 +666,26 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
   if (p < p1) load(p);
 
   const float scale = abs_scale(a.sl2);
-  const int f0 = 32 * rb, f = f0 + ln;
-  const int i = (int)fdiv_u((uint32_t)min(f, sq.R - 1), a.g);
-  const int head = min(f, sq.R - 1) - i * a.G;
-  const int lim = f < sq.R ? sq.base + i : -1;
-  const uint16_t* qr = a.q + (int64_t)(a.row0[s] + i) * a.q_tok + (hk * a.G + head) * a.q_head + 16 * h;
+  int lim[NB];  // a row's position
+#pragma unroll
+  for (int t = 0; t < NB; ++t) {
+    const int f = f0 + 32 * t + ln;
+    lim[t] = f < sq.R ? sq.base + (int)fdiv_u((uint32_t)f, a.g) : -1;
+  }
   __syncthreads();  // the sequence before is written
   // q in K's order of dims: step 2 j + x holds dims 16 (2 j + h) + 8 x .. + 7
-  for (int kk = wv; kk < 8; kk += WV)
-    sm.q[kk][lane] = signed_q(*reinterpret_cast<const uint4*>(qr + 32 * (kk >> 1) + 8 * (kk & 1)), a.sl2);
-  Rows32 st;
-  st.clear();
+#pragma unroll
+  for (int t = 0; t < NB; ++t) {
+    const int f = min(f0 + 32 * t + ln, sq.R - 1), i = (int)fdiv_u((uint32_t)f, a.g);
+    const uint16_t* qr = a.q + (int64_t)(a.row0[s] + i) * a.q_tok + (hk * a.G + f - i * a.G) * a.q_head + 16 * h;
+    for (int kk = wv; kk < 8; kk += WV)
+      sm.q[t][kk][lane] = signed_q(*reinterpret_cast<const uint4*>(qr + 32 * (kk >> 1) + 8 * (kk & 1)), a.sl2);
+  }
+  Rows32 st[NB];
+#pragma unroll
+  for (int t = 0; t < NB; ++t) st[t].clear();
   const int lim_lo = sq.base + (int)fdiv_u((uint32_t)f0, a.g);
-  const int open_from = sq.base + (int)fdiv_u((uint32_t)min(f0 + 31, sq.R - 1), a.g) - a.window + 1;
+  const int open_from = sq.base + (int)fdiv_u((uint32_t)min(f0 + 32 * NB - 1, sq.R - 1), a.g) - a.window + 1;
   uint8_t* const kp = sm.codes[wv][0];
   uint8_t* const vp = sm.codes[wv][1];
   __syncthreads();  // q
@@ -710,24 +718,32 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
     if (p + WV < p1) load(p + WV);
     wave_fence();
     // scores
-    f16v_t c[1];
+    f16v_t c[NB][1];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) c[0][i] = 0.0f;
+    for (int t = 0; t < NB; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[t][0][i] = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float sc = sm.w[wv][0][j >> 1][ln], z = sm.w[wv][1][j >> 1][ln];
       const u4_t w = reinterpret_cast<const u4_t*>(kp)[8 * ln + ((2 * j + h) ^ kswz(ln))];
       const uint2 d0 = dequant4(w[0], sc, z), d1 = dequant4(w[1], sc, z);
       const uint2 d2 = dequant4(w[2], sc, z), d3 = dequant4(w[3], sc, z);
-      c[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d0.x, d0.y, d1.x, d1.y),
-                                                     u4_as_bf8(sm.q[2 * j][lane]), c[0], 0, 0, 0);
-      c[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d2.x, d2.y, d3.x, d3.y),
-                                                     u4_as_bf8(sm.q[2 * j + 1][lane]), c[0], 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < NB; ++t) {
+        c[t][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d0.x, d0.y, d1.x, d1.y),
+                                                          u4_as_bf8(sm.q[t][2 * j][lane]), c[t][0], 0, 0, 0);
+        c[t][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(words_as_bf8(d2.x, d2.y, d3.x, d3.y),
+                                                          u4_as_bf8(sm.q[t][2 * j + 1][lane]), c[t][0], 0, 0, 0);
+      }
     }
-    if (masked) mask32(c, lim - UNIT * p - 4 * h, a.window);  // uniform
-    bf16x8_t pr[2];
-    softmax32(c, st, scale, pr);
-    sums32(st, pr);
+    bf16x8_t pr[NB][2];
+#pragma unroll
+    for (int t = 0; t < NB; ++t) {
+      if (masked) mask32(c[t], lim[t] - UNIT * p - 4 * h, a.window);  // uniform
+      softmax32(c[t], st[t], scale, pr[t]);
+      sums32(st[t], pr[t]);
+    }
     // values: of keys 16 e + 8 (j / 4) + 4 h + j % 4, j < 8, this lane's dim of each window of 32
     const int r8 = (lane >> 1) & 7, src = 4 * h + 8 * (r8 >> 2) + (r8 & 3);
 #pragma unroll
@@ -748,34 +764,42 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             v[j] = fmaf(sc[j], (float)(((uint32_t)(j < 4 ? raw.x : raw.y) >> (8 * (j & 3))) & 0xffu), z[j]);
-          st.o[w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              words_as_bf8(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])),
-              pr[e], st.o[w], 0, 0, 0);
+          const bf16x8_t vb = words_as_bf8(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]),
+                                           pack_bf2(v[6], v[7]));
+#pragma unroll
+          for (int t = 0; t < NB; ++t)
+            st[t].o[w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, pr[t][e], st[t].o[w], 0, 0, 0);
         }
       }
     for (; wilds; wilds &= wilds - 1) {  // rare
       const int key = __builtin_ctzll(wilds);
-      add_wild(a.buf, row + key, key, lim - UNIT * p - key, st, lane, pr, a.window);
+#pragma unroll
+      for (int t = 0; t < NB; ++t)
+        add_wild(a.buf, row + key, key, lim[t] - UNIT * p - key, st[t], lane, pr[t], a.window);
     }
   }
 
   // ---- the waves' rows meet in LDS, 16 at a time
-  const int R = min(32, sq.R - f0);
+  const int R = min(32 * NB, sq.R - f0);
   f4_t* acc = reinterpret_cast<f4_t*>(sm.codes[wv]);
-  st.l = sum_xor32(st.l);
-  if (h == 0) sm.ml[wv][ln] = make_float2(st.m, st.l);
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
+  for (int t = 0; t < NB; ++t) {
+    const float l = sum_xor32(st[t].l);
+    if (h == 0) sm.ml[wv][32 * t + ln] = make_float2(st[t].m, l);
+  }
+#pragma unroll
+  for (int part = 0; part < 2 * NB; ++part) {
+    const Rows32& rt = st[part >> 1];
     if (16 * part >= R) break;  // uniform
     if (part) __syncthreads();  // the 16 before are read
     wave_fence();
-    if (ln >> 4 == part) {
+    if (ln >> 4 == (part & 1)) {
 #pragma unroll
       for (int w = 0; w < 4; ++w)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           acc[32 * (ln & 15) + ((8 * w + 2 * j + h) ^ (ln & 15))] =
-              f4_t{st.o[w][4 * j], st.o[w][4 * j + 1], st.o[w][4 * j + 2], st.o[w][4 * j + 3]};
+              f4_t{rt.o[w][4 * j], rt.o[w][4 * j + 1], rt.o[w][4 * j + 2], rt.o[w][4 * j + 3]};
     }
     __syncthreads();
     for (int x = tid; x < 32 * min(16, R - 16 * part); x += 64 * WV) {
@@ -805,15 +829,24 @@ __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV>& sm, in
   }
 }
 
-// Partial rows of a KV head and row block: 32 for each share and sequence (along both each part adds one to their sum).
+// Partial rows of a KV head and row block: a block's for each share and sequence (along both each part adds one to
+// their sum).
 __device__ __forceinline__ int64_t few_slot(const ChunkArgs& a, int hk, int rb, int x) {
-  return ((int64_t)(hk * a.blocks + rb) * (a.shares + a.nseq) + x) * 32;
+  return ((int64_t)(hk * a.blocks + rb) * (a.shares + a.nseq) + x) << a.row_bits;
+}
+template <int NB, bool WHOLE, bool AGAIN, int WV>
+__device__ __forceinline__ void few_rows(const ChunkArgs& a, FewSmem<WV, NB>& sm, int s, const Seq& sq, int f0, int hk,
+                                         int p0, int p1, int64_t slot) {
+  if (sq.R - f0 > 32)  // uniform
+    few_part<NB, WHOLE, AGAIN>(a, sm, s, sq, f0, hk, p0, p1, slot);
+  else if (sq.R > f0)
+    few_part<1, WHOLE, AGAIN>(a, sm, s, sq, f0, hk, p0, p1, slot);
 }
 
 // A share of the sequences' half pages, dealt out one sequence behind the other.
-template <bool AGAIN>
+template <int NB, bool AGAIN>
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void few_kernel(const ChunkArgs a) {
-  __shared__ FewSmem<FEW_WAVES> sm;
+  __shared__ FewSmem<FEW_WAVES, NB> sm;
   const int hk = blockIdx.x % a.Hkv, y = blockIdx.x / a.Hkv, x = y / a.blocks, rb = y - x * a.blocks;
   const int lane = threadIdx.x & 63;
   const Deal deal = few_deal(a, lane);
@@ -827,29 +860,29 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void few_kernel(const ChunkArgs 
     if (pg.n == 0) continue;
     begin += SEQ_COST;
     const int p0 = max(u - begin, 0), p1 = min(u1 - begin, pg.n);
-    if (p0 < p1 && 32 * rb < sq.R)
-      few_part<FEW_WAVES, false, AGAIN>(a, sm, s, sq, rb, hk, pg.lo + p0, pg.lo + p1, few_slot(a, hk, rb, x + s));
+    if (p0 < p1)
+      few_rows<NB, false, AGAIN>(a, sm, s, sq, 32 * NB * rb, hk, pg.lo + p0, pg.lo + p1, few_slot(a, hk, rb, x + s));
     begin += pg.n;
     u = begin;
   }
 }
 
 // A whole sequence per workgroup: nothing to merge.
-template <int WV, bool AGAIN>
+template <int NB, int WV>
 __global__ __launch_bounds__(64 * WV, 2) void few_whole_kernel(const ChunkArgs a) {
-  __shared__ FewSmem<WV> sm;
-  const int hk = blockIdx.x % a.Hkv, y = blockIdx.x / a.Hkv, s = y / a.blocks, rb = y - s * a.blocks;
+  __shared__ FewSmem<WV, NB> sm;
+  const int hk = blockIdx.x % a.Hkv, y = blockIdx.x / a.Hkv, s = y / a.blocks, f0 = 32 * NB * (y - s * a.blocks);
   const Seq sq = seq_of(a, s);
-  const int R = min(32, sq.R - 32 * rb);
+  const int R = min(32 * NB, sq.R - f0);
   if (sq.len < 0) {
     for (int x = threadIdx.x; x < R * D; x += 64 * WV) {
-      const int f = 32 * rb + x / D, p = (int)fdiv_u((uint32_t)f, a.g);
+      const int f = f0 + x / D, p = (int)fdiv_u((uint32_t)f, a.g);
       a.out[((int64_t)(a.row0[s] + p) * a.Hkv * a.G + hk * a.G + f - p * a.G) * D + x % D] = 0x7fc0;
     }
     return;
   }
   const Units pg = few_units(a, sq);
-  if (R > 0) few_part<WV, true, AGAIN>(a, sm, s, sq, rb, hk, pg.lo, pg.lo + pg.n, 0);
+  few_rows<NB, true, false>(a, sm, s, sq, f0, hk, pg.lo, pg.lo + pg.n, 0);
 }
 
 // An output row by GR groups of 32 lanes (4 dims each), 8 / GR rows per workgroup: group g takes every GR-th
@@ -859,9 +892,9 @@ __global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
   __shared__ float2 sh_ml[8];
   __shared__ f4_t sh_acc[8][32];
   const int lane = threadIdx.x & 63;
-  // wave-uniform: a row has at least a wave. Rows of a sequence and KV head: 32 per block
+  // wave-uniform: a row has at least a wave. Rows of a sequence and KV head: as many as its blocks'
   const int row = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (8 / GR) + threadIdx.x / (32 * GR)));
-  const int per = 32 * a.blocks, y = row / per, f = row - y * per, s = min(y / a.Hkv, a.nseq - 1), hk = y % a.Hkv;
+  const int per = a.blocks << a.row_bits, y = row / per, f = row - y * per, s = min(y / a.Hkv, a.nseq - 1), hk = y % a.Hkv;
   const Deal deal = few_deal(a, lane);
   const Seq sq = seq_at(deal, s);
   const int pages = few_units(a, sq).n;
@@ -869,7 +902,7 @@ __global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
   const int first = before / deal.share;
   const bool mine = f < sq.R;
   const int parts = mine && pages ? (before + pages - 1) / deal.share - first + 1 : 0;
-  const int64_t slot = few_slot(a, hk, f >> 5, first + s) + (f & 31);
+  const int64_t slot = few_slot(a, hk, f >> a.row_bits, first + s) + (f & ((1 << a.row_bits) - 1));
   const int grp = (threadIdx.x >> 5) % GR, ch = threadIdx.x & 31;
   float M = -INFINITY, den = 0.0f;
   f4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -878,7 +911,7 @@ __global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
     f4_t x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t at = slot + 32 * (int64_t)min(i0 + GR * j, parts - 1);
+      const int64_t at = slot + ((int64_t)min(i0 + GR * j, parts - 1) << a.row_bits);
       ml[j] = a.part_ml[at];
       x[j] = *reinterpret_cast<const f4_t*>(a.part_acc + at * D + 4 * ch);
     }
@@ -922,6 +955,11 @@ constexpr int64_t FEW_ROWS = 96;
 // 4,099 653 / 623, 24 chunks of up to 300 rows behind up to 5,985 365 / 348 (in shares all the same); 32/8 heads: 5
 // prompts of up to 2,049 rows 123 / 103, 4 of 500 38 / 27, one of 5,000 254 / 244, 64 of 400 220 / 234.
 constexpr int64_t IDLE_TILES = 8, LONGEST = 40;
+// Of more than 32 rows, 64 go as one block where a workgroup (two per CU) has TWO_UNITS half pages or more, or a sequence
+// and KV head of its own: its waves dequantize a page once for both halves, but have as much to join at the end. us, 32 /
+// 64 rows: 48 of 16 sessions of 8,000 positions 105 / 86, of 100 to 4,100 39 / 43; 48 of 4 of 20,000 75 / 63, of one 27 /
+// 34; 64 behind 65,536 61 / 57; 48 of 64 windows of 512 40 / 34, of 8 13.5 / 21.
+constexpr int64_t TWO_UNITS = 36;
 // Calls of few pages per sequence take each whole: one launch, nothing to merge. Many sequences also where they are
 // longer. us on the GPU, dealt out / whole: 1 session of 512 positions, 8 KV heads 9.9 / 9.5, of 1,038 10.0 / 13.8 (with
 // the host, whose launches bound such a call, 16.3 / 14); 8 of 1,500 16.4 / 20.3, 16 windows of 1,100 20.6 / 17.6, 32
@@ -958,14 +996,16 @@ ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G
   if (idle * tiles > IDLE_TILES * blocks * Hkv || tiles > std::max(LONGEST, own * Hkv / slots))
     p.many.shares = (int)std::max<int64_t>(1, slots / Hkv);
   p.many.slots = p.many.nseq ? 2 * p.many.shares * Hkv * p.many.rows_of : 0;
-  p.few.rows_of = 32;
-  p.few.blocks = (int)((few + 31) / 32);
-  const int64_t wgs = p.few.nseq * p.few.blocks * Hkv;
   int rows = 0;
   for (int s = 0; s < p.few.nseq; ++s) rows = std::max(rows, p.few.rows[s]);
+  const int64_t units = p.few.nseq * Hkv * seen(rows) * (PAGE / UNIT);
+  const bool two = few > 32 && (units >= TWO_UNITS * 2 * cus || p.few.nseq * Hkv >= 2 * cus);
+  p.few.rows_of = two ? 64 : 32;
+  p.few.blocks = (int)((few + p.few.rows_of - 1) / p.few.rows_of);
+  const int64_t wgs = p.few.nseq * p.few.blocks * Hkv;
   if (seen(rows) > (2 * wgs >= cus ? WHOLE_PAGES_MANY : WHOLE_PAGES)) {
     p.few.shares = (int)std::max<int64_t>(1, 2 * cus / (Hkv * std::max(1, p.few.blocks)));
-    p.few.slots = Hkv * p.few.blocks * (int64_t)(p.few.shares + p.few.nseq) * 32;
+    p.few.slots = Hkv * p.few.blocks * (int64_t)(p.few.shares + p.few.nseq) * p.few.rows_of;
   }
   return p;
 }
@@ -1008,17 +1048,19 @@ int launch_many(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
 int launch_few(const ChunkArgs& a, const ChunkPart& c, hipStream_t st) {
   if (a.shares == 0) {
     const int64_t wgs = (int64_t)c.nseq * c.blocks * a.Hkv;
-    const bool wide = wgs <= device_cu_count();
-    auto* whole = c.blocks > 1 ? wide ? few_whole_kernel<8, true> : few_whole_kernel<4, true>
-                               : wide ? few_whole_kernel<8, false> : few_whole_kernel<4, false>;
+    const bool wide = c.rows_of == 32 && wgs <= device_cu_count();
+    // blocks of 64 rows are only formed for more workgroups than CUs
+    auto* whole = c.rows_of > 32 ? few_whole_kernel<2, 4> : wide ? few_whole_kernel<1, 8> : few_whole_kernel<1, 4>;
     whole<<<dim3((unsigned)wgs), dim3(wide ? 512 : 256), 0, st>>>(a);
     LQ_CHECK_LAUNCH("few_whole_kernel");
     return LQ_OK;
   }
-  auto* few = c.blocks > 1 ? few_kernel<true> : few_kernel<false>;
+  const bool again = c.blocks > 1;
+  auto* few = c.rows_of > 32 ? again ? few_kernel<2, true> : few_kernel<2, false>
+                             : again ? few_kernel<1, true> : few_kernel<1, false>;
   few<<<dim3((unsigned)(a.shares * c.blocks * a.Hkv)), dim3(64 * FEW_WAVES), 0, st>>>(a);
   LQ_CHECK_LAUNCH("few_kernel");
-  const int64_t n = (int64_t)c.nseq * a.Hkv * 32 * c.blocks;
+  const int64_t n = (int64_t)c.nseq * a.Hkv * c.rows_of * c.blocks;
   if (a.shares / std::min(c.nseq, 4) > 16)
     few_merge_kernel<8><<<dim3((unsigned)n), dim3(256), 0, st>>>(a);
   else
@@ -1089,6 +1131,7 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
     a.part_ml = (float2*)(a.part_acc + c->slots * 128);
     a.shares = c->shares;
     a.blocks = c->blocks;
+    a.row_bits = c->rows_of > 32 ? 6 : 5;
     a.nseq = c->nseq;
     a.lanes = 6;
     while ((c->nseq << a.lanes) > 64) --a.lanes;

@@ -227,3 +227,46 @@ def test_blocks_whole_and_in_shares(dev, hq, kv, lens, counts, window, whole):
     want, bound = exact(q, pool, table, lens, counts, window, SCALE)
     if len(lens) > 1:
         assert_within(out[counts[0]:], want[counts[0]:], bound[counts[0]:])
+
+
+@pytest.mark.parametrize("spare", [0, 60])  # a short table, taken whole, and a long one, dealt out
+@pytest.mark.parametrize("window", [None, 70])
+@pytest.mark.parametrize("longest", [10, 16])  # of 6 query heads each: 60 rows, one block, and 96, two
+def test_many_verified_blocks(dev, longest, window, spare):
+    """More than 32 query rows of so many sequences that 64 go as one block, beside single tokens: values, a V row that some rows see and others do not, a page and a length that are not there."""
+    g = gen(7)
+    hq, kv, B = 48, 8, 64
+    lens = [(37 * i * i) % 400 + 17 for i in range(B)]
+    counts = [[6, 1, 8, longest, min(11, longest), 5][i % 6] for i in range(B)]
+    lens[9], counts[9], counts[10] = 0, 3, 0
+    pool, table = sessions(g, kv, lens, dev, spare=spare)
+    q = randn(g, sum(counts), hq, D).to(dev)
+    args = (ints(lens, dev), SCALE, counts, window)
+    clean = paged_chunk_attention(q, *pool, table.to(dev), *args)
+    want_all, bound = exact(q, pool, table, lens, counts, window, SCALE)
+    assert_within(clean, want_all, bound)
+    ends = torch.tensor(counts).cumsum(0).tolist()
+    for b in (3, 2, 34):  # the longest, 48 rows of a KV head, the next longest
+        first = ends[b] - counts[b]
+        at = lens[b] - counts[b] // 2
+        spoiled = [tuple(t.clone() for t in buf) for buf in pool]
+        spoiled[1][1][int(table[b, at // PAGE]), 5, at % PAGE, 0] = float("inf")
+        got = paged_chunk_attention(q, *spoiled, table.to(dev), *args)
+        see = slice(ends[b] - counts[b] // 2, ends[b])
+        assert not torch.isfinite(got[see][:, 30:36, :64]).any()
+        want = clean.clone()
+        want[see, 30:36, :64] = got[see, 30:36, :64] = 0
+        assert torch.equal(got, want)
+        bad = table.clone()
+        bad[b, (lens[b] - 1) // PAGE] = pool[0][0].shape[0]
+        got = paged_chunk_attention(q, *pool, bad.to(dev), *args)
+        sees = (lens[b] - 1) // PAGE * PAGE - (lens[b] - counts[b])  # the first row that does
+        assert got[first + max(0, sees):ends[b]].isnan().all()
+        assert torch.equal(got[:first + max(0, sees)], clean[:first + max(0, sees)]) and torch.equal(got[ends[b]:], clean[ends[b]:])
+        for n in (-1, PAGE * table.shape[1] + 1):
+            now = list(lens)
+            now[b] = n
+            got = paged_chunk_attention(q, *pool, table.to(dev), ints(now, dev), *args[1:])
+            assert got[first:ends[b]].isnan().all()
+            for part in (slice(0, first), slice(ends[b], None)):  # other lengths cut the others' keys elsewhere
+                assert_within(got[part], want_all[part], bound[part])
