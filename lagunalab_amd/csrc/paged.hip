@@ -200,7 +200,8 @@ __device__ __forceinline__ float sum16(float x) {
   return x + dpp<DPP_ROW_ROR8>(x);
 }
 
-// Turns of a wave where the heads of all tokens fill this many waves per CU.
+// Turns of a wave where the heads of all tokens fill this many waves per CU: its norm weights and angles are loaded once.
+// us, of 2, 4 and 8: 2,048 rows of 48/8 heads 21.1, 20.6, 20.0; 7 packed prompts of up to 4,099 78.5, 82.4, 96.4.
 constexpr int ROTATE_TURNS = 4, ROTATE_MANY = 32;
 
 template <bool PAIRS, bool WIDE, int RT>

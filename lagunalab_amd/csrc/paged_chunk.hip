@@ -4,15 +4,18 @@
 // p = lens[b] - counts[b] + i and sees max(0, p - window + 1) .. p. lens is read on the device, so that a
 // recorded call follows growing sequences.
 //
-// A workgroup takes a block of query rows of a KV head, numbered position-major (row f is position f / G of
-// query head f % G), walks the pages that the block sees, dequantizes each once into LDS as bf16 -- one tile of
-// 64 keys, what paged_gather reads -- and runs it through attn_tile.h. The pages' codes are loaded into registers
-// a tile ahead and staged into one of two tiles; one barrier per tile.
+// Query rows of a KV head are numbered position-major (row f is position f / G of query head f % G), so that any
+// grouping fills a matrix tile; a wave has 32 of them as the columns of v_mfma_f32_32x32x16_bf16 (attn_tile32.h). K and V
+// are dequantized, scale * code + bias in fp32, to the bf16 rows that paged_gather reads. Softmax in fp32 with a running
+// maximum; the weights are rounded to bf16, in the values and in the row sums alike: outputs are 0.0023 of their size off
+// those in 64 bits, where the rounding of the output alone makes 0.0017.
 //
-// The work is dealt out in equal shares of tiles: the blocks of all sequences stand one behind the other, a
-// block costing its tiles and BLOCK_COST for its start and end, and a workgroup takes one share, which may begin
-// and end inside blocks. Parts of blocks go to the workspace and a second launch merges them. Every workgroup
-// adds the costs up itself, from the lengths.
+// Sequences of many rows go as blocks of 256 rows (128 where no sequence has more): a workgroup walks the pages that its
+// block sees, one tile of 64 keys each, dequantized once into LDS. Those of few rows (up to FEW_ROWS) go through waves
+// that take half pages each (further down). Blocks are taken whole, or all blocks stand one behind the other, a block
+// costing its tiles and BLOCK_COST for its start and end, and a workgroup takes an equal share of that, which may begin
+// and end inside blocks: parts go to the workspace and a second launch merges them. Every workgroup adds the costs up
+// itself, from the lengths. The rules and what they measured are at chunk_plan.
 //
 // Keys that a row does not see reach it in no way: masked scores are -infinity, pages that no row of a block
 // sees are not read, and a V row with infinities or NaN in a tile that is masked for some row is taken out of
@@ -237,6 +240,14 @@ struct ChunkSmem {
   uint32_t wild[3][2];       // keys of tile t % 3, if masked, whose V is wild
 };
 
+// Blocks of many rows. Eight waves are two halves that run a phase apart: while one has the matrix cores (S of tile t + 1,
+// O of tile t), the other does softmax and brings a tile in, its codes loaded two tiles ahead and K staged there, V between
+// the MFMAs of the matrix phase; one barrier per phase, and the waves in the matrix phase go first (s_setprio). Bound by
+// the vector work beside the MFMAs and, in long calls, by power. 2,048 rows of 32/8 heads behind 30,720 positions 1,090
+// to 1,130 us, 1,050 to 1,080 TFLOP/s, a tile 4,000 cycles: MFMAs alone 878, with the softmax 978, with staging 1,090.
+// Without priorities 1,173, with the vector phase first 1,222; K staged in the matrix phase 1,223; row sums between the
+// MFMAs 1,212, in the softmax 1,135; fragments two / four steps ahead instead of three 1,135 / 1,120.
+// Four waves, two workgroups per CU, run a tile's phases one behind the other.
 template <int PW>  // waves, of 32 rows each: 8 or 4
 __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
   constexpr bool HALVES = PW == 8;
@@ -591,11 +602,12 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkArgs a) {
   }
 }
 
-// ---- sequences of few rows (single tokens, verified blocks): up to 32 query rows per workgroup, all of them in
-// every wave, which takes half a page (32 keys) at a time through LDS of its own (no barriers), dequantized on its way
-// into the matrix cores, the next one's loads out. Reading the pages bounds long calls, a wave's way through a half
-// page short ones: with whole pages per wave, and two waves per SIMD for it instead of three, 1,024 positions of one
-// session took 15.1 us in one launch.
+// ---- sequences of few rows (single tokens, verified blocks): 32 query rows per workgroup, or 64, all of them in every
+// wave, which takes half a page (32 keys) at a time through LDS of its own (no barriers), dequantized on its way into the
+// matrix cores, the next one's loads out. Reading the pages bounds long calls of one block (5 rows behind 65,536
+// positions, 8 KV heads: 39 us, 3.6 TB/s; 8 single tokens of 42,771 to 82,671 194, 5.6), dequantization and softmax those
+// of more rows (about 2,800 cycles of vector work per half page), the way through a half page short ones. Whole pages per
+// wave took 44.6 for the first, and 25.0 instead of 20.8 for 64 tokens of windows of 512.
 constexpr int UNIT = 32;  // keys of a wave's step
 
 template <int WV, int NB>  // waves, 32 rows each of a block
