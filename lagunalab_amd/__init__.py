@@ -6,7 +6,8 @@ Python surface (drop-in names of ``laguna_mlx``):
   lookup.NgramIndex, lookup.ngram_propose, lookup.greedy_accept, lookup.DeviceNgramIndex
   quant.quantize / quant.dequantize / quant.quantize_into
 Several sessions on one GPU (no counterpart there):
-  paged.PagedKVCache, paged.PagedBatch (+ paged_append, paged_gather, paged_decode_attention, copy_pages)
+  paged.PagedKVCache, paged.PagedBatch (+ paged_append, paged_append_rotated, paged_gather, paged_decode_attention,
+  paged_chunk_attention, copy_pages); rotary.Rotary
   prompt_attn.prompt_attention
 All compute runs in liblaguna_hip.so (hand-written HIP for gfx950); there is no CPU fallback.
 """

@@ -243,7 +243,7 @@ struct ChunkSmem {
 // Blocks of many rows. Eight waves are two halves that run a phase apart: while one has the matrix cores (S of tile t + 1,
 // O of tile t), the other does softmax and brings a tile in, its codes loaded two tiles ahead and K staged there, V between
 // the MFMAs of the matrix phase; one barrier per phase, and the waves in the matrix phase go first (s_setprio). Bound by
-// the vector work beside the MFMAs and, in long calls, by power. 2,048 rows of 32/8 heads behind 30,720 positions 1,090
+// the vector work beside the MFMAs and, in long calls, by power. 2,048 rows of 32/8 heads behind 32,771 positions 1,090
 // to 1,130 us, 1,050 to 1,080 TFLOP/s, a tile 4,000 cycles: MFMAs alone 878, with the softmax 978, with staging 1,090.
 // Without priorities 1,173, with the vector phase first 1,222; K staged in the matrix phase 1,223; row sums between the
 // MFMAs 1,212, in the softmax 1,135; fragments two / four steps ahead instead of three 1,135 / 1,120.
@@ -964,7 +964,7 @@ constexpr int64_t FEW_ROWS = 96;
 // long block among short ones would be waited for: whole blocks have at most LONGEST tiles, or those that the rows see
 // of each other alone keep the other workgroups busy for as long. us, shares / whole, 48/8 heads: 2,048 rows of a window
 // of 512 66.8 / 57.4, of 4,096 240 / 263, 1,024 behind 1,000 68.4 / 67.5, behind 8,000 235 / 258, 7 prompts of up to
-// 4,099 653 / 623, 24 chunks of up to 300 rows behind up to 5,985 365 / 348 (in shares all the same); 32/8 heads: 5
+// 4,099 653 / 623, 24 chunks of up to 301 rows behind up to 6,007 365 / 348 (in shares all the same); 32/8 heads: 5
 // prompts of up to 2,049 rows 123 / 103, 4 of 500 38 / 27, one of 5,000 254 / 244, 64 of 400 220 / 234.
 constexpr int64_t IDLE_TILES = 8, LONGEST = 40;
 // Of more than 32 rows, 64 go as one block where a workgroup (two per CU) has TWO_UNITS half pages or more, or a sequence
