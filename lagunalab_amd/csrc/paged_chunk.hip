@@ -1007,7 +1007,7 @@ ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G
   const int64_t tiles = seen(p.many.rows_of / G + 1);
   if (idle * tiles > IDLE_TILES * blocks * Hkv || tiles > std::max(LONGEST, own * Hkv / slots))
     p.many.shares = (int)std::max<int64_t>(1, slots / Hkv);
-  p.many.slots = p.many.nseq ? 2 * p.many.shares * Hkv * p.many.rows_of : 0;
+  p.many.slots = p.many.nseq && p.many.shares > 1 ? 2 * p.many.shares * Hkv * p.many.rows_of : 0;
   int rows = 0;
   for (int s = 0; s < p.few.nseq; ++s) rows = std::max(rows, p.few.rows[s]);
   const int64_t units = p.few.nseq * Hkv * seen(rows) * (PAGE / UNIT);
@@ -1115,11 +1115,11 @@ extern "C" int lq_paged_chunk_attn(const uint16_t* q, int64_t q_tok, int64_t q_h
   LQ_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0 && ((q_tok | q_head) & 7) == 0,
                "rows must be 16-byte aligned (strides a multiple of 8)");
   LQ_CHECK_ARG((int64_t)plan.many.blocks * Hkv <= 1 << 22, "too many rows");  // workgroups of a launch
-  int64_t most = 0;  // cost, if every block sees the whole table
+  int64_t most = 0;  // cost, if every block sees the whole table: twice as much has to fit 32 bits
   for (int s = 0; s < plan.many.nseq; ++s)
     most += (plan.many.rows[s] * G + plan.many.rows_of - 1) / plan.many.rows_of * (table_width + lq::BLOCK_COST);
   most = std::max<int64_t>(most, plan.few.nseq * (2 * table_width + lq::SEQ_COST));
-  LQ_CHECK_ARG(most < (1ll << 31) - (1 << 20), "too many rows for table rows of %lld pages", (long long)table_width);
+  LQ_CHECK_ARG(most < 1ll << 30, "too many rows for table rows of %lld pages", (long long)table_width);
   const int64_t need = chunk_bytes(plan);
   if (need > 0 && (!workspace || workspace_bytes < need)) {
     set_error("workspace of %lld bytes is smaller than the %lld needed", (long long)workspace_bytes, (long long)need);

@@ -84,6 +84,7 @@ def attend(lib, **kw):
     # more rows than all the workgroups of a launch, or costs than 32 bits
     (dict(hq=1024, kv=1024, counts=ints(1 << 24, 1 << 24), q_tok=1 << 17), b"too many rows"),
     (dict(hq=2, counts=ints(1 << 23, 2), width=1 << 18, stride=1 << 18), b"too many rows"),
+    (dict(hq=2, counts=ints(1 << 20, 2), width=1 << 18, stride=1 << 18), b"too many rows"),
 ])
 def test_chunk_refusals(lib, bad, word):
     assert attend(lib, **bad) == _lib.LQ_EINVAL
@@ -106,6 +107,8 @@ def test_workspace_sizes(lib):
     for bad in ((None, 1, 8, 2, 4, 0), (ints(1), 0, 8, 2, 4, 0), (ints(1), 65, 8, 2, 4, 0), (ints(-1), 1, 8, 2, 4, 0),
                 (ints(1), 1, 7, 2, 4, 0), (ints(1), 1, 8, 2, 0, 0), (ints(1), 1, 8, 2, 4, -1)):
         assert need(*bad) < 0, bad
+    # a share per KV head is not cut
+    assert need(ints(5000), 1, 512, 512, 1 << 18, 0) == 0
     # partial rows, whatever the lengths: below 128 MiB up to 64 KV heads
     for hq, kv in ((8, 1), (32, 8), (48, 8), (64, 64), (512, 8)):
         for counts in ([1], [1] * 64, [500] * 64, [4096], [5, 4096]):
