@@ -1037,8 +1037,8 @@ int check_chunk(int64_t Hq, int64_t Hkv, const int32_t* counts, int64_t nseq, in
     rows += counts[s];
   }
   LQ_CHECK_ARG(rows < (1 << 30), "too many rows");
-  LQ_CHECK_ARG(width >= 1 && window >= 0 && window < ((int64_t)1 << 40), "a window of %lld positions, or table rows of %lld pages",
-               (long long)window, (long long)width);
+  LQ_CHECK_ARG(width >= 1 && window >= 0 && window < ((int64_t)1 << 40),
+               "a window of %lld positions, or table rows of %lld pages", (long long)window, (long long)width);
   return LQ_OK;
 }
 
