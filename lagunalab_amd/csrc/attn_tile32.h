@@ -75,9 +75,9 @@ __device__ __forceinline__ void mask32(f16v_t (&c)[MT], int rel, int window) {
 }
 
 // Scores of MT key tiles to weights: raises the running maximum where needed (and rescales the row), P in bf16 as the
-// B operands of the 16-key steps.
-template <int MT>
-__device__ __forceinline__ void softmax32(f16v_t (&c)[MT], Rows32& st, float scale, bf16x8_t (&p)[2 * MT]) {
+// B operands of the 16-key steps. work(): done when half of the scores are weights and their registers free.
+template <int MT, typename Work>
+__device__ __forceinline__ void softmax32(f16v_t (&c)[MT], Rows32& st, float scale, bf16x8_t (&p)[2 * MT], Work work) {
   float x[2 * MT];
 #pragma unroll
   for (int j = 0; j < 2 * MT; ++j) {  // chains
@@ -105,6 +105,7 @@ __device__ __forceinline__ void softmax32(f16v_t (&c)[MT], Rows32& st, float sca
   }
 #pragma unroll
   for (int e = 0; e < 2 * MT; ++e) {
+    if (e == MT) work();
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -116,6 +117,11 @@ __device__ __forceinline__ void softmax32(f16v_t (&c)[MT], Rows32& st, float sca
     asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
     p[e] = words_as_bf8(w[0], w[1], w[2], w[3]);
   }
+}
+
+template <int MT>
+__device__ __forceinline__ void softmax32(f16v_t (&c)[MT], Rows32& st, float scale, bf16x8_t (&p)[2 * MT]) {
+  softmax32(c, st, scale, p, []() {});
 }
 
 // Adds the rounded weights to the row sums.
@@ -165,27 +171,27 @@ __device__ __forceinline__ bf16x8_t v_operand32(uint32_t v, int w, int e) {
 // Q.K^T of one tile, then P.V of another: 32 MFMAs in 16 steps of two, whose fragments are read three steps ahead
 // (ahead32: the first three steps', which may lie in the phase before). k, v: the lane's place
 // in the tiles.
-// work(u): what else there is to do at step u, between its MFMAs and the next's.
+// work(n): what else there is to do behind MFMA n. It and one fragment's read fit beside the MFMA that runs; all of a
+// step's behind its second MFMA did not (a phase 1,870 cycles instead of 1,640).
 constexpr int AHEAD = 3;
 struct Ahead32 {
   bf16x8_t f[AHEAD + 1][2];
 };
-__device__ __forceinline__ void fetch32(uint32_t k, uint32_t v, int step, bf16x8_t (&f)[2]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    f[j] = step < 8 ? k_operand32(k, j, step) : v_operand32(v, 2 * (step & 1) + j, (step - 8) >> 1);
+__device__ __forceinline__ void fetch32(uint32_t k, uint32_t v, int step, int j, Ahead32& a) {
+  a.f[step % (AHEAD + 1)][j] =
+      step < 8 ? k_operand32(k, j, step) : v_operand32(v, 2 * (step & 1) + j, (step - 8) >> 1);
 }
 __device__ __forceinline__ void ahead32(uint32_t k, Ahead32& a) {
 #pragma unroll
-  for (int u = 0; u < AHEAD; ++u) fetch32(k, 0, u, a.f[u]);
+  for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fetch32(k, 0, u, j, a);
 }
 template <typename Work>
 __device__ __forceinline__ void matrix32(uint32_t k, uint32_t v, Rows32& st, f16v_t (&c)[2],
                                          const bf16x8_t (&p)[4], Ahead32& a, Work work) {
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
-    if (u + AHEAD < 16) fetch32(k, v, u + AHEAD, a.f[(u + AHEAD) % (AHEAD + 1)]);
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if (u < 8) {
@@ -199,10 +205,11 @@ __device__ __forceinline__ void matrix32(uint32_t k, uint32_t v, Rows32& st, f16
         const int w = 2 * (u & 1) + j;
         st.o[w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f[u % (AHEAD + 1)][j], p[(u - 8) >> 1], st.o[w], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      if (u + AHEAD < 16) fetch32(k, v, u + AHEAD, j, a);
+      work(2 * u + j);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    work(u);
-    __builtin_amdgcn_sched_barrier(0);
   }
   // behind the last MFMA: beside MFMAs, of either wave of the SIMD, v_dot2 stalls both (2,048 rows behind 32,771
   // positions, 32/8 heads: 1,113 us here, 1,212 between the steps, 1,135 in the softmax)
@@ -214,7 +221,10 @@ __device__ __forceinline__ void scores32(uint32_t k, const Rows32& st, f16v_t (&
   ahead32(k, a);
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
-    if (u + AHEAD < 8) fetch32(k, 0, u + AHEAD, a.f[(u + AHEAD) % (AHEAD + 1)]);
+    if (u + AHEAD < 8) {
+      fetch32(k, 0, u + AHEAD, 0, a);
+      fetch32(k, 0, u + AHEAD, 1, a);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {

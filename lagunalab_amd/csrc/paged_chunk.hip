@@ -234,6 +234,15 @@ __device__ __forceinline__ uint32_t lane_offset(uint32_t o) {
   return o;
 }
 
+// lds_barrier, with its wait known to the compiler: operands read ahead of it need none of their own behind it, where
+// one would wait for later reads as well.
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 template <int STAGES>
 struct ChunkSmem {
   KvTile tile[STAGES];       // K of tile t in tile[t % STAGES], V likewise
@@ -241,13 +250,14 @@ struct ChunkSmem {
 };
 
 // Blocks of many rows. Eight waves are two halves that run a phase apart: while one has the matrix cores (S of tile t + 1,
-// O of tile t), the other does softmax and brings a tile in, its codes loaded two tiles ahead and K staged there, V between
-// the MFMAs of the matrix phase; one barrier per phase, and the waves in the matrix phase go first (s_setprio). Bound by
-// the vector work beside the MFMAs and, in long calls, by power. 2,048 rows of 32/8 heads behind 32,771 positions 1,090
-// to 1,130 us, 1,050 to 1,080 TFLOP/s, a tile 4,000 cycles: MFMAs alone 878, with the softmax 978, with staging 1,090.
-// Without priorities 1,173, with the vector phase first 1,222; K staged in the matrix phase 1,223; row sums between the
-// MFMAs 1,212, in the softmax 1,135; fragments two / four steps ahead instead of three 1,135 / 1,120.
-// Four waves, two workgroups per CU, run a tile's phases one behind the other.
+// O of tile t), the other does softmax and brings a tile in, its codes loaded two tiles ahead and K staged there, V a code
+// at a time beside the MFMAs; one barrier per phase, and the waves in the matrix phase go first (s_setprio). Bound by the
+// phases' own lengths (a wave's vector phase 1,850 cycles, of them 400 staging and 270 exponentials; its matrix phase 1,640
+// for 32 MFMAs of 32) and, in long calls, by power. 2,048 rows of 32/8 heads behind 32,771 positions 1,060 to 1,090 us,
+// 1,080 to 1,110 TFLOP/s. There, without priorities 1,115, with the vector phase first 1,180; V staged two codes behind
+// every second MFMA 1,085; K staged in the matrix phase too 1,127 (the vector phase 1,640, the matrix phase 1,950); row
+// sums between the MFMAs 1,212 instead of 1,100, in the softmax 1,135; the row maximum between the MFMAs 1,072 instead of
+// 1,063. Four waves, two workgroups per CU, run a tile's phases one behind the other.
 template <int PW>  // waves, of 32 rows each: 8 or 4
 __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
   constexpr bool HALVES = PW == 8;
@@ -401,16 +411,20 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
           }
         }
       };
-      // two codes of each chunk per step, eight steps
+      // one code of each chunk at a time, 16 of them
       uint32_t vd[C][4];
-      auto stage_v = [&](int t, int step) {
+      float before[C];
+      auto stage_v = [&](int t, int n) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-          const uint32_t w = rv[i][step >> 1] >> (16 * (step & 1));
           const float sc = bf16_pick(vs[i], group), z = bf16_pick(vb[i], group);
-          vd[i][step & 3] = pack_bf2(fmaf(sc, (float)(w & 0xffu), z), fmaf(sc, (float)((w >> 8) & 0xffu), z));
-          if ((step & 3) == 3)
-            *v_chunk32(sm.tile[t % STAGES], key0 + 8 * PW * i, 2 * chunk + (step >> 2)) =
+          const float x = fmaf(sc, (float)((rv[i][n >> 2] >> (8 * (n & 3))) & 0xffu), z);
+          if (n & 1)
+            vd[i][(n >> 1) & 3] = pack_bf2(before[i], x);
+          else
+            before[i] = x;
+          if ((n & 7) == 7)
+            *v_chunk32(sm.tile[t % STAGES], key0 + 8 * PW * i, 2 * chunk + (n >> 3)) =
                 make_uint4(vd[i][0], vd[i][1], vd[i][2], vd[i][3]);
         }
       };
@@ -425,7 +439,7 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
       bf16x8_t p[4];
       const uint32_t k_at = k_lane32(sm.tile[0], lane), v_at = v_lane32(sm.tile[0], lane);
       auto tile_at = [](int t) { return (uint32_t)(t % STAGES) * (uint32_t)sizeof(KvTile); };
-      lds_barrier();  // the block before is done with LDS
+      tile_barrier();  // the block before is done with LDS
       if (a.sl2 < 0.0f) {
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) st.q[kk] = u4_as_bf8(signed_q(__builtin_bit_cast(uint4, st.q[kk]), a.sl2));
@@ -438,22 +452,22 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
           stage_k(t0 + 1, rk, ks, kb, k_ok);
           settle_v(t0);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) stage_v(t0, i);
+          for (int n = 0; n < 16; ++n) stage_v(t0, n);
           load_k();
           load_v();
-          next_row(t0 + 3);
         };
-        lds_barrier();
+        tile_barrier();
         if (HALVES && !grp_a) {  // half a tile behind
           begin();
-          lds_barrier();
+          tile_barrier();
         }
         scores32(k_at + tile_at(t0), st, c);
         if (!HALVES || grp_a) begin();
         for (int t = t0; t < t1; ++t) {
-          lds_barrier();
+          tile_barrier();
           // vector phase
           __builtin_amdgcn_s_setprio(0);
+          next_row(t + 3);
           stage_k(t + 2, rk, ks, kb, k_ok);
           load_k();
           if (TKEYS * t + TKEYS - 1 > lim_lo || TKEYS * t < open_from) {  // wave-uniform: masked for some row
@@ -462,9 +476,11 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
           Ahead32 ahead;
           const uint32_t kt = k_at + tile_at(t + 1);
           if constexpr (HALVES) {
-            softmax32(c, st, scale, p);
-            ahead32(kt, ahead);
-            lds_barrier();
+            softmax32(c, st, scale, p, [&]() {
+              ahead32(kt, ahead);
+              __builtin_amdgcn_sched_barrier(0);
+            });
+            tile_barrier();
           } else {
             ahead32(kt, ahead);
             softmax32(c, st, scale, p);
@@ -473,13 +489,9 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
           __builtin_amdgcn_s_setprio(1);
           // between them V of tile t + 1 is staged, and the tiles behind are loaded
           settle_v(t + 1);
-          matrix32(kt, v_at + tile_at(t), st, c, p, ahead, [&](int u) {
-            if (u < 8) stage_v(t + 1, u);
-            if (u == 8) load_v();
-            if (u == 12) {
-              next_row(t + 4);
-              asm volatile("" : "+s"(row_next));  // here, not behind the last step
-            }
+          matrix32(kt, v_at + tile_at(t), st, c, p, ahead, [&](int n) {
+            if (n < 16) stage_v(t + 1, n);
+            if (n == 16) load_v();
           });
           if (t >= t_masked || t < t_open) {
             uint64_t w = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sm.wild[t % 3][0]) |
@@ -493,7 +505,7 @@ __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
           // last read before the barrier ahead of this phase: what tile t + 2 will note
           if (tid < 2) sm.wild[(t + 2) % 3][tid] = 0;
         }
-        if (HALVES && grp_a) lds_barrier();
+        if (HALVES && grp_a) tile_barrier();
       }
 
       // ---- rows out: dims 32 w + 8 j + 4 h ..
