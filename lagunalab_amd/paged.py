@@ -763,7 +763,8 @@ class PagedBatch:
         self._refresh(states)
         q = queries.to(torch.bfloat16)
         keys, values = self.cache.keys, self.cache.values
-        if self.window is not None or (self.rotates and L > 1):
+        # single tokens by the decode kernels, which take up to 16 query heads per KV head
+        if self.window is not None or (self.rotates and (L > 1 or Hq > 16 * keys[0].shape[1])):
             out = paged_chunk_attention(q.transpose(1, 2).reshape(B * L, Hq, D), keys, values, self._table, self._lens,
                                         scale, [L] * B, self.window)
             out = out.view(B, L, Hq, D).transpose(1, 2)

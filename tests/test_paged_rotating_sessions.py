@@ -118,6 +118,8 @@ def test_attention_gets_the_sessions_tables(rotating, monkeypatch):
     two, one = torch.arange(2 * 4 * 2 * D).view(2, 4, 2, D).to(torch.bfloat16), torch.zeros((2, 4, 1, D), dtype=torch.bfloat16)
     wide = cache.batch([a, b], rotates=True)
     assert torch.equal(wide.attend(two, 0.1), two) and (wide.attend(one, 0.1) == 1).all()
+    many = torch.zeros((2, 17 * H, 1, D), dtype=torch.bfloat16)
+    assert torch.equal(wide.attend(many, 0.1), many) and seen.pop()[0] == (2, 17 * H, D)
     slide = cache.batch([a, b], window=9)
     assert torch.equal(slide.attend(two, 0.1), two) and torch.equal(slide.attend(one, 0.1), one)
     assert seen == [((4, 4, D), [70, 3], [2, 2], None), ((4, 4, D), [70, 3], [2, 2], 9), ((2, 4, D), [70, 3], [1, 1], 9)]
