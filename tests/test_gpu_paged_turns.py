@@ -272,3 +272,45 @@ def test_many_verified_blocks(dev, longest, window, spare):
             assert got[first:ends[b]].isnan().all()
             for part in (slice(0, first), slice(ends[b], None)):  # other lengths cut the others' keys elsewhere
                 assert_within(got[part], want_all[part], bound[part])
+
+
+def test_views_and_many_sequences(dev):
+    """One sequence's pages under several lengths (a table of one expanded row), queries and keys expanded over heads,
+    more sequences than a launch takes, a table far wider than the sequences, another stream."""
+    g = gen(8)
+    pool, table = sessions(g, 2, [700], dev)
+    lens, counts = [700, 130, 1, 64, 699], [90, 1, 1, 64, 40]
+    one = randn(g, sum(counts), 1, D).to(dev)
+    q = one.expand(-1, 8, -1)
+    wide = table.to(dev).expand(len(lens), -1)
+    out = paged_chunk_attention(q, *pool, wide, ints(lens, dev), SCALE, counts, 100)
+    assert_within(out, *exact(q, pool, wide.cpu(), lens, counts, 100, SCALE))
+    far = torch.full((len(lens), 3000), -1, dtype=torch.int32, device=dev)
+    far[:, :wide.shape[1]] = wide
+    for window in (None, 100):
+        out = paged_chunk_attention(q, *pool, far, ints(lens, dev), SCALE, counts, window)
+        assert_within(out, *exact(q, pool, wide.cpu(), lens, counts, window, SCALE))
+
+    starts = [(7 * i) % 200 for i in range(150)]
+    counts = [i % 4 for i in range(150)]
+    T = sum(counts)
+    table, pages = make_table(g, [s + c for s, c in zip(starts, counts)], 0)
+    rotary = Rotary.of(ROPE, dev)
+    x, k, v = randn(g, T, 4, D).to(dev), randn(g, T, 1, D).to(dev).expand(-1, 2, -1), randn(g, T, 2, D).to(dev)
+    pools = [[tuple(t.clone() for t in buf) for buf in p] for p in [fill_pool(g, pages, 2, dev, poison=False)] * 2]
+    got = paged_append_rotated(x, k, v, *pools[0], table.to(dev), ints(starts, dev), rotary, counts, fetch=True)
+    stream = torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):  # a sequence at a time
+        at = 0
+        for b, (s, c) in enumerate(zip(starts, counts)):
+            part = paged_append_rotated(x[at:at + c], k[at:at + c], v[at:at + c], *pools[1], table[b:b + 1].to(dev),
+                                        ints([s], dev), rotary, [c], fetch=True)
+            for t, p in zip(got, part):
+                assert torch.equal(t[at:at + c], p)
+            at += c
+    torch.cuda.current_stream(dev).wait_stream(stream)
+    for a, b in zip((*pools[0][0], *pools[0][1]), (*pools[1][0], *pools[1][1])):
+        assert torch.equal(a, b)
+    want, off = exact_rows(x, torch.cat([torch.arange(s, s + c) for s, c in zip(starts, counts)]), None, rotary)
+    assert ((got[0].double().cpu() - want).abs() <= want.abs() * 2.0 ** -8 + 2 * off).all()
