@@ -240,6 +240,8 @@ __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateArgs a, c
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   float c[8], s[8];
   rotation8<PAIRS>(pairs, d0, a.dims, c, s);
+  // a dim's partner among neighbours; of dims that stay 0, as partner8's: 0 times an infinite one is no 0
+  auto neighbour = [&](const float (&v)[8], int j) { return d0 + j < a.dims ? v[j ^ 1] : 0.0f; };
   float cw[8], sw[8];  // with the norm weights of the dim and of its partner
   const uint16_t* of = nullptr;
 #pragma unroll
@@ -264,12 +266,17 @@ __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateArgs a, c
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         cw[j] = c[j] * g[j];
-        sw[j] = s[j] * (PAIRS ? g[j ^ 1] : o[j]);
+        sw[j] = s[j] * (PAIRS ? neighbour(g, j) : o[j]);
       }
     }
     float x[8], y[8];
     unpack8(own[i], x);
-    if constexpr (!PAIRS) unpack8(other[i], y);
+    if constexpr (PAIRS) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = neighbour(x, j);
+    } else {
+      unpack8(other[i], y);
+    }
     if (!is_v) {
       float inv = 1.0f;
       if (w) {
@@ -280,7 +287,7 @@ __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateArgs a, c
       }
       float r[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = fmaf(PAIRS ? x[j ^ 1] : y[j], sw[j], x[j] * cw[j]) * inv;
+      for (int j = 0; j < 8; ++j) r[j] = fmaf(y[j], sw[j], x[j] * cw[j]) * inv;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = r[j];
     }
