@@ -191,7 +191,7 @@ class Attention:
         inv, self.rot_dims, self.mscale = rope_frequencies(head_dim, rope)
         self.inv_freq = inv.to(dev)
         from .rotary import Rotary
-        self.rotary = Rotary(self.inv_freq, self.mscale)
+        self.rotary = Rotary.of(rope, dev, head_dim=head_dim)
         H, Hkv, D = n_heads, n_kv_heads, head_dim
         self._splits = [H * D, Hkv * D, Hkv * D, wg.shape[0]]
 

@@ -27,5 +27,7 @@ class Rotary:
     @classmethod
     def of(cls, params: dict, device="cuda", interleaved: bool = False, head_dim: int = 128) -> "Rotary":
         """Of a rope config, as :func:`lagunalab_amd.attention.rope_frequencies` reads it."""
-        inv_freq, _, mscale = rope_frequencies(head_dim, params)
+        inv_freq, dims, mscale = rope_frequencies(head_dim, params)
+        if dims != 2 * len(inv_freq):
+            raise ValueError(f"{dims} rotated dims are not pairs")
         return cls(inv_freq.to(device), mscale, interleaved)
