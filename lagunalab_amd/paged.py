@@ -311,7 +311,7 @@ def paged_chunk_attention(q, keys, values, table, lens, scale, counts=None, wind
     lens = _ints(lens, B, "lens", dev)
     out = q.new_empty((T, Hq, HEAD_DIM))
     qp, op, tp, np = q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr()
-    seen = window or 0
+    seen = 0 if window is None or window >= PAGE * width else window  # as long as the table: it hides nothing
     lib = _lib.load()
     with _lib.on_device(dev):
         for a, n, at, cp in _launches(counts):
