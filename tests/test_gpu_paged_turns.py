@@ -15,7 +15,7 @@ from lagunalab_amd.rotary import Rotary
 from paged_util import D, PAGE, fill_pool, make_table, randn
 from test_gpu_paged_chunk import SCALE, assert_within, exact, sessions
 from test_gpu_paged_rotate import exact_rows
-from tiny_model import TinyArgs, TinyLM
+from tiny_model import TinyArgs, TinyLM, _rms, _rope, sdpa
 
 pytestmark = pytest.mark.gpu
 ROPE = {"rope_theta": 1e4, "partial_rotary_factor": 0.5}
@@ -314,3 +314,79 @@ def test_views_and_many_sequences(dev):
         assert torch.equal(a, b)
     want, off = exact_rows(x, torch.cat([torch.arange(s, s + c) for s, c in zip(starts, counts)]), None, rotary)
     assert ((got[0].double().cpu() - want).abs() <= want.abs() * 2.0 ** -8 + 2 * off).all()
+
+
+class RotatingLM(TinyLM):
+    """The tiny model with its projections rounded to bf16, as the rows of a rotating batch are: over one its attention
+    hands them on, norm and rotation are the append's."""
+
+    def _attention(self, m, x, mask, cache):
+        a, bf = self.args, torch.bfloat16
+        B, L, _ = x.shape
+        heads = (a.num_attention_heads, a.num_key_value_heads, a.num_key_value_heads)
+        q, k, v = ((x @ w.T).to(bf).view(B, L, h, D) for w, h in zip((m.q_proj, m.k_proj, m.v_proj), heads))
+        if cache.rotates:
+            q = cache.append_rotated(q, k, v, Rotary.of({"rope_theta": a.rope_theta}, x.device), m.q_norm.to(bf),
+                                     m.k_norm.to(bf), a.rms_norm_eps)
+            out = cache.attend(q, SCALE)
+        else:
+            q, k = (_rope(_rms(t.float(), w, a.rms_norm_eps).transpose(1, 2), cache.offset, a.rope_theta).to(bf)
+                    for t, w in ((q, m.q_norm), (k, m.k_norm)))
+            k, v = cache.update_and_fetch(k.contiguous(), v.transpose(1, 2).contiguous())
+            out = cache.attend(q.contiguous(), SCALE) if cache.fused_step else sdpa(q, k, v, mask, SCALE)
+        gate = torch.nn.functional.softplus(x @ m.g_proj.T)[..., None]
+        return (out.to(x.dtype).transpose(1, 2) * gate).reshape(B, L, -1) @ m.o_proj.T
+
+
+@torch.no_grad()
+def test_a_model_over_sessions_of_different_lengths(dev):
+    """Full and sliding layers over rotating batches, a pool per layer: prompts of three lengths, a chunk, tokens, a
+    session forked and one trimmed on the way; every session's logits as over dequantizing caches of its own with the
+    layers' masks. The tolerance is the one of the model above: the bf16 rows, weights and outputs of either side are off
+    by 2^-8 of their size, an 8-bit row by half a step."""
+    types = ["full_attention", "sliding_attention", "full_attention", "sliding_attention"]
+    model = RotatingLM(TinyArgs(layer_types=types), device="cuda", seed=4)
+    for m in model.layers:
+        for w in (m.q_norm, m.k_norm):
+            w.copy_(w.to(torch.bfloat16))
+    windows = [model.args.sliding_window if t == "sliding_attention" else None for t in types]
+
+    class Masked(DequantKVCache):
+        rotates = False
+
+        def make_mask(self, N, return_array=False, window_size=None):
+            from lagunalab_amd.cache import create_attention_mask
+            return create_attention_mask(N, self.offset, return_array, window_size)
+
+    g = gen(9)
+    pools = [PagedKVCache(40, 2, dev) for _ in types]
+    who, plain = [], []
+
+    def near_logits(got, want):
+        assert (got - want).abs().max() < 5e-2 * want.abs().max()
+
+    for n in (150, 67, 3):
+        s, own = [p.open() for p in pools], [Masked() for _ in types]
+        ids = torch.randint(0, 1024, (1, n), generator=g).to(dev)
+        near_logits(model(ids, cache=[p.batch([x], w, rotates=True) for p, x, w in zip(pools, s, windows)]),
+                    model(ids, cache=own))
+        who.append(s)
+        plain.append(own)
+
+    def steps(*lengths):
+        batches = [p.batch([s[i] for s in who], w, rotates=True) for i, (p, w) in enumerate(zip(pools, windows))]
+        for L in lengths:
+            ids = torch.randint(0, 1024, (len(who), L), generator=g).to(dev)
+            got = model(ids, cache=batches)
+            for i, own in enumerate(plain):
+                near_logits(got[i:i + 1], model(ids[i:i + 1], cache=own))
+
+    steps(1, 40, 1, 5)
+    who.append([p.fork(x) for p, x in zip(pools, who[0])])
+    plain.append([Masked() for _ in types])
+    for old, new in zip(plain[0], plain[-1]):
+        new.state = tuple(tuple(t.clone() for t in x) for x in old.state)
+    for p, x, own in zip(pools, who[1], plain[1]):
+        assert p.trim(x, 3) == own.trim(3) == 3
+    steps(1, 6, 1)
+    assert [pools[0].length(s[0]) for s in who] == [205, 119, 58, 205]
