@@ -254,10 +254,13 @@ struct ChunkSmem {
 // at a time beside the MFMAs; one barrier per phase, and the waves in the matrix phase go first (s_setprio). Bound by the
 // phases' own lengths (a wave's vector phase 1,850 cycles, of them 400 staging and 270 exponentials; its matrix phase 1,640
 // for 32 MFMAs of 32) and, in long calls, by power. 2,048 rows of 32/8 heads behind 32,771 positions 1,060 to 1,090 us,
-// 1,080 to 1,110 TFLOP/s. There, without priorities 1,115, with the vector phase first 1,180; V staged two codes behind
-// every second MFMA 1,085; K staged in the matrix phase too 1,127 (the vector phase 1,640, the matrix phase 1,950); row
-// sums between the MFMAs 1,212 instead of 1,100, in the softmax 1,135; the row maximum between the MFMAs 1,072 instead of
-// 1,063. Four waves, two workgroups per CU, run a tile's phases one behind the other.
+// 1,040 to 1,070 TFLOP/s. There, without priorities 1,115, with the vector phase first 1,180; V staged two codes behind
+// every second MFMA 1,085; K staged in the matrix phase too 1,127 (the vector phase 1,640, the matrix phase 1,950); the
+// row maximum between the MFMAs 1,072 instead of 1,063; where the row sums go: attn_tile32.h. Rows read back as bf16 and
+// attended by the packed prompt kernel are faster in such calls and slower in shorter or smaller ones (us, here / read
+// back): 2,048 rows behind 32,771 1,058 / 963, of 48/8 heads behind 7,000 402 / 371, 512 of 48/8 behind 7,681 117 / 122,
+// of 32/8 behind 82,159 649 / 670, 256 of 48/8 behind 1,000 30 / 43, 64 of 32/8 behind 20,000 53 / 82. Four waves, two
+// workgroups per CU, run a tile's phases one behind the other.
 template <int PW>  // waves, of 32 rows each: 8 or 4
 __global__ __launch_bounds__(64 * PW, 2) void chunk_kernel(const ChunkArgs a) {
   constexpr bool HALVES = PW == 8;
@@ -652,7 +655,10 @@ __device__ __forceinline__ Deal few_deal(const ChunkArgs& a, int lane) {
 
 // Units [p0, p1) of sequence s for its rows f0 .. f0 + 32 NB - 1: partial rows to slot .., or with WHOLE output rows.
 // AGAIN: other blocks read the pages too, and they stay in the L2 (streaming / staying, us: 48 rows of 16
-// sessions of 100 to 4,100 positions 42.6 / 39.2; of one block 64 single tokens of up to 8,200 118 / 124).
+// sessions of 100 to 4,100 positions 42.6 / 39.2; of one block 64 single tokens of up to 8,200 118 / 124). Sequences
+// taken whole stream their pages whatever their blocks, which run side by side and are few pages apart: staying is
+// within 5% either way there (48 rows of 16 windows of 512 14.9 / 15.4, of 16 sessions of 1,000 19.2 / 19.9, 96 of 8
+// windows 14.0 / 14.1, of 32 32.2 / 30.6, of 64 57.2 / 55.5, 80 of 16 of 2 KV heads 13.6 / 13.2).
 template <int NB, bool WHOLE, bool AGAIN, int WV, int MB>
 __device__ __forceinline__ void few_part(const ChunkArgs& a, FewSmem<WV, MB>& sm, int s, const Seq& sq, int f0, int hk,
                                          int p0, int p1, int64_t slot) {
@@ -956,7 +962,11 @@ __global__ __launch_bounds__(256) void few_merge_kernel(const ChunkArgs a) {
       make_uint2(pack_bf2(acc[0] * inv, acc[1] * inv), pack_bf2(acc[2] * inv, acc[3] * inv));
 }
 
-// How a call's sequences are dealt out.
+// How a call's sequences are dealt out. The lengths are the device's: the rules below take the table's width for them
+// (the window's, where it is shorter), so a table wider than its sequences may get the way that suits long ones. us,
+// table as wide as the sequences / 1,300 pages: a row behind 1,037 positions 15.0 / 9.5, of each of 64 sessions of 100 to
+// 1,500 34.5 / 39.6, 8 of 16 of 97 to 4,099 40 / 42, 8 prompts of 300 rows 26 / 35, 512 rows behind 1,000 41.9 / 42.1,
+// behind 7,681 121 / 121, 5 behind 65,536 39.0 / 38.3.
 struct ChunkPart {  // the sequences of few rows, or of many
   int nseq, rows_of, shares, blocks;  // rows of a block, shares (0: whole blocks) and blocks per KV head
   int seq[LQ_MAX_SEQS], row0[LQ_MAX_SEQS], rows[LQ_MAX_SEQS];
@@ -965,10 +975,12 @@ struct ChunkPart {  // the sequences of few rows, or of many
 struct ChunkPlan {
   ChunkPart few, many;
 };
-// Up to FEW_ROWS query rows of a sequence and KV head go as blocks of 32 that read the pages each, from the L2 but
-// the first, more as blocks that share a dequantized page. us, shared / each, 8 KV heads: 36 rows behind 20,000 positions
-// 54 / 27, 64 behind 65,536 87 / 60, 96 behind 5,000 27 / 22, 48 of 16 sessions of 100 to 4,100 44 / 45, 96 of 4 of
-// 9,000 51 / 53, 126 behind 65,536 90 / more.
+// Up to FEW_ROWS query rows of a sequence and KV head go as blocks of 32 (64) that read the pages each, those dealt out
+// from the L2 but the first, more as blocks that share a dequantized page. us, shared / each, 8 KV heads: 36 rows behind
+// 20,000 positions 54 / 27, 64 behind 65,536 87 / 60, 96 behind 65,536 86 / 74, behind 5,000 27 / 22, of 4 sessions of
+// 9,000 51 / 53, of 16 of 4,099 65 / 81, 48 of 16 of 100 to 4,100 44 / 45; above the limit 126 behind 65,536 88 / 91,
+// behind 20,000 57 / 40, behind 5,000 26 / 24, of 4 of 9,000 51 / 59, of 16 of 4,099 69 / 95: one session of up to 20,000
+// would gain, several lose more.
 constexpr int64_t FEW_ROWS = 96;
 // Blocks of many rows are taken whole, a workgroup each and the longest first, where that leaves few compute units
 // idle: IDLE_TILES per block, were all blocks as long as the table (or window) lets them be. Else the call is dealt out
@@ -981,13 +993,16 @@ constexpr int64_t FEW_ROWS = 96;
 constexpr int64_t IDLE_TILES = 8, LONGEST = 40;
 // Of more than 32 rows, 64 go as one block where a workgroup (two per CU) has TWO_UNITS half pages or more, or a sequence
 // and KV head of its own: its waves dequantize a page once for both halves, but have as much to join at the end. us, 32 /
-// 64 rows: 48 of 16 sessions of 8,000 positions 105 / 86, of 100 to 4,100 39 / 43; 48 of 4 of 20,000 75 / 63, of one 27 /
-// 34; 64 behind 65,536 61 / 57; 48 of 64 windows of 512 40 / 34, of 8 13.5 / 21.
+// 64 rows: 48 of 16 sessions of 100 to 4,100 positions 39 / 43, of 2,050 each (17 half pages) 41 / 42, of 4,099 (32) 60
+// / 57, of 4,608 (36) 65 / 60, of 6,000 77 / 67, of 8,000 97 / 81, of 100 to 8,000 60 / 55; 48 of 4 of 20,000 75 / 63, of
+// one 27 / 34; 64 behind 65,536 61 / 57; 48 of 64 windows of 512 40 / 34, of 8 13.5 / 21. Half pages by the table's
+// width: sequences that fill it gain from 32 on, those of half its width on average still lose there.
 constexpr int64_t TWO_UNITS = 36;
 // Calls of few pages per sequence take each whole: one launch, nothing to merge. Many sequences also where they are
-// longer. us on the GPU, dealt out / whole: 1 session of 512 positions, 8 KV heads 9.9 / 9.5, of 1,038 10.0 / 13.8 (with
-// the host, whose launches bound such a call, 16.3 / 14); 8 of 1,500 16.4 / 20.3, 16 windows of 1,100 20.6 / 17.6, 32
-// of 1,500 32.1 / 24.3, 64 of 100 to 1,500 39.1 / 33.2.
+// longer. us on the GPU, dealt out / whole: 1 session of 512 positions, 8 KV heads 9.3 / 10.2, of 1,038 9.5 / 15.0 (with
+// the host, whose launches bound such a call, 16.3 / 14: the limit is set for calls made one by one, a recorded step
+// would take shares from the first pages on); 8 of 1,500 16.4 / 20.3, 16 windows of 1,100 20.6 / 17.6, 32 of 1,500 32.1 /
+// 24.3, 64 of 100 to 1,500 39.1 / 33.2.
 constexpr int64_t WHOLE_PAGES = 20, WHOLE_PAGES_MANY = 32;
 ChunkPlan chunk_plan(const int32_t* counts, int64_t nseq, int64_t Hkv, int64_t G, int64_t width, int64_t window, int cus) {
   ChunkPlan p{};
